@@ -9,8 +9,9 @@
  * multiplies) lives in this one library, compiled once for sm_100a.
  *
  * Conventions
- *  - Every pointer is a device pointer unless stated otherwise. Inputs are
- *    C-contiguous, the output is fp32 C-contiguous in the planned order.
+ *  - Every pointer is a device pointer unless stated otherwise. Inputs of the
+ *    contractions are C-contiguous, their output is fp32 C-contiguous in the
+ *    planned order.
  *  - `stream` is a cudaStream_t passed as void* (torch.cuda.current_stream()
  *    .cuda_stream). All calls only enqueue work on that stream.
  *  - Functions return 0 on success or a PE_ERR_* code; the code is also
@@ -31,7 +32,8 @@ extern "C" {
 
 #define PE_MAX_RANK 8
 
-enum pe_dtype { PE_F32 = 0, PE_F16 = 1 };
+/* PE_BF16: the recurrent-mixer operators only; einsum plans take the first two. */
+enum pe_dtype { PE_F32 = 0, PE_F16 = 1, PE_BF16 = 2 };
 
 enum pe_status {
     PE_OK = 0,
@@ -174,6 +176,165 @@ int pe_broadcast_mul(const pe_broadcast_plan* plan, const void* full, const void
 /* ---- permute --------------------------------------------------------------- */
 
 int pe_permute(const pe_permute_plan* plan, const void* in, void* out, void* stream);
+
+/* ---- recurrent-mixer operators ------------------------------------------------
+ *
+ * Channels-last operators beside the contractions of a state space or linear
+ * attention layer. dtype (pe_dtype) is the element type of activations; sums,
+ * states and statistics are fp32. Strides are in elements; the channel axis has
+ * stride 1. Optional pointers may be NULL. Sequences: cu == NULL takes `batch`
+ * rows of `tokens` tokens (nseq = batch); else batch is 1 and sequence s is tokens
+ * cu[s] .. cu[s + 1] - 1 of the row, cu[0] = 0, cu[nseq] = tokens, never falling (a
+ * table that is not so gives PE_ERR_INVALID in the device word and outputs of no
+ * meaning). Sequences may be empty. Every field is 8 bytes wide.
+ */
+
+/*
+ * Selective scan. Per sequence, channel d (of group g = d / (channels / groups))
+ * and state n < states:
+ *   dt = delta + delta_bias, softplus(dt) if `softplus`
+ *   h  = exp(dt A[d, n]) h + dt u B[t, g, n]
+ *   out = (sum_n C[t, g, n] h + D[d] u) * silu(z)
+ * h0 / state: first and last h of each sequence, fp32 [nseq, channels, states]
+ * contiguous. A [channels, states], D and delta_bias [channels] fp32 contiguous;
+ * out [batch, tokens, channels] contiguous. ckpt (for the backward pass) receives
+ * h before every 16th token, pe_scan_ckpt_floats floats. ws: pe_scan_ws_bytes.
+ */
+typedef struct pe_scan_args {
+    int64_t dtype, softplus;
+    int64_t batch, tokens, channels, states, groups, nseq;
+    const int32_t* cu;
+    const void *u, *delta, *z, *B, *C;
+    const float *A, *D, *delta_bias, *h0;
+    int64_t u_sb, u_st, delta_sb, delta_st, z_sb, z_st, B_sb, B_st, B_sg, C_sb, C_st, C_sg;
+    void* out;
+    float* state;
+    float* ckpt;
+    void* ws;
+    int64_t ws_bytes;
+} pe_scan_args;
+int64_t pe_scan_ckpt_floats(int64_t tokens, int64_t nseq, int64_t packed, int64_t channels, int64_t states);
+int64_t pe_scan_ws_bytes(const pe_scan_args* args);
+int pe_selective_scan(const pe_scan_args* args, void* stream);
+
+/*
+ * Gradients of the scan from those of out (dout, strides dout_sb / dout_st) and of
+ * the last states (dstate, may be NULL). du, ddelta, dz [batch, tokens, channels]
+ * and dB, dC [batch, tokens, groups, states] in dtype; dA, dD, ddelta_bias, dh0
+ * fp32; all contiguous. dz, dD, ddelta_bias, dh0 may be NULL. The same inputs give
+ * the same bits: no sum goes through an atomic.
+ */
+typedef struct pe_scan_grad_args {
+    pe_scan_args fwd; /* out, state unused; ckpt as the forward pass wrote it */
+    const void* dout;
+    int64_t dout_sb, dout_st;
+    const float* dstate;
+    void *du, *ddelta, *dz, *dB, *dC;
+    float *dA, *dD, *ddelta_bias, *dh0;
+    void* ws;
+    int64_t ws_bytes;
+} pe_scan_grad_args;
+int64_t pe_scan_grad_ws_bytes(const pe_scan_grad_args* args);
+int pe_selective_scan_grad(const pe_scan_grad_args* args, void* stream);
+
+/*
+ * One token of each of `batch` requests. state [slots, channels, states] fp32
+ * contiguous, updated in place; request b's state is row slot[b] (slots32 or
+ * slots64; b itself if both are NULL). A negative slot skips the request (out = 0); one past
+ * the end does too and sets PE_ERR_INVALID in the device word. u, delta, z, out
+ * [batch, channels] (row strides, out contiguous); B, C [batch, groups, states].
+ */
+typedef struct pe_scan_step_args {
+    int64_t dtype, softplus;
+    int64_t batch, channels, states, groups, slots;
+    const int32_t* slots32;
+    const int64_t* slots64;
+    const void *u, *delta, *z, *B, *C;
+    const float *A, *D, *delta_bias;
+    int64_t u_sb, delta_sb, z_sb, B_sb, B_sg, C_sb, C_sg;
+    float* state;
+    void* out;
+} pe_scan_step_args;
+int pe_selective_scan_step(const pe_scan_step_args* args, void* stream);
+
+/*
+ * Short causal convolution along the tokens, one filter of `width` (2 to 4) taps a
+ * channel: p[t] = bias + sum_k weight[c, k] x[t - (width - 1) + k], out = p or silu(p)
+ * (`silu`). x before the sequence: init [nseq, width - 1, channels] (contiguous,
+ * dtype) or zeros. state receives the last width - 1 inputs of each sequence, in the
+ * same form. weight [channels, width] and bias [channels] have dtype; out contiguous.
+ */
+typedef struct pe_conv_args {
+    int64_t dtype, silu, width;
+    int64_t batch, tokens, channels, nseq;
+    const int32_t* cu;
+    const void *x, *weight, *bias, *init;
+    int64_t x_sb, x_st;
+    void *out, *state;
+} pe_conv_args;
+int pe_causal_conv(const pe_conv_args* args, void* stream);
+
+/* Its gradients, from dout (strided) and dstate (may be NULL). dx, dinit (may be
+ * NULL), dweight and dbias (may be NULL) in dtype, contiguous. */
+typedef struct pe_conv_grad_args {
+    pe_conv_args fwd; /* out and state unused */
+    const void *dout, *dstate;
+    int64_t dout_sb, dout_st;
+    void *dx, *dinit, *dweight, *dbias;
+    void* ws;
+    int64_t ws_bytes;
+} pe_conv_grad_args;
+int64_t pe_causal_conv_grad_ws_bytes(const pe_conv_grad_args* args);
+int pe_causal_conv_grad(const pe_conv_grad_args* args, void* stream);
+
+/* One token of each of `batch` requests; state [slots, width - 1, channels] (dtype,
+ * contiguous) is shifted in place. Slots as in pe_scan_step_args. */
+typedef struct pe_conv_step_args {
+    int64_t dtype, silu, width;
+    int64_t batch, channels, slots;
+    const int32_t* slots32;
+    const int64_t* slots64;
+    const void *x, *weight, *bias;
+    int64_t x_sb;
+    void *state, *out;
+} pe_conv_step_args;
+int pe_causal_conv_step(const pe_conv_step_args* args, void* stream);
+
+/*
+ * Group norm, channels last. x [batch, places, channels] (strides x_sb, x_sp): per
+ * row and group of channels / groups channels, over its places and channels,
+ *   xn = (x - mean) / sqrt(var + eps),   v = xn weight[c] + bias[c]
+ *   out = v | silu(v) (`silu`) | v silu(gate) (gate given)
+ * weight, bias [channels] (dtype, may be NULL), gate strided like x; out contiguous.
+ * mean, rstd: fp32 [batch, groups], written (needed by the backward pass), may be
+ * NULL. ws: pe_group_norm_ws_bytes.
+ */
+typedef struct pe_norm_args {
+    int64_t dtype, silu;
+    int64_t batch, places, channels, groups;
+    double eps;
+    const void *x, *weight, *bias, *gate;
+    int64_t x_sb, x_sp, gate_sb, gate_sp;
+    void* out;
+    float *mean, *rstd;
+    void* ws;
+    int64_t ws_bytes;
+} pe_norm_args;
+int64_t pe_group_norm_ws_bytes(const pe_norm_args* args);
+int pe_group_norm(const pe_norm_args* args, void* stream);
+
+/* Its gradients from dout (strided): dx, dgate (with a gate), dweight, dbias (with
+ * those) in dtype, contiguous. fwd.mean and fwd.rstd as the forward pass wrote them. */
+typedef struct pe_norm_grad_args {
+    pe_norm_args fwd; /* out unused */
+    const void* dout;
+    int64_t dout_sb, dout_sp;
+    void *dx, *dgate, *dweight, *dbias;
+    void* ws;
+    int64_t ws_bytes;
+} pe_norm_grad_args;
+int64_t pe_group_norm_grad_ws_bytes(const pe_norm_grad_args* args);
+int pe_group_norm_grad(const pe_norm_grad_args* args, void* stream);
 
 /* ---- status ---------------------------------------------------------------- */
 

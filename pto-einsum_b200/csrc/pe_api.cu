@@ -156,6 +156,39 @@ int pe_permute(const pe_permute_plan* plan, const void* in, void* out, void* str
     return permute(plan, in, out, (cudaStream_t)stream);
 }
 
+int64_t pe_scan_ckpt_floats(int64_t tokens, int64_t nseq, int64_t packed, int64_t channels, int64_t states) {
+    return scan_ckpt_floats(tokens, nseq, packed, channels, states);
+}
+int64_t pe_scan_ws_bytes(const pe_scan_args* args) { return scan_ws_bytes(args); }
+int pe_selective_scan(const pe_scan_args* args, void* stream) {
+    return set_last_error(selective_scan(args, (cudaStream_t)stream));
+}
+int64_t pe_scan_grad_ws_bytes(const pe_scan_grad_args* args) { return scan_grad_ws_bytes(args); }
+int pe_selective_scan_grad(const pe_scan_grad_args* args, void* stream) {
+    return set_last_error(selective_scan_grad(args, (cudaStream_t)stream));
+}
+int pe_selective_scan_step(const pe_scan_step_args* args, void* stream) {
+    return set_last_error(selective_scan_step(args, (cudaStream_t)stream));
+}
+int pe_causal_conv(const pe_conv_args* args, void* stream) {
+    return set_last_error(causal_conv(args, (cudaStream_t)stream));
+}
+int64_t pe_causal_conv_grad_ws_bytes(const pe_conv_grad_args* args) { return conv_grad_ws_bytes(args); }
+int pe_causal_conv_grad(const pe_conv_grad_args* args, void* stream) {
+    return set_last_error(causal_conv_grad(args, (cudaStream_t)stream));
+}
+int pe_causal_conv_step(const pe_conv_step_args* args, void* stream) {
+    return set_last_error(causal_conv_step(args, (cudaStream_t)stream));
+}
+int64_t pe_group_norm_ws_bytes(const pe_norm_args* args) { return norm_ws_bytes(args); }
+int pe_group_norm(const pe_norm_args* args, void* stream) {
+    return set_last_error(group_norm(args, (cudaStream_t)stream));
+}
+int64_t pe_group_norm_grad_ws_bytes(const pe_norm_grad_args* args) { return norm_grad_ws_bytes(args); }
+int pe_group_norm_grad(const pe_norm_grad_args* args, void* stream) {
+    return set_last_error(group_norm_grad(args, (cudaStream_t)stream));
+}
+
 int pe_last_error(void) { return t_last_error; }
 
 const char* pe_error_string(int code) {
@@ -174,7 +207,10 @@ const char* pe_error_string(int code) {
 
 int pe_device_error(void* stream) {
     if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return set_last_error(PE_ERR_CUDA);
+    // each of these reads (and clears) its own translation unit's word
     int v = gemm_device_error(true);
+    for (int w : {scan_device_error(true), scan_grad_device_error(true), conv_device_error(true)})
+        if (v == 0 || w < 0) v = w;
     if (v < 0) return set_last_error(PE_ERR_CUDA);
     set_last_error(PE_OK);
     return v;

@@ -1,0 +1,489 @@
+// pe_conv.cu - short causal convolution along the tokens (channels last), its
+// gradients and its single-token form, for sm_100a.
+//
+//   p[t] = bias + sum_k w[k] x[t - (W - 1) + k],   out = p or silu(p)
+//   g = dout act'(p),  dx[i] = sum_j w[W - 1 - j] g[i + j],  dw[k] = sum_t g[t] x[t - (W - 1) + k]
+//
+// All of it is bound by memory: two FMAs a tap against 2 (forward) or 3 (backward)
+// elements moved. A thread owns 16 bytes of channels and walks a tile of tokens with
+// the last W - 1 inputs in registers, four tokens' loads in flight, so that each
+// input is read once apart from the W - 1 tokens before (after) a tile.
+#include "pe_mixer.cuh"
+
+namespace pe {
+
+namespace {
+
+constexpr int U = 4;          // tokens loaded ahead
+constexpr int kBlock = 256;
+constexpr int kSiteOffsets = 34, kSiteSlot = 35;
+
+template <typename T>
+struct ConvP {
+    Seqs seqs;
+    int64_t C, CV;            // channels, channel vectors
+    int64_t tiles, tile;      // token tiles in all, tokens a tile
+    int silu;
+    const T *x, *w, *bias, *init;
+    int64_t x_sb, x_st;
+    T *out, *state;
+};
+
+template <typename T, int W, int V>
+struct Filter {
+    float w[W][V], b[V];
+    __device__ __forceinline__ void load(const T* weight, const T* bias, int64_t c) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][v] = to_float(__ldg(weight + (c + v) * W + k));
+            b[v] = bias ? to_float(__ldg(bias + c + v)) : 0.0f;
+        }
+    }
+};
+
+// Inputs before token `pos` (counted from the sequence's start): win[j] = x[pos - (W - 1) + j].
+template <typename T, int W, int V>
+__device__ __forceinline__ void load_before(const ConvP<T>& p, const T* xs, int64_t pos, int s, int64_t c,
+                                            float (&win)[W][V]) {
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+        const int64_t i = pos - (W - 1) + j;
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[j][v] = 0.0f;
+        if (i >= 0)
+            unpack(load_vec<T, V>(xs + i * p.x_st + c), win[j]);
+        else if (p.init)
+            unpack(load_vec<T, V>(p.init + ((int64_t)s * (W - 1) + (W - 1) + i) * p.C + c), win[j]);
+    }
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kBlock) conv_fwd(const __grid_constant__ ConvP<T> p) {
+    if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.seqs, threadIdx.x, kSiteOffsets);
+    int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    const int64_t tile = id / p.CV, c = (id - tile * p.CV) * V;
+    if (tile >= p.tiles) {
+        // the sequences' last W - 1 inputs
+        const int64_t s = tile - p.tiles;
+        if (!p.state || s >= p.seqs.nseq) return;
+        const Span sp = seq_span(p.seqs, (int)s);
+        const T* xs = p.x + sp.row * p.x_sb + sp.start * p.x_st;
+        float win[W][V];
+        load_before<T, W, V>(p, xs, sp.len, (int)s, c, win);
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) store_vec(p.state + (s * (W - 1) + j) * p.C + c, pack<T, V>(win[j]));
+        return;
+    }
+    Filter<T, W, V> f;
+    f.load(p.w, p.bias, c);
+    const int64_t per = ceil_div(p.seqs.tokens, p.tile);   // tiles a row
+    int64_t t = tile % per * p.tile;
+    const int64_t end = min(p.seqs.tokens, t + p.tile);
+    int s = p.seqs.cu ? seq_of_token(p.seqs, t) : (int)(tile / per);
+    for (; t < end && s < p.seqs.nseq; ++s) {
+        const Span sp = seq_span(p.seqs, s);
+        const int64_t stop = min(end, sp.start + sp.len);   // of the tile's tokens in this sequence
+        if (stop <= t || sp.start > t) continue;
+        const T* xr = p.x + sp.row * p.x_sb + c;
+        T* o = p.out + sp.row * p.seqs.tokens * p.C + c;
+        float win[W][V];
+        load_before<T, W, V>(p, xr - c + sp.start * p.x_st, t - sp.start, s, c, win);
+        for (; t < stop; t += U) {
+            Vec<T, V> raw[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (t + i < stop) raw[i] = load_vec<T, V>(xr + (t + i) * p.x_st);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (t + i < stop) {
+                    unpack(raw[i], win[W - 1]);
+                    float y[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        float a = f.b[v];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) a = fmaf(f.w[k][v], win[k][v], a);
+                        y[v] = p.silu ? a * sigmoidf(a) : a;
+#pragma unroll
+                        for (int k = 0; k < W - 1; ++k) win[k][v] = win[k + 1][v];
+                    }
+                    store_vec(o + (t + i) * p.C, pack<T, V>(y));
+                }
+            }
+        }
+        t = stop;
+    }
+}
+
+// ---- backward -------------------------------------------------------------------
+template <typename T>
+struct ConvGradP {
+    ConvP<T> f;
+    const T *dout, *dstate;
+    int64_t o_sb, o_st;
+    T *dx, *dinit;
+    float *pw, *pb;     // [blocks along the tokens][C W] and [..][C]
+    int bx;             // channel vectors a block (power of two <= 32)
+};
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kBlock) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
+    __shared__ float red[(W + 1) * V * kBlock];
+    const ConvP<T>& f = p.f;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) check_offsets(f.seqs, threadIdx.x, kSiteOffsets);
+    const int by = kBlock / p.bx, x = threadIdx.x % p.bx, y = threadIdx.x / p.bx;
+    const int64_t cv = (int64_t)blockIdx.y * p.bx + x, c = cv * V;
+    const int64_t tile = (int64_t)blockIdx.x * by + y;
+    float dw[W][V], db[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        db[v] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) dw[k][v] = 0.0f;
+    }
+    if (cv < f.CV && tile < f.tiles) {
+        Filter<T, W, V> flt;
+        flt.load(f.w, f.bias, c);
+        const int64_t per = ceil_div(f.seqs.tokens, f.tile);
+        int64_t t = tile % per * f.tile;
+        const int64_t end = min(f.seqs.tokens, t + f.tile);
+        int s = f.seqs.cu ? seq_of_token(f.seqs, t) : (int)(tile / per);
+        for (; t < end && s < f.seqs.nseq; ++s) {
+            const Span sp = seq_span(f.seqs, s);
+            const int64_t fin = sp.start + sp.len, stop = min(end, fin);
+            if (stop <= t || sp.start > t) continue;
+            const T* xr = f.x + sp.row * f.x_sb + c;
+            const T* dor = p.dout + sp.row * p.o_sb + c;
+            T* dx = p.dx + sp.row * f.seqs.tokens * f.C + c;
+            float win[W][V], g[W][V];   // inputs and g of the tokens up to the current one
+            load_before<T, W, V>(f, xr - c + sp.start * f.x_st, t - sp.start, s, c, win);
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) g[k][v] = 0.0f;
+            // g of the tokens t .. stop + W - 2 gives dx of t .. stop - 1 (and of the
+            // inputs before the sequence where t starts it)
+            const int64_t last = stop + W - 1;
+            for (int64_t k0 = t; k0 < last; k0 += U) {
+                Vec<T, V> rx[U], ro[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+                    if (k0 + i < min(last, fin)) {
+                        rx[i] = load_vec<T, V>(xr + (k0 + i) * f.x_st);
+                        ro[i] = load_vec<T, V>(dor + (k0 + i) * p.o_st);
+                    }
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int64_t k = k0 + i;
+                    if (k >= last) break;
+                    if (k < fin) {
+                        unpack(rx[i], win[W - 1]);
+                        unpack(ro[i], g[W - 1]);
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            if (f.silu) {
+                                float a = flt.b[v];
+#pragma unroll
+                                for (int q = 0; q < W; ++q) a = fmaf(flt.w[q][v], win[q][v], a);
+                                g[W - 1][v] *= silu_slope(a, sigmoidf(a));
+                            }
+                            if (k < stop) {
+                                db[v] += g[W - 1][v];
+#pragma unroll
+                                for (int q = 0; q < W; ++q) dw[q][v] = fmaf(g[W - 1][v], win[q][v], dw[q][v]);
+                            }
+#pragma unroll
+                            for (int q = 0; q < W - 1; ++q) win[q][v] = win[q + 1][v];
+                        }
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) g[W - 1][v] = 0.0f;
+                    }
+                    const int64_t i0 = k - (W - 1);          // the input whose sum is complete
+                    const int64_t pos = i0 - sp.start;
+                    if (i0 >= t || (pos < 0 && t == sp.start && p.dinit)) {
+                        float d[V];
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            d[v] = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < W; ++j) d[v] = fmaf(flt.w[W - 1 - j][v], g[j][v], d[v]);
+                        }
+                        const int64_t j = pos + W - 1 - sp.len;  // its place in the last state
+                        if (p.dstate && j >= 0) {
+                            float e[V];
+                            unpack(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
+#pragma unroll
+                            for (int v = 0; v < V; ++v) d[v] += e[v];
+                        }
+                        if (i0 >= t)
+                            store_vec(dx + i0 * f.C, pack<T, V>(d));
+                        else
+                            store_vec(p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c, pack<T, V>(d));
+                    }
+#pragma unroll
+                    for (int q = 0; q < W - 1; ++q)
+#pragma unroll
+                        for (int v = 0; v < V; ++v) g[q][v] = g[q + 1][v];
+                }
+            }
+            t = stop;
+        }
+    }
+    // the block's tiles, in order
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) red[(k * V + v) * kBlock + threadIdx.x] = dw[k][v];
+        red[(W * V + v) * kBlock + threadIdx.x] = db[v];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (W + 1) * V * p.bx; i += kBlock) {
+        const int xi = i % p.bx, kv = i / p.bx, k = kv / V, v = kv % V;
+        const int64_t ci = ((int64_t)blockIdx.y * p.bx + xi) * V + v;
+        if (ci >= f.C) continue;
+        float a = 0.0f;
+        for (int r = 0; r < by; ++r) a += red[kv * kBlock + r * p.bx + xi];
+        if (k < W)
+            p.pw[(int64_t)blockIdx.x * f.C * W + ci * W + k] = a;
+        else
+            p.pb[(int64_t)blockIdx.x * f.C + ci] = a;
+    }
+}
+
+// dinit of the sequences without tokens: their last state is their first.
+template <typename T>
+__global__ void __launch_bounds__(kBlock) conv_empty(Seqs q, int64_t n, const T* dstate, T* dinit) {
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i >= n * q.nseq || seq_span(q, (int)(i / n)).len) return;
+    dinit[i] = dstate ? dstate[i] : from_float<T>(0.0f);
+}
+
+// ---- one token --------------------------------------------------------------------
+template <typename T>
+struct ConvStepP {
+    int64_t C, CV, batch, slots, x_sb;
+    const int32_t* s32;
+    const int64_t* s64;
+    int silu;
+    const T *x, *w, *bias;
+    T *state, *out;
+};
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(128) conv_step(const __grid_constant__ ConvStepP<T> p) {
+    const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    const int64_t b = id / p.CV, c = (id - b * p.CV) * V;
+    if (b >= p.batch) return;
+    int64_t slot = b;
+    if (p.s32) slot = __ldg(p.s32 + b);
+    if (p.s64) slot = __ldg(p.s64 + b);
+    float y[V];
+    if (slot < 0 || slot >= p.slots) {
+        if (slot >= 0 && c == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = 0.0f;
+        store_vec(p.out + b * p.C + c, pack<T, V>(y));
+        return;
+    }
+    T* st = p.state + slot * (W - 1) * p.C + c;
+    Vec<T, V> win[W];
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) win[k] = *reinterpret_cast<const Vec<T, V>*>(st + k * p.C);
+    win[W - 1] = load_vec<T, V>(p.x + b * p.x_sb + c);
+    Filter<T, W, V> f;
+    f.load(p.w, p.bias, c);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float a = f.b[v];
+#pragma unroll
+        for (int k = 0; k < W; ++k) a = fmaf(f.w[k][v], to_float(win[k].v[v]), a);
+        y[v] = p.silu ? a * sigmoidf(a) : a;
+    }
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) store_vec(st + k * p.C, win[k + 1]);
+    store_vec(p.out + b * p.C + c, pack<T, V>(y));
+}
+
+// ---- host -------------------------------------------------------------------------
+int check_conv(const pe_conv_args* a) {
+    if (!a || a->dtype < PE_F32 || a->dtype > PE_BF16 || a->width < 2 || a->width > 4) return PE_ERR_INVALID;
+    if (a->batch < 0 || a->tokens < 0 || a->channels < 1 || a->nseq < 0) return PE_ERR_INVALID;
+    if (a->cu ? a->batch != 1 : a->nseq != a->batch) return PE_ERR_INVALID;
+    if (a->channels > (1 << 24) || a->nseq > (1 << 24)) return PE_ERR_UNSUPPORTED;
+    if (!a->weight || (a->tokens && a->batch && !a->x)) return PE_ERR_INVALID;
+    return PE_OK;
+}
+
+int elem_bytes(int64_t dtype) { return dtype == PE_F32 ? 4 : 2; }
+
+// 16-byte accesses: every row of every tensor starts on a 16-byte boundary.
+bool wide(int64_t dtype, int64_t channels, std::initializer_list<const void*> ptrs,
+          std::initializer_list<int64_t> strides) {
+    const int64_t v = 16 / elem_bytes(dtype);
+    if (channels % v) return false;
+    for (const void* q : ptrs)
+        if ((uintptr_t)q % 16) return false;
+    for (int64_t st : strides)
+        if (st % v) return false;
+    return true;
+}
+
+template <typename T>
+ConvP<T> conv_params(const pe_conv_args* a, int v, int64_t tile) {
+    ConvP<T> p;
+    p.seqs = Seqs{a->cu, a->tokens, (int32_t)a->nseq};
+    p.C = a->channels; p.CV = a->channels / v;
+    p.tile = tile;
+    p.tiles = ceil_div(a->tokens, tile) * a->batch;
+    p.silu = a->silu != 0;
+    p.x = (const T*)a->x; p.w = (const T*)a->weight; p.bias = (const T*)a->bias; p.init = (const T*)a->init;
+    p.x_sb = a->x_sb; p.x_st = a->x_st;
+    p.out = (T*)a->out; p.state = (T*)a->state;
+    return p;
+}
+
+// Tokens a thread walks in the forward pass.
+int64_t fwd_tile(const pe_conv_args*) { return 16; }
+constexpr int64_t kBwdTile = 16;
+
+template <typename T, int W, int V>
+int conv_run(const pe_conv_args* a, cudaStream_t s) {
+    const ConvP<T> p = conv_params<T>(a, V, fwd_tile(a));
+    const int64_t ids = (p.tiles + (p.state ? a->nseq : 0)) * p.CV, blocks = ceil_div(ids, kBlock);
+    if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+    if (!blocks) return PE_OK;
+    conv_fwd<T, W, V><<<(unsigned)blocks, kBlock, 0, s>>>(p);
+    count_launch();
+    return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
+}
+
+struct ConvGradShape {
+    int bx;
+    int64_t rows;       // blocks along the tokens
+};
+ConvGradShape grad_shape(const pe_conv_args* a, int v) {
+    const int64_t cv = a->channels / v;
+    ConvGradShape g{1, 0};
+    while (g.bx < 32 && g.bx < cv) g.bx *= 2;
+    g.rows = ceil_div(ceil_div(a->tokens, kBwdTile) * a->batch, kBlock / g.bx);
+    return g;
+}
+
+template <typename T, int W, int V>
+int conv_grad_run(const pe_conv_grad_args* g, cudaStream_t s) {
+    const pe_conv_args* a = &g->fwd;
+    const ConvGradShape sh = grad_shape(a, V);
+    ConvGradP<T> p;
+    p.f = conv_params<T>(a, V, kBwdTile);
+    p.dout = (const T*)g->dout; p.dstate = (const T*)g->dstate;
+    p.o_sb = g->dout_sb; p.o_st = g->dout_st;
+    p.dx = (T*)g->dx; p.dinit = (T*)g->dinit;
+    p.pw = (float*)g->ws;
+    p.pb = p.pw + sh.rows * a->channels * W;
+    p.bx = sh.bx;
+    const int64_t cblocks = ceil_div(p.f.CV, sh.bx);
+    if (sh.rows > 0x7fffffffll || cblocks > 65535) return PE_ERR_UNSUPPORTED;
+    if (sh.rows) {
+        conv_bwd<T, W, V><<<dim3((unsigned)sh.rows, (unsigned)cblocks), kBlock, 0, s>>>(p);
+        count_launch();
+        if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
+    }
+    const int64_t n = (W - 1) * a->channels;
+    if (g->dinit && a->nseq && (a->cu || a->tokens == 0)) {
+        conv_empty<T><<<(unsigned)ceil_div(n * a->nseq, kBlock), kBlock, 0, s>>>(p.f.seqs, n, p.dstate, p.dinit);
+        count_launch();
+        if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
+    }
+    int rc = sum_rows(p.pw, sh.rows, a->channels * W, (int)a->dtype, g->dweight, s);
+    if (!rc && g->dbias) rc = sum_rows(p.pb, sh.rows, a->channels, (int)a->dtype, g->dbias, s);
+    return rc;
+}
+
+template <typename T, int W, int V>
+int conv_step_run(const pe_conv_step_args* a, cudaStream_t s) {
+    ConvStepP<T> p;
+    p.C = a->channels; p.CV = a->channels / V; p.batch = a->batch; p.slots = a->slots; p.x_sb = a->x_sb;
+    p.s32 = a->slots32; p.s64 = a->slots64;
+    p.silu = a->silu != 0;
+    p.x = (const T*)a->x; p.w = (const T*)a->weight; p.bias = (const T*)a->bias;
+    p.state = (T*)a->state; p.out = (T*)a->out;
+    const int64_t blocks = ceil_div(p.batch * p.CV, 128);
+    if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+    conv_step<T, W, V><<<(unsigned)blocks, 128, 0, s>>>(p);
+    count_launch();
+    return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
+}
+
+#define PE_CONV_W(F, T, V, w, ...)                    \
+    switch (w) {                                      \
+        case 2: return F<T, 2, V>(__VA_ARGS__);       \
+        case 3: return F<T, 3, V>(__VA_ARGS__);       \
+        default: return F<T, 4, V>(__VA_ARGS__);      \
+    }
+template <typename T, int V>
+int conv_w(const pe_conv_args* a, cudaStream_t s) { PE_CONV_W(conv_run, T, V, a->width, a, s) }
+template <typename T, int V>
+int conv_grad_w(const pe_conv_grad_args* a, cudaStream_t s) { PE_CONV_W(conv_grad_run, T, V, a->fwd.width, a, s) }
+template <typename T, int V>
+int conv_step_w(const pe_conv_step_args* a, cudaStream_t s) { PE_CONV_W(conv_step_run, T, V, a->width, a, s) }
+
+#define PE_CONV_T(F, dtype, vec, ...)                                                               \
+    switch (dtype) {                                                                                \
+        case PE_F32: return vec ? F<float, 4>(__VA_ARGS__) : F<float, 1>(__VA_ARGS__);              \
+        case PE_F16: return vec ? F<__half, 8>(__VA_ARGS__) : F<__half, 1>(__VA_ARGS__);            \
+        default: return vec ? F<__nv_bfloat16, 8>(__VA_ARGS__) : F<__nv_bfloat16, 1>(__VA_ARGS__);  \
+    }
+int conv_any(const pe_conv_args* a, bool vec, cudaStream_t s) { PE_CONV_T(conv_w, a->dtype, vec, a, s) }
+int conv_grad_any(const pe_conv_grad_args* a, bool vec, cudaStream_t s) {
+    PE_CONV_T(conv_grad_w, a->fwd.dtype, vec, a, s)
+}
+int conv_step_any(const pe_conv_step_args* a, bool vec, cudaStream_t s) { PE_CONV_T(conv_step_w, a->dtype, vec, a, s) }
+
+bool grad_wide(const pe_conv_grad_args* g) {
+    const pe_conv_args* a = &g->fwd;
+    return wide(a->dtype, a->channels, {a->x, a->init, g->dout, g->dstate, g->dx, g->dinit},
+                {a->x_sb, a->x_st, g->dout_sb, g->dout_st});
+}
+
+}  // namespace
+
+int causal_conv(const pe_conv_args* a, cudaStream_t s) {
+    if (int rc = check_conv(a)) return rc;
+    if (a->tokens && a->batch && !a->out) return PE_ERR_INVALID;
+    return conv_any(a, wide(a->dtype, a->channels, {a->x, a->init, a->out, a->state}, {a->x_sb, a->x_st}), s);
+}
+
+int64_t conv_grad_ws_bytes(const pe_conv_grad_args* g) {
+    if (!g || check_conv(&g->fwd) != PE_OK) return 0;
+    const pe_conv_args* a = &g->fwd;
+    return grad_shape(a, grad_wide(g) ? 16 / elem_bytes(a->dtype) : 1).rows * a->channels * (a->width + 1) * 4;
+}
+
+int causal_conv_grad(const pe_conv_grad_args* g, cudaStream_t s) {
+    if (!g) return PE_ERR_INVALID;
+    if (int rc = check_conv(&g->fwd)) return rc;
+    if (!g->dweight || (g->fwd.tokens && g->fwd.batch && (!g->dout || !g->dx))) return PE_ERR_INVALID;
+    const int64_t need = conv_grad_ws_bytes(g);
+    if (need && (!g->ws || g->ws_bytes < need)) return PE_ERR_WORKSPACE;
+    return conv_grad_any(g, grad_wide(g), s);
+}
+
+int causal_conv_step(const pe_conv_step_args* a, cudaStream_t s) {
+    if (!a || a->dtype < PE_F32 || a->dtype > PE_BF16 || a->width < 2 || a->width > 4 || a->batch < 0 ||
+        a->channels < 1 || a->slots < 0)
+        return PE_ERR_INVALID;
+    if (a->batch == 0) return PE_OK;
+    if (!a->x || !a->weight || !a->state || !a->out) return PE_ERR_INVALID;
+    return conv_step_any(a, wide(a->dtype, a->channels, {a->x, a->state, a->out}, {a->x_sb}), s);
+}
+
+int conv_device_error(bool clear) {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v && clear) cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+    return v;
+}
+
+}  // namespace pe

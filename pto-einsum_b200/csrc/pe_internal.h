@@ -41,4 +41,26 @@ int contract_cached(void* cache, const pe_contract_plan* plan, const void* in0, 
 int gemm_device_error(bool clear);
 int wait_timeout_selftest(uint64_t timeout_ns, cudaStream_t s);
 
+// out[c] = sum over r < rows of part[r][c], rounded to dtype; a fixed order of additions.
+int sum_rows(const float* part, int64_t rows, int64_t cols, int dtype, void* out, cudaStream_t s);
+
+// Recurrent-mixer operators.
+int64_t scan_ckpt_floats(int64_t tokens, int64_t nseq, int64_t packed, int64_t channels, int64_t states);
+int64_t scan_ws_bytes(const pe_scan_args* a);
+int selective_scan(const pe_scan_args* a, cudaStream_t s);
+int64_t scan_grad_ws_bytes(const pe_scan_grad_args* a);
+int selective_scan_grad(const pe_scan_grad_args* a, cudaStream_t s);
+int selective_scan_step(const pe_scan_step_args* a, cudaStream_t s);
+int scan_device_error(bool clear);
+int scan_grad_device_error(bool clear);
+int causal_conv(const pe_conv_args* a, cudaStream_t s);
+int64_t conv_grad_ws_bytes(const pe_conv_grad_args* a);
+int causal_conv_grad(const pe_conv_grad_args* a, cudaStream_t s);
+int causal_conv_step(const pe_conv_step_args* a, cudaStream_t s);
+int conv_device_error(bool clear);
+int64_t norm_ws_bytes(const pe_norm_args* a);
+int group_norm(const pe_norm_args* a, cudaStream_t s);
+int64_t norm_grad_ws_bytes(const pe_norm_grad_args* a);
+int group_norm_grad(const pe_norm_grad_args* a, cudaStream_t s);
+
 }  // namespace pe

@@ -1,0 +1,183 @@
+// pe_mixer.cuh - what the recurrent-mixer kernels share: element types, packed
+// sequences, the activations and warp reductions.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "pe_common.cuh"
+
+namespace pe {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// V elements that one load moves (V * sizeof(T) is 16 bytes, or V is 1).
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+    T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+    if constexpr (V * sizeof(T) == 16) {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+        return *reinterpret_cast<const Vec<T, V>*>(&r);
+    } else {
+        static_assert(V == 1, "16 bytes or one element");
+        Vec<T, V> r;
+        r.v[0] = __ldg(p);
+        return r;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& r) {
+    *reinterpret_cast<Vec<T, V>*>(p) = r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V>& r, float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = to_float(r.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(f[i]);
+    return r;
+}
+
+// 1 / (1 + exp(-x)). Where exp(-x) overflows the quotient is 0, its limit.
+__device__ __forceinline__ float sigmoidf(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// d silu(x) / dx with s = sigmoid(x).
+__device__ __forceinline__ float silu_slope(float x, float s) { return s * (1.0f + x * (1.0f - s)); }
+
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1]. log1p(e) =
+// 2 artanh(s) with s = e / (2 + e) <= 1/3, whose odd power series through s^13
+// leaves a relative error below (1/9)^7 / 15 = 1.4e-8. A logarithm of the
+// rounded 1 + e would lose the small step sizes (e = 1e-3 keeps 13 bits).
+__device__ __forceinline__ float softplusf(float x) {
+    const float e = __expf(-fabsf(x));
+    const float s = __fdividef(e, 2.0f + e);
+    const float q = s * s;
+    float r = fmaf(q, 1.0f / 13, 1.0f / 11);
+    r = fmaf(r, q, 1.0f / 9);
+    r = fmaf(r, q, 1.0f / 7);
+    r = fmaf(r, q, 1.0f / 5);
+    r = fmaf(r, q, 1.0f / 3);
+    r = fmaf(r, q, 1.0f);
+    // NaN stays NaN: fmaxf alone would drop it, the product with s does not
+    return fmaxf(x, 0.0f) + 2.0f * s * r;
+}
+
+// 2^x of one instruction (relative error 2^-22, denormal results flushed).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- sequences ----------------------------------------------------------------
+// Uniform batches (cu == nullptr): nseq rows of `tokens` tokens. Packed: one row of
+// `tokens` tokens that holds nseq sequences, the s-th from cu[s] to cu[s + 1].
+struct Seqs {
+    const int32_t* cu;
+    int64_t tokens;
+    int32_t nseq;
+};
+struct Span {
+    int64_t row;    // batch row of the sequence's tokens
+    int64_t start;  // its first token in that row
+    int64_t len;
+};
+
+// Offsets read from the device are clamped, so that a wrong table cannot lead out
+// of the tensors; check_offsets reports it.
+__device__ __forceinline__ int64_t seq_offset(const Seqs& q, int s) {
+    const int64_t c = __ldg(q.cu + s);
+    return c < 0 ? 0 : (c > q.tokens ? q.tokens : c);
+}
+__device__ __forceinline__ Span seq_span(const Seqs& q, int s) {
+    if (!q.cu) return Span{s, 0, q.tokens};
+    const int64_t a = seq_offset(q, s), b = seq_offset(q, s + 1);
+    return Span{0, a, b > a ? b - a : 0};
+}
+
+// Pieces of `size` tokens, counted from each sequence's own start, are numbered so
+// that a number can be found and inverted without a table: piece j of sequence s is
+// piece_base(s) + j with piece_base(s) = cu[s] / size + s. Since
+// floor(a + b) - floor(a) + 1 >= ceil(b), the numbers of a sequence end before the
+// next one's begin; an empty sequence owns one number, and numbers without tokens
+// are skipped. Uniform batches use s * ceil(tokens / size).
+__host__ __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int64_t piece_base(const Seqs& q, int s, int64_t size) {
+    if (!q.cu) return (int64_t)s * (q.tokens > size ? ceil_div(q.tokens, size) : 1);
+    return seq_offset(q, s) / size + s;
+}
+__host__ __device__ __forceinline__ int64_t piece_count(const Seqs& q, int64_t size) {
+    const int64_t n = q.tokens > size ? ceil_div(q.tokens, size) : 1;
+    return q.cu ? n + q.nseq : n * q.nseq;
+}
+// Sequence and index of a piece number.
+__device__ __forceinline__ void piece_find(const Seqs& q, int64_t piece, int64_t size, int& s, int64_t& j) {
+    if (!q.cu) {
+        const int64_t n = q.tokens > size ? ceil_div(q.tokens, size) : 1;
+        s = (int)(piece / n);
+        j = piece - s * n;
+        return;
+    }
+    int lo = 0, hi = q.nseq;  // the last s with piece_base(s) <= piece
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (piece_base(q, mid, size) <= piece) lo = mid; else hi = mid;
+    }
+    s = lo;
+    j = piece - piece_base(q, s, size);
+    if (j < 0) j = 0;
+}
+// Last sequence that starts at or before token t of a packed row.
+__device__ __forceinline__ int seq_of_token(const Seqs& q, int64_t t) {
+    int lo = 0, hi = q.nseq;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (seq_offset(q, mid) <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+// One warp of the grid looks the offsets over: 0 first, `tokens` last, never falling.
+__device__ __forceinline__ void check_offsets(const Seqs& q, int lane, int site) {
+    if (!q.cu) return;
+    bool bad = __ldg(q.cu) != 0 || __ldg(q.cu + q.nseq) != q.tokens;
+    for (int s = lane; s < q.nseq; s += 32) bad |= __ldg(q.cu + s) > __ldg(q.cu + s + 1);
+    if (bad) record_error(PE_ERR_INVALID | (site << 8));
+}
+
+// ---- warp reduction --------------------------------------------------------------
+// R values a lane, summed over the R lanes that differ in the bits STEP .. STEP * R / 2
+// of the lane number: lane bit pattern i of those bits ends with the sum of value i.
+// Each level halves the values (R - 1 shuffles in all, against R log2 R for R sums
+// that every lane keeps).
+template <int R, int STEP>
+__device__ __forceinline__ float reduce_scatter(float (&v)[R], int lane) {
+#pragma unroll
+    for (int m = R / 2; m >= 1; m /= 2) {
+        const bool hi = lane & (m * STEP);
+#pragma unroll
+        for (int i = 0; i < m; ++i) {
+            const float send = hi ? v[i] : v[i + m];
+            const float keep = hi ? v[i + m] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m * STEP);
+        }
+    }
+    return v[0];
+}
+
+}  // namespace pe

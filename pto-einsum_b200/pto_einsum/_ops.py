@@ -1,0 +1,141 @@
+"""Calls into the core library for operators that take strided torch tensors: argument
+structs, streams and the checks they share."""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from ._core import core_lib, error_string
+from .builder import _raw_stream_getter
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+_get_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = None
+_fns: dict = {}
+
+
+def packer(fields: str) -> struct.Struct:
+    """An argument struct of 8-byte fields: q integers, Q pointers, d doubles."""
+    return struct.Struct("=" + fields)
+
+
+def function(name: str, restype=ctypes.c_int, sizes: bool = False):
+    """The core library's `name`(args, stream), or `name`(args) for the workspace sizes."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = getattr(core_lib(), name)
+        fn.argtypes = [ctypes.c_char_p] if sizes else [ctypes.c_char_p, ctypes.c_void_p]
+        fn.restype = ctypes.c_int64 if sizes else restype
+        _fns[name] = fn
+    return fn
+
+
+def call(name: str, args: bytes, dev: torch.device):
+    """Enqueue on the device's current stream; a nonzero status raises RuntimeError."""
+    global _raw_stream
+    if _raw_stream is None:
+        _raw_stream = _raw_stream_getter()
+    fn, idx = function(name), dev.index
+    if idx == _get_device():
+        rc = fn(args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(args, torch.cuda.current_stream(idx).cuda_stream)
+    if rc:
+        raise RuntimeError(f"pto_einsum: {name} failed: {error_string(rc)} ({rc})")
+
+
+def sized(name: str, args: bytes, dev: torch.device) -> int:
+    """Workspace bytes; the rule may ask the device for its number of SMs."""
+    fn = function(name, sizes=True)
+    if dev.index == _get_device():
+        return fn(args)
+    with torch.cuda.device(dev.index):
+        return fn(args)
+
+
+def workspace(nbytes: int, dev: torch.device):
+    """Scratch from torch's caching allocator, so it belongs to the current stream."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def check_tensor(name: str, t, shape, dtype, dev):
+    """`t` must be a tensor of that shape, type and device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor (got {type(t).__name__})")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev} (got {t.device})")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+    if t.shape != torch.Size(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+
+
+def check_activations(name: str, t, dims):
+    """The tensor whose type and device the others follow."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor (got {type(t).__name__})")
+    if t.device.type != "cuda":
+        raise ValueError(f"pto_einsum: {name} must be a CUDA tensor (got {t.device})")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16 (got {t.dtype})")
+    if t.dim() not in dims:
+        raise ValueError(f"{name} must have {' or '.join(map(str, dims))} dimensions (got shape {tuple(t.shape)})")
+
+
+def rows(t):
+    """`t` with a last axis of stride 1 (a copy where it has another)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def stride(t, axis: int) -> int:
+    """Stride of an axis, 0 for one of length one (whatever the tensor says of it)."""
+    return 0 if t is None or t.shape[axis] == 1 else t.stride(axis)
+
+
+def offsets(cu_seqlens, batch: int, tokens: int, dev):
+    """cu_seqlens as an int32 tensor on `dev`, and the number of sequences.
+
+    A list or a host tensor is checked here; one on the device is not read by the host
+    (the kernels keep within the tensors whatever it holds and report a wrong table in
+    the device error word)."""
+    if cu_seqlens is None:
+        return None, batch
+    if batch != 1:
+        raise ValueError(f"cu_seqlens takes one row of packed sequences (got a batch of {batch})")
+    if tokens > 2 ** 31 - 1:
+        raise ValueError("cu_seqlens takes rows of less than 2**31 tokens")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.device.type == "cpu":
+        cu = [int(v) for v in (cu_seqlens.tolist() if hasattr(cu_seqlens, "tolist") else cu_seqlens)]
+        if len(cu) < 2 or cu[0] != 0 or cu[-1] != tokens or any(a > b for a, b in zip(cu, cu[1:])):
+            raise ValueError(f"cu_seqlens must rise from 0 to the {tokens} tokens of the row")
+        return torch.tensor(cu, dtype=torch.int32, device=dev), len(cu) - 1
+    if cu_seqlens.device != dev:
+        raise ValueError(f"cu_seqlens must be on {dev} (got {cu_seqlens.device})")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        raise ValueError(f"cu_seqlens must be one row of at least two offsets (got {tuple(cu_seqlens.shape)})")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"cu_seqlens must be int32 or int64 (got {cu_seqlens.dtype})")
+    return cu_seqlens.to(torch.int32).contiguous(), cu_seqlens.shape[0] - 1
+
+
+def slot_pointers(slots, batch: int, dev):
+    """(pointer to int32 slots, pointer to int64 slots); the caller keeps `slots` alive."""
+    if slots is None:
+        return 0, 0
+    if not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int32, torch.int64):
+        raise TypeError("slots must be an int32 or int64 tensor")
+    if slots.device != dev or slots.shape != (batch,) or (batch > 1 and slots.stride(0) != 1):
+        raise ValueError(f"slots must be a contiguous tensor of {batch} indices on {dev}")
+    return (slots.data_ptr(), 0) if slots.dtype == torch.int32 else (0, slots.data_ptr())
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
