@@ -9,6 +9,8 @@
 // (softplus, the gate) is computed once by all threads of the block and passed in
 // shared memory, and so are B and C in fp32; the sums over states of 16 tokens are
 // reduced together (reduce_scatter: LPC - 1 shuffles for LPC tokens).
+#include <cmath>
+
 #include "pe_scan.cuh"
 
 namespace pe {
@@ -16,17 +18,54 @@ namespace pe {
 namespace {
 
 // ---- forward --------------------------------------------------------------------
+// What a thread has loaded of a tile: I items of four tokens of one channel, and its
+// part of the tile's B and C. Loads of the next tile are issued before the current
+// one's recurrence and used after it.
+template <typename T, int LPC, bool STATE_ONLY>
+struct TileRegs {
+    static constexpr int CH = kThreads / LPC, I = LPC < 4 ? 4 / LPC : 1, J = LPC * 4 * TS / kThreads > 0 ? LPC * 4 * TS / kThreads : 1;
+    T d[I][4], u[I][4], z[STATE_ONLY ? 1 : I][4];
+    T b[J], c[STATE_ONLY ? 1 : J];
+
+    __device__ __forceinline__ void load(const ScanP<T>& p, const Place& w, const T* up, const T* dp, const T* zp,
+                                         const T* Bp, const T* Cp, int64_t at, int cnt) {
+        constexpr int NP = 4 * LPC;
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int k = 0; k < I; ++k) {
+            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
+            const int64_t cc = w.c0 + ic;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = ic < w.nch && t4 + i < cnt;
+                const int64_t t = at + t4 + i;
+                d[k][i] = in ? __ldg(dp + t * p.d_st + cc) : from_float<T>(0.0f);
+                u[k][i] = in ? __ldg(up + t * p.u_st + cc) : from_float<T>(0.0f);
+                if (!STATE_ONLY) z[k][i] = in && zp ? __ldg(zp + t * p.z_st + cc) : from_float<T>(0.0f);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + j * kThreads, t = i / NP, n = i % NP;
+            const bool in = t < cnt && n < p.N;
+            b[j] = in ? __ldg(Bp + (at + t) * p.B_st + n) : from_float<T>(0.0f);
+            if (!STATE_ONLY) c[j] = in ? __ldg(Cp + (at + t) * p.C_st + n) : from_float<T>(0.0f);
+        }
+    }
+};
+
 // STATE_ONLY: a piece's last state from a zero start and its sum of dt (first half of
 // a split scan); else the whole, starting from what the sequence's earlier pieces left.
 template <typename T, int LPC, bool STATE_ONLY>
-__global__ void __launch_bounds__(kThreads) scan_fwd(const __grid_constant__ ScanP<T> p) {
+__global__ void __launch_bounds__(kThreads, LPC == 4 || LPC == 8 ? 4 : 2) scan_fwd(const __grid_constant__ ScanP<T> p) {
     constexpr int CH = kThreads / LPC, NP = 4 * LPC, R = LPC < TS ? LPC : TS;
-    __shared__ __align__(16) float sdt[CH * LD], sx[CH * LD], sy[STATE_ONLY ? 1 : CH * LD];
-    __shared__ __align__(16) float sB[TS * NP], sC[STATE_ONLY ? 1 : TS * NP];
+    using Regs = TileRegs<T, LPC, STATE_ONLY>;
+    constexpr int I = Regs::I, J = Regs::J, BUF = (STATE_ONLY ? 2 : 3) * CH * LD + (STATE_ONLY ? 1 : 2) * TS * NP;
+    extern __shared__ __align__(16) float smem[];   // two buffers: dt, dt u, y [CH][LD] and B, C [TS][NP]
     const int tid = threadIdx.x, lane = tid & 31;
     if (blockIdx.x == 0 && tid < 32) check_offsets(p.seqs, lane, kSiteOffsets);
     const Place w = place_of<CH>(p);
-    if (!w.any) return;
+    if (!w.any || (STATE_ONLY && w.t1 == w.sp.len)) return;   // nothing starts from the last piece's state
     const int ch = tid / LPC, q = tid % LPC, c = w.c0 + ch, n0 = 4 * q;
     const bool live = ch < w.nch;
     const int64_t tok = w.sp.start;
@@ -39,112 +78,158 @@ __global__ void __launch_bounds__(kThreads) scan_fwd(const __grid_constant__ Sca
         h[i] = 0.0f;
     }
     const int64_t DN = (int64_t)p.D * p.N, cn = (int64_t)c * p.N + n0;
-    if (!STATE_ONLY) {
-        const int64_t first = w.number - w.j;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p.h0 && live && n0 + i < p.N) h[i] = __ldg(p.h0 + w.s * DN + cn + i);
-        for (int64_t k = first; k < w.number; ++k) {
-            const float sum = live ? __ldg(p.dtsum + k * p.D + c) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (live && n0 + i < p.N) h[i] = fmaf(exp2_fast(A[i] * sum), h[i], __ldg(p.hloc + k * DN + cn + i));
-        }
-    }
-    float dtsum = 0.0f;
     const T* u = p.u + w.sp.row * p.u_sb;
     const T* delta = p.delta + w.sp.row * p.d_sb;
     const T* z = p.z ? p.z + w.sp.row * p.z_sb : nullptr;
     const T* B = p.B + w.sp.row * p.B_sb + w.g * p.B_sg;
     const T* C = p.C + w.sp.row * p.C_sb + w.g * p.C_sg;
-    T* out = p.out + (w.sp.row * p.seqs.tokens) * p.D;
+    T* out = STATE_ONLY ? nullptr : p.out + (w.sp.row * p.seqs.tokens) * p.D;
+    Regs r;
+    r.load(p, w, u, delta, z, B, C, tok + w.t0, (int)min((int64_t)TS, w.t1 - w.t0));
+    float bias[I], Dw[I];
+#pragma unroll
+    for (int k = 0; k < I; ++k) {
+        const int ic = (tid + k * kThreads) % CH;
+        bias[k] = p.bias && ic < w.nch ? __ldg(p.bias + w.c0 + ic) : 0.0f;
+        Dw[k] = !STATE_ONLY && p.Dw && ic < w.nch ? __ldg(p.Dw + w.c0 + ic) : 0.0f;
+    }
+    if (!STATE_ONLY) {
+        const float* from = p.hloc ? p.hloc + w.number * DN : p.h0 ? p.h0 + w.s * DN : nullptr;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (from && live && n0 + i < p.N) h[i] = from[cn + i];
+    }
+    const f32x2 A01 = pack2(A[0], A[1]), A23 = pack2(A[2], A[3]);
+    f32x2 h01 = pack2(h[0], h[1]), h23 = pack2(h[2], h[3]);
+    float dtsum = 0.0f;
+    float add[STATE_ONLY ? 1 : I][4], gate[STATE_ONLY ? 1 : I][4];   // of the tile before: D u and silu(z)
+    int buf = 0, last = 0;
+    float* ckpt = !STATE_ONLY && p.ckpt && live ? p.ckpt + (piece_base(p.seqs, w.s, TS) + w.t0 / TS) * DN + cn : nullptr;
+
+    // out of the tile that ended at token `end`: (y + D u) silu(z)
+    auto finish = [&](int64_t at, int cnt, const float* sy) {
+#pragma unroll
+        for (int k = 0; k < I; ++k) {
+            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
+            if (it >= CH * (TS / 4) || ic >= w.nch) continue;
+            const float4 y4 = *reinterpret_cast<const float4*>(sy + ic * LD + t4);
+            const float yv[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t4 + i < cnt)
+                    out[(at + t4 + i) * p.D + w.c0 + ic] = from_float<T>((yv[i] + add[k][i]) * gate[k][i]);
+        }
+    };
 
     for (int64_t t = w.t0; t < w.t1; t += TS) {
         const int cnt = (int)min((int64_t)TS, w.t1 - t);
         const int64_t at = tok + t;
-        for (int it = tid; it < CH * (TS / 4); it += kThreads) {
-            const int ic = it % CH, t4 = it / CH * 4;
-            const int64_t cc = w.c0 + ic;
+        float* sdt = smem + buf * BUF;
+        float* sx = sdt + CH * LD;
+        float* sB = sx + CH * LD;
+        float* sC = sB + TS * NP;
+        float* sy = sC + TS * NP;
+        float gadd[STATE_ONLY ? 1 : I][4], ggate[STATE_ONLY ? 1 : I][4];
+#pragma unroll
+        for (int k = 0; k < I; ++k) {
+            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
             float dt[4], x[4];
-            const float bias = p.bias && ic < w.nch ? __ldg(p.bias + cc) : 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool in = ic < w.nch && t4 + i < cnt;
-                dt[i] = in ? to_float(__ldg(delta + (at + t4 + i) * p.d_st + cc)) + bias : 0.0f;
+                const float uv = to_float(r.u[k][i]);
+                dt[i] = to_float(r.d[k][i]) + bias[k];
                 if (p.softplus) dt[i] = softplusf(dt[i]);
-                x[i] = in ? dt[i] * to_float(__ldg(u + (at + t4 + i) * p.u_st + cc)) : 0.0f;
+                x[i] = dt[i] * uv;
+                if (!STATE_ONLY) {
+                    const float zv = to_float(r.z[k][i]);
+                    gadd[k][i] = Dw[k] * uv;
+                    ggate[k][i] = z ? zv * sigmoidf(zv) : 1.0f;
+                }
             }
-            *reinterpret_cast<float4*>(sdt + ic * LD + t4) = make_float4(dt[0], dt[1], dt[2], dt[3]);
-            *reinterpret_cast<float4*>(sx + ic * LD + t4) = make_float4(x[0], x[1], x[2], x[3]);
+            if (it < CH * (TS / 4)) {
+                *reinterpret_cast<float4*>(sdt + ic * LD + t4) = make_float4(dt[0], dt[1], dt[2], dt[3]);
+                *reinterpret_cast<float4*>(sx + ic * LD + t4) = make_float4(x[0], x[1], x[2], x[3]);
+            }
         }
-        stage_cols<LPC>(sB, B + at * p.B_st, p.B_st, cnt, p.N);
-        if (!STATE_ONLY) stage_cols<LPC>(sC, C + at * p.C_st, p.C_st, cnt, p.N);
-        __syncthreads();
-        if (!STATE_ONLY && p.ckpt && live) {
-            float* k = p.ckpt + (piece_base(p.seqs, w.s, TS) + t / TS) * DN + cn;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (n0 + i < p.N) k[i] = h[i];
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + j * kThreads;
+            if (i < TS * NP) {
+                sB[i] = to_float(r.b[j]);
+                if (!STATE_ONLY) sC[i] = to_float(r.c[j]);
+            }
+        }
+        __syncthreads();
+        if (!STATE_ONLY && t > w.t0) finish(at - TS, last, smem + (buf ^ 1) * BUF + 2 * CH * LD + 2 * TS * NP);
+        if (t + TS < w.t1)
+            r.load(p, w, u, delta, z, B, C, at + TS, (int)min((int64_t)TS, w.t1 - t - TS));
+        if (!STATE_ONLY) {
+#pragma unroll
+            for (int k = 0; k < I; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) add[k][i] = gadd[k][i], gate[k][i] = ggate[k][i];
+            if (ckpt) {
+                unpack2(h01, h[0], h[1]);
+                unpack2(h23, h[2], h[3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n0 + i < p.N) ckpt[i] = h[i];
+                ckpt += DN;
+            }
         }
         float y[TS];
+        auto token = [&](int k, float dt, float x) {
+            const f32x2 dt2 = pack2(dt, dt), x2 = pack2(x, x);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sB + k * NP + n0);
+            h01 = fma2(exp2_2(mul2(dt2, A01)), h01, mul2(x2, b.x));
+            h23 = fma2(exp2_2(mul2(dt2, A23)), h23, mul2(x2, b.y));
+            if (STATE_ONLY) {
+                dtsum += dt;
+            } else {
+                const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sC + k * NP + n0);
+                float lo, hi;
+                unpack2(fma2(cv.y, h23, mul2(cv.x, h01)), lo, hi);
+                y[k] = lo + hi;
+            }
+        };
+        if (cnt == TS) {
 #pragma unroll
-        for (int t4 = 0; t4 < TS; t4 += 4) {
-            const float4 dt4 = *reinterpret_cast<const float4*>(sdt + ch * LD + t4);
-            const float4 x4 = *reinterpret_cast<const float4*>(sx + ch * LD + t4);
-            const float dt[4] = {dt4.x, dt4.y, dt4.z, dt4.w}, x[4] = {x4.x, x4.y, x4.z, x4.w};
+            for (int t4 = 0; t4 < TS; t4 += 4) {
+                const float4 d4 = *reinterpret_cast<const float4*>(sdt + ch * LD + t4);
+                const float4 x4 = *reinterpret_cast<const float4*>(sx + ch * LD + t4);
+                token(t4, d4.x, x4.x);
+                token(t4 + 1, d4.y, x4.y);
+                token(t4 + 2, d4.z, x4.z);
+                token(t4 + 3, d4.w, x4.w);
+            }
+        } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                y[t4 + k] = 0.0f;
-                if (t4 + k < cnt) {
-                    const float4 b = *reinterpret_cast<const float4*>(sB + (t4 + k) * NP + n0);
-                    h[0] = fmaf(exp2_fast(dt[k] * A[0]), h[0], x[k] * b.x);
-                    h[1] = fmaf(exp2_fast(dt[k] * A[1]), h[1], x[k] * b.y);
-                    h[2] = fmaf(exp2_fast(dt[k] * A[2]), h[2], x[k] * b.z);
-                    h[3] = fmaf(exp2_fast(dt[k] * A[3]), h[3], x[k] * b.w);
-                    if (STATE_ONLY) {
-                        dtsum += dt[k];
-                    } else {
-                        const float4 cv = *reinterpret_cast<const float4*>(sC + (t4 + k) * NP + n0);
-                        y[t4 + k] = fmaf(cv.x, h[0], cv.y * h[1]) + fmaf(cv.z, h[2], cv.w * h[3]);
-                    }
-                }
+            for (int k = 0; k < TS; ++k) {
+                y[k] = 0.0f;
+                if (k < cnt) token(k, sdt[ch * LD + k], sx[ch * LD + k]);
             }
         }
         if (!STATE_ONLY) {
 #pragma unroll
-            for (int r = 0; r < TS; r += R) {
+            for (int k = 0; k < TS; k += R) {
                 float v[R];
 #pragma unroll
-                for (int i = 0; i < R; ++i) v[i] = y[r + i];
+                for (int i = 0; i < R; ++i) v[i] = y[k + i];
                 float sum = reduce_scatter<R, 1>(v, lane);
                 if (LPC > R) sum += __shfl_xor_sync(0xffffffffu, sum, R);
-                if (q < R) sy[ch * LD + r + q] = sum;
+                if (q < R) sy[ch * LD + k + q] = sum;
             }
         }
+        last = cnt;
+        buf ^= 1;
+    }
+    if (!STATE_ONLY && w.t1 > w.t0) {
         __syncthreads();
-        if (!STATE_ONLY) {
-            for (int it = tid; it < CH * (TS / 4); it += kThreads) {
-                const int ic = it % CH, t4 = it / CH * 4;
-                const int64_t cc = w.c0 + ic;
-                if (ic >= w.nch) continue;
-                const float4 y4 = *reinterpret_cast<const float4*>(sy + ic * LD + t4);
-                float yv[4] = {y4.x, y4.y, y4.z, y4.w};
-                const float Dw = p.Dw ? __ldg(p.Dw + cc) : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (t4 + i >= cnt) break;
-                    if (p.Dw) yv[i] = fmaf(Dw, to_float(__ldg(u + (at + t4 + i) * p.u_st + cc)), yv[i]);
-                    if (z) {
-                        const float zv = to_float(__ldg(z + (at + t4 + i) * p.z_st + cc));
-                        yv[i] *= zv * sigmoidf(zv);
-                    }
-                    out[(at + t4 + i) * p.D + cc] = from_float<T>(yv[i]);
-                }
-            }
-            // sy is written again only after the next tile's first barrier
-        }
+        finish(tok + w.t0 + (w.t1 - w.t0 - 1) / TS * TS, last, smem + (buf ^ 1) * BUF + 2 * CH * LD + 2 * TS * NP);
     }
     if (!live) return;
+    unpack2(h01, h[0], h[1]);
+    unpack2(h23, h[2], h[3]);
     if (STATE_ONLY) {
         if (q == 0) p.dtsum[w.number * p.D + c] = dtsum;
 #pragma unroll
@@ -154,6 +239,38 @@ __global__ void __launch_bounds__(kThreads) scan_fwd(const __grid_constant__ Sca
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (n0 + i < p.N) p.state[w.s * DN + cn + i] = h[i];
+    }
+}
+
+// Between the halves of a split scan: each piece's own last state gives way to the state
+// before the piece. One thread a (sequence, channel, state); the products exp(A sum dt)
+// do not depend on one another, so the loads of eight pieces are in flight together.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) scan_carry(const __grid_constant__ ScanP<T> p) {
+    const int64_t DN = (int64_t)p.D * p.N, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= DN) return;
+    const int s = blockIdx.y;
+    const int64_t len = seq_span(p.seqs, s).len, base = piece_base(p.seqs, s, p.piece);
+    const int64_t n = len > p.piece ? ceil_div(len, p.piece) : 1;
+    const int c = (int)(i / p.N);
+    const float A = __ldg(p.A + i) * kLog2e;
+    float h = p.h0 ? __ldg(p.h0 + s * DN + i) : 0.0f;
+    float* hp = p.hloc + base * DN + i;
+    const float* sp = p.dtsum + base * p.D + c;
+    for (int64_t k0 = 0; k0 < n; k0 += 8) {
+        float own[8], keep[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k0 + k < n - 1) {
+                own[k] = hp[(k0 + k) * DN];
+                keep[k] = exp2_fast(A * __ldg(sp + (k0 + k) * p.D));
+            }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k0 + k < n) {
+                hp[(k0 + k) * DN] = h;
+                if (k0 + k < n - 1) h = fmaf(keep[k], h, own[k]);
+            }
     }
 }
 
@@ -233,7 +350,26 @@ __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ St
 
 // ---- host -------------------------------------------------------------------------
 // Tokens a piece of a scan split along time; 0 = not split.
-int64_t piece_tokens(const pe_scan_args*) { return 0; }
+//
+// Not split, a block (4 warps) takes its channels through a whole sequence: at best
+// kFull clocks a token of SM time, kAlone when it has the SM to itself. Split, all SMs
+// work, for the price of computing every exponential twice (kState more clocks a
+// token) and of two more launches. The longest of n packed sequences, whose lengths
+// the host does not know, is taken as (1 + ln n) average ones, as random cuts make it.
+constexpr double kAlone = 60, kFull = 42, kState = 36, kLaunches = 15000;
+int64_t piece_tokens(const pe_scan_args* a) {
+    const int64_t ch = kThreads / lanes_for(a->states), dg = a->channels / a->groups;
+    const int64_t tiles = a->groups * ceil_div(dg, ch);
+    if (a->nseq < 1 || a->nseq > 65535 || a->tokens < 256) return 0;
+    const double sms = num_sms(), total = (double)a->tokens * (a->cu ? 1 : a->nseq) * tiles;
+    double longest = (double)a->tokens;
+    if (a->cu) longest = min(longest, longest / a->nseq * (1.0 + log((double)a->nseq)));
+    const double whole = max(longest * kAlone, total / sms * kFull);
+    const double split = total / sms * (kFull + kState) * 1.1 + kLaunches;
+    if (split >= whole) return 0;
+    const int64_t piece = (int64_t)(total / (3.0 * sms));   // three blocks an SM
+    return max((int64_t)64, ceil_div(piece, TS) * TS);
+}
 
 template <typename T, int LPC>
 int scan_run(const pe_scan_args* a, cudaStream_t s) {
@@ -247,13 +383,15 @@ int scan_run(const pe_scan_args* a, cudaStream_t s) {
     }
     unsigned grid;
     if (int rc = grid_of(piece_count(p.seqs, p.piece) * p.G * p.ntile, &grid)) return rc;
+    constexpr int CH = kThreads / LPC, cols = TS * 4 * LPC;
     if (piece) {
-        scan_fwd<T, LPC, true><<<grid, kThreads, 0, s>>>(p);
+        if (int rc = launch(scan_fwd<T, LPC, true>, p, grid, 2 * (2 * CH * LD + cols) * 4, s)) return rc;
+        const dim3 carry((unsigned)ceil_div((int64_t)p.D * p.N, kThreads), (unsigned)p.seqs.nseq);
+        scan_carry<T><<<carry, kThreads, 0, s>>>(p);
         count_launch();
+        if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
-    scan_fwd<T, LPC, false><<<grid, kThreads, 0, s>>>(p);
-    count_launch();
-    return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
+    return launch(scan_fwd<T, LPC, false>, p, grid, 2 * (3 * CH * LD + 2 * cols) * 4, s);
 }
 
 template <typename T>

@@ -60,14 +60,31 @@ __device__ __forceinline__ Place place_of(const P& p) {
     return w;
 }
 
-// B or C of a tile's tokens as fp32 [TS][4 LPC], zero past the last state and token.
-template <int LPC, typename T>
-__device__ __forceinline__ void stage_cols(float* dst, const T* src, int64_t st, int cnt, int N) {
-    constexpr int NP = 4 * LPC;
-    for (int i = threadIdx.x; i < TS * NP; i += kThreads) {
-        const int t = i / NP, n = i % NP;
-        dst[i] = t < cnt && n < N ? to_float(__ldg(src + t * st + n)) : 0.0f;
-    }
+// ---- packed pairs --------------------------------------------------------------
+// Two fp32 lanes in one 64-bit register, one instruction for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
+    float lo, hi;
+    unpack2(x, lo, hi);
+    return pack2(exp2_fast(lo), exp2_fast(hi));
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -114,6 +131,16 @@ inline int grid_of(int64_t blocks, unsigned* grid) {
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     *grid = (unsigned)blocks;
     return PE_OK;
+}
+
+template <typename K, typename P>
+int launch(K kernel, const P& p, unsigned grid, int smem, cudaStream_t s) {
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return PE_ERR_CUDA;
+    kernel<<<grid, kThreads, smem, s>>>(p);
+    count_launch();
+    return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }
 
 #define PE_LANES(F, l, ...)                    \
