@@ -198,7 +198,7 @@ int pe_permute(const pe_permute_plan* plan, const void* in, void* out, void* str
  * h0 / state: first and last h of each sequence, fp32 [nseq, channels, states]
  * contiguous. A [channels, states], D and delta_bias [channels] fp32 contiguous;
  * out [batch, tokens, channels] contiguous. ckpt (for the backward pass) receives
- * h before every 16th token, pe_scan_ckpt_floats floats. ws: pe_scan_ws_bytes.
+ * h before every 64th token, pe_scan_ckpt_floats floats. ws: pe_scan_ws_bytes.
  */
 typedef struct pe_scan_args {
     int64_t dtype, softplus;

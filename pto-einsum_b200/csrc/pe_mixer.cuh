@@ -55,8 +55,23 @@ __device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
     return r;
 }
 
-// 1 / (1 + exp(-x)). Where exp(-x) overflows the quotient is 0, its limit.
-__device__ __forceinline__ float sigmoidf(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// 2^x and 1/x of one instruction each (relative errors of 2^-22 and 2^-23; denormal
+// arguments and results count as zero).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// 1 / (1 + exp(-x)); 0, its limit, where exp(-x) overflows.
+__device__ __forceinline__ float sigmoidf(float x) { return rcp_fast(1.0f + exp2_fast(-kLog2e * x)); }
 // d silu(x) / dx with s = sigmoid(x).
 __device__ __forceinline__ float silu_slope(float x, float s) { return s * (1.0f + x * (1.0f - s)); }
 
@@ -65,8 +80,8 @@ __device__ __forceinline__ float silu_slope(float x, float s) { return s * (1.0f
 // leaves a relative error below (1/9)^7 / 15 = 1.4e-8. A logarithm of the
 // rounded 1 + e would lose the small step sizes (e = 1e-3 keeps 13 bits).
 __device__ __forceinline__ float softplusf(float x) {
-    const float e = __expf(-fabsf(x));
-    const float s = __fdividef(e, 2.0f + e);
+    const float e = exp2_fast(-kLog2e * fabsf(x));
+    const float s = e * rcp_fast(2.0f + e);
     const float q = s * s;
     float r = fmaf(q, 1.0f / 13, 1.0f / 11);
     r = fmaf(r, q, 1.0f / 9);
@@ -76,13 +91,6 @@ __device__ __forceinline__ float softplusf(float x) {
     r = fmaf(r, q, 1.0f);
     // NaN stays NaN: fmaxf alone would drop it, the product with s does not
     return fmaxf(x, 0.0f) + 2.0f * s * r;
-}
-
-// 2^x of one instruction (relative error 2^-22, denormal results flushed).
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // ---- sequences ----------------------------------------------------------------

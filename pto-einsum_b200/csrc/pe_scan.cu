@@ -3,12 +3,12 @@
 //
 //   h[n] = exp(dt A[n]) h[n] + dt u B[n],   y = sum_n C[n] h[n] + D u
 //
-// per channel, dt = softplus(delta + bias). A thread keeps four states of one
-// channel in registers; LPC = 1 .. 32 neighbouring lanes share a channel (4 LPC >=
-// states). Tokens go through in tiles of 16: what depends on (token, channel) alone
-// (softplus, the gate) is computed once by all threads of the block and passed in
-// shared memory, and so are B and C in fp32; the sums over states of 16 tokens are
-// reduced together (reduce_scatter: LPC - 1 shuffles for LPC tokens).
+// per channel, dt = softplus(delta + bias). A thread keeps four states of one channel in
+// registers; LPC = 1 .. 32 neighbouring lanes share a channel (4 LPC >= states). Tokens
+// go through in tiles of 16: what depends on (token, channel) alone (softplus, the gate)
+// is computed once by all threads of the block and passed in shared memory, and so are
+// B and C in fp32; the sums over states are reduced for LPC tokens together
+// (reduce_scatter: LPC - 1 shuffles for LPC tokens).
 #include <cmath>
 
 #include "pe_scan.cuh"
@@ -18,57 +18,93 @@ namespace pe {
 namespace {
 
 // ---- forward --------------------------------------------------------------------
-// What a thread has loaded of a tile: I items of four tokens of one channel, and its
-// part of the tile's B and C. Loads of the next tile are issued before the current
-// one's recurrence and used after it.
-template <typename T, int LPC, bool STATE_ONLY>
-struct TileRegs {
-    static constexpr int CH = kThreads / LPC, I = LPC < 4 ? 4 / LPC : 1, J = LPC * 4 * TS / kThreads > 0 ? LPC * 4 * TS / kThreads : 1;
-    T d[I][4], u[I][4], z[STATE_ONLY ? 1 : I][4];
-    T b[J], c[STATE_ONLY ? 1 : J];
+constexpr int TS = 16;       // tokens a tile
 
-    __device__ __forceinline__ void load(const ScanP<T>& p, const Place& w, const T* up, const T* dp, const T* zp,
-                                         const T* Bp, const T* Cp, int64_t at, int cnt) {
-        constexpr int NP = 4 * LPC;
-        const int tid = threadIdx.x;
+template <int LPC>
+struct Lanes {
+    static constexpr int CH = kThreads / LPC;    // channels a block
+    static constexpr int NP = 4 * LPC;           // states, padded
+    static constexpr int R = LPC < TS ? LPC : TS;
+    // (token pair, channel pair) items of the element-wise work: I a thread
+    static constexpr int ITEMS = CH / 2 * (TS / 2), I = (ITEMS + kThreads - 1) / kThreads;
+    // row of a [token][channel] tile of floats: the lanes of a warp hold 32 / LPC channels of
+    // LPC tokens, which fall on different banks with these
+    static constexpr int Y = LPC == 1 ? 128 : LPC == 2 ? 80 : LPC == 4 ? 40 : LPC == 8 ? 20 : LPC == 16 ? 10 : 6;
+};
+
+// B or C of a tile: fp32 [TS][NP], zero past the last token and state.
+template <int NP, typename T>
+__device__ __forceinline__ void widen_rows(float* dst, const T* src, int cnt, int N) {
+    constexpr int J = TS * NP / 2 / kThreads;
 #pragma unroll
-        for (int k = 0; k < I; ++k) {
-            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
-            const int64_t cc = w.c0 + ic;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = ic < w.nch && t4 + i < cnt;
-                const int64_t t = at + t4 + i;
-                d[k][i] = in ? __ldg(dp + t * p.d_st + cc) : from_float<T>(0.0f);
-                u[k][i] = in ? __ldg(up + t * p.u_st + cc) : from_float<T>(0.0f);
-                if (!STATE_ONLY) z[k][i] = in && zp ? __ldg(zp + t * p.z_st + cc) : from_float<T>(0.0f);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = tid + j * kThreads, t = i / NP, n = i % NP;
-            const bool in = t < cnt && n < p.N;
-            b[j] = in ? __ldg(Bp + (at + t) * p.B_st + n) : from_float<T>(0.0f);
-            if (!STATE_ONLY) c[j] = in ? __ldg(Cp + (at + t) * p.C_st + n) : from_float<T>(0.0f);
-        }
+    for (int j = 0; j < (J > 0 ? J : 1); ++j) {
+        const int i = 2 * (threadIdx.x + j * kThreads), t = i / NP, n = i % NP;
+        if (J == 0 && i >= TS * NP) break;
+        const Vec<T, 2> v = *reinterpret_cast<const Vec<T, 2>*>(src + i);
+        *reinterpret_cast<float2*>(dst + i) = make_float2(t < cnt && n < N ? to_float(v.v[0]) : 0.0f,
+                                                          t < cnt && n + 1 < N ? to_float(v.v[1]) : 0.0f);
     }
+}
+
+// Shared memory of a block; two of each part, for even and odd tiles.
+template <typename T, int LPC, bool STATE_ONLY>
+struct FwdSmem {
+    using L = Lanes<LPC>;
+    struct __align__(16) Raw {       // as in memory
+        T u[TS * L::CH], d[TS * L::CH], b[TS * L::NP];
+        T z[STATE_ONLY ? 8 : TS * L::CH], c[STATE_ONLY ? 8 : TS * L::NP];
+    } raw[2];
+    struct __align__(16) Wide {      // (dt, dt u) of each token and channel; B, C
+        float2 dx[TS][L::CH];
+        float B[TS * L::NP], C[STATE_ONLY ? 4 : TS * L::NP];
+    } fp[2];
+    float y[2][STATE_ONLY ? 4 : TS * L::Y];
 };
 
 // STATE_ONLY: a piece's last state from a zero start and its sum of dt (first half of
 // a split scan); else the whole, starting from what the sequence's earlier pieces left.
+//
+// Three tiles are under way between two barriers: the copies of tile i + 2 from memory,
+// the element-wise work before tile i + 1 and after tile i - 1, and the recurrence of
+// tile i; what one barrier interval writes, the next one reads. Tokens past the end have
+// dt = 0 and B = 0: they leave the state as it is.
 template <typename T, int LPC, bool STATE_ONLY>
-__global__ void __launch_bounds__(kThreads, LPC == 4 || LPC == 8 ? 4 : 2) scan_fwd(const __grid_constant__ ScanP<T> p) {
-    constexpr int CH = kThreads / LPC, NP = 4 * LPC, R = LPC < TS ? LPC : TS;
-    using Regs = TileRegs<T, LPC, STATE_ONLY>;
-    constexpr int I = Regs::I, J = Regs::J, BUF = (STATE_ONLY ? 2 : 3) * CH * LD + (STATE_ONLY ? 1 : 2) * TS * NP;
-    extern __shared__ __align__(16) float smem[];   // two buffers: dt, dt u, y [CH][LD] and B, C [TS][NP]
+__global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
+    scan_fwd(const __grid_constant__ ScanP<T> p) {
+    using L = Lanes<LPC>;
+    constexpr int CH = L::CH, NP = L::NP, R = L::R, I = L::I, Y = L::Y;
+    using F = FwdSmem<T, LPC, STATE_ONLY>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    F& m = *reinterpret_cast<F*>(smem);
     const int tid = threadIdx.x, lane = tid & 31;
     if (blockIdx.x == 0 && tid < 32) check_offsets(p.seqs, lane, kSiteOffsets);
     const Place w = place_of<CH>(p);
     if (!w.any || (STATE_ONLY && w.t1 == w.sp.len)) return;   // nothing starts from the last piece's state
     const int ch = tid / LPC, q = tid % LPC, c = w.c0 + ch, n0 = 4 * q;
     const bool live = ch < w.nch;
-    const int64_t tok = w.sp.start;
+
+    // rows of the piece's first token
+    const int64_t row0 = w.sp.start + w.t0;
+    const T* u = p.u + w.sp.row * p.u_sb + row0 * p.u_st + w.c0;
+    const T* delta = p.delta + w.sp.row * p.d_sb + row0 * p.d_st + w.c0;
+    const T* z = p.z ? p.z + w.sp.row * p.z_sb + row0 * p.z_st + w.c0 : nullptr;
+    const T* B = p.B + w.sp.row * p.B_sb + row0 * p.B_st + w.g * p.B_sg;
+    const T* C = p.C + w.sp.row * p.C_sb + row0 * p.C_st + w.g * p.C_sg;
+    const int64_t count = w.t1 - w.t0;                        // tokens
+    auto copy = [&](int64_t t, int b) {
+        if (t < count) {
+            const int cnt = (int)min((int64_t)TS, count - t);
+            stage<TS, CH>(m.raw[b].u, u + t * p.u_st, p.u_st, cnt, w.nch, p.u_cb);
+            stage<TS, CH>(m.raw[b].d, delta + t * p.d_st, p.d_st, cnt, w.nch, p.d_cb);
+            stage<TS, NP>(m.raw[b].b, B + t * p.B_st, p.B_st, cnt, p.N, p.B_cb);
+            if constexpr (!STATE_ONLY) {
+                stage<TS, NP>(m.raw[b].c, C + t * p.C_st, p.C_st, cnt, p.N, p.C_cb);
+                if (z) stage<TS, CH>(m.raw[b].z, z + t * p.z_st, p.z_st, cnt, w.nch, p.z_cb);
+            }
+        }
+        cp_commit();
+    };
+    copy(0, 0);
 
     float A[4], h[4];
 #pragma unroll
@@ -78,20 +114,17 @@ __global__ void __launch_bounds__(kThreads, LPC == 4 || LPC == 8 ? 4 : 2) scan_f
         h[i] = 0.0f;
     }
     const int64_t DN = (int64_t)p.D * p.N, cn = (int64_t)c * p.N + n0;
-    const T* u = p.u + w.sp.row * p.u_sb;
-    const T* delta = p.delta + w.sp.row * p.d_sb;
-    const T* z = p.z ? p.z + w.sp.row * p.z_sb : nullptr;
-    const T* B = p.B + w.sp.row * p.B_sb + w.g * p.B_sg;
-    const T* C = p.C + w.sp.row * p.C_sb + w.g * p.C_sg;
-    T* out = STATE_ONLY ? nullptr : p.out + (w.sp.row * p.seqs.tokens) * p.D;
-    Regs r;
-    r.load(p, w, u, delta, z, B, C, tok + w.t0, (int)min((int64_t)TS, w.t1 - w.t0));
-    float bias[I], Dw[I];
+    // this thread's items: token pairs 2 tp of channel pairs 2 cp
+    float bias[I][2], Dw[I][2];
 #pragma unroll
     for (int k = 0; k < I; ++k) {
-        const int ic = (tid + k * kThreads) % CH;
-        bias[k] = p.bias && ic < w.nch ? __ldg(p.bias + w.c0 + ic) : 0.0f;
-        Dw[k] = !STATE_ONLY && p.Dw && ic < w.nch ? __ldg(p.Dw + w.c0 + ic) : 0.0f;
+        const int cp = (tid + k * kThreads) % (CH / 2) * 2;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const bool in = cp + e < w.nch;
+            bias[k][e] = p.bias && in ? __ldg(p.bias + w.c0 + cp + e) : 0.0f;
+            Dw[k][e] = !STATE_ONLY && p.Dw && in ? __ldg(p.Dw + w.c0 + cp + e) : 0.0f;
+        }
     }
     if (!STATE_ONLY) {
         const float* from = p.hloc ? p.hloc + w.number * DN : p.h0 ? p.h0 + w.s * DN : nullptr;
@@ -102,130 +135,151 @@ __global__ void __launch_bounds__(kThreads, LPC == 4 || LPC == 8 ? 4 : 2) scan_f
     const f32x2 A01 = pack2(A[0], A[1]), A23 = pack2(A[2], A[3]);
     f32x2 h01 = pack2(h[0], h[1]), h23 = pack2(h[2], h[3]);
     float dtsum = 0.0f;
-    float add[STATE_ONLY ? 1 : I][4], gate[STATE_ONLY ? 1 : I][4];   // of the tile before: D u and silu(z)
-    int buf = 0, last = 0;
-    float* ckpt = !STATE_ONLY && p.ckpt && live ? p.ckpt + (piece_base(p.seqs, w.s, TS) + w.t0 / TS) * DN + cn : nullptr;
+    float* ckpt = !STATE_ONLY && p.ckpt && live
+                      ? p.ckpt + (piece_base(p.seqs, w.s, KCK) + w.t0 / KCK) * DN + cn : nullptr;
+    T* out = STATE_ONLY ? nullptr : p.out + (w.sp.row * p.seqs.tokens + row0) * p.D + w.c0;
 
-    // out of the tile that ended at token `end`: (y + D u) silu(z)
-    auto finish = [&](int64_t at, int cnt, const float* sy) {
+    // D u and silu(z) of the thread's items: [0] of the tile whose recurrence runs, [1] of the next
+    float add[2][I][2][2], gate[2][I][2][2];
+    auto before = [&](int64_t t, int b) {
+        const int cnt = (int)max((int64_t)0, min((int64_t)TS, count - t));
 #pragma unroll
         for (int k = 0; k < I; ++k) {
-            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
-            if (it >= CH * (TS / 4) || ic >= w.nch) continue;
-            const float4 y4 = *reinterpret_cast<const float4*>(sy + ic * LD + t4);
-            const float yv[4] = {y4.x, y4.y, y4.z, y4.w};
+            const int it = tid + k * kThreads, cp = it % (CH / 2) * 2, tp = it / (CH / 2) * 2;
+            if (L::ITEMS % kThreads && it >= L::ITEMS) break;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (t4 + i < cnt)
-                    out[(at + t4 + i) * p.D + w.c0 + ic] = from_float<T>((yv[i] + add[k][i]) * gate[k][i]);
-        }
-    };
-
-    for (int64_t t = w.t0; t < w.t1; t += TS) {
-        const int cnt = (int)min((int64_t)TS, w.t1 - t);
-        const int64_t at = tok + t;
-        float* sdt = smem + buf * BUF;
-        float* sx = sdt + CH * LD;
-        float* sB = sx + CH * LD;
-        float* sC = sB + TS * NP;
-        float* sy = sC + TS * NP;
-        float gadd[STATE_ONLY ? 1 : I][4], ggate[STATE_ONLY ? 1 : I][4];
+            for (int i = 0; i < 2; ++i) {
+                const Vec<T, 2> dv = *reinterpret_cast<const Vec<T, 2>*>(m.raw[b].d + (tp + i) * CH + cp);
+                const Vec<T, 2> uv = *reinterpret_cast<const Vec<T, 2>*>(m.raw[b].u + (tp + i) * CH + cp);
+                float f[4];
 #pragma unroll
-        for (int k = 0; k < I; ++k) {
-            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
-            float dt[4], x[4];
+                for (int e = 0; e < 2; ++e) {
+                    const float x = to_float(uv.v[e]);
+                    float dt = to_float(dv.v[e]) + bias[k][e];
+                    if (p.softplus) dt = softplusf(dt);
+                    f[2 * e] = tp + i < cnt ? dt : 0.0f;
+                    f[2 * e + 1] = tp + i < cnt ? dt * x : 0.0f;
+                    if constexpr (!STATE_ONLY) add[1][k][i][e] = Dw[k][e] * x;
+                }
+                *reinterpret_cast<float4*>(&m.fp[b].dx[tp + i][cp]) = make_float4(f[0], f[1], f[2], f[3]);
+                if constexpr (!STATE_ONLY) {
+                    gate[1][k][i][0] = gate[1][k][i][1] = 1.0f;
+                    if (z) {
+                        const Vec<T, 2> zv = *reinterpret_cast<const Vec<T, 2>*>(m.raw[b].z + (tp + i) * CH + cp);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float uv = to_float(r.u[k][i]);
-                dt[i] = to_float(r.d[k][i]) + bias[k];
-                if (p.softplus) dt[i] = softplusf(dt[i]);
-                x[i] = dt[i] * uv;
-                if (!STATE_ONLY) {
-                    const float zv = to_float(r.z[k][i]);
-                    gadd[k][i] = Dw[k] * uv;
-                    ggate[k][i] = z ? zv * sigmoidf(zv) : 1.0f;
+                        for (int e = 0; e < 2; ++e) {
+                            const float g = to_float(zv.v[e]);
+                            gate[1][k][i][e] = g * sigmoidf(g);
+                        }
+                    }
                 }
             }
-            if (it < CH * (TS / 4)) {
-                *reinterpret_cast<float4*>(sdt + ic * LD + t4) = make_float4(dt[0], dt[1], dt[2], dt[3]);
-                *reinterpret_cast<float4*>(sx + ic * LD + t4) = make_float4(x[0], x[1], x[2], x[3]);
-            }
         }
+        widen_rows<NP>(m.fp[b].B, m.raw[b].b, cnt, p.N);
+        if constexpr (!STATE_ONLY) widen_rows<NP>(m.fp[b].C, m.raw[b].c, cnt, p.N);
+    };
+    auto after = [&](int64_t t, int cnt, int b) {   // out = (y + D u) silu(z)
+        if constexpr (!STATE_ONLY) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < TS * NP) {
-                sB[i] = to_float(r.b[j]);
-                if (!STATE_ONLY) sC[i] = to_float(r.c[j]);
+            for (int k = 0; k < I; ++k) {
+                const int it = tid + k * kThreads, cp = it % (CH / 2) * 2, tp = it / (CH / 2) * 2;
+                if (L::ITEMS % kThreads && it >= L::ITEMS) break;
+                T* o = out + (t + tp) * p.D + cp;
+#pragma unroll
+                for (int i = 0; i < 2; ++i, o += p.D) {
+                    if (tp + i >= cnt) break;
+                    const float2 y = *reinterpret_cast<const float2*>(&m.y[b][(tp + i) * Y + cp]);
+                    Vec<T, 2> v;
+                    v.v[0] = from_float<T>((y.x + add[0][k][i][0]) * gate[0][k][i][0]);
+                    v.v[1] = from_float<T>((y.y + add[0][k][i][1]) * gate[0][k][i][1]);
+                    if (p.pairs && cp < w.nch) {
+                        *reinterpret_cast<Vec<T, 2>*>(o) = v;
+                    } else {
+                        if (cp < w.nch) o[0] = v.v[0];
+                        if (cp + 1 < w.nch) o[1] = v.v[1];
+                    }
+                }
             }
         }
-        __syncthreads();
-        if (!STATE_ONLY && t > w.t0) finish(at - TS, last, smem + (buf ^ 1) * BUF + 2 * CH * LD + 2 * TS * NP);
-        if (t + TS < w.t1)
-            r.load(p, w, u, delta, z, B, C, at + TS, (int)min((int64_t)TS, w.t1 - t - TS));
-        if (!STATE_ONLY) {
+    };
+    auto shift = [&]() {
+        if constexpr (!STATE_ONLY) {
 #pragma unroll
             for (int k = 0; k < I; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) add[k][i] = gadd[k][i], gate[k][i] = ggate[k][i];
-            if (ckpt) {
-                unpack2(h01, h[0], h[1]);
-                unpack2(h23, h[2], h[3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n0 + i < p.N) ckpt[i] = h[i];
-                ckpt += DN;
-            }
+                for (int i = 0; i < 4; ++i) {
+                    add[0][k][i / 2][i % 2] = add[1][k][i / 2][i % 2];
+                    gate[0][k][i / 2][i % 2] = gate[1][k][i / 2][i % 2];
+                }
         }
-        float y[TS];
-        auto token = [&](int k, float dt, float x) {
-            const f32x2 dt2 = pack2(dt, dt), x2 = pack2(x, x);
-            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sB + k * NP + n0);
-            h01 = fma2(exp2_2(mul2(dt2, A01)), h01, mul2(x2, b.x));
-            h23 = fma2(exp2_2(mul2(dt2, A23)), h23, mul2(x2, b.y));
-            if (STATE_ONLY) {
-                dtsum += dt;
-            } else {
-                const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sC + k * NP + n0);
-                float lo, hi;
-                unpack2(fma2(cv.y, h23, mul2(cv.x, h01)), lo, hi);
-                y[k] = lo + hi;
-            }
-        };
-        if (cnt == TS) {
-#pragma unroll
-            for (int t4 = 0; t4 < TS; t4 += 4) {
-                const float4 d4 = *reinterpret_cast<const float4*>(sdt + ch * LD + t4);
-                const float4 x4 = *reinterpret_cast<const float4*>(sx + ch * LD + t4);
-                token(t4, d4.x, x4.x);
-                token(t4 + 1, d4.y, x4.y);
-                token(t4 + 2, d4.z, x4.z);
-                token(t4 + 3, d4.w, x4.w);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < TS; ++k) {
-                y[k] = 0.0f;
-                if (k < cnt) token(k, sdt[ch * LD + k], sx[ch * LD + k]);
-            }
-        }
-        if (!STATE_ONLY) {
-#pragma unroll
-            for (int k = 0; k < TS; k += R) {
-                float v[R];
-#pragma unroll
-                for (int i = 0; i < R; ++i) v[i] = y[k + i];
-                float sum = reduce_scatter<R, 1>(v, lane);
-                if (LPC > R) sum += __shfl_xor_sync(0xffffffffu, sum, R);
-                if (q < R) sy[ch * LD + k + q] = sum;
-            }
-        }
-        last = cnt;
-        buf ^= 1;
-    }
-    if (!STATE_ONLY && w.t1 > w.t0) {
+    };
+
+    cp_wait();
+    __syncthreads();
+    copy(TS, 1);
+    before(0, 0);
+    int b = 0;
+    for (int64_t t = 0; t < count; t += TS, b ^= 1) {
+        cp_wait();
         __syncthreads();
-        finish(tok + w.t0 + (w.t1 - w.t0 - 1) / TS * TS, last, smem + (buf ^ 1) * BUF + 2 * CH * LD + 2 * TS * NP);
+        copy(t + 2 * TS, b);
+        if (t > 0) after(t - TS, TS, b ^ 1);
+        shift();
+        before(t + TS, b ^ 1);
+        if (ckpt && t % KCK == 0) {
+            unpack2(h01, h[0], h[1]);
+            unpack2(h23, h[2], h[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n0 + i < p.N) ckpt[i] = h[i];
+            ckpt += DN;
+        }
+        // four tokens at a time: all that does not depend on the state first
+        float y[TS];
+#pragma unroll
+        for (int k0 = 0; k0 < TS; k0 += 4) {
+            f32x2 a[4][2], x[4][2];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 dx = m.fp[b].dx[k0 + k][ch];
+                const f32x2 dt2 = pack2(dx.x, dx.x), x2 = pack2(dx.y, dx.y);
+                const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&m.fp[b].B[(k0 + k) * NP + n0]);
+                a[k][0] = exp2_2(mul2(dt2, A01));
+                a[k][1] = exp2_2(mul2(dt2, A23));
+                x[k][0] = mul2(x2, bv.x);
+                x[k][1] = mul2(x2, bv.y);
+                if constexpr (STATE_ONLY) dtsum += dx.x;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h01 = fma2(a[k][0], h01, x[k][0]);
+                h23 = fma2(a[k][1], h23, x[k][1]);
+                if constexpr (!STATE_ONLY) {
+                    const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&m.fp[b].C[(k0 + k) * NP + n0]);
+                    float lo, hi;
+                    unpack2(fma2(cv.y, h23, mul2(cv.x, h01)), lo, hi);
+                    y[k0 + k] = lo + hi;
+                }
+            }
+            if constexpr (!STATE_ONLY) {
+                if ((k0 + 4) % R == 0) {   // R = 8, 16: after so many tokens; R < 4: several sums
+#pragma unroll
+                    for (int r0 = k0 + 4 - (R > 4 ? R : 4); r0 < k0 + 4; r0 += R) {
+                        float v[R];
+#pragma unroll
+                        for (int i = 0; i < R; ++i) v[i] = y[r0 + i];
+                        float sum = reduce_scatter<R, 1>(v, lane);
+                        if (LPC > R) sum += __shfl_xor_sync(0xffffffffu, sum, R);
+                        if (q < R) m.y[b][(r0 + q) * Y + ch] = sum;
+                    }
+                }
+            }
+        }
+    }
+    if (!STATE_ONLY && count > 0) {
+        __syncthreads();
+        const int64_t t = (count - 1) / TS * TS;
+        after(t, (int)(count - t), b ^ 1);
     }
     if (!live) return;
     unpack2(h01, h[0], h[1]);
@@ -349,6 +403,12 @@ __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ St
 }
 
 // ---- host -------------------------------------------------------------------------
+int lanes_for(int64_t states) {
+    int l = 1;
+    while (4 * l < states) l *= 2;
+    return l;
+}
+
 // Tokens a piece of a scan split along time; 0 = not split.
 //
 // Not split, a block (4 warps) takes its channels through a whole sequence: at best
@@ -356,7 +416,7 @@ __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ St
 // work, for the price of computing every exponential twice (kState more clocks a
 // token) and of two more launches. The longest of n packed sequences, whose lengths
 // the host does not know, is taken as (1 + ln n) average ones, as random cuts make it.
-constexpr double kAlone = 60, kFull = 42, kState = 36, kLaunches = 15000;
+constexpr double kAlone = 150, kFull = 80, kState = 55, kLaunches = 15000;
 int64_t piece_tokens(const pe_scan_args* a) {
     const int64_t ch = kThreads / lanes_for(a->states), dg = a->channels / a->groups;
     const int64_t tiles = a->groups * ceil_div(dg, ch);
@@ -365,15 +425,15 @@ int64_t piece_tokens(const pe_scan_args* a) {
     double longest = (double)a->tokens;
     if (a->cu) longest = min(longest, longest / a->nseq * (1.0 + log((double)a->nseq)));
     const double whole = max(longest * kAlone, total / sms * kFull);
-    const double split = total / sms * (kFull + kState) * 1.1 + kLaunches;
+    const double split = total / sms * (kFull + kState) + kLaunches;
     if (split >= whole) return 0;
-    const int64_t piece = (int64_t)(total / (3.0 * sms));   // three blocks an SM
-    return max((int64_t)64, ceil_div(piece, TS) * TS);
+    const int64_t piece = (int64_t)(total / (4.0 * sms));   // four blocks an SM
+    return max((int64_t)KCK, ceil_div(piece, KCK) * KCK);
 }
 
 template <typename T, int LPC>
 int scan_run(const pe_scan_args* a, cudaStream_t s) {
-    ScanP<T> p = scan_params<T>(a, kThreads / LPC);
+    ScanP<T> p = scan_params<T>(a, kThreads / LPC, 4 * LPC);
     const int64_t piece = piece_tokens(a);
     if (piece) {
         p.piece = piece;
@@ -383,19 +443,28 @@ int scan_run(const pe_scan_args* a, cudaStream_t s) {
     }
     unsigned grid;
     if (int rc = grid_of(piece_count(p.seqs, p.piece) * p.G * p.ntile, &grid)) return rc;
-    constexpr int CH = kThreads / LPC, cols = TS * 4 * LPC;
     if (piece) {
-        if (int rc = launch(scan_fwd<T, LPC, true>, p, grid, 2 * (2 * CH * LD + cols) * 4, s)) return rc;
-        const dim3 carry((unsigned)ceil_div((int64_t)p.D * p.N, kThreads), (unsigned)p.seqs.nseq);
-        scan_carry<T><<<carry, kThreads, 0, s>>>(p);
+        if (int rc = launch(scan_fwd<T, LPC, true>, p, grid, sizeof(FwdSmem<T, LPC, true>), s)) return rc;
+        const dim3 blocks((unsigned)ceil_div((int64_t)p.D * p.N, kThreads), (unsigned)p.seqs.nseq);
+        scan_carry<T><<<blocks, kThreads, 0, s>>>(p);
         count_launch();
         if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
-    return launch(scan_fwd<T, LPC, false>, p, grid, 2 * (3 * CH * LD + 2 * cols) * 4, s);
+    return launch(scan_fwd<T, LPC, false>, p, grid, sizeof(FwdSmem<T, LPC, false>), s);
 }
 
+#define PE_LANES(F, l, ...)                    \
+    switch (l) {                               \
+        case 1: return F<T, 1>(__VA_ARGS__);   \
+        case 2: return F<T, 2>(__VA_ARGS__);   \
+        case 4: return F<T, 4>(__VA_ARGS__);   \
+        case 8: return F<T, 8>(__VA_ARGS__);   \
+        case 16: return F<T, 16>(__VA_ARGS__); \
+        default: return F<T, 32>(__VA_ARGS__); \
+    }
+
 template <typename T>
-int scan_lanes(const pe_scan_args* a, cudaStream_t s) {
+int scan_type(const pe_scan_args* a, cudaStream_t s) {
     PE_LANES(scan_run, lanes_for(a->states), a, s)
 }
 
@@ -422,18 +491,18 @@ int step_run(const pe_scan_step_args* a, cudaStream_t s) {
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }
 template <typename T>
-int step_lanes(const pe_scan_step_args* a, cudaStream_t s) {
+int step_type(const pe_scan_step_args* a, cudaStream_t s) {
     PE_LANES(step_run, lanes_for(a->states), a, s)
 }
 
-int scan_any(const pe_scan_args* a, cudaStream_t s) { PE_TYPES(scan_lanes, a->dtype, a, s) }
-int step_any(const pe_scan_step_args* a, cudaStream_t s) { PE_TYPES(step_lanes, a->dtype, a, s) }
+int scan_any(const pe_scan_args* a, cudaStream_t s) { PE_TYPES(scan_type, a->dtype, a, s) }
+int step_any(const pe_scan_step_args* a, cudaStream_t s) { PE_TYPES(step_type, a->dtype, a, s) }
 
 }  // namespace
 
 int64_t scan_ckpt_floats(int64_t tokens, int64_t nseq, int64_t packed, int64_t channels, int64_t states) {
     const int32_t none = 0;
-    return piece_count(Seqs{packed ? &none : nullptr, tokens, (int32_t)nseq}, TS) * channels * states;
+    return piece_count(Seqs{packed ? &none : nullptr, tokens, (int32_t)nseq}, KCK) * channels * states;
 }
 
 int64_t scan_ws_bytes(const pe_scan_args* a) {

@@ -1,6 +1,8 @@
 // pe_scan.cuh - what the forward and the backward scan share: parameters, the
-// placement of blocks, staging, and the host's checks.
+// placement of blocks, tiles and staging, and the host's checks.
 #pragma once
+
+#include <initializer_list>
 
 #include "pe_mixer.cuh"
 
@@ -8,12 +10,8 @@ namespace pe {
 
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int TS = 16;       // tokens a tile, and between two checkpoints
-constexpr int LD = TS + 4;   // row of a [channel][token] tile: 16-byte rows whose float4 reads by
-                             // neighbouring channels fall on different banks
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int KCK = 64;      // tokens between two checkpoints
 constexpr int kSiteOffsets = 32, kSiteSlot = 33;
 
 template <typename T>
@@ -27,7 +25,10 @@ struct ScanP {
     int64_t u_sb, u_st, d_sb, d_st, z_sb, z_st, B_sb, B_st, B_sg, C_sb, C_st, C_sg;
     T* out;
     float *state, *ckpt;
-    int64_t piece;        // tokens a piece (a multiple of TS, or more than any sequence has)
+    // copies to shared memory: rows of these tensors in chunks (see chunk_of), 0 = element by element
+    int u_cb, d_cb, z_cb, B_cb, C_cb;
+    bool pairs;           // out's rows take aligned pairs of elements
+    int64_t piece;        // tokens a piece (a multiple of KCK, or more than any sequence has)
     float *hloc, *dtsum;  // ws of a split scan: each piece's own last state and sum of dt
 };
 
@@ -87,13 +88,48 @@ __device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
     return pack2(exp2_fast(lo), exp2_fast(hi));
 }
 
-// ---- host -------------------------------------------------------------------------
-inline int lanes_for(int64_t states) {
-    int l = 1;
-    while (4 * l < states) l *= 2;
-    return l;
+// ---- copies to shared memory ------------------------------------------------------
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* dst, const void* src, int valid) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// cnt (at most ROWS) rows of `width` (at most W) elements into rows of W, in chunks of
+// `cb` bytes that arrive asynchronously where the rows are aligned for them. Nothing
+// past the width or the count is read; there the tile stays as it was.
+template <int ROWS, int W, int BYTES, typename T>
+__device__ __forceinline__ void stage_chunks(T* dst, const T* src, int64_t st, int cnt, int width) {
+    constexpr int E = BYTES / (int)sizeof(T), PER = W / E;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < ROWS * PER; i += kThreads) {
+        const int t = i / PER, k = i % PER * E;
+        if (t < cnt && k < width)
+            cp_async<BYTES>(dst + t * W + k, src + t * st + k, min(BYTES, (width - k) * (int)sizeof(T)));
+    }
+}
+template <int ROWS, int W, typename T>
+__device__ __forceinline__ void stage(T* dst, const T* src, int64_t st, int cnt, int width, int cb) {
+    constexpr int ROW = W * (int)sizeof(T);
+    static_assert(ROW % 8 == 0, "rows of whole chunks");
+    if (ROW % 16 == 0 && cb == 16) {
+        stage_chunks<ROWS, W, 16>(dst, src, st, cnt, width);
+    } else if (cb >= 8) {
+        stage_chunks<ROWS, W, 8>(dst, src, st, cnt, width);
+    } else {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < ROWS * W; i += kThreads) {
+            const int t = i / W, k = i % W;
+            if (t < cnt && k < width) dst[i] = __ldg(src + t * st + k);
+        }
+    }
 }
 
+// ---- host -------------------------------------------------------------------------
 inline int check_scan(const pe_scan_args* a) {
     if (!a || a->dtype < PE_F32 || a->dtype > PE_BF16) return PE_ERR_INVALID;
     if (a->batch < 0 || a->tokens < 0 || a->channels < 1 || a->groups < 1 || a->nseq < 0 || a->states < 1)
@@ -107,8 +143,20 @@ inline int check_scan(const pe_scan_args* a) {
 
 inline Seqs seqs_of(const pe_scan_args* a) { return Seqs{a->cu, a->tokens, (int32_t)a->nseq}; }
 
+// Bytes a copy of rows of `width` elements moves at once: the largest of 16 and 8 that a
+// row of the tile holds and that divides the base address, the strides and `step` (what
+// a block's first element may be a multiple of); 0 where none does.
+inline int chunk_of(const void* p, int es, int64_t row_bytes, std::initializer_list<int64_t> strides, int64_t step) {
+    for (int cb : {16, 8}) {
+        bool ok = row_bytes >= cb && (uintptr_t)p % cb == 0 && step * es % cb == 0;
+        for (int64_t s : strides) ok = ok && s * es % cb == 0;
+        if (ok) return cb;
+    }
+    return 0;
+}
+
 template <typename T>
-ScanP<T> scan_params(const pe_scan_args* a, int ch) {
+ScanP<T> scan_params(const pe_scan_args* a, int ch, int nc) {
     ScanP<T> p;
     p.seqs = seqs_of(a);
     p.D = (int)a->channels; p.N = (int)a->states; p.G = (int)a->groups; p.Dg = p.D / p.G;
@@ -122,8 +170,17 @@ ScanP<T> scan_params(const pe_scan_args* a, int ch) {
     p.B_sb = a->B_sb; p.B_st = a->B_st; p.B_sg = a->B_sg;
     p.C_sb = a->C_sb; p.C_st = a->C_st; p.C_sg = a->C_sg;
     p.out = (T*)a->out; p.state = a->state; p.ckpt = a->ckpt;
-    p.piece = (a->tokens / TS + 1) * TS;   // longer than any sequence: one piece each, numbered like it
+    p.piece = (a->tokens / KCK + 1) * KCK;   // longer than any sequence: one piece each, numbered like it
     p.hloc = p.dtsum = nullptr;
+    const int es = sizeof(T);
+    const int64_t step = p.G > 1 ? p.Dg : ch, row = (int64_t)ch * es;   // of a block's first channel
+    const int64_t cols = (int64_t)nc * es;
+    p.u_cb = chunk_of(p.u, es, row, {p.u_sb, p.u_st, (int64_t)ch}, step);
+    p.d_cb = chunk_of(p.delta, es, row, {p.d_sb, p.d_st, (int64_t)ch}, step);
+    p.z_cb = p.z ? chunk_of(p.z, es, row, {p.z_sb, p.z_st, (int64_t)ch}, step) : 0;
+    p.B_cb = chunk_of(p.B, es, cols, {p.B_sb, p.B_st, p.B_sg}, nc);
+    p.C_cb = chunk_of(p.C, es, cols, {p.C_sb, p.C_st, p.C_sg}, nc);
+    p.pairs = p.Dg % 2 == 0;
     return p;
 }
 
@@ -142,16 +199,6 @@ int launch(K kernel, const P& p, unsigned grid, int smem, cudaStream_t s) {
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }
-
-#define PE_LANES(F, l, ...)                    \
-    switch (l) {                               \
-        case 1: return F<T, 1>(__VA_ARGS__);   \
-        case 2: return F<T, 2>(__VA_ARGS__);   \
-        case 4: return F<T, 4>(__VA_ARGS__);   \
-        case 8: return F<T, 8>(__VA_ARGS__);   \
-        case 16: return F<T, 16>(__VA_ARGS__); \
-        default: return F<T, 32>(__VA_ARGS__); \
-    }
 
 #define PE_TYPES(F, dtype, ...)                            \
     switch (dtype) {                                       \

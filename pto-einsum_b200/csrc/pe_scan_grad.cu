@@ -5,338 +5,500 @@ namespace pe {
 
 namespace {
 
+constexpr int K = 8;         // tokens a lane
+constexpr int SEG = K + 4;   // a lane's K tokens in a shared row: float4 reads of eight lanes fall on
+                             // all banks once
+// A warp takes 32 / LT channel pairs and LT K consecutive tokens, a lane one pair's K
+// tokens; the block's warps have other channels and the same tokens.
+template <int LT>
+struct Tile {
+    static constexpr int TT = LT * K;                 // tokens
+    static constexpr int CB = 2 * (32 / LT) * kWarps; // channels
+    static constexpr int RS = LT * SEG + 4;           // row of a [..][token] array
+};
+__device__ __forceinline__ int at_token(int t) { return t / K * SEG + t % K; }
+
+// B or C of a tile's tokens, rows of NC states as in memory, into fp32 [state][token];
+// zero past the last token (a token there must leave the state alone) and state.
+template <int LT, int NC, typename T>
+__device__ __forceinline__ void widen_cols(float* dst, const T* src, int cnt, int nn) {
+    constexpr int TT = Tile<LT>::TT, RS = Tile<LT>::RS;
+#pragma unroll
+    for (int i = threadIdx.x; i < TT * NC / 4; i += kThreads) {
+        const int t = i / (NC / 4), n = i % (NC / 4) * 4;
+        const Vec<T, 4> v = *reinterpret_cast<const Vec<T, 4>*>(src + t * NC + n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            dst[(n + e) * RS + at_token(t)] = t < cnt && n + e < nn ? to_float(v.v[e]) : 0.0f;
+    }
+}
+
+// Eight consecutive floats as four pairs, 16-byte aligned.
+struct Pairs {
+    f32x2 p[K / 2];
+};
+__device__ __forceinline__ Pairs load_pairs(const float* s) {
+    Pairs r;
+#pragma unroll
+    for (int i = 0; i < K / 4; ++i) {
+        const ulonglong2 v = reinterpret_cast<const ulonglong2*>(s)[i];
+        r.p[2 * i] = v.x;
+        r.p[2 * i + 1] = v.y;
+    }
+    return r;
+}
+__device__ __forceinline__ void store_pairs(float* s, const Pairs& r) {
+#pragma unroll
+    for (int i = 0; i < K / 4; ++i)
+        reinterpret_cast<ulonglong2*>(s)[i] = ulonglong2{r.p[2 * i], r.p[2 * i + 1]};
+}
+__device__ __forceinline__ void to_scalars(const Pairs& r, float (&f)[K]) {
+#pragma unroll
+    for (int i = 0; i < K / 2; ++i) unpack2(r.p[i], f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ float product(const Pairs& a) {
+    float lo, hi;
+    unpack2(mul2(mul2(a.p[0], a.p[1]), mul2(a.p[2], a.p[3])), lo, hi);
+    return lo * hi;
+}
+__device__ __forceinline__ f32x2 shfl2_up(f32x2 v, int d, int width) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    return pack2(__shfl_up_sync(0xffffffffu, lo, d, width), __shfl_up_sync(0xffffffffu, hi, d, width));
+}
+__device__ __forceinline__ f32x2 shfl2_down(f32x2 v, int d, int width) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    return pack2(__shfl_down_sync(0xffffffffu, lo, d, width), __shfl_down_sync(0xffffffffu, hi, d, width));
+}
+
+// What the lanes of a channel pair do to the state, composed along the tokens. Lane tl
+// maps the state before it, h, to P h + H (both channels at once). Returns the state
+// before the lane, and in `last` the state after it, given the state `h0` before lane 0.
+template <int LT>
+__device__ __forceinline__ f32x2 scan_lanes_up(f32x2 P, f32x2 H, f32x2 h0, int tl, f32x2& last) {
+    if (tl == 0) H = fma2(P, h0, H);
+#pragma unroll
+    for (int d = 1; d < LT; d *= 2) {
+        const f32x2 Hu = shfl2_up(H, d, LT), Pu = shfl2_up(P, d, LT);
+        if (tl >= d) {
+            H = fma2(P, Hu, H);
+            P = mul2(P, Pu);
+        }
+    }
+    last = H;
+    const f32x2 before = shfl2_up(H, 1, LT);
+    return tl == 0 ? h0 : before;
+}
+// The same from the last token to the first.
+template <int LT>
+__device__ __forceinline__ f32x2 scan_lanes_down(f32x2 P, f32x2 H, f32x2 h0, int tl, f32x2& last) {
+    if (tl == LT - 1) H = fma2(P, h0, H);
+#pragma unroll
+    for (int d = 1; d < LT; d *= 2) {
+        const f32x2 Hu = shfl2_down(H, d, LT), Pu = shfl2_down(P, d, LT);
+        if (tl < LT - d) {
+            H = fma2(P, Hu, H);
+            P = mul2(P, Pu);
+        }
+    }
+    last = H;
+    const f32x2 after = shfl2_down(H, 1, LT);
+    return tl == LT - 1 ? h0 : after;
+}
+
+constexpr int LT = 8;         // lanes along the tokens: tiles of 64 tokens, one a checkpoint
+using L = Tile<LT>;
+constexpr int TT = L::TT, CB = L::CB, RS = L::RS;
+static_assert(TT == KCK, "a checkpoint a tile");
+
 // ---- backward -------------------------------------------------------------------
 template <typename T>
 struct GradP {
     ScanP<T> f;
     const T* dout;
     int64_t o_sb, o_st;
+    int o_cb;
     const float* dstate;
     T *du, *ddelta, *dz;
     float *dh0;
-    float *pBC;       // [2][tiles][batch * tokens][G][N]: each channel tile's share of dB and dC
+    float *pBC;       // [2][tiles][G][N][batch * tokens]: each channel tile's share of dB and dC
     float *pA;        // [nseq][D][N]
     float *pD, *pb;   // [nseq][D]
 };
 
-// Adds v to a sum that keeps its rounding errors (Kahan): a sum over thousands of
-// tokens would lose what two passes of a pairwise sum keep.
-__device__ __forceinline__ void add_exactly(float& sum, float& err, float v) {
-    const float y = __fsub_rn(v, err), t = __fadd_rn(sum, y);
-    err = __fsub_rn(__fsub_rn(t, sum), y);
-    sum = t;
-}
-
-// A tile's inputs on their way from memory: loaded while the tile before is worked on.
-template <typename T, int LPC>
-struct GradRegs {
-    static constexpr int CH = kThreads / LPC, I = LPC < 4 ? 4 / LPC : 1, J = LPC * 4 * TS / kThreads > 0 ? LPC * 4 * TS / kThreads : 1;
-    T d[I][4], u[I][4], z[I][4], o[I][4], b[J], c[J];
-
-    __device__ __forceinline__ void load(const GradP<T>& p, const Place& w, const T* up, const T* dp, const T* zp,
-                                         const T* op, const T* Bp, const T* Cp, int64_t at, int cnt) {
-        constexpr int NP = 4 * LPC;
-        const int tid = threadIdx.x;
-        const T zero = from_float<T>(0.0f);
-#pragma unroll
-        for (int k = 0; k < I; ++k) {
-            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
-            const int64_t cc = w.c0 + ic;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = ic < w.nch && t4 + i < cnt;
-                const int64_t t = at + t4 + i;
-                d[k][i] = in ? __ldg(dp + t * p.f.d_st + cc) : zero;
-                u[k][i] = in ? __ldg(up + t * p.f.u_st + cc) : zero;
-                o[k][i] = in ? __ldg(op + t * p.o_st + cc) : zero;
-                z[k][i] = in && zp ? __ldg(zp + t * p.f.z_st + cc) : zero;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = tid + j * kThreads, t = i / NP, n = i % NP;
-            const bool in = t < cnt && n < p.f.N;
-            b[j] = in ? __ldg(Bp + (at + t) * p.f.B_st + n) : zero;
-            c[j] = in ? __ldg(Cp + (at + t) * p.f.C_st + n) : zero;
-        }
-    }
+template <typename T>
+struct GradSmem {
+    static constexpr int NC = sizeof(T) == 2 ? 16 : 8;   // states at a time: two blocks fit an SM
+    alignas(16) T u[TT * CB];                            // as in memory
+    T d[TT * CB], z[TT * CB], o[TT * CB], b[TT * NC], c[TT * NC];
+    // fp32, [channel or state][token]; the first three end as du, q u + r and y + D u
+    alignas(16) float dt[CB * RS];
+    float x[CB * RS], dy[CB * RS];
+    float B[NC * RS], C[NC * RS];
+    float red[kWarps][NC][2][TT];                        // a warp's share of dB and dC
+    float rows[];   // [N][CB] adjoint states, A log2(e), dA; [CB][N] checkpoint
 };
 
-// Sums of R values over the LPC lanes of a channel, TS values in: lane q of the channel
-// stores value k + q of each run of R.
-template <int LPC>
-__device__ __forceinline__ void sum_states(const float (&y)[TS], float* row, int q, int lane, float scale) {
-    constexpr int R = LPC < TS ? LPC : TS;
+// One block takes 32 channels through a whole sequence, tile by tile from its end. Per
+// state n a lane composes the maps of its K tokens forwards (from the checkpoint) and
+// backwards (from the tile after), scans them with the other lanes of its channels, and
+// runs both recurrences again in registers:
+//   h = a h' + b,  a = exp(dt A),  b = dt u B;   g = C dy + a' g'
+//   q = sum_n g B,  r = sum_n g a h' A:   du = q dt + D dy,  ddt = q u + r
+//   dB = sum_c g dt u,  dC = sum_c dy h,  dA = sum_t g a h' dt
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ GradP<T> p) {
+    using M = GradSmem<T>;
+    constexpr int NC = M::NC;
+    extern __shared__ __align__(16) unsigned char smem[];
+    M& m = *reinterpret_cast<M*>(smem);
+    const ScanP<T>& f = p.f;
+    float *sG = m.rows, *sA = sG + f.N * CB, *sD = sA + f.N * CB, *sK = sD + f.N * CB;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    if (blockIdx.x == 0 && tid < 32) check_offsets(f.seqs, lane, kSiteOffsets);
+    const Place w = place_of<CB>(f);
+    const int tl = lane % LT, cl = lane / LT, c = 2 * (warp * (32 / LT) + cl);
+    const int64_t DN = (int64_t)f.D * f.N;
+    const int tile = (w.c0 - w.g * f.Dg) / CB;
+
+    const int64_t start = w.sp.start, len = w.sp.len;
+    const T* u = f.u + w.sp.row * f.u_sb + start * f.u_st + w.c0;
+    const T* delta = f.delta + w.sp.row * f.d_sb + start * f.d_st + w.c0;
+    const T* z = f.z ? f.z + w.sp.row * f.z_sb + start * f.z_st + w.c0 : nullptr;
+    const T* dout = p.dout + w.sp.row * p.o_sb + start * p.o_st + w.c0;
+    const T* B = f.B + w.sp.row * f.B_sb + start * f.B_st + w.g * f.B_sg;
+    const T* C = f.C + w.sp.row * f.C_sb + start * f.C_st + w.g * f.C_sg;
+    const int64_t row0 = w.sp.row * f.seqs.tokens + start;
+    const int64_t rows = f.seqs.tokens * (f.seqs.cu ? 1 : f.seqs.nseq);
+    const float* ckpt = f.ckpt + piece_base(f.seqs, w.s, KCK) * DN + (int64_t)w.c0 * f.N;
+    auto copy_states = [&](int64_t t, int n0) {
+        const int cnt = (int)min((int64_t)TT, len - t), nn = min(NC, f.N - n0);
+        stage<TT, NC>(m.b, B + t * f.B_st + n0, f.B_st, cnt, nn, f.B_cb);
+        stage<TT, NC>(m.c, C + t * f.C_st + n0, f.C_st, cnt, nn, f.C_cb);
+    };
+    auto copy = [&](int64_t t) {
+        const int cnt = (int)min((int64_t)TT, len - t);
+        stage<TT, CB>(m.u, u + t * f.u_st, f.u_st, cnt, w.nch, f.u_cb);
+        stage<TT, CB>(m.d, delta + t * f.d_st, f.d_st, cnt, w.nch, f.d_cb);
+        stage<TT, CB>(m.o, dout + t * p.o_st, p.o_st, cnt, w.nch, p.o_cb);
+        if (z) stage<TT, CB>(m.z, z + t * f.z_st, f.z_st, cnt, w.nch, f.z_cb);
+        copy_states(t, 0);
+        const float* k = ckpt + t / KCK * DN;
+        for (int i = tid; i < w.nch * f.N; i += kThreads) cp_async<4>(sK + i, k + i, 4);
+    };
+    const int64_t top = len > 0 ? (len - 1) / TT * TT : -1;
+    if (top >= 0) copy(top);
+    cp_commit();
+    for (int i = tid; i < CB * f.N; i += kThreads) {
+        const int ci = i / f.N, n = i - ci * f.N;
+        const int64_t k = (int64_t)(w.c0 + ci) * f.N + n;
+        const bool in = ci < w.nch;
+        sG[n * CB + ci] = in && p.dstate ? __ldg(p.dstate + w.s * DN + k) : 0.0f;
+        sA[n * CB + ci] = in ? __ldg(f.A + k) * kLog2e : 0.0f;
+        sD[n * CB + ci] = 0.0f;
+        if (!in) sK[i] = 0.0f;
+    }
+    float Dw[2], dD[2] = {0.0f, 0.0f}, db[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < TS; k += R) {
-        float v[R];
+    for (int e = 0; e < 2; ++e) Dw[e] = f.Dw && c + e < w.nch ? __ldg(f.Dw + w.c0 + c + e) : 0.0f;
+    // of the element-wise work: channels cp, cp + 1
+    const int cp = tid % (CB / 2) * 2;
+    float bias[2];
 #pragma unroll
-        for (int i = 0; i < R; ++i) v[i] = y[k + i];
-        float sum = reduce_scatter<R, 1>(v, lane);
-        if (LPC > R) sum += __shfl_xor_sync(0xffffffffu, sum, R);
-        if (q < R) row[k + q] = sum * scale;
+    for (int e = 0; e < 2; ++e) bias[e] = f.bias && cp + e < w.nch ? __ldg(f.bias + w.c0 + cp + e) : 0.0f;
+    float* dtr = m.dt + c * RS + tl * SEG;
+    float* xr = m.x + c * RS + tl * SEG;
+    float* dyr = m.dy + c * RS + tl * SEG;
+
+    for (int64_t t = top; t >= 0; t -= TT) {
+        const int cnt = (int)min((int64_t)TT, len - t);
+        Pairs dt[2], x[2], dy[2], y[2], q[2], r[2];
+        for (int n0 = 0; n0 < f.N; n0 += NC) {
+            const int nn = min(NC, f.N - n0);
+            cp_wait();
+            __syncthreads();
+            if (n0 == 0) {
+                // dt, u and dy = dout silu(z), transposed; zero past the last token and channel
+#pragma unroll 2
+                for (int i = tid; i < TT / 4 * (CB / 2); i += kThreads) {
+                    const int t4 = i / (CB / 2) * 4;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float fd[4], fu[4], fy[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int at = (t4 + k) * CB + cp + e;
+                            const bool ok = cp + e < w.nch && t4 + k < cnt;
+                            float v = to_float(m.d[at]) + bias[e];
+                            if (f.softplus) v = softplusf(v);
+                            fd[k] = ok ? v : 0.0f;
+                            fu[k] = ok ? to_float(m.u[at]) : 0.0f;
+                            v = to_float(m.o[at]);
+                            if (z) {
+                                const float zv = to_float(m.z[at]);
+                                v *= zv * sigmoidf(zv);
+                            }
+                            fy[k] = ok ? v : 0.0f;
+                        }
+                        const int to = (cp + e) * RS + at_token(t4);
+                        *reinterpret_cast<float4*>(m.dt + to) = make_float4(fd[0], fd[1], fd[2], fd[3]);
+                        *reinterpret_cast<float4*>(m.x + to) = make_float4(fu[0], fu[1], fu[2], fu[3]);
+                        *reinterpret_cast<float4*>(m.dy + to) = make_float4(fy[0], fy[1], fy[2], fy[3]);
+                    }
+                }
+            }
+            widen_cols<LT, NC>(m.B, m.b, cnt, nn);
+            widen_cols<LT, NC>(m.C, m.c, cnt, nn);
+            __syncthreads();
+            if (n0 + NC < f.N) {
+                copy_states(t, n0 + NC);
+                cp_commit();
+            }
+            if (n0 == 0) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    dt[e] = load_pairs(dtr + e * RS);
+                    x[e] = load_pairs(xr + e * RS);
+                    dy[e] = load_pairs(dyr + e * RS);
+                    f32x2 s = 0;
+#pragma unroll
+                    for (int i = 0; i < K / 2; ++i) {
+                        s = fma2(x[e].p[i], dy[e].p[i], s);
+                        x[e].p[i] = mul2(dt[e].p[i], x[e].p[i]);
+                        y[e].p[i] = q[e].p[i] = r[e].p[i] = 0;
+                    }
+                    float lo, hi;
+                    unpack2(s, lo, hi);
+                    dD[e] += lo + hi;
+                }
+            }
+#pragma unroll 1
+            for (int n = 0; n < nn; ++n) {
+                const Pairs Bn = load_pairs(m.B + n * RS + tl * SEG), Cn = load_pairs(m.C + n * RS + tl * SEG);
+                const int at = (n0 + n) * CB + c;
+                const float2 A = *reinterpret_cast<const float2*>(sA + at);
+                f32x2* gp = reinterpret_cast<f32x2*>(sG + at);
+                const f32x2 g0 = *gp, h0 = pack2(sK[c * f.N + n0 + n], sK[(c + 1) * f.N + n0 + n]);
+                float a[2][K], b[2][K], v[2][K], P[2], H[2], G[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float Ae = e ? A.y : A.x;
+                    const f32x2 A2 = pack2(Ae, Ae);
+                    Pairs ap, bp, vp;
+#pragma unroll
+                    for (int i = 0; i < K / 2; ++i) {
+                        ap.p[i] = exp2_2(mul2(dt[e].p[i], A2));
+                        bp.p[i] = mul2(x[e].p[i], Bn.p[i]);
+                        vp.p[i] = mul2(dy[e].p[i], Cn.p[i]);
+                    }
+                    P[e] = product(ap);
+                    to_scalars(ap, a[e]);
+                    to_scalars(bp, b[e]);
+                    to_scalars(vp, v[e]);
+                    H[e] = b[e][0];
+                    G[e] = v[e][K - 1];
+#pragma unroll
+                    for (int k = 1; k < K; ++k) {
+                        H[e] = fmaf(a[e][k], H[e], b[e][k]);
+                        G[e] = fmaf(a[e][K - k], G[e], v[e][K - 1 - k]);
+                    }
+                    G[e] *= a[e][0];
+                }
+                f32x2 last;
+                const f32x2 P2 = pack2(P[0], P[1]);
+                const f32x2 before = scan_lanes_up<LT>(P2, pack2(H[0], H[1]), h0, tl, last);
+                const f32x2 after = scan_lanes_down<LT>(P2, pack2(G[0], G[1]), g0, tl, last);
+                if (tl == 0) *gp = last;   // the last lane read it before the shuffles
+                float hb[2], ga[2], da[2];
+                unpack2(before, hb[0], hb[1]);
+                unpack2(after, ga[0], ga[1]);
+                Pairs dB, dC;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float Ae = e ? A.y : A.x;
+                    const f32x2 A2 = pack2(Ae, Ae);
+                    float h = hb[e], g = ga[e], s[K], gs[K], hs[K];   // s = a h'
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        s[k] = a[e][k] * h;
+                        h = hs[k] = s[k] + b[e][k];
+                    }
+#pragma unroll
+                    for (int k = K - 1; k >= 0; --k) {
+                        gs[k] = g + v[e][k];
+                        g = gs[k] * a[e][k];
+                    }
+                    f32x2 sum = 0;
+#pragma unroll
+                    for (int i = 0; i < K / 2; ++i) {
+                        const f32x2 g2 = pack2(gs[2 * i], gs[2 * i + 1]), h2 = pack2(hs[2 * i], hs[2 * i + 1]);
+                        y[e].p[i] = fma2(Cn.p[i], h2, y[e].p[i]);
+                        q[e].p[i] = fma2(Bn.p[i], g2, q[e].p[i]);
+                        const f32x2 e2 = mul2(g2, pack2(s[2 * i], s[2 * i + 1]));
+                        r[e].p[i] = fma2(e2, A2, r[e].p[i]);
+                        sum = fma2(e2, dt[e].p[i], sum);
+                        dB.p[i] = e ? fma2(g2, x[e].p[i], dB.p[i]) : mul2(g2, x[e].p[i]);
+                        dC.p[i] = e ? fma2(h2, dy[e].p[i], dC.p[i]) : mul2(h2, dy[e].p[i]);
+                    }
+                    float lo, hi;
+                    unpack2(sum, lo, hi);
+                    da[e] = lo + hi;
+                }
+#pragma unroll
+                for (int d = LT / 2; d >= 1; d /= 2) {
+                    da[0] += __shfl_xor_sync(0xffffffffu, da[0], d);
+                    da[1] += __shfl_xor_sync(0xffffffffu, da[1], d);
+                }
+                if (tl == 0) {
+                    float2* o = reinterpret_cast<float2*>(sD + at);
+                    *o = make_float2(o->x + da[0], o->y + da[1]);
+                }
+                // over the warp's four channel pairs: lanes 16 .. 31 end with dC, odd pairs with
+                // the second half of the tokens
+                float vb[K], vc[K];
+                to_scalars(dB, vb);
+                to_scalars(dC, vc);
+                const bool hi = lane & 16, odd = lane & 8;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const float send = hi ? vb[k] : vc[k], keep = hi ? vc[k] : vb[k];
+                    vb[k] = keep + __shfl_xor_sync(0xffffffffu, send, 16);
+                }
+#pragma unroll
+                for (int k = 0; k < K / 2; ++k) {
+                    const float send = odd ? vb[k] : vb[k + K / 2], keep = odd ? vb[k + K / 2] : vb[k];
+                    vb[k] = keep + __shfl_xor_sync(0xffffffffu, send, 8);
+                }
+                *reinterpret_cast<float4*>(&m.red[warp][n][hi][tl * K + (odd ? K / 2 : 0)]) =
+                    make_float4(vb[0], vb[1], vb[2], vb[3]);
+            }
+            __syncthreads();
+            for (int i = tid; i < nn * 2 * TT; i += kThreads) {
+                const int k = i % TT, which = i / TT % 2, n = i / (2 * TT);
+                if (k >= cnt) continue;
+                float s = 0.0f;
+#pragma unroll
+                for (int v = 0; v < kWarps; ++v) s += m.red[v][n][which][k];
+                p.pBC[((((int64_t)which * f.ntile + tile) * f.G + w.g) * f.N + n0 + n) * rows + row0 + t + k] = s;
+            }
+        }
+        // a lane's own parts of the rows take what the element-wise work needs
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const Pairs uv = load_pairs(xr + e * RS);
+            const f32x2 D2 = pack2(Dw[e], Dw[e]), ln2 = pack2(kLn2, kLn2);
+#pragma unroll
+            for (int i = 0; i < K / 2; ++i) {
+                dt[e].p[i] = fma2(q[e].p[i], dt[e].p[i], mul2(D2, dy[e].p[i]));
+                r[e].p[i] = fma2(q[e].p[i], uv.p[i], mul2(ln2, r[e].p[i]));
+                y[e].p[i] = fma2(D2, uv.p[i], y[e].p[i]);
+            }
+            store_pairs(dtr + e * RS, dt[e]);
+            store_pairs(xr + e * RS, r[e]);
+            store_pairs(dyr + e * RS, y[e]);
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int i = tid; i < TT / 4 * (CB / 2); i += kThreads) {
+            const int t4 = i / (CB / 2) * 4;
+            float du[2][4], dd[2][4], yv[2][4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int at = (cp + e) * RS + at_token(t4);
+                const float4 v0 = *reinterpret_cast<const float4*>(m.dt + at);
+                const float4 v1 = *reinterpret_cast<const float4*>(m.x + at);
+                const float4 v2 = *reinterpret_cast<const float4*>(m.dy + at);
+                du[e][0] = v0.x, du[e][1] = v0.y, du[e][2] = v0.z, du[e][3] = v0.w;
+                dd[e][0] = v1.x, dd[e][1] = v1.y, dd[e][2] = v1.z, dd[e][3] = v1.w;
+                yv[e][0] = v2.x, yv[e][1] = v2.y, yv[e][2] = v2.z, yv[e][3] = v2.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (t4 + k >= cnt || cp >= w.nch) break;
+                Vec<T, 2> vu, vd, vz;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int at = (t4 + k) * CB + cp + e;
+                    float g = dd[e][k];
+                    if (f.softplus) g *= sigmoidf(to_float(m.d[at]) + bias[e]);
+                    if (cp + e < w.nch) db[e] += g;
+                    vu.v[e] = from_float<T>(du[e][k]);
+                    vd.v[e] = from_float<T>(g);
+                    if (p.dz) {
+                        const float zv = to_float(m.z[at]);
+                        vz.v[e] = from_float<T>(to_float(m.o[at]) * silu_slope(zv, sigmoidf(zv)) * yv[e][k]);
+                    }
+                }
+                const int64_t o = (row0 + t + t4 + k) * f.D + w.c0 + cp;
+                if (f.pairs) {
+                    *reinterpret_cast<Vec<T, 2>*>(p.du + o) = vu;
+                    *reinterpret_cast<Vec<T, 2>*>(p.ddelta + o) = vd;
+                    if (p.dz) *reinterpret_cast<Vec<T, 2>*>(p.dz + o) = vz;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (cp + e < w.nch) {
+                            p.du[o + e] = vu.v[e];
+                            p.ddelta[o + e] = vd.v[e];
+                            if (p.dz) p.dz[o + e] = vz.v[e];
+                        }
+                }
+            }
+        }
+        if (t > 0) {
+            __syncthreads();
+            copy(t - TT);
+            cp_commit();
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < w.nch * f.N; i += kThreads) {
+        const int ci = i / f.N, n = i - ci * f.N;
+        const int64_t k = w.s * DN + (int64_t)(w.c0 + ci) * f.N + n;
+        p.pA[k] = sD[n * CB + ci];
+        if (p.dh0) p.dh0[k] = sG[n * CB + ci];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = LT / 2; d >= 1; d /= 2) dD[e] += __shfl_xor_sync(0xffffffffu, dD[e], d);
+        if (tl == 0 && c + e < w.nch) p.pD[(int64_t)w.s * f.D + w.c0 + c + e] = dD[e];
+        m.dt[e * kThreads + tid] = db[e];
+    }
+    __syncthreads();
+    if (tid < w.nch) {
+        float s = 0.0f;
+        for (int k = tid / 2; k < kThreads; k += CB / 2) s += m.dt[tid % 2 * kThreads + k];
+        p.pb[(int64_t)w.s * f.D + w.c0 + tid] = s;
     }
 }
 
-// One block takes the channel tile through a whole sequence, tile by tile from its
-// end: the 16 states of a tile are computed again from its checkpoint and stay in
-// registers, then the adjoint runs back over them.
-//   g = C dy + a' g' ;  q = sum_n g B ;  r = sum_n g h' a A
-//   du = q dt + D dy ;  ddt = q u + r ;  dB += g dt u ;  dC += dy h ;  dA += g h' a dt
-template <typename T, int LPC>
-__global__ void __launch_bounds__(kThreads, LPC == 4 || LPC == 8 ? 3 : 2) scan_bwd(const __grid_constant__ GradP<T> p) {
-    constexpr int CH = kThreads / LPC, NP = 4 * LPC;
-    constexpr int CW = 32 / LPC;              // channels a warp
-    constexpr int RC = CW < 8 ? CW : 8;       // lanes that share the eight dB and dC sums
-    constexpr int VL = 8 / RC;                // sums a lane ends with
-    using Regs = GradRegs<T, LPC>;
-    constexpr int I = Regs::I, J = Regs::J;
-    extern __shared__ __align__(16) float smem[];
-    float *sdt = smem, *sx = sdt + CH * LD, *sdy = sx + CH * LD, *sy = sdy + CH * LD, *sq = sy + CH * LD,
-          *sr = sq + CH * LD;             // [CH][LD] each
-    float *sB = sr + CH * LD, *sC = sB + TS * NP;
-    float* sred = sC + TS * NP;           // [4 warps][TS][2][NP]
-    const ScanP<T>& f = p.f;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
-    if (blockIdx.x == 0 && tid < 32) check_offsets(f.seqs, lane, kSiteOffsets);
-    const Place w = place_of<CH>(f);
-    const int ch = tid / LPC, q = tid % LPC, c = w.c0 + ch, n0 = 4 * q;
-    const bool live = ch < w.nch;
-    const int64_t DN = (int64_t)f.D * f.N, cn = (int64_t)c * f.N + n0;
-    const int tile = (w.c0 - w.g * f.Dg) / CH;
-
-    float A[4], dA[4], eA[4], carry[4];
+// dB and dC [row][G N] from the channel tiles' shares [tile][G N][row]: 32 rows by 32
+// columns a block, transposed in shared memory; blockIdx.z 0 is dB, 1 dC.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_tiles(const float* __restrict__ part, int ntile, int64_t rows, int cols,
+                                                 T* dB, T* dC) {
+    __shared__ float s[32][33];
+    const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+    const int64_t r0 = (int64_t)blockIdx.x * 32;
+    const int c0 = blockIdx.y * 32;
+    part += (int64_t)blockIdx.z * ntile * cols * rows;
+    T* out = blockIdx.z ? dC : dB;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool in = live && n0 + i < f.N;
-        A[i] = in ? __ldg(f.A + cn + i) * kLog2e : 0.0f;
-        carry[i] = in && p.dstate ? __ldg(p.dstate + w.s * DN + cn + i) : 0.0f;
-        dA[i] = eA[i] = 0.0f;
+    for (int k = y; k < 32; k += 8) {
+        float a = 0.0f;
+        if (c0 + k < cols && r0 + x < rows) {
+            const float* b = part + (int64_t)(c0 + k) * rows + r0 + x;
+#pragma unroll 8
+            for (int i = 0; i < ntile; ++i) a += __ldg(b + (int64_t)i * cols * rows);
+        }
+        s[k][x] = a;
     }
-    const f32x2 A01 = pack2(A[0], A[1]), A23 = pack2(A[2], A[3]);
-    f32x2 c01 = pack2(carry[0], carry[1]), c23 = pack2(carry[2], carry[3]);
-    float dD = 0.0f, db = 0.0f, eD = 0.0f, eb = 0.0f;   // of channel tid % CH, this thread's tokens
-    const T* u = f.u + w.sp.row * f.u_sb;
-    const T* delta = f.delta + w.sp.row * f.d_sb;
-    const T* z = f.z ? f.z + w.sp.row * f.z_sb : nullptr;
-    const T* dout = p.dout + w.sp.row * p.o_sb;
-    const T* B = f.B + w.sp.row * f.B_sb + w.g * f.B_sg;
-    const T* C = f.C + w.sp.row * f.C_sb + w.g * f.C_sg;
-    const int64_t row0 = w.sp.row * f.seqs.tokens;
-    const int64_t rows = f.seqs.tokens * (f.seqs.cu ? 1 : f.seqs.nseq);
-    float bias[I], Dw[I];
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < I; ++k) {
-        const int ic = (tid + k * kThreads) % CH;
-        bias[k] = f.bias && ic < w.nch ? __ldg(f.bias + w.c0 + ic) : 0.0f;
-        Dw[k] = f.Dw && ic < w.nch ? __ldg(f.Dw + w.c0 + ic) : 0.0f;
-    }
-    const int64_t top = w.sp.len > 0 ? (w.sp.len - 1) / TS * TS : -1;
-    const float* ckpt = f.ckpt + (piece_base(f.seqs, w.s, TS) + (top >= 0 ? top / TS : 0)) * DN + cn;
-    Regs r;
-    float hc[4];
-    auto load_state = [&]() {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) hc[i] = live && n0 + i < f.N ? ckpt[i] : 0.0f;
-        ckpt -= DN;
-    };
-    if (top >= 0) {
-        r.load(p, w, u, delta, z, dout, B, C, w.sp.start + top, (int)(w.sp.len - top));
-        load_state();
-    }
-
-    for (int64_t t = top; t >= 0; t -= TS) {
-        const int cnt = (int)min((int64_t)TS, w.sp.len - t);
-        const int64_t at = w.sp.start + t;
-        // what the tile's gradients need of each (token, channel) after the recurrence:
-        // u, slope of softplus, d out / d z without y
-        float ku[I][4], ks[I][4], kz[I][4];
-#pragma unroll
-        for (int k = 0; k < I; ++k) {
-            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
-            float dt[4], x[4], dy[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = ic < w.nch && t4 + i < cnt;
-                const float raw = to_float(r.d[k][i]) + bias[k], zv = to_float(r.z[k][i]);
-                ku[k][i] = to_float(r.u[k][i]);
-                dy[i] = to_float(r.o[k][i]);
-                dt[i] = f.softplus ? softplusf(raw) : raw;
-                ks[k][i] = f.softplus ? sigmoidf(raw) : 1.0f;
-                kz[k][i] = 0.0f;
-                if (z) {
-                    const float s = sigmoidf(zv);
-                    kz[k][i] = dy[i] * silu_slope(zv, s);
-                    dy[i] *= zv * s;
-                }
-                x[i] = dt[i] * ku[k][i];
-                if (!in) dt[i] = x[i] = dy[i] = 0.0f;
-            }
-            if (it < CH * (TS / 4)) {
-                *reinterpret_cast<float4*>(sdt + ic * LD + t4) = make_float4(dt[0], dt[1], dt[2], dt[3]);
-                *reinterpret_cast<float4*>(sx + ic * LD + t4) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(sdy + ic * LD + t4) = make_float4(dy[0], dy[1], dy[2], dy[3]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = tid + j * kThreads;
-            if (i < TS * NP) {
-                sB[i] = to_float(r.b[j]);
-                sC[i] = to_float(r.c[j]);
-            }
-        }
-        __syncthreads();
-
-        f32x2 hs[TS + 1][2];   // hs[0] before the tile, hs[k + 1] after its token k
-        hs[0][0] = pack2(hc[0], hc[1]);
-        hs[0][1] = pack2(hc[2], hc[3]);
-        if (t > 0) {
-            r.load(p, w, u, delta, z, dout, B, C, at - TS, TS);
-            load_state();
-        }
-        {
-            float yv[TS];
-#pragma unroll
-            for (int k = 0; k < TS; ++k) {
-                yv[k] = 0.0f;
-                hs[k + 1][0] = hs[k][0];
-                hs[k + 1][1] = hs[k][1];
-                if (k < cnt) {
-                    const float dt = sdt[ch * LD + k], x = sx[ch * LD + k];
-                    const f32x2 dt2 = pack2(dt, dt), x2 = pack2(x, x);
-                    const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sB + k * NP + n0);
-                    hs[k + 1][0] = fma2(exp2_2(mul2(dt2, A01)), hs[k][0], mul2(x2, b.x));
-                    hs[k + 1][1] = fma2(exp2_2(mul2(dt2, A23)), hs[k][1], mul2(x2, b.y));
-                    if (z) {
-                        const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sC + k * NP + n0);
-                        float lo, hi;
-                        unpack2(fma2(cv.y, hs[k + 1][1], mul2(cv.x, hs[k + 1][0])), lo, hi);
-                        yv[k] = lo + hi;
-                    }
-                }
-            }
-            if (z) sum_states<LPC>(yv, sy + ch * LD, q, lane, 1.0f);
-        }
-        float qv[TS], rv[TS];
-        f32x2 t01 = 0, t23 = 0;   // the tile's dA
-#pragma unroll
-        for (int k = TS - 1; k >= 0; --k) {
-            qv[k] = rv[k] = 0.0f;
-            if (k < cnt) {
-                const float dt = sdt[ch * LD + k], x = sx[ch * LD + k], dy = sdy[ch * LD + k];
-                const f32x2 dt2 = pack2(dt, dt), x2 = pack2(x, x), dy2 = pack2(dy, dy);
-                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sB + k * NP + n0);
-                const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sC + k * NP + n0);
-                const f32x2 g01 = fma2(cv.x, dy2, c01), g23 = fma2(cv.y, dy2, c23);
-                float lo, hi, v[8];
-                unpack2(fma2(g23, b.y, mul2(g01, b.x)), lo, hi);
-                qv[k] = lo + hi;
-                unpack2(mul2(g01, x2), v[0], v[1]);
-                unpack2(mul2(g23, x2), v[2], v[3]);
-                unpack2(mul2(dy2, hs[k + 1][0]), v[4], v[5]);
-                unpack2(mul2(dy2, hs[k + 1][1]), v[6], v[7]);
-                c01 = mul2(g01, exp2_2(mul2(dt2, A01)));
-                c23 = mul2(g23, exp2_2(mul2(dt2, A23)));
-                const f32x2 e01 = mul2(c01, hs[k][0]), e23 = mul2(c23, hs[k][1]);
-                unpack2(fma2(e23, A23, mul2(e01, A01)), lo, hi);
-                rv[k] = lo + hi;
-                t01 = fma2(e01, dt2, t01);
-                t23 = fma2(e23, dt2, t23);
-                // sum over the warp's channels: lanes that differ in the bits LPC .. 16
-                float* dst = sred + ((warp * TS + k) * 2) * NP + n0;
-                if constexpr (RC == 8) {
-                    float s = reduce_scatter<8, LPC>(v, lane);
-#pragma unroll
-                    for (int m = 8 * LPC; m < 32; m *= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
-                    const int i = (lane / LPC) % 8;
-                    if (lane < 8 * LPC) dst[(i / 4) * NP + i % 4] = s;
-                } else {
-                    // fewer lanes than sums: every lane halves its set until RC lanes hold VL each
-#pragma unroll
-                    for (int m = 4, half = RC / 2; half >= 1; m /= 2, half /= 2) {
-                        const bool hi_half = lane & (half * LPC);
-#pragma unroll
-                        for (int i = 0; i < m; ++i) {
-                            const float send = hi_half ? v[i] : v[i + m];
-                            const float keep = hi_half ? v[i + m] : v[i];
-                            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, half * LPC);
-                        }
-                    }
-                    const int first = (lane / LPC) % RC * VL;
-#pragma unroll
-                    for (int i = 0; i < VL; ++i) dst[((first + i) / 4) * NP + (first + i) % 4] = v[i];
-                }
-            }
-        }
-        {
-            float td[4];
-            unpack2(t01, td[0], td[1]);
-            unpack2(t23, td[2], td[3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) add_exactly(dA[i], eA[i], td[i]);
-        }
-        sum_states<LPC>(qv, sq + ch * LD, q, lane, 1.0f);
-        sum_states<LPC>(rv, sr + ch * LD, q, lane, kLn2);
-        __syncthreads();
-        float tD = 0.0f, tb = 0.0f;
-#pragma unroll
-        for (int k = 0; k < I; ++k) {
-            const int it = tid + k * kThreads, ic = it % CH, t4 = it / CH * 4;
-            if (it >= CH * (TS / 4) || ic >= w.nch) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t4 + i >= cnt) continue;
-                const int64_t o = (row0 + at + t4 + i) * f.D + w.c0 + ic;
-                const int m = ic * LD + t4 + i;
-                const float dy = sdy[m], gq = sq[m];
-                p.du[o] = from_float<T>(fmaf(gq, sdt[m], Dw[k] * dy));
-                const float dd = fmaf(gq, ku[k][i], sr[m]) * ks[k][i];
-                p.ddelta[o] = from_float<T>(dd);
-                tD = fmaf(dy, ku[k][i], tD);
-                tb += dd;
-                if (p.dz) p.dz[o] = from_float<T>(kz[k][i] * fmaf(Dw[k], ku[k][i], sy[m]));
-            }
-        }
-        add_exactly(dD, eD, tD);
-        add_exactly(db, eb, tb);
-        for (int i = tid; i < cnt * 2 * NP; i += kThreads) {
-            const int n = i % NP, which = i / NP % 2, k = i / (2 * NP);
-            if (n >= f.N) continue;
-            float s = 0.0f;
-#pragma unroll
-            for (int v = 0; v < kThreads / 32; ++v) s += sred[((v * TS + k) * 2 + which) * NP + n];
-            p.pBC[(((int64_t)which * f.ntile + tile) * rows + row0 + at + k) * f.G * f.N + w.g * f.N + n] = s;
-        }
-        __syncthreads();
-    }
-    // sums over the tokens: dA by its own lane, dD and dbias over the threads of a channel
-    if (live) {
-        unpack2(c01, carry[0], carry[1]);
-        unpack2(c23, carry[2], carry[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n0 + i < f.N) {
-                p.pA[w.s * DN + cn + i] = dA[i];
-                if (p.dh0) p.dh0[w.s * DN + cn + i] = carry[i];
-            }
-    }
-    if (CH >= kThreads) {
-        if (tid < w.nch) {
-            p.pD[(int64_t)w.s * f.D + w.c0 + tid] = dD;
-            p.pb[(int64_t)w.s * f.D + w.c0 + tid] = db;
-        }
-    } else {
-        sred[tid] = dD;   // read last before the loop's final barrier
-        sred[kThreads + tid] = db;
-        __syncthreads();
-        if (tid < w.nch) {
-            float a = 0.0f, b = 0.0f;
-            for (int k = tid; k < kThreads; k += CH) { a += sred[k]; b += sred[kThreads + k]; }
-            p.pD[(int64_t)w.s * f.D + w.c0 + tid] = a;
-            p.pb[(int64_t)w.s * f.D + w.c0 + tid] = b;
-        }
-    }
+    for (int k = y; k < 32; k += 8)
+        if (r0 + k < rows && c0 + x < cols) out[(r0 + k) * cols + c0 + x] = from_float<T>(s[x][k]);
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -344,59 +506,48 @@ struct GradWs {
     int64_t bc, a, d, b, total;   // float offsets
 };
 GradWs grad_ws(const pe_scan_args* a) {
-    const int64_t ch = kThreads / lanes_for(a->states), dg = a->channels / a->groups;
     const int64_t rows = a->tokens * (a->cu ? 1 : a->nseq);
     GradWs w;
     w.bc = 0;
-    w.a = 2 * ceil_div(dg, ch) * rows * a->groups * a->states;
+    w.a = 2 * ceil_div(a->channels / a->groups, CB) * rows * a->groups * a->states;
     w.d = w.a + a->nseq * a->channels * a->states;
     w.b = w.d + a->nseq * a->channels;
     w.total = w.b + a->nseq * a->channels;
     return w;
 }
 
-template <typename T, int LPC>
-int grad_run(const pe_scan_grad_args* a, cudaStream_t s) {
-    constexpr int CH = kThreads / LPC;
+template <typename T>
+int grad_type(const pe_scan_grad_args* a, cudaStream_t s) {
     const pe_scan_args* f = &a->fwd;
     GradP<T> p;
-    p.f = scan_params<T>(f, CH);
+    p.f = scan_params<T>(f, CB, GradSmem<T>::NC);
     const GradWs w = grad_ws(f);
     float* ws = (float*)a->ws;
     p.dout = (const T*)a->dout; p.o_sb = a->dout_sb; p.o_st = a->dout_st;
+    p.o_cb = chunk_of(p.dout, sizeof(T), CB * sizeof(T), {p.o_sb, p.o_st, CB}, p.f.G > 1 ? p.f.Dg : CB);
     p.dstate = a->dstate;
     p.du = (T*)a->du; p.ddelta = (T*)a->ddelta; p.dz = (T*)a->dz;
     p.dh0 = a->dh0;
     p.pBC = ws + w.bc; p.pA = ws + w.a; p.pD = ws + w.d; p.pb = ws + w.b;
     unsigned grid;
     if (int rc = grid_of((int64_t)p.f.seqs.nseq * p.f.G * p.f.ntile, &grid)) return rc;
-    // every sequence is one piece here, numbered by itself
-    const int smem = (6 * CH * LD + (2 + 2 * kThreads / 32) * TS * 4 * LPC) * 4;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(scan_bwd<T, LPC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return PE_ERR_CUDA;
-    }
-    if (grid) {
-        scan_bwd<T, LPC><<<grid, kThreads, smem, s>>>(p);
+    if (grid)   // every sequence is one piece here, numbered by itself
+        if (int rc = launch(scan_bwd<T>, p, grid, sizeof(GradSmem<T>) + 4 * p.f.N * CB * 4, s)) return rc;
+    const int64_t rows = f->tokens * (f->cu ? 1 : f->nseq), cols = f->groups * f->states;
+    if (rows) {
+        if (ceil_div(rows, 32) > 0x7fffffffll || ceil_div(cols, 32) > 65535) return PE_ERR_UNSUPPORTED;
+        const dim3 blocks((unsigned)ceil_div(rows, 32), (unsigned)ceil_div(cols, 32), 2);
+        sum_tiles<T><<<blocks, 256, 0, s>>>(p.pBC, p.f.ntile, rows, (int)cols, (T*)a->dB, (T*)a->dC);
         count_launch();
         if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
-    const int64_t rows = f->tokens * (f->cu ? 1 : f->nseq), cols = rows * f->groups * f->states;
-    const int64_t DN = f->channels * f->states;
-    int rc = sum_rows(p.pBC, p.f.ntile, cols, (int)f->dtype, a->dB, s);
-    if (!rc) rc = sum_rows(p.pBC + p.f.ntile * cols, p.f.ntile, cols, (int)f->dtype, a->dC, s);
-    if (!rc) rc = sum_rows(p.pA, f->nseq, DN, PE_F32, a->dA, s);
+    int rc = sum_rows(p.pA, f->nseq, f->channels * f->states, PE_F32, a->dA, s);
     if (!rc && a->dD) rc = sum_rows(p.pD, f->nseq, f->channels, PE_F32, a->dD, s);
     if (!rc && a->ddelta_bias) rc = sum_rows(p.pb, f->nseq, f->channels, PE_F32, a->ddelta_bias, s);
     return rc;
 }
 
-template <typename T>
-int grad_lanes(const pe_scan_grad_args* a, cudaStream_t s) {
-    PE_LANES(grad_run, lanes_for(a->fwd.states), a, s)
-}
-
-int grad_any(const pe_scan_grad_args* a, cudaStream_t s) { PE_TYPES(grad_lanes, a->fwd.dtype, a, s) }
+int grad_any(const pe_scan_grad_args* a, cudaStream_t s) { PE_TYPES(grad_type, a->fwd.dtype, a, s) }
 
 }  // namespace
 
