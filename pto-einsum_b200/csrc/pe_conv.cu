@@ -32,13 +32,18 @@ struct ConvP {
 template <typename T, int W, int V>
 struct Filter {
     float w[W][V], b[V];
+    // weight [C][W]: the V channels' taps are V W consecutive elements, W loads
     __device__ __forceinline__ void load(const T* weight, const T* bias, int64_t c) {
+        Vec<T, V> r[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) r[k] = load_vec<T, V>(weight + c * W + k * V);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
+            b[v] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < W; ++k) w[k][v] = to_float(__ldg(weight + (c + v) * W + k));
-            b[v] = bias ? to_float(__ldg(bias + c + v)) : 0.0f;
+            for (int k = 0; k < W; ++k) w[k][v] = to_float(r[(v * W + k) / V].v[(v * W + k) % V]);
         }
+        if (bias) unpack(load_vec<T, V>(bias + c), b);
     }
 };
 
@@ -59,7 +64,7 @@ __device__ __forceinline__ void load_before(const ConvP<T>& p, const T* xs, int6
 }
 
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(kBlock) conv_fwd(const __grid_constant__ ConvP<T> p) {
+__global__ void __launch_bounds__(kBlock, 2) conv_fwd(const __grid_constant__ ConvP<T> p) {
     if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.seqs, threadIdx.x, kSiteOffsets);
     int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
     const int64_t tile = id / p.CV, c = (id - tile * p.CV) * V;
@@ -89,30 +94,30 @@ __global__ void __launch_bounds__(kBlock) conv_fwd(const __grid_constant__ ConvP
         T* o = p.out + sp.row * p.seqs.tokens * p.C + c;
         float win[W][V];
         load_before<T, W, V>(p, xr - c + sp.start * p.x_st, t - sp.start, s, c, win);
-        for (; t < stop; t += U) {
+        auto token = [&](const Vec<T, V>& raw, T* to) {
+            unpack(raw, win[W - 1]);
+            float y[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float a = f.b[v];
+#pragma unroll
+                for (int k = 0; k < W; ++k) a = fmaf(f.w[k][v], win[k][v], a);
+                y[v] = p.silu ? a * sigmoidf(a) : a;
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) win[k][v] = win[k + 1][v];
+            }
+            store_vec(to, pack<T, V>(y));
+        };
+        const T* xt = xr + t * p.x_st;
+        T* ot = o + t * p.C;
+        for (; t + U <= stop; t += U, xt += U * p.x_st, ot += U * p.C) {
             Vec<T, V> raw[U];
 #pragma unroll
-            for (int i = 0; i < U; ++i)
-                if (t + i < stop) raw[i] = load_vec<T, V>(xr + (t + i) * p.x_st);
+            for (int i = 0; i < U; ++i) raw[i] = load_vec<T, V>(xt + i * p.x_st);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (t + i < stop) {
-                    unpack(raw[i], win[W - 1]);
-                    float y[V];
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        float a = f.b[v];
-#pragma unroll
-                        for (int k = 0; k < W; ++k) a = fmaf(f.w[k][v], win[k][v], a);
-                        y[v] = p.silu ? a * sigmoidf(a) : a;
-#pragma unroll
-                        for (int k = 0; k < W - 1; ++k) win[k][v] = win[k + 1][v];
-                    }
-                    store_vec(o + (t + i) * p.C, pack<T, V>(y));
-                }
-            }
+            for (int i = 0; i < U; ++i) token(raw[i], ot + i * p.C);
         }
-        t = stop;
+        for (; t < stop; ++t, xt += p.x_st, ot += p.C) token(load_vec<T, V>(xt), ot);
     }
 }
 
@@ -128,7 +133,7 @@ struct ConvGradP {
 };
 
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(kBlock) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
+__global__ void __launch_bounds__(kBlock, 2) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
     __shared__ float red[(W + 1) * V * kBlock];
     const ConvP<T>& f = p.f;
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) check_offsets(f.seqs, threadIdx.x, kSiteOffsets);
@@ -165,11 +170,45 @@ __global__ void __launch_bounds__(kBlock) conv_bwd(const __grid_constant__ ConvG
             // g of the tokens t .. stop + W - 2 gives dx of t .. stop - 1 (and of the
             // inputs before the sequence where t starts it)
             const int64_t last = stop + W - 1;
-            for (int64_t k0 = t; k0 < last; k0 += U) {
+            // a token's g, into the sums if it is the tile's own
+            auto slope = [&](const Vec<T, V>& rx, const Vec<T, V>& ro, bool own) {
+                unpack(rx, win[W - 1]);
+                unpack(ro, g[W - 1]);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (f.silu) {
+                        float a = flt.b[v];
+#pragma unroll
+                        for (int q = 0; q < W; ++q) a = fmaf(flt.w[q][v], win[q][v], a);
+                        g[W - 1][v] *= silu_slope(a, sigmoidf(a));
+                    }
+                    if (own) {
+                        db[v] += g[W - 1][v];
+#pragma unroll
+                        for (int q = 0; q < W; ++q) dw[q][v] = fmaf(g[W - 1][v], win[q][v], dw[q][v]);
+                    }
+#pragma unroll
+                    for (int q = 0; q < W - 1; ++q) win[q][v] = win[q + 1][v];
+                }
+            };
+            auto sum_taps = [&](float (&d)[V]) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    d[v] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) d[v] = fmaf(flt.w[W - 1 - j][v], g[j][v], d[v]);
+#pragma unroll
+                    for (int q = 0; q < W - 1; ++q) g[q][v] = g[q + 1][v];
+                }
+            };
+            // U tokens from k0 on: their g, and dx of the inputs W - 1 earlier, whose sums they
+            // complete. Some may lie past the last one, and some inputs before the tile.
+            auto any = [&](int64_t k0) {
                 Vec<T, V> rx[U], ro[U];
+                const int64_t have = min(last, fin);
 #pragma unroll
                 for (int i = 0; i < U; ++i)
-                    if (k0 + i < min(last, fin)) {
+                    if (k0 + i < have) {
                         rx[i] = load_vec<T, V>(xr + (k0 + i) * f.x_st);
                         ro[i] = load_vec<T, V>(dor + (k0 + i) * p.o_st);
                     }
@@ -178,54 +217,45 @@ __global__ void __launch_bounds__(kBlock) conv_bwd(const __grid_constant__ ConvG
                     const int64_t k = k0 + i;
                     if (k >= last) break;
                     if (k < fin) {
-                        unpack(rx[i], win[W - 1]);
-                        unpack(ro[i], g[W - 1]);
-#pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            if (f.silu) {
-                                float a = flt.b[v];
-#pragma unroll
-                                for (int q = 0; q < W; ++q) a = fmaf(flt.w[q][v], win[q][v], a);
-                                g[W - 1][v] *= silu_slope(a, sigmoidf(a));
-                            }
-                            if (k < stop) {
-                                db[v] += g[W - 1][v];
-#pragma unroll
-                                for (int q = 0; q < W; ++q) dw[q][v] = fmaf(g[W - 1][v], win[q][v], dw[q][v]);
-                            }
-#pragma unroll
-                            for (int q = 0; q < W - 1; ++q) win[q][v] = win[q + 1][v];
-                        }
+                        slope(rx[i], ro[i], k < stop);
                     } else {
 #pragma unroll
                         for (int v = 0; v < V; ++v) g[W - 1][v] = 0.0f;
                     }
-                    const int64_t i0 = k - (W - 1);          // the input whose sum is complete
-                    const int64_t pos = i0 - sp.start;
-                    if (i0 >= t || (pos < 0 && t == sp.start && p.dinit)) {
-                        float d[V];
+                    float d[V];
+                    sum_taps(d);
+                    const int64_t i0 = k - (W - 1), pos = i0 - sp.start;
+                    const bool first = pos < 0 && t == sp.start && p.dinit;   // an input before the sequence
+                    if (i0 < t && !first) continue;
+                    const int64_t j = pos + W - 1 - sp.len;                    // its place in the last state
+                    if (p.dstate && j >= 0) {
+                        float e[V];
+                        unpack(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
 #pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            d[v] = 0.0f;
-#pragma unroll
-                            for (int j = 0; j < W; ++j) d[v] = fmaf(flt.w[W - 1 - j][v], g[j][v], d[v]);
-                        }
-                        const int64_t j = pos + W - 1 - sp.len;  // its place in the last state
-                        if (p.dstate && j >= 0) {
-                            float e[V];
-                            unpack(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
-#pragma unroll
-                            for (int v = 0; v < V; ++v) d[v] += e[v];
-                        }
-                        if (i0 >= t)
-                            store_vec(dx + i0 * f.C, pack<T, V>(d));
-                        else
-                            store_vec(p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c, pack<T, V>(d));
+                        for (int v = 0; v < V; ++v) d[v] += e[v];
                     }
+                    T* to = first ? p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c : dx + i0 * f.C;
+                    store_vec(to, pack<T, V>(d));
+                }
+            };
+#pragma unroll 1
+            for (int64_t k = t; k < last; k += U) {
+                if (k == t || k + U > stop) {
+                    any(k);
+                    continue;
+                }
+                Vec<T, V> rx[U], ro[U];
 #pragma unroll
-                    for (int q = 0; q < W - 1; ++q)
+                for (int i = 0; i < U; ++i) {
+                    rx[i] = load_vec<T, V>(xr + (k + i) * f.x_st);
+                    ro[i] = load_vec<T, V>(dor + (k + i) * p.o_st);
+                }
 #pragma unroll
-                        for (int v = 0; v < V; ++v) g[q][v] = g[q + 1][v];
+                for (int i = 0; i < U; ++i) {
+                    slope(rx[i], ro[i], true);
+                    float d[V];
+                    sum_taps(d);
+                    store_vec(dx + (k + i - (W - 1)) * f.C, pack<T, V>(d));
                 }
             }
             t = stop;
@@ -344,13 +374,21 @@ ConvP<T> conv_params(const pe_conv_args* a, int v, int64_t tile) {
     return p;
 }
 
-// Tokens a thread walks in the forward pass.
-int64_t fwd_tile(const pe_conv_args*) { return 16; }
-constexpr int64_t kBwdTile = 16;
+// Tokens a thread walks in the forward pass: as many as leave two warps' worth of loads
+// to every scheduler (the W - 1 tokens read again and the filter weigh less on a longer
+// walk), 4 to 32.
+int64_t fwd_tile(const pe_conv_args* a, int v) {
+    const int64_t cells = a->tokens * a->batch * (a->channels / v), want = (int64_t)num_sms() * 1536;
+    int64_t tile = 4;
+    while (tile < 32 && cells / (2 * tile) >= want) tile *= 2;
+    return tile;
+}
+// Backward, tokens a thread; the block's threads along the tokens add up their sums.
+constexpr int64_t kBwdTile = 32;
 
 template <typename T, int W, int V>
 int conv_run(const pe_conv_args* a, cudaStream_t s) {
-    const ConvP<T> p = conv_params<T>(a, V, fwd_tile(a));
+    const ConvP<T> p = conv_params<T>(a, V, fwd_tile(a, V));
     const int64_t ids = (p.tiles + (p.state ? a->nseq : 0)) * p.CV, blocks = ceil_div(ids, kBlock);
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     if (!blocks) return PE_OK;
@@ -396,9 +434,9 @@ int conv_grad_run(const pe_conv_grad_args* g, cudaStream_t s) {
         count_launch();
         if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
-    int rc = sum_rows(p.pw, sh.rows, a->channels * W, (int)a->dtype, g->dweight, s);
-    if (!rc && g->dbias) rc = sum_rows(p.pb, sh.rows, a->channels, (int)a->dtype, g->dbias, s);
-    return rc;
+    const SumJob sums[2] = {{p.pw, sh.rows, a->channels * W, (int)a->dtype, g->dweight},
+                            {p.pb, sh.rows, a->channels, (int)a->dtype, g->dbias}};
+    return sum_rows(sums, 2, s);
 }
 
 template <typename T, int W, int V>
@@ -436,14 +474,20 @@ int conv_step_w(const pe_conv_step_args* a, cudaStream_t s) { PE_CONV_W(conv_ste
         default: return vec ? F<__nv_bfloat16, 8>(__VA_ARGS__) : F<__nv_bfloat16, 1>(__VA_ARGS__);  \
     }
 int conv_any(const pe_conv_args* a, bool vec, cudaStream_t s) { PE_CONV_T(conv_w, a->dtype, vec, a, s) }
+// The backward pass keeps 2 (W + 1) sums and taps a channel besides two windows: four
+// channels a thread in every type.
 int conv_grad_any(const pe_conv_grad_args* a, bool vec, cudaStream_t s) {
-    PE_CONV_T(conv_grad_w, a->fwd.dtype, vec, a, s)
+    switch (a->fwd.dtype) {
+        case PE_F32: return vec ? conv_grad_w<float, 4>(a, s) : conv_grad_w<float, 1>(a, s);
+        case PE_F16: return vec ? conv_grad_w<__half, 4>(a, s) : conv_grad_w<__half, 1>(a, s);
+        default: return vec ? conv_grad_w<__nv_bfloat16, 4>(a, s) : conv_grad_w<__nv_bfloat16, 1>(a, s);
+    }
 }
 int conv_step_any(const pe_conv_step_args* a, bool vec, cudaStream_t s) { PE_CONV_T(conv_step_w, a->dtype, vec, a, s) }
 
 bool grad_wide(const pe_conv_grad_args* g) {
     const pe_conv_args* a = &g->fwd;
-    return wide(a->dtype, a->channels, {a->x, a->init, g->dout, g->dstate, g->dx, g->dinit},
+    return wide(a->dtype, a->channels, {a->x, a->weight, a->bias, a->init, g->dout, g->dstate, g->dx, g->dinit},
                 {a->x_sb, a->x_st, g->dout_sb, g->dout_st});
 }
 
@@ -452,13 +496,13 @@ bool grad_wide(const pe_conv_grad_args* g) {
 int causal_conv(const pe_conv_args* a, cudaStream_t s) {
     if (int rc = check_conv(a)) return rc;
     if (a->tokens && a->batch && !a->out) return PE_ERR_INVALID;
-    return conv_any(a, wide(a->dtype, a->channels, {a->x, a->init, a->out, a->state}, {a->x_sb, a->x_st}), s);
+    return conv_any(a, wide(a->dtype, a->channels, {a->x, a->weight, a->bias, a->init, a->out, a->state}, {a->x_sb, a->x_st}), s);
 }
 
 int64_t conv_grad_ws_bytes(const pe_conv_grad_args* g) {
     if (!g || check_conv(&g->fwd) != PE_OK) return 0;
     const pe_conv_args* a = &g->fwd;
-    return grad_shape(a, grad_wide(g) ? 16 / elem_bytes(a->dtype) : 1).rows * a->channels * (a->width + 1) * 4;
+    return grad_shape(a, grad_wide(g) ? 4 : 1).rows * a->channels * (a->width + 1) * 4;
 }
 
 int causal_conv_grad(const pe_conv_grad_args* g, cudaStream_t s) {
@@ -476,7 +520,7 @@ int causal_conv_step(const pe_conv_step_args* a, cudaStream_t s) {
         return PE_ERR_INVALID;
     if (a->batch == 0) return PE_OK;
     if (!a->x || !a->weight || !a->state || !a->out) return PE_ERR_INVALID;
-    return conv_step_any(a, wide(a->dtype, a->channels, {a->x, a->state, a->out}, {a->x_sb}), s);
+    return conv_step_any(a, wide(a->dtype, a->channels, {a->x, a->weight, a->bias, a->state, a->out}, {a->x_sb}), s);
 }
 
 int conv_device_error(bool clear) {

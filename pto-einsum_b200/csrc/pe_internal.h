@@ -41,8 +41,15 @@ int contract_cached(void* cache, const pe_contract_plan* plan, const void* in0, 
 int gemm_device_error(bool clear);
 int wait_timeout_selftest(uint64_t timeout_ns, cudaStream_t s);
 
-// out[c] = sum over r < rows of part[r][c], rounded to dtype; a fixed order of additions.
-int sum_rows(const float* part, int64_t rows, int64_t cols, int dtype, void* out, cudaStream_t s);
+// out[c] = sum over r < rows of part[r][c], rounded to dtype, in a fixed order of
+// additions; up to three at once, those without an `out` left out.
+struct SumJob {
+    const float* part;
+    int64_t rows, cols;
+    int dtype;
+    void* out;
+};
+int sum_rows(const SumJob* jobs, int count, cudaStream_t s);
 
 // Recurrent-mixer operators.
 int64_t scan_ckpt_floats(int64_t tokens, int64_t nseq, int64_t packed, int64_t channels, int64_t states);

@@ -21,7 +21,7 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// V elements that one load moves (V * sizeof(T) is 16 bytes, or V is 1).
+// V elements that one load moves (V * sizeof(T) is 16 or 8 bytes, or V is 1).
 template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {
     T v[V];
@@ -31,8 +31,11 @@ __device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
     if constexpr (V * sizeof(T) == 16) {
         const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
         return *reinterpret_cast<const Vec<T, V>*>(&r);
+    } else if constexpr (V * sizeof(T) == 8) {
+        const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
+        return *reinterpret_cast<const Vec<T, V>*>(&r);
     } else {
-        static_assert(V == 1, "16 bytes or one element");
+        static_assert(V == 1, "16 or 8 bytes, or one element");
         Vec<T, V> r;
         r.v[0] = __ldg(p);
         return r;

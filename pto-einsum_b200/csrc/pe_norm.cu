@@ -5,8 +5,8 @@
 //   g = d out / d v . dout,  dw = sum g xn,  db = sum g,
 //   dx = rstd (g w - mean(g w) - xn mean(g w xn))          (means over the group)
 //
-// Bound by memory. A group of up to 1024 loads (16 bytes each where the layout
-// allows) stays in the registers of the lanes that share it: one read of x, two-pass
+// Bound by memory. A group of up to 1024 loads (512 backward; 16 bytes each where
+// the layout allows) stays in the registers of the lanes that share it: one read of x, two-pass
 // statistics. A larger one goes over the tensor twice: per-channel sums of row chunks,
 // their combination, then the result; the second read comes from L2 while the tensor
 // fits there. Variances are never formed as a difference of large squares: two passes
@@ -64,72 +64,100 @@ __device__ __forceinline__ void group_sum(float (&v)[NV], int L, float* red) {
     }
 }
 
-// Item i of a group: place i / per, channel vector i % per (per = vectors a place).
-template <int V>
-struct Item {
-    bool in;
-    int64_t place;
-    int64_t c;
-    __device__ __forceinline__ Item(int i, int per, int items, int c0) {
-        in = i < items;
-        place = i / per;
-        c = c0 + (i - (int)place * per) * V;
+// Blocks an SM holds of the kernels below, by loads a lane.
+__host__ __device__ constexpr int reg_blocks(int k, bool grad) {
+    return grad ? (k == 1 ? 2 : 1) : k == 1 ? 3 : k == 2 ? 2 : 1;
+}
+
+// The items of a lane: item i of a group is channel vector i % per of place i / per.
+template <int V, int K>
+struct Items {
+    bool in[K];
+    int place[K], c[K];
+    __device__ __forceinline__ Items(int l, int L, int per, int items, int c0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = l + k * L;
+            in[k] = i < items;
+            place[k] = in[k] ? i / per : 0;
+            c[k] = in[k] ? c0 + (i - place[k] * per) * V : 0;
+        }
     }
 };
 
+// L lanes share a group and take its rows r, r + R, ...; the next row's loads are on the
+// way while the current one is reduced. All lanes make the same number of rounds, for
+// the shuffles take all of them.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kBlock) norm_reg(const __grid_constant__ NormP<T> p, int L, int64_t units) {
+__global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const __grid_constant__ NormP<T> p, int L, int R) {
     __shared__ float red[8];
-    const int64_t unit = ((int64_t)blockIdx.x * kBlock + threadIdx.x) / L;
-    const int l = threadIdx.x % L;
-    const bool live = unit < units;     // lanes past the end still take part in the shuffles
-    const int64_t n = live ? unit / p.G : 0;
-    const int g = live ? (int)(unit - n * p.G) : 0, c0 = g * p.cg;
-    const int per = p.cg / V, items = live ? per * (int)p.S : 0;
-    const float inv = 1.0f / (float)((int64_t)p.cg * p.S);
-    float x[K][V];
-    float sum[1] = {0.0f};
+    const int unit = (int)(((int64_t)blockIdx.x * kBlock + threadIdx.x) / L), l = threadIdx.x % L;
+    const bool live = unit / p.G < R;
+    const int r = live ? unit / p.G : 0, g = live ? unit % p.G : 0;
+    const int per = p.cg / V;
+    const Items<V, K> it(l, L, per, live ? per * (int)p.S : 0, g * p.cg);
+    const float inv = 1.0f / (float)(p.cg * (int)p.S);
+    int64_t xo[K], go[K];
+    Vec<T, V> w[K], b[K], x[K], z[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const Item<V> it(l + k * L, per, items, c0);
-        if (it.in) unpack(load_vec<T, V>(p.x + n * p.x_sb + it.place * p.x_sp + it.c), x[k]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[0] += it.in ? x[k][v] : 0.0f;
+        xo[k] = it.place[k] * p.x_sp + it.c[k];
+        go[k] = it.place[k] * p.g_sp + it.c[k];
+        if (it.in[k] && p.w) w[k] = load_vec<T, V>(p.w + it.c[k]);
+        if (it.in[k] && p.b) b[k] = load_vec<T, V>(p.b + it.c[k]);
     }
-    group_sum(sum, L, red);
-    const float mean = sum[0] * inv;
-    sum[0] = 0.0f;
+    auto load = [&](int64_t n) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k)
+            if (it.in[k] && n < p.N) {
+                x[k] = load_vec<T, V>(p.x + n * p.x_sb + xo[k]);
+                if (p.mode == kGate) z[k] = load_vec<T, V>(p.gate + n * p.g_sb + go[k]);
+            }
+    };
+    load(r);
+    for (int64_t n0 = 0; n0 < p.N; n0 += R) {
+        const int64_t n = n0 + r;
+        const bool on = n < p.N;
+        float f[K][V], ga[K][V], sum[1] = {0.0f};
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float d = x[k][v] - mean;
-            sum[0] += l + k * L < items ? d * d : 0.0f;
+        for (int k = 0; k < K; ++k) {
+            unpack(x[k], f[k]);
+            if (p.mode == kGate) unpack(z[k], ga[k]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[0] += it.in[k] ? f[k][v] : 0.0f;
         }
-    group_sum(sum, L, red);
-    const float rstd = rsqrtf(sum[0] * inv + p.eps);
-    if (!live) return;
-    if (l == 0 && p.mean) {
-        p.mean[unit] = mean;
-        p.rstd[unit] = rstd;
-    }
+        load(n + R);
+        group_sum(sum, L, red);
+        const float mean = sum[0] * inv;
+        sum[0] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const Item<V> it(l + k * L, per, items, c0);
-        if (!it.in) continue;
-        float w[V], b[V], y[V], ga[V];
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int v = 0; v < V; ++v) w[v] = 1.0f, b[v] = 0.0f;
-        if (p.w) unpack(load_vec<T, V>(p.w + it.c), w);
-        if (p.b) unpack(load_vec<T, V>(p.b + it.c), b);
-        if (p.mode == kGate) unpack(load_vec<T, V>(p.gate + n * p.g_sb + it.place * p.g_sp + it.c), ga);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            y[v] = fmaf((x[k][v] - mean) * rstd, w[v], b[v]);
-            if (p.mode == kSilu) y[v] *= sigmoidf(y[v]);
-            if (p.mode == kGate) y[v] *= ga[v] * sigmoidf(ga[v]);
+            for (int v = 0; v < V; ++v) {
+                f[k][v] -= mean;
+                sum[0] += it.in[k] ? f[k][v] * f[k][v] : 0.0f;
+            }
+        group_sum(sum, L, red);
+        const float rstd = rsqrtf(sum[0] * inv + p.eps);
+        if (!live || !on) continue;
+        if (l == 0 && p.mean) {
+            p.mean[n * p.G + g] = mean;
+            p.rstd[n * p.G + g] = rstd;
         }
-        store_vec(p.out + (n * p.S + it.place) * p.C + it.c, pack<T, V>(y));
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (!it.in[k]) continue;
+            float y[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                y[v] = f[k][v] * rstd;
+                if (p.w) y[v] *= to_float(w[k].v[v]);
+                if (p.b) y[v] += to_float(b[k].v[v]);
+                if (p.mode == kSilu) y[v] *= sigmoidf(y[v]);
+                if (p.mode == kGate) y[v] *= ga[k][v] * sigmoidf(ga[k][v]);
+            }
+            store_vec(p.out + (n * p.S + it.place[k]) * p.C + it.c[k], pack<T, V>(y));
+        }
     }
 }
 
@@ -151,81 +179,93 @@ __device__ __forceinline__ void through_act(int mode, const float (&xn)[V], cons
     }
 }
 
-// A group of lanes takes rows r, r + R, ... of one group of channels and keeps the sums
-// of g xn and g of its own channels: pw, pb [R][C]. One place a row (S = 1).
+// L lanes take rows r, r + R, ... of one group of channels (one place a row) and keep the
+// sums of g xn and g of their own channels: pw, pb [R][C].
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kBlock) norm_reg_bwd(const __grid_constant__ NormP<T> p, int L, int64_t R, float* pw,
+__global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(const __grid_constant__ NormP<T> p, int L, int R, float* pw,
                                                        float* pb) {
     __shared__ float red[16];
-    const int64_t unit = ((int64_t)blockIdx.x * kBlock + threadIdx.x) / L;
-    const int l = threadIdx.x % L;
-    const bool live = unit < R * p.G;
-    const int64_t r = live ? unit / p.G : 0;
-    const int g = live ? (int)(unit - r * p.G) : 0, c0 = g * p.cg;
-    const int per = p.cg / V, items = live ? per : 0;
+    const int unit = (int)(((int64_t)blockIdx.x * kBlock + threadIdx.x) / L), l = threadIdx.x % L;
+    const bool live = unit / p.G < R;
+    const int r = live ? unit / p.G : 0, g = live ? unit % p.G : 0;
+    const int per = p.cg / V;
+    const Items<V, K> it(l, L, per, live ? per : 0, g * p.cg);
     const float inv = 1.0f / (float)p.cg;
-    float w[K][V], b[K][V], aw[K][V], ab[K][V];
+    float aw[K][V], ab[K][V];
+    Vec<T, V> w[K], b[K], x[K], z[K], o[K];
+    float mean = 0.0f, rstd = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const Item<V> it(l + k * L, per, items, c0);
 #pragma unroll
-        for (int v = 0; v < V; ++v) w[k][v] = 1.0f, b[k][v] = aw[k][v] = ab[k][v] = 0.0f;
-        if (it.in && p.w) unpack(load_vec<T, V>(p.w + it.c), w[k]);
-        if (it.in && p.b) unpack(load_vec<T, V>(p.b + it.c), b[k]);
+        for (int v = 0; v < V; ++v) {
+            aw[k][v] = ab[k][v] = 0.0f;
+            w[k].v[v] = from_float<T>(1.0f);
+            b[k].v[v] = from_float<T>(0.0f);
+        }
+        if (it.in[k] && p.w) w[k] = load_vec<T, V>(p.w + it.c[k]);
+        if (it.in[k] && p.b) b[k] = load_vec<T, V>(p.b + it.c[k]);
     }
-    // every lane of the warp (and, with L = kBlock, of the block) does as many rounds as
-    // the largest r needs: the shuffles take all lanes
-    const int64_t rounds = ceil_div(p.N, R);
-    for (int64_t i = 0; i < rounds; ++i) {
-        const int64_t n = r + i * R;
-        const bool on = live && n < p.N;
-        const float mean = on ? __ldg(p.mean + n * p.G + g) : 0.0f, rstd = on ? __ldg(p.rstd + n * p.G + g) : 0.0f;
-        float xn[K][V], go[K][V];
-        float sum[2] = {0.0f, 0.0f};
+    auto load = [&](int64_t n) {
+        if (n < p.N) {
+            mean = __ldg(p.mean + n * p.G + g);
+            rstd = __ldg(p.rstd + n * p.G + g);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (it.in[k] && n < p.N) {
+                x[k] = load_vec<T, V>(p.x + n * p.x_sb + it.c[k]);
+                o[k] = load_vec<T, V>(p.dout + n * p.o_sb + it.c[k]);
+                if (p.mode == kGate) z[k] = load_vec<T, V>(p.gate + n * p.g_sb + it.c[k]);
+            }
+    };
+    load(r);
+    for (int64_t n0 = 0; n0 < p.N; n0 += R) {
+        const int64_t n = n0 + r;
+        const bool on = n < p.N;
+        const float scale = rstd;
+        float xn[K][V], go[K][V], sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const Item<V> it(l + k * L, per, items, c0);
-#pragma unroll
-            for (int v = 0; v < V; ++v) xn[k][v] = go[k][v] = 0.0f;
-            if (!it.in || !on) continue;
-            float ga[V];
-            unpack(load_vec<T, V>(p.x + n * p.x_sb + it.place * p.x_sp + it.c), xn[k]);
-            unpack(load_vec<T, V>(p.dout + n * p.o_sb + it.place * p.o_sp + it.c), go[k]);
-            if (p.mode == kGate) unpack(load_vec<T, V>(p.gate + n * p.g_sb + it.place * p.g_sp + it.c), ga);
+            if (!it.in[k] || !on) continue;
+            float ga[V], wf[V], bf[V];
+            unpack(x[k], xn[k]);
+            unpack(o[k], go[k]);
+            unpack(w[k], wf);
+            unpack(b[k], bf);
+            if (p.mode == kGate) unpack(z[k], ga);
 #pragma unroll
             for (int v = 0; v < V; ++v) xn[k][v] = (xn[k][v] - mean) * rstd;
-            through_act<V>(p.mode, xn[k], w[k], b[k], go[k], ga);
-            if (p.mode == kGate) store_vec(p.dgate + (n * p.S + it.place) * p.C + it.c, pack<T, V>(ga));
+            through_act<V>(p.mode, xn[k], wf, bf, go[k], ga);
+            if (p.mode == kGate) store_vec(p.dgate + n * p.C + it.c[k], pack<T, V>(ga));
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 aw[k][v] = fmaf(go[k][v], xn[k][v], aw[k][v]);
                 ab[k][v] += go[k][v];
-                go[k][v] *= w[k][v];
+                go[k][v] *= wf[v];
                 sum[0] += go[k][v];
                 sum[1] = fmaf(go[k][v], xn[k][v], sum[1]);
             }
         }
+        load(n + R);
         group_sum(sum, L, red);
         const float m0 = sum[0] * inv, m1 = sum[1] * inv;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const Item<V> it(l + k * L, per, items, c0);
-            if (!it.in || !on) continue;
+            if (!it.in[k] || !on) continue;
             float d[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) d[v] = rstd * (go[k][v] - m0 - xn[k][v] * m1);
-            store_vec(p.dx + (n * p.S + it.place) * p.C + it.c, pack<T, V>(d));
+            for (int v = 0; v < V; ++v) d[v] = scale * (go[k][v] - m0 - xn[k][v] * m1);
+            store_vec(p.dx + n * p.C + it.c[k], pack<T, V>(d));
         }
     }
     if (!pw) return;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const Item<V> it(l + k * L, per, items, c0);
-        if (!it.in) continue;
+        if (!it.in[k]) continue;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            pw[r * p.C + it.c + v] = aw[k][v];
-            pb[r * p.C + it.c + v] = ab[k][v];
+            pw[(int64_t)r * p.C + it.c[k] + v] = aw[k][v];
+            pb[(int64_t)r * p.C + it.c[k] + v] = ab[k][v];
         }
     }
 }
@@ -254,7 +294,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kBlock) norm_stats(const __grid_constant__ NormP<T> p, Chunks q, float* part) {
     __shared__ float red[3][V][kBlock];
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
-    const int64_t n = blockIdx.x / q.chunks, chunk = blockIdx.x - n * q.chunks;
+    const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
     const int64_t s0 = chunk * q.rows, s1 = min(p.S, s0 + q.rows);
     float s[V], ss[V], pv[V];
@@ -337,7 +377,7 @@ struct Channel {
         if (p.b) unpack(load_vec<T, V>(p.b + c), b);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int64_t g = n * p.G + (c + v) / p.cg;
+            const int64_t g = n * p.G + (int)(c + v) / p.cg;
             mean[v] = __ldg(p.mean + g);
             rstd[v] = __ldg(p.rstd + g);
         }
@@ -347,7 +387,7 @@ struct Channel {
 template <typename T, int V>
 __global__ void __launch_bounds__(kBlock) norm_apply(const __grid_constant__ NormP<T> p, Chunks q) {
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
-    const int64_t n = blockIdx.x / q.chunks, chunk = blockIdx.x - n * q.chunks;
+    const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
     if (c >= p.C) return;
     const int64_t s0 = chunk * q.rows, s1 = min(p.S, s0 + q.rows);
@@ -372,7 +412,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kBlock) norm_sums(const __grid_constant__ NormP<T> p, Chunks q, float* part) {
     __shared__ float red[2][V][kBlock];
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
-    const int64_t n = blockIdx.x / q.chunks, chunk = blockIdx.x - n * q.chunks;
+    const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
     const int64_t s0 = chunk * q.rows, s1 = min(p.S, s0 + q.rows);
     float aw[V], ab[V];
@@ -453,7 +493,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kBlock) norm_apply_bwd(const __grid_constant__ NormP<T> p, Chunks q,
                                                          const float* gm) {
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
-    const int64_t n = blockIdx.x / q.chunks, chunk = blockIdx.x - n * q.chunks;
+    const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
     if (c >= p.C) return;
     const int64_t s0 = chunk * q.rows, s1 = min(p.S, s0 + q.rows);
@@ -461,7 +501,7 @@ __global__ void __launch_bounds__(kBlock) norm_apply_bwd(const __grid_constant__
     float m0[V], m1[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int64_t g = n * p.G + (c + v) / p.cg;
+        const int64_t g = n * p.G + (int)(c + v) / p.cg;
         m0[v] = __ldg(gm + 2 * g);
         m1[v] = __ldg(gm + 2 * g + 1);
     }
@@ -510,7 +550,7 @@ int vec_of(const pe_norm_args* a, std::initializer_list<const void*> more, std::
 struct Plan {
     int v;            // elements a load
     int lanes, k;     // groups in registers: lanes a group, loads a lane; lanes 0: too large for that
-    int64_t R;        // backward, in registers: rows of partial sums
+    int64_t R;        // in registers: rows at work, a lane takes every R-th
     Chunks q;
 };
 
@@ -520,9 +560,11 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
     const int vr = cg % vec == 0 ? vec : 1;      // in registers a load stays within its group
     const int64_t items = a->places <= 1024 ? cg / vr * a->places : 1 << 20;
     // the backward pass keeps sums a channel in registers, where an item is a channel vector
-    if (items <= 4 * kBlock && (!grad || a->places == 1)) {
+    // (two loads a lane at most: four need more registers than there are)
+    const int most = grad ? 2 : 4;
+    if (items <= most * kBlock && (!grad || a->places == 1)) {
         p.v = vr;
-        if (items <= 128) {
+        if (items <= 32 * most) {
             p.lanes = 1;
             while (p.lanes < 32 && p.lanes < items) p.lanes *= 2;
         } else {
@@ -530,9 +572,10 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
         }
         const int64_t k = ceil_div(items, p.lanes);
         p.k = k <= 1 ? 1 : k <= 2 ? 2 : 4;
-        // half of the SMs' threads, and rows of sums that stay small beside the tensor
-        const int64_t want = (int64_t)num_sms() * 1024 / p.lanes / a->groups;
-        p.R = a->batch < 1 ? 0 : a->batch < want ? a->batch : want < 1 ? 1 : want;
+        // rows of groups at work: one wave of blocks; each then takes further rows, so that
+        // its filter and its sums weigh less
+        const int64_t want = (int64_t)num_sms() * reg_blocks(p.k, grad) * kBlock / p.lanes / a->groups;
+        p.R = a->batch < want ? a->batch : want < 1 ? 1 : want;
         return p;
     }
     p.v = vec;
@@ -574,11 +617,11 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
     NormP<T> p = norm_params<T>(a);
     const int64_t units = p.N * p.G;
     if (pl.lanes) {
-        const int64_t blocks = ceil_div(units * pl.lanes, kBlock);
-        if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
-        if (pl.k == 1) norm_reg<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, units);
-        else if (pl.k == 2) norm_reg<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, units);
-        else norm_reg<T, V, 4><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, units);
+        const int64_t blocks = ceil_div(pl.R * p.G * pl.lanes, kBlock);
+        if (blocks > 0x7fffffll) return PE_ERR_UNSUPPORTED;
+        if (pl.k == 1) norm_reg<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
+        else if (pl.k == 2) norm_reg<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
+        else norm_reg<T, V, 4><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
         return launched();
     }
     float* part = (float*)a->ws;
@@ -613,15 +656,14 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
     int64_t rows;
     if (pl.lanes) {
         const int64_t blocks = ceil_div(pl.R * p.G * pl.lanes, kBlock);
-        if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+        if (blocks > 0x7fffffll) return PE_ERR_UNSUPPORTED;
         rows = pl.R;
         const bool sums = ga->dweight || ga->dbias;
         sw = ws;
         sb = ws + rows * p.C;
         float* pw = sums ? sw : nullptr;
-        if (pl.k == 1) norm_reg_bwd<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, pl.R, pw, sb);
-        else if (pl.k == 2) norm_reg_bwd<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, pl.R, pw, sb);
-        else norm_reg_bwd<T, V, 4><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, pl.R, pw, sb);
+        if (pl.k == 1) norm_reg_bwd<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R, pw, sb);
+        else norm_reg_bwd<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R, pw, sb);
         if (int rc = launched()) return rc;
     } else {
         float* part = ws;
@@ -639,9 +681,8 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
         norm_apply_bwd<T, V><<<grid, kBlock, 0, s>>>(p, pl.q, gm);
         if (int rc = launched()) return rc;
     }
-    int rc = ga->dweight ? sum_rows(sw, rows, p.C, (int)a->dtype, ga->dweight, s) : PE_OK;
-    if (!rc && ga->dbias) rc = sum_rows(sb, rows, p.C, (int)a->dtype, ga->dbias, s);
-    return rc;
+    const SumJob sums[2] = {{sw, rows, p.C, (int)a->dtype, ga->dweight}, {sb, rows, p.C, (int)a->dtype, ga->dbias}};
+    return sum_rows(sums, 2, s);
 }
 
 #define PE_NORM_T(F, dtype, vec, ...)                                                                       \
@@ -684,9 +725,9 @@ int group_norm_grad(const pe_norm_grad_args* g, cudaStream_t s) {
     const pe_norm_args* a = &g->fwd;
     if (int rc = check_norm(a)) return rc;
     if (a->batch == 0 || a->places == 0) {
-        int rc = g->dweight ? sum_rows(nullptr, 0, a->channels, (int)a->dtype, g->dweight, s) : PE_OK;
-        if (!rc && g->dbias) rc = sum_rows(nullptr, 0, a->channels, (int)a->dtype, g->dbias, s);
-        return rc;
+        const SumJob none[2] = {{nullptr, 0, a->channels, (int)a->dtype, g->dweight},
+                                {nullptr, 0, a->channels, (int)a->dtype, g->dbias}};
+        return sum_rows(none, 2, s);
     }
     if (!a->mean || !a->rstd || !g->dout || !g->dx || (a->gate && !g->dgate)) return PE_ERR_INVALID;
     const Plan pl = grad_plan(g);

@@ -5,27 +5,41 @@ namespace pe {
 
 namespace {
 
-// out[c] = sum_r part[r][c]. A block has 32 columns and 8 row lanes: lane y adds the
-// rows y, y + 8, ..., then the eight sums are added in order, so that the same input
-// gives the same bits. Reads of a warp are 128 contiguous bytes.
-template <typename T>
-__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ part, int64_t rows, int64_t cols,
-                                                       T* __restrict__ out) {
-    __shared__ float s[8][33];
+// out[c] = sum_r part[r][c] of each job (blockIdx.y). A block has 32 columns and 32 row
+// lanes: lane y adds the rows y, y + 32, ..., eight loads in flight, then the 32 sums are
+// added in order, so that the same input gives the same bits. Reads of a warp are 128
+// contiguous bytes. Bound by latency at the usual sizes (a few hundred rows), so all of
+// an operator's sums go in one launch.
+struct Jobs {
+    SumJob j[3];
+};
+
+__device__ __forceinline__ void store_sum(const SumJob& j, int64_t c, float a) {
+    if (j.dtype == PE_F32)
+        ((float*)j.out)[c] = a;
+    else if (j.dtype == PE_F16)
+        ((__half*)j.out)[c] = from_float<__half>(a);
+    else
+        ((__nv_bfloat16*)j.out)[c] = from_float<__nv_bfloat16>(a);
+}
+
+__global__ void __launch_bounds__(1024) sum_rows_kernel(const __grid_constant__ Jobs jobs) {
+    __shared__ float s[32][33];
+    const SumJob& j = jobs.j[blockIdx.y];
     const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < j.cols; c0 += (int64_t)gridDim.x * 32) {
         const int64_t c = c0 + x;
         float a = 0.0f;
-        if (c < cols) {
-#pragma unroll 4
-            for (int64_t r = y; r < rows; r += 8) a += __ldg(part + r * cols + c);
+        if (c < j.cols) {
+#pragma unroll 8
+            for (int64_t r = y; r < j.rows; r += 32) a += __ldg(j.part + r * j.cols + c);
         }
         s[y][x] = a;
         __syncthreads();
-        if (y == 0 && c < cols) {
+        if (y == 0 && c < j.cols) {
 #pragma unroll
-            for (int k = 1; k < 8; ++k) a += s[k][x];
-            out[c] = from_float<T>(a);
+            for (int k = 1; k < 32; ++k) a += s[k][x];
+            store_sum(j, c, a);
         }
         __syncthreads();
     }
@@ -33,16 +47,18 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__
 
 }  // namespace
 
-int sum_rows(const float* part, int64_t rows, int64_t cols, int dtype, void* out, cudaStream_t s) {
-    if (cols <= 0) return PE_OK;
-    const int64_t blocks = ceil_div(cols, 32);
-    const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
-    if (dtype == PE_F32)
-        sum_rows_kernel<<<grid, 256, 0, s>>>(part, rows, cols, (float*)out);
-    else if (dtype == PE_F16)
-        sum_rows_kernel<<<grid, 256, 0, s>>>(part, rows, cols, (__half*)out);
-    else
-        sum_rows_kernel<<<grid, 256, 0, s>>>(part, rows, cols, (__nv_bfloat16*)out);
+int sum_rows(const SumJob* jobs, int count, cudaStream_t s) {
+    Jobs all{};
+    int n = 0;
+    int64_t most = 0;
+    for (int i = 0; i < count; ++i)
+        if (jobs[i].out && jobs[i].cols > 0) {
+            all.j[n++] = jobs[i];
+            most = jobs[i].cols > most ? jobs[i].cols : most;
+        }
+    if (!n) return PE_OK;
+    const int64_t blocks = ceil_div(most, 32);
+    sum_rows_kernel<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), n), 1024, 0, s>>>(all);
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }

@@ -342,63 +342,100 @@ struct StepP {
     T* out;
 };
 
-template <typename T, int LPC, bool VEC>
+// A lane has four states of one channel, LPC lanes a channel, for RB requests: A is read
+// once for them, and all their states are on the way before the first is used. Bound by
+// memory: the states, 8 bytes a (request, channel, state).
+template <typename T, int LPC, int RB, bool VEC>
 __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ StepP<T> p) {
     constexpr int CH = kThreads / LPC;
     const int tid = threadIdx.x, q = tid % LPC, n0 = 4 * q;
     const int c = blockIdx.x * CH + tid / LPC;
     const bool live = c < p.D;
-    const int64_t b = blockIdx.y;
-    int64_t slot = b;
-    if (p.s32) slot = __ldg(p.s32 + b);
-    if (p.s64) slot = __ldg(p.s64 + b);
-    if (slot < 0 || slot >= p.slots) {
-        if (slot >= 0 && blockIdx.x == 0 && tid == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
-        if (live && q == 0) p.out[b * p.D + c] = from_float<T>(0.0f);
-        return;
+    const int64_t b0 = (int64_t)blockIdx.y * RB, cn = (int64_t)c * p.N + n0;
+    bool in[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[i] = live && n0 + i < p.N;
+    float h[RB][4], B[RB][4], C[RB][4], A[4], u[RB], dt[RB], z[RB];
+    int64_t slot[RB];
+    const int g = live ? c / p.Dg : 0;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        const int64_t b = b0 + r;
+        slot[r] = b < p.batch ? (p.s32 ? (int64_t)__ldg(p.s32 + b) : p.s64 ? __ldg(p.s64 + b) : b) : -1;
+        if (slot[r] >= p.slots) {
+            if (blockIdx.x == 0 && tid == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
+            slot[r] = -1;
+        }
     }
-    float y = 0.0f, uv = 0.0f;
-    if (live) {
-        uv = to_float(__ldg(p.u + b * p.u_sb + c));
-        float dt = to_float(__ldg(p.delta + b * p.d_sb + c)) + (p.bias ? __ldg(p.bias + c) : 0.0f);
-        if (p.softplus) dt = softplusf(dt);
-        const float x = dt * uv;
-        const int g = c / p.Dg;
-        const T* B = p.B + b * p.B_sb + g * p.B_sg + n0;
-        const T* C = p.C + b * p.C_sb + g * p.C_sg + n0;
-        const int64_t cn = (int64_t)c * p.N + n0;
-        float* hp = p.state + slot * p.D * p.N + cn;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        const bool on = slot[r] >= 0;
+        const float* hp = p.state + slot[r] * p.D * p.N + cn;
         if (VEC) {
-            if (n0 < p.N) {
-                float4 h = *reinterpret_cast<const float4*>(hp);
-                const float4 a = __ldg(reinterpret_cast<const float4*>(p.A + cn));
-                h.x = fmaf(exp2_fast(dt * (a.x * kLog2e)), h.x, x * to_float(__ldg(B)));
-                h.y = fmaf(exp2_fast(dt * (a.y * kLog2e)), h.y, x * to_float(__ldg(B + 1)));
-                h.z = fmaf(exp2_fast(dt * (a.z * kLog2e)), h.z, x * to_float(__ldg(B + 2)));
-                h.w = fmaf(exp2_fast(dt * (a.w * kLog2e)), h.w, x * to_float(__ldg(B + 3)));
-                y = to_float(__ldg(C)) * h.x + to_float(__ldg(C + 1)) * h.y + to_float(__ldg(C + 2)) * h.z +
-                    to_float(__ldg(C + 3)) * h.w;
-                *reinterpret_cast<float4*>(hp) = h;
-            }
+            const float4 v = on && in[0] ? __ldcs(reinterpret_cast<const float4*>(hp)) : make_float4(0, 0, 0, 0);
+            h[r][0] = v.x, h[r][1] = v.y, h[r][2] = v.z, h[r][3] = v.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (n0 + i >= p.N) break;
-                const float h = fmaf(exp2_fast(dt * (__ldg(p.A + cn + i) * kLog2e)), hp[i], x * to_float(__ldg(B + i)));
-                y = fmaf(to_float(__ldg(C + i)), h, y);
-                hp[i] = h;
+            for (int i = 0; i < 4; ++i) h[r][i] = on && in[i] ? hp[i] : 0.0f;
+        }
+    }
+    if (VEC) {
+        const float4 v = in[0] ? __ldg(reinterpret_cast<const float4*>(p.A + cn)) : make_float4(0, 0, 0, 0);
+        A[0] = v.x * kLog2e, A[1] = v.y * kLog2e, A[2] = v.z * kLog2e, A[3] = v.w * kLog2e;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A[i] = in[i] ? __ldg(p.A + cn + i) * kLog2e : 0.0f;
+    }
+    const float bias = live && p.bias ? __ldg(p.bias + c) : 0.0f, Dw = live && p.Dw ? __ldg(p.Dw + c) : 0.0f;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        const int64_t b = b0 + r;
+        const bool on = slot[r] >= 0;
+        u[r] = on && live ? to_float(__ldg(p.u + b * p.u_sb + c)) : 0.0f;
+        dt[r] = on && live ? to_float(__ldg(p.delta + b * p.d_sb + c)) + bias : 0.0f;
+        z[r] = on && live && p.z ? to_float(__ldg(p.z + b * p.z_sb + c)) : 0.0f;
+        if (VEC) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) B[r][i] = C[r][i] = 0.0f;
+            if (on && in[0]) {
+                unpack(load_vec<T, 4>(p.B + b * p.B_sb + g * p.B_sg + n0), B[r]);
+                unpack(load_vec<T, 4>(p.C + b * p.C_sb + g * p.C_sg + n0), C[r]);
             }
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            B[r][i] = on && in[i] ? to_float(__ldg(p.B + b * p.B_sb + g * p.B_sg + n0 + i)) : 0.0f;
+            C[r][i] = on && in[i] ? to_float(__ldg(p.C + b * p.C_sb + g * p.C_sg + n0 + i)) : 0.0f;
         }
     }
 #pragma unroll
-    for (int m = LPC / 2; m >= 1; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
-    if (live && q == 0) {
-        if (p.Dw) y = fmaf(__ldg(p.Dw + c), uv, y);
-        if (p.z) {
-            const float zv = to_float(__ldg(p.z + b * p.z_sb + c));
-            y *= zv * sigmoidf(zv);
+    for (int r = 0; r < RB; ++r) {
+        if (b0 + r >= p.batch) break;
+        const float d = p.softplus ? softplusf(dt[r]) : dt[r], x = d * u[r];
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            h[r][i] = fmaf(exp2_fast(d * A[i]), h[r][i], x * B[r][i]);
+            y = fmaf(C[r][i], h[r][i], y);
         }
-        p.out[b * p.D + c] = from_float<T>(y);
+        if (slot[r] >= 0) {
+            float* hp = p.state + slot[r] * p.D * p.N + cn;
+            if (VEC) {
+                if (in[0]) __stcs(reinterpret_cast<float4*>(hp), make_float4(h[r][0], h[r][1], h[r][2], h[r][3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (in[i]) hp[i] = h[r][i];
+            }
+        }
+#pragma unroll
+        for (int m = LPC / 2; m >= 1; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
+        if (live && q == 0) {
+            y = fmaf(Dw, u[r], y);
+            if (p.z) y *= z[r] * sigmoidf(z[r]);
+            p.out[(b0 + r) * p.D + c] = from_float<T>(slot[r] >= 0 ? y : 0.0f);
+        }
     }
 }
 
@@ -427,8 +464,10 @@ int64_t piece_tokens(const pe_scan_args* a) {
     const double whole = max(longest * kAlone, total / sms * kFull);
     const double split = total / sms * (kFull + kState) + kLaunches;
     if (split >= whole) return 0;
-    const int64_t piece = (int64_t)(total / (4.0 * sms));   // four blocks an SM
-    return max((int64_t)KCK, ceil_div(piece, KCK) * KCK);
+    // four blocks an SM, one wave of them: pieces are rounded up
+    const int64_t slots = 4 * num_sms(), rows = a->cu ? 1 : a->nseq;
+    const int64_t pieces = max((int64_t)1, slots / (rows * tiles) - (a->cu ? a->nseq : 0));
+    return max((int64_t)KCK, ceil_div(ceil_div(a->tokens, pieces), KCK) * KCK);
 }
 
 template <typename T, int LPC>
@@ -481,12 +520,22 @@ int step_run(const pe_scan_step_args* a, cudaStream_t s) {
     p.u_sb = a->u_sb; p.d_sb = a->delta_sb; p.z_sb = a->z_sb;
     p.B_sb = a->B_sb; p.B_sg = a->B_sg; p.C_sb = a->C_sb; p.C_sg = a->C_sg;
     p.state = a->state; p.out = (T*)a->out;
-    const dim3 grid((unsigned)ceil_div(p.D, kThreads / LPC), (unsigned)a->batch);
-    const bool vec = p.N % 4 == 0 && ((uintptr_t)p.state | (uintptr_t)p.A) % 16 == 0;
-    if (vec)
-        scan_step<T, LPC, true><<<grid, kThreads, 0, s>>>(p);
+    const int64_t tiles = ceil_div(p.D, kThreads / LPC);
+    // four states at once: fp32 of the state and of A, and of B and C in their type
+    const int cb = 4 * sizeof(T);
+    const bool vec = p.N % 4 == 0 && ((uintptr_t)p.state | (uintptr_t)p.A) % 16 == 0 &&
+                     ((uintptr_t)p.B | (uintptr_t)p.C) % cb == 0 && (p.B_sb | p.B_sg | p.C_sb | p.C_sg) % 4 == 0;
+    // two requests a thread once that still gives every SM its 16 blocks
+    const bool two = tiles * a->batch >= 32ll * num_sms();
+    const dim3 grid((unsigned)tiles, (unsigned)(two ? ceil_div(a->batch, 2) : a->batch));
+    if (vec && two)
+        scan_step<T, LPC, 2, true><<<grid, kThreads, 0, s>>>(p);
+    else if (two)
+        scan_step<T, LPC, 2, false><<<grid, kThreads, 0, s>>>(p);
+    else if (vec)
+        scan_step<T, LPC, 1, true><<<grid, kThreads, 0, s>>>(p);
     else
-        scan_step<T, LPC, false><<<grid, kThreads, 0, s>>>(p);
+        scan_step<T, LPC, 1, false><<<grid, kThreads, 0, s>>>(p);
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }

@@ -123,8 +123,9 @@ struct GradP {
     T *du, *ddelta, *dz;
     float *dh0;
     float *pBC;       // [2][tiles][G][N][batch * tokens]: each channel tile's share of dB and dC
-    float *pA;        // [nseq][D][N]
-    float *pD, *pb;   // [nseq][D]
+    float *pA;        // [pieces][D][N]
+    float *pD, *pb;   // [pieces][D]
+    float *gloc, *dtsum;   // split: each piece's own adjoint state at its start, later the one after it; sum of dt
 };
 
 template <typename T>
@@ -140,7 +141,8 @@ struct GradSmem {
     float rows[];   // [N][CB] adjoint states, A log2(e), dA; [CB][N] checkpoint
 };
 
-// One block takes 32 channels through a whole sequence, tile by tile from its end. Per
+// One block takes 32 channels through a sequence (or a piece of it), tile by tile from
+// its end. Per
 // state n a lane composes the maps of its K tokens forwards (from the checkpoint) and
 // backwards (from the tile after), scans them with the other lanes of its channels, and
 // runs both recurrences again in registers:
@@ -162,7 +164,12 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
     const int64_t DN = (int64_t)f.D * f.N;
     const int tile = (w.c0 - w.g * f.Dg) / CB;
 
-    const int64_t start = w.sp.start, len = w.sp.len;
+    if (!w.any) {   // a number that stands for no piece: nothing in the sums
+        for (int i = tid; i < w.nch * f.N; i += kThreads) p.pA[w.number * DN + (int64_t)w.c0 * f.N + i] = 0.0f;
+        if (tid < w.nch) p.pD[w.number * f.D + w.c0 + tid] = p.pb[w.number * f.D + w.c0 + tid] = 0.0f;
+        return;
+    }
+    const int64_t start = w.sp.start, len = w.t1;   // tokens are counted from the sequence's start
     const T* u = f.u + w.sp.row * f.u_sb + start * f.u_st + w.c0;
     const T* delta = f.delta + w.sp.row * f.d_sb + start * f.d_st + w.c0;
     const T* z = f.z ? f.z + w.sp.row * f.z_sb + start * f.z_st + w.c0 : nullptr;
@@ -187,14 +194,15 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
         const float* k = ckpt + t / KCK * DN;
         for (int i = tid; i < w.nch * f.N; i += kThreads) cp_async<4>(sK + i, k + i, 4);
     };
-    const int64_t top = len > 0 ? (len - 1) / TT * TT : -1;
+    const int64_t top = len > w.t0 ? (len - 1) / TT * TT : -1;
     if (top >= 0) copy(top);
     cp_commit();
+    const float* from = p.gloc ? p.gloc + w.number * DN : p.dstate ? p.dstate + w.s * DN : nullptr;
     for (int i = tid; i < CB * f.N; i += kThreads) {
         const int ci = i / f.N, n = i - ci * f.N;
         const int64_t k = (int64_t)(w.c0 + ci) * f.N + n;
         const bool in = ci < w.nch;
-        sG[n * CB + ci] = in && p.dstate ? __ldg(p.dstate + w.s * DN + k) : 0.0f;
+        sG[n * CB + ci] = in && from ? from[k] : 0.0f;
         sA[n * CB + ci] = in ? __ldg(f.A + k) * kLog2e : 0.0f;
         sD[n * CB + ci] = 0.0f;
         if (!in) sK[i] = 0.0f;
@@ -211,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
     float* xr = m.x + c * RS + tl * SEG;
     float* dyr = m.dy + c * RS + tl * SEG;
 
-    for (int64_t t = top; t >= 0; t -= TT) {
+    for (int64_t t = top; t >= w.t0; t -= TT) {
         const int cnt = (int)min((int64_t)TT, len - t);
         Pairs dt[2], x[2], dy[2], y[2], q[2], r[2];
         for (int n0 = 0; n0 < f.N; n0 += NC) {
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
                 }
             }
         }
-        if (t > 0) {
+        if (t > w.t0) {
             __syncthreads();
             copy(t - TT);
             cp_commit();
@@ -455,22 +463,207 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
     __syncthreads();
     for (int i = tid; i < w.nch * f.N; i += kThreads) {
         const int ci = i / f.N, n = i - ci * f.N;
-        const int64_t k = w.s * DN + (int64_t)(w.c0 + ci) * f.N + n;
-        p.pA[k] = sD[n * CB + ci];
-        if (p.dh0) p.dh0[k] = sG[n * CB + ci];
+        const int64_t k = (int64_t)(w.c0 + ci) * f.N + n;
+        p.pA[w.number * DN + k] = sD[n * CB + ci];
+        if (p.dh0 && w.j == 0) p.dh0[w.s * DN + k] = sG[n * CB + ci];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int d = LT / 2; d >= 1; d /= 2) dD[e] += __shfl_xor_sync(0xffffffffu, dD[e], d);
-        if (tl == 0 && c + e < w.nch) p.pD[(int64_t)w.s * f.D + w.c0 + c + e] = dD[e];
+        if (tl == 0 && c + e < w.nch) p.pD[w.number * f.D + w.c0 + c + e] = dD[e];
         m.dt[e * kThreads + tid] = db[e];
     }
     __syncthreads();
     if (tid < w.nch) {
         float s = 0.0f;
         for (int k = tid / 2; k < kThreads; k += CB / 2) s += m.dt[tid % 2 * kThreads + k];
-        p.pb[(int64_t)w.s * f.D + w.c0 + tid] = s;
+        p.pb[w.number * f.D + w.c0 + tid] = s;
+    }
+}
+
+// The first half of a backward pass split along the tokens: the adjoint state at a
+// piece's start that the piece's own tokens give, and its sum of dt. As scan_bwd, with
+// nothing but g's recurrence.
+template <typename T>
+struct AdjSmem {
+    static constexpr int NC = GradSmem<T>::NC;
+    alignas(16) T d[TT * CB];
+    T z[TT * CB], o[TT * CB], c[TT * NC];
+    alignas(16) float dt[CB * RS];
+    float dy[CB * RS], C[NC * RS];
+    float rows[];   // [N][CB] adjoint states, A log2(e)
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 3) scan_adjoint(const __grid_constant__ GradP<T> p) {
+    using M = AdjSmem<T>;
+    constexpr int NC = M::NC;
+    extern __shared__ __align__(16) unsigned char smem[];
+    M& m = *reinterpret_cast<M*>(smem);
+    const ScanP<T>& f = p.f;
+    float *sG = m.rows, *sA = sG + f.N * CB;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const Place w = place_of<CB>(f);
+    if (!w.any || w.j == 0) return;   // nothing comes before a sequence's first piece
+    const int tl = lane % LT, c = 2 * (tid / 32 * (32 / LT) + lane / LT);
+    const int64_t DN = (int64_t)f.D * f.N;
+    const int64_t start = w.sp.start, len = w.t1;
+    const T* delta = f.delta + w.sp.row * f.d_sb + start * f.d_st + w.c0;
+    const T* z = f.z ? f.z + w.sp.row * f.z_sb + start * f.z_st + w.c0 : nullptr;
+    const T* dout = p.dout + w.sp.row * p.o_sb + start * p.o_st + w.c0;
+    const T* C = f.C + w.sp.row * f.C_sb + start * f.C_st + w.g * f.C_sg;
+    auto copy_states = [&](int64_t t, int n0) {
+        stage<TT, NC>(m.c, C + t * f.C_st + n0, f.C_st, (int)min((int64_t)TT, len - t), min(NC, f.N - n0), f.C_cb);
+    };
+    auto copy = [&](int64_t t) {
+        const int cnt = (int)min((int64_t)TT, len - t);
+        stage<TT, CB>(m.d, delta + t * f.d_st, f.d_st, cnt, w.nch, f.d_cb);
+        stage<TT, CB>(m.o, dout + t * p.o_st, p.o_st, cnt, w.nch, p.o_cb);
+        if (z) stage<TT, CB>(m.z, z + t * f.z_st, f.z_st, cnt, w.nch, f.z_cb);
+    };
+    const int64_t top = (len - 1) / TT * TT;
+    copy(top);
+    copy_states(top, 0);
+    cp_commit();
+    for (int i = tid; i < CB * f.N; i += kThreads) {
+        const int ci = i / f.N, n = i - ci * f.N;
+        sG[n * CB + ci] = 0.0f;
+        sA[n * CB + ci] = ci < w.nch ? __ldg(f.A + (int64_t)(w.c0 + ci) * f.N + n) * kLog2e : 0.0f;
+    }
+    const int cp = tid % (CB / 2) * 2;
+    float bias[2], dtsum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) bias[e] = f.bias && cp + e < w.nch ? __ldg(f.bias + w.c0 + cp + e) : 0.0f;
+
+    for (int64_t t = top; t >= w.t0; t -= TT) {
+        const int cnt = (int)min((int64_t)TT, len - t);
+        Pairs dt[2], dy[2];
+        for (int n0 = 0; n0 < f.N; n0 += NC) {
+            const int nn = min(NC, f.N - n0);
+            cp_wait();
+            __syncthreads();
+            if (n0 == 0) {
+#pragma unroll 2
+                for (int i = tid; i < TT / 4 * (CB / 2); i += kThreads) {
+                    const int t4 = i / (CB / 2) * 4;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float fd[4], fy[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int at = (t4 + k) * CB + cp + e;
+                            const bool ok = cp + e < w.nch && t4 + k < cnt;
+                            float v = to_float(m.d[at]) + bias[e];
+                            if (f.softplus) v = softplusf(v);
+                            fd[k] = ok ? v : 0.0f;
+                            v = to_float(m.o[at]);
+                            if (z) {
+                                const float zv = to_float(m.z[at]);
+                                v *= zv * sigmoidf(zv);
+                            }
+                            fy[k] = ok ? v : 0.0f;
+                        }
+                        const int to = (cp + e) * RS + at_token(t4);
+                        *reinterpret_cast<float4*>(m.dt + to) = make_float4(fd[0], fd[1], fd[2], fd[3]);
+                        *reinterpret_cast<float4*>(m.dy + to) = make_float4(fy[0], fy[1], fy[2], fy[3]);
+                    }
+                }
+            }
+            widen_cols<LT, NC>(m.C, m.c, cnt, nn);
+            __syncthreads();
+            if (n0 + NC < f.N) {
+                copy_states(t, n0 + NC);
+            } else if (t > w.t0) {
+                copy(t - TT);
+                copy_states(t - TT, 0);
+            }
+            cp_commit();
+            if (n0 == 0) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    dt[e] = load_pairs(m.dt + (c + e) * RS + tl * SEG);
+                    dy[e] = load_pairs(m.dy + (c + e) * RS + tl * SEG);
+                    float s[K];
+                    to_scalars(dt[e], s);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) dtsum[e] += s[k];
+                }
+            }
+#pragma unroll 1
+            for (int n = 0; n < nn; ++n) {
+                const Pairs Cn = load_pairs(m.C + n * RS + tl * SEG);
+                const int at = (n0 + n) * CB + c;
+                const float2 A = *reinterpret_cast<const float2*>(sA + at);
+                f32x2* gp = reinterpret_cast<f32x2*>(sG + at);
+                const f32x2 g0 = *gp;
+                float P[2], G[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float Ae = e ? A.y : A.x;
+                    const f32x2 A2 = pack2(Ae, Ae);
+                    Pairs ap, vp;
+                    float a[K], v[K];
+#pragma unroll
+                    for (int i = 0; i < K / 2; ++i) {
+                        ap.p[i] = exp2_2(mul2(dt[e].p[i], A2));
+                        vp.p[i] = mul2(dy[e].p[i], Cn.p[i]);
+                    }
+                    P[e] = product(ap);
+                    to_scalars(ap, a);
+                    to_scalars(vp, v);
+                    G[e] = v[K - 1];
+#pragma unroll
+                    for (int k = 1; k < K; ++k) G[e] = fmaf(a[K - k], G[e], v[K - 1 - k]);
+                    G[e] *= a[0];
+                }
+                f32x2 last;
+                scan_lanes_down<LT>(pack2(P[0], P[1]), pack2(G[0], G[1]), g0, tl, last);
+                if (tl == 0) *gp = last;   // the last lane read it before the shuffles
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < w.nch * f.N; i += kThreads) {
+        const int ci = i / f.N, n = i - ci * f.N;
+        p.gloc[w.number * DN + (int64_t)(w.c0 + ci) * f.N + n] = sG[n * CB + ci];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = LT / 2; d >= 1; d /= 2) dtsum[e] += __shfl_xor_sync(0xffffffffu, dtsum[e], d);
+        if (tl == 0 && c + e < w.nch) p.dtsum[w.number * f.D + w.c0 + c + e] = dtsum[e];
+    }
+}
+
+// Each piece's own adjoint state gives way to the one after the piece, from the
+// sequence's end. One thread a (sequence, channel, state).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) adjoint_carry(const __grid_constant__ GradP<T> p) {
+    const ScanP<T>& f = p.f;
+    const int64_t DN = (int64_t)f.D * f.N, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= DN) return;
+    const int s = blockIdx.y;
+    const int64_t len = seq_span(f.seqs, s).len, base = piece_base(f.seqs, s, f.piece);
+    const int64_t n = len > f.piece ? ceil_div(len, f.piece) : 1;
+    const float A = __ldg(f.A + i) * kLog2e;
+    float g = p.dstate ? __ldg(p.dstate + s * DN + i) : 0.0f;
+    float* gp = p.gloc + base * DN + i;
+    const float* sp = p.dtsum + base * f.D + i / f.N;
+    for (int64_t k0 = n - 1; k0 >= 0; k0 -= 8) {
+        float own[8], keep[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k0 - k > 0) {
+                own[k] = gp[(k0 - k) * DN];
+                keep[k] = exp2_fast(A * __ldg(sp + (k0 - k) * f.D));
+            }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k0 - k >= 0) {
+                gp[(k0 - k) * DN] = g;
+                if (k0 - k > 0) g = fmaf(keep[k], g, own[k]);
+            }
     }
 }
 
@@ -502,17 +695,35 @@ __global__ void __launch_bounds__(256) sum_tiles(const float* __restrict__ part,
 }
 
 // ---- host -------------------------------------------------------------------------
+// Tokens a piece of the backward pass; 0 = whole sequences. A block that has an SM to
+// itself leaves most of it idle, and the pass that finds the adjoint states between
+// pieces costs half as much as the pass itself: split where the sequences' blocks fill
+// less than 0.6 of the SMs, into as many pieces as two blocks an SM take.
+int64_t grad_piece(const pe_scan_args* a) {
+    const int64_t tiles = a->groups * ceil_div(a->channels / a->groups, CB), rows = a->cu ? 1 : a->nseq;
+    const int64_t blocks = a->nseq * tiles;
+    if (blocks < 1 || a->nseq > 65535 || blocks * 10 >= num_sms() * 6 || a->tokens / (a->nseq / rows) < 4 * KCK)
+        return 0;
+    int64_t pieces = 2 * num_sms() / (rows * tiles) - (a->cu ? a->nseq : 0);
+    if (pieces < 2) return 0;
+    return ceil_div(ceil_div(a->tokens, pieces), KCK) * KCK;
+}
+
 struct GradWs {
-    int64_t bc, a, d, b, total;   // float offsets
+    int64_t piece, pieces, bc, a, d, b, g, s, total;   // tokens a piece, pieces; float offsets
 };
 GradWs grad_ws(const pe_scan_args* a) {
-    const int64_t rows = a->tokens * (a->cu ? 1 : a->nseq);
+    const int64_t rows = a->tokens * (a->cu ? 1 : a->nseq), DN = a->channels * a->states;
     GradWs w;
+    w.piece = grad_piece(a);
+    w.pieces = piece_count(seqs_of(a), w.piece ? w.piece : (a->tokens / KCK + 1) * KCK);
     w.bc = 0;
     w.a = 2 * ceil_div(a->channels / a->groups, CB) * rows * a->groups * a->states;
-    w.d = w.a + a->nseq * a->channels * a->states;
-    w.b = w.d + a->nseq * a->channels;
-    w.total = w.b + a->nseq * a->channels;
+    w.d = w.a + w.pieces * DN;
+    w.b = w.d + w.pieces * a->channels;
+    w.g = w.b + w.pieces * a->channels;
+    w.s = w.g + (w.piece ? w.pieces * DN : 0);
+    w.total = w.s + (w.piece ? w.pieces * a->channels : 0);
     return w;
 }
 
@@ -529,9 +740,21 @@ int grad_type(const pe_scan_grad_args* a, cudaStream_t s) {
     p.du = (T*)a->du; p.ddelta = (T*)a->ddelta; p.dz = (T*)a->dz;
     p.dh0 = a->dh0;
     p.pBC = ws + w.bc; p.pA = ws + w.a; p.pD = ws + w.d; p.pb = ws + w.b;
+    p.gloc = p.dtsum = nullptr;
     unsigned grid;
-    if (int rc = grid_of((int64_t)p.f.seqs.nseq * p.f.G * p.f.ntile, &grid)) return rc;
-    if (grid)   // every sequence is one piece here, numbered by itself
+    if (int rc = grid_of(w.pieces * p.f.G * p.f.ntile, &grid)) return rc;
+    if (f->nseq == 0) grid = 0;
+    if (grid && w.piece) {
+        p.f.piece = w.piece;
+        p.gloc = ws + w.g;
+        p.dtsum = ws + w.s;
+        if (int rc = launch(scan_adjoint<T>, p, grid, sizeof(AdjSmem<T>) + 2 * p.f.N * CB * 4, s)) return rc;
+        const dim3 blocks((unsigned)ceil_div(f->channels * f->states, kThreads), (unsigned)f->nseq);
+        adjoint_carry<T><<<blocks, kThreads, 0, s>>>(p);
+        count_launch();
+        if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
+    }
+    if (grid)
         if (int rc = launch(scan_bwd<T>, p, grid, sizeof(GradSmem<T>) + 4 * p.f.N * CB * 4, s)) return rc;
     const int64_t rows = f->tokens * (f->cu ? 1 : f->nseq), cols = f->groups * f->states;
     if (rows) {
@@ -541,10 +764,10 @@ int grad_type(const pe_scan_grad_args* a, cudaStream_t s) {
         count_launch();
         if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
-    int rc = sum_rows(p.pA, f->nseq, f->channels * f->states, PE_F32, a->dA, s);
-    if (!rc && a->dD) rc = sum_rows(p.pD, f->nseq, f->channels, PE_F32, a->dD, s);
-    if (!rc && a->ddelta_bias) rc = sum_rows(p.pb, f->nseq, f->channels, PE_F32, a->ddelta_bias, s);
-    return rc;
+    const SumJob sums[3] = {{p.pA, grid ? w.pieces : 0, f->channels * f->states, PE_F32, a->dA},
+                            {p.pD, grid ? w.pieces : 0, f->channels, PE_F32, a->dD},
+                            {p.pb, grid ? w.pieces : 0, f->channels, PE_F32, a->ddelta_bias}};
+    return sum_rows(sums, 3, s);
 }
 
 int grad_any(const pe_scan_grad_args* a, cudaStream_t s) { PE_TYPES(grad_type, a->fwd.dtype, a, s) }

@@ -17,28 +17,50 @@ _raw_stream = None
 _fns: dict = {}
 
 
+# Argument checks and layouts of earlier calls, by signature: the shapes, strides, types
+# and devices of the tensors (never their addresses or values). A call whose signature
+# is here needs no further checks; only calls that copy nothing are kept.
+_MOST_PLANS = 4096
+_plans: dict = {}
+
+
+def sig(t):
+    """What a plan may depend on of a tensor."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def plan(key):
+    return _plans.get(key)
+
+
+def keep_plan(key, value):
+    if len(_plans) >= _MOST_PLANS:
+        _plans.clear()
+    _plans[key] = value
+    return value
+
+
 def packer(fields: str) -> struct.Struct:
     """An argument struct of 8-byte fields: q integers, Q pointers, d doubles."""
     return struct.Struct("=" + fields)
 
 
-def function(name: str, restype=ctypes.c_int, sizes: bool = False):
-    """The core library's `name`(args, stream), or `name`(args) for the workspace sizes."""
+def function(name: str, restype=ctypes.c_int, argtypes=(ctypes.c_char_p, ctypes.c_void_p)):
+    """The core library's `name`; the operators take (argument struct, stream)."""
     fn = _fns.get(name)
     if fn is None:
         fn = getattr(core_lib(), name)
-        fn.argtypes = [ctypes.c_char_p] if sizes else [ctypes.c_char_p, ctypes.c_void_p]
-        fn.restype = ctypes.c_int64 if sizes else restype
+        fn.argtypes, fn.restype = list(argtypes), restype
         _fns[name] = fn
     return fn
 
 
-def call(name: str, args: bytes, dev: torch.device):
-    """Enqueue on the device's current stream; a nonzero status raises RuntimeError."""
+def call(name: str, args: bytes, idx: int):
+    """Enqueue on the current stream of device `idx`; a nonzero status raises RuntimeError."""
     global _raw_stream
     if _raw_stream is None:
         _raw_stream = _raw_stream_getter()
-    fn, idx = function(name), dev.index
+    fn = _fns.get(name) or function(name)
     if idx == _get_device():
         rc = fn(args, _raw_stream(idx))
     else:
@@ -48,12 +70,12 @@ def call(name: str, args: bytes, dev: torch.device):
         raise RuntimeError(f"pto_einsum: {name} failed: {error_string(rc)} ({rc})")
 
 
-def sized(name: str, args: bytes, dev: torch.device) -> int:
+def sized(name: str, args: bytes, idx: int) -> int:
     """Workspace bytes; the rule may ask the device for its number of SMs."""
-    fn = function(name, sizes=True)
-    if dev.index == _get_device():
+    fn = _fns.get(name) or function(name, ctypes.c_int64, (ctypes.c_char_p,))
+    if idx == _get_device():
         return fn(args)
-    with torch.cuda.device(dev.index):
+    with torch.cuda.device(idx):
         return fn(args)
 
 
@@ -123,19 +145,28 @@ def offsets(cu_seqlens, batch: int, tokens: int, dev):
         raise ValueError(f"cu_seqlens must be one row of at least two offsets (got {tuple(cu_seqlens.shape)})")
     if cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"cu_seqlens must be int32 or int64 (got {cu_seqlens.dtype})")
-    return cu_seqlens.to(torch.int32).contiguous(), cu_seqlens.shape[0] - 1
+    return cu_seqlens.to(torch.int32).contiguous(), cu_seqlens.shape[0] - 1   # itself if it is that
 
 
-def slot_pointers(slots, batch: int, dev):
-    """(pointer to int32 slots, pointer to int64 slots); the caller keeps `slots` alive."""
+def check_slots(slots, batch: int, dev):
     if slots is None:
-        return 0, 0
+        return
     if not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int32, torch.int64):
         raise TypeError("slots must be an int32 or int64 tensor")
     if slots.device != dev or slots.shape != (batch,) or (batch > 1 and slots.stride(0) != 1):
         raise ValueError(f"slots must be a contiguous tensor of {batch} indices on {dev}")
+
+
+def slot_pointers(slots):
+    """(pointer to int32 slots, pointer to int64 slots)."""
+    if slots is None:
+        return 0, 0
     return (slots.data_ptr(), 0) if slots.dtype == torch.int32 else (0, slots.data_ptr())
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False

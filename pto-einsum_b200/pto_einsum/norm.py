@@ -13,11 +13,13 @@ in a fixed order.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _ops
-from ._ops import DTYPES, call, check_tensor, packer, ptr, rows, stride, wants_grad
+from ._ops import DTYPES, call, check_tensor, packer, plan, ptr, rows, sig, stride, wants_grad
 
 __all__ = ["group_norm", "group_norm_reference"]
 
@@ -25,52 +27,69 @@ _NORM = packer("6q" "d" "4Q" "4q" "Q" "2Q" "Qq")
 _NORM_GRAD = packer("6q" "d" "4Q" "4q" "Q" "2Q" "Qq" "Q" "2q" "4Q" "Qq")
 
 
-def _fields(x, gate, weight, bias, groups, eps, silu, out, mean, rstd):
-    N, S, C = x.shape
-    return (DTYPES[x.dtype], silu, N, S, C, groups, eps, x.data_ptr(), ptr(weight), ptr(bias), ptr(gate),
-            stride(x, 0), stride(x, 1), *((0, 0) if gate is None else (stride(gate, 0), stride(gate, 1))), ptr(out),
-            ptr(mean), ptr(rstd))
+def _fields(lay, x, weight, bias, gate, out, mean, rstd):
+    ints, strides, _ = lay
+    return (*ints, x.data_ptr(), ptr(weight), ptr(bias), ptr(gate), *strides, ptr(out), ptr(mean), ptr(rstd))
 
 
-def _forward(x, weight, bias, gate, groups, eps, silu, stats):
+def _forward(lay, x, weight, bias, gate, stats):
     dev = x.device
     out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2, x.shape[0], groups), dtype=torch.float32, device=dev).unbind(0)
-    fields = _fields(x, gate, weight, bias, groups, eps, silu, out, mean, rstd)
-    nbytes = _ops.sized("pe_group_norm_ws_bytes", _NORM.pack(*fields, 0, 0), dev)
+        mean, rstd = torch.empty((2, lay[0][2], lay[0][5]), dtype=torch.float32, device=dev).unbind(0)
+    fields = _fields(lay, x, weight, bias, gate, out, mean, rstd)
+    nbytes = _ops.sized("pe_group_norm_ws_bytes", _NORM.pack(*fields, 0, 0), lay[2])
     ws = _ops.workspace(nbytes, dev)
-    call("pe_group_norm", _NORM.pack(*fields, ptr(ws), nbytes), dev)
+    call("pe_group_norm", _NORM.pack(*fields, ptr(ws), nbytes), lay[2])
     return out, mean, rstd
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, gate, groups, eps, silu):
-        out, mean, rstd = _forward(x, weight, bias, gate, groups, eps, silu, True)
+    def forward(ctx, x, weight, bias, gate, lay):
+        out, mean, rstd = _forward(lay, x, weight, bias, gate, True)
         ctx.save_for_backward(x, weight, bias, gate, mean, rstd)
-        ctx.plan = groups, eps, silu
+        ctx.lay = lay
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         x, weight, bias, gate, mean, rstd = ctx.saved_tensors
-        groups, eps, silu = ctx.plan
-        dev = x.device
-        dout = rows(dout)
+        lay, dev = ctx.lay, x.device
+        dout = _fold(dout)
 
         def like(t):
             return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
 
         dx, dw, db, dgate = like(x), like(weight), like(bias), like(gate)
-        fields = (*_fields(x, gate, weight, bias, groups, eps, silu, None, mean, rstd), 0, 0, dout.data_ptr(),
-                  stride(dout, 0), stride(dout, 1), dx.data_ptr(), ptr(dgate), ptr(dw), ptr(db))
-        nbytes = _ops.sized("pe_group_norm_grad_ws_bytes", _NORM_GRAD.pack(*fields, 0, 0), dev)
+        fields = (*_fields(lay, x, weight, bias, gate, None, mean, rstd), 0, 0, dout.data_ptr(), *_strides(dout),
+                  dx.data_ptr(), ptr(dgate), ptr(dw), ptr(db))
+        nbytes = _ops.sized("pe_group_norm_grad_ws_bytes", _NORM_GRAD.pack(*fields, 0, 0), lay[2])
         ws = _ops.workspace(nbytes, dev)
-        call("pe_group_norm_grad", _NORM_GRAD.pack(*fields, ptr(ws), nbytes), dev)
-        return dx, dw, db, dgate, None, None, None
+        call("pe_group_norm_grad", _NORM_GRAD.pack(*fields, ptr(ws), nbytes), lay[2])
+        return dx, dw, db, dgate, None
+
+
+def _fold(t):
+    """`t` itself, or a copy, such that its middle axes are one axis of one stride."""
+    t = rows(t)
+    if t.dim() <= 3:
+        return t
+    try:
+        t.view(t.shape[0], -1, t.shape[-1]) if t.numel() else None
+        return t
+    except RuntimeError:
+        return t.contiguous()
+
+
+def _strides(t):
+    """Strides of a row and of a place (0 for an axis of one)."""
+    if t.dim() == 2:
+        return stride(t, 0), 0
+    places = [i for i in range(1, t.dim() - 1) if t.shape[i] > 1]
+    return stride(t, 0), stride(t, places[-1]) if places else 0
 
 
 def group_norm(x, groups: int, weight=None, bias=None, *, eps: float = 1e-5, activation=None, gate=None):
@@ -79,36 +98,41 @@ def group_norm(x, groups: int, weight=None, bias=None, *, eps: float = 1e-5, act
     weight and bias [C] and gate (x's shape) have x's type; activation is None or
     "silu" and excludes a gate. The channels are contiguous; other strides are free
     where the middle axes fold into one. Returns a contiguous tensor of x's shape."""
-    if activation not in (None, "silu"):
-        raise ValueError(f"activation must be None or 'silu' (got {activation!r})")
-    if activation and gate is not None:
-        raise ValueError("activation and gate exclude each other")
-    if not isinstance(x, torch.Tensor) or x.dim() < 2:
-        raise ValueError("x must be a tensor of at least two dimensions, channels last")
-    _ops.check_activations("x", x, (x.dim(),))
-    C = x.shape[-1]
-    if groups < 1 or C < 1 or C % groups:
-        raise ValueError(f"groups must divide the {C} channels (got {groups})")
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative (got {eps})")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            check_tensor(name, t, (C,), x.dtype, x.device)
-    if gate is not None:
-        check_tensor("gate", gate, x.shape, x.dtype, x.device)
-    shape = x.shape
-
-    def fold(t):
-        t = rows(t)
-        return t.unsqueeze(1) if t.dim() == 2 else t if t.dim() == 3 else t.flatten(1, -2)
-
-    x = fold(x)
-    gate = None if gate is None else fold(gate)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    args = (x, weight, bias, gate, int(groups), float(eps), 1 if activation else 0)
-    out = _GroupNorm.apply(*args) if wants_grad(x, weight, bias, gate) else _forward(*args, False)[0]
-    return out if out.shape == shape else out.view(shape)
+    try:
+        key = ("norm", groups, eps, activation, sig(x), sig(weight), sig(bias), sig(gate))
+        lay = plan(key)
+    except (AttributeError, TypeError):      # not tensors: the checks say which
+        key = lay = None
+    if lay is None:
+        if activation not in (None, "silu"):
+            raise ValueError(f"activation must be None or 'silu' (got {activation!r})")
+        if activation and gate is not None:
+            raise ValueError("activation and gate exclude each other")
+        if not isinstance(x, torch.Tensor) or x.dim() < 2:
+            raise ValueError("x must be a tensor of at least two dimensions, channels last")
+        _ops.check_activations("x", x, (x.dim(),))
+        C = x.shape[-1]
+        if groups < 1 or C < 1 or C % groups:
+            raise ValueError(f"groups must divide the {C} channels (got {groups})")
+        if not eps >= 0:
+            raise ValueError(f"eps must not be negative (got {eps})")
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None:
+                check_tensor(name, t, (C,), x.dtype, x.device)
+        if gate is not None:
+            check_tensor("gate", gate, x.shape, x.dtype, x.device)
+        given = (x, weight, bias, gate)
+        x, gate = _fold(x), None if gate is None else _fold(gate)
+        weight = None if weight is None else weight.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        places = math.prod(x.shape[1:-1])
+        lay = ((DTYPES[x.dtype], 1 if activation else 0, x.shape[0], places, C, int(groups), float(eps)),
+               (*_strides(x), *((0, 0) if gate is None else _strides(gate))), x.device.index)
+        if key is not None and all(a is b for a, b in zip(given, (x, weight, bias, gate))):
+            _ops.keep_plan(key, lay)
+    if wants_grad(x, weight, bias, gate):
+        return _GroupNorm.apply(x, weight, bias, gate, lay)
+    return _forward(lay, x, weight, bias, gate, False)[0]
 
 
 def group_norm_reference(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, gate=None):

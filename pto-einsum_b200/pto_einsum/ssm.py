@@ -28,11 +28,14 @@ request).
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _ops
-from ._ops import DTYPES, call, check_activations, check_tensor, offsets, packer, ptr, rows, stride, wants_grad
+from ._ops import (DTYPES, call, check_activations, check_tensor, offsets, packer, plan, ptr, rows, sig, stride,
+                   wants_grad)
 
 __all__ = ["causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step",
            "causal_conv_reference", "selective_scan_reference", "MAX_STATES"]
@@ -67,48 +70,51 @@ def _check_filter(x, weight, bias):
     return weight.shape[1]
 
 
-def _conv_fields(x, weight, bias, init, cu, nseq, silu, out, state):
-    B, T, C = x.shape
-    return (DTYPES[x.dtype], silu, weight.shape[1], B, T, C, nseq, ptr(cu), x.data_ptr(), weight.data_ptr(),
-            ptr(bias), ptr(init), stride(x, 0), stride(x, 1), ptr(out), ptr(state))
+def _conv_layout(x, weight, nseq, silu):
+    """The numbers of a call, its strides and its device: all but the pointers."""
+    return (DTYPES[x.dtype], silu, weight.shape[1], *x.shape, nseq), (stride(x, 0), stride(x, 1)), x.device.index
 
 
-def _conv_forward(x, weight, bias, init, cu, nseq, silu, want_state):
-    B, T, C = x.shape
-    out = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
-    state = torch.empty((nseq, weight.shape[1] - 1, C), dtype=x.dtype, device=x.device) if want_state else None
-    call("pe_causal_conv", _CONV.pack(*_conv_fields(x, weight, bias, init, cu, nseq, silu, out, state)), x.device)
+def _conv_fields(lay, x, weight, bias, init, cu, out, state):
+    return (*lay[0], ptr(cu), x.data_ptr(), weight.data_ptr(), ptr(bias), ptr(init), *lay[1], ptr(out), ptr(state))
+
+
+def _conv_forward(lay, x, weight, bias, init, cu, want_state):
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    state = None
+    if want_state:
+        _, _, W, _, _, C, nseq = lay[0]
+        state = torch.empty((nseq, W - 1, C), dtype=x.dtype, device=x.device)
+    call("pe_causal_conv", _CONV.pack(*_conv_fields(lay, x, weight, bias, init, cu, out, state)), lay[2])
     return out, state
 
 
 class _CausalConv(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, init, cu, nseq, silu, want_state):
+    def forward(ctx, x, weight, bias, init, cu, lay, want_state):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, init, cu)
-        ctx.plan = nseq, silu
-        out, state = _conv_forward(x, weight, bias, init, cu, nseq, silu, want_state)
+        ctx.lay = lay
+        out, state = _conv_forward(lay, x, weight, bias, init, cu, want_state)
         return (out, state) if want_state else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dstate=None):
         x, weight, bias, init, cu = ctx.saved_tensors
-        nseq, silu = ctx.plan
-        B, T, C = x.shape
-        dev, dt = x.device, x.dtype
-        dout = torch.zeros((B, T, C), dtype=dt, device=dev) if dout is None else rows(dout)
+        lay, dev, dt = ctx.lay, x.device, x.dtype
+        dout = torch.zeros(x.shape, dtype=dt, device=dev) if dout is None else rows(dout)
         dstate = None if dstate is None else dstate.contiguous()
-        dx = torch.empty((B, T, C), dtype=dt, device=dev)
+        dx = torch.empty(x.shape, dtype=dt, device=dev)
         dw = torch.empty(weight.shape, dtype=dt, device=dev)
-        db = torch.empty(C, dtype=dt, device=dev) if bias is not None else None
+        db = torch.empty(bias.shape, dtype=dt, device=dev) if bias is not None else None
         dinit = torch.empty(init.shape, dtype=dt, device=dev) if init is not None else None
-        fields = (*_conv_fields(x, weight, bias, init, cu, nseq, silu, None, None), dout.data_ptr(), ptr(dstate),
+        fields = (*_conv_fields(lay, x, weight, bias, init, cu, None, None), dout.data_ptr(), ptr(dstate),
                   stride(dout, 0), stride(dout, 1), dx.data_ptr(), ptr(dinit), dw.data_ptr(), ptr(db))
-        nbytes = _ops.sized("pe_causal_conv_grad_ws_bytes", _CONV_GRAD.pack(*fields, 0, 0), dev)
+        nbytes = _ops.sized("pe_causal_conv_grad_ws_bytes", _CONV_GRAD.pack(*fields, 0, 0), lay[2])
         ws = _ops.workspace(nbytes, dev)
-        call("pe_causal_conv_grad", _CONV_GRAD.pack(*fields, ptr(ws), nbytes), dev)
-        return dx, dw, db, dinit, None, None, None, None
+        call("pe_causal_conv_grad", _CONV_GRAD.pack(*fields, ptr(ws), nbytes), lay[2])
+        return dx, dw, db, dinit, None, None, None
 
 
 def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, cu_seqlens=None,
@@ -120,19 +126,29 @@ def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, cu
     W - 1 inputs of each sequence [S, W - 1, C], for `causal_conv_step` or the next
     piece of the prompt. All tensors have x's type; x's channels are contiguous, its
     other strides are free."""
-    silu = _silu(activation)
-    check_activations("x", x, (3,))
-    W = _check_filter(x, weight, bias)
-    B, T, C = x.shape
-    cu, nseq = offsets(cu_seqlens, B, T, x.device)
-    if initial_state is not None:
-        check_tensor("initial_state", initial_state, (nseq, W - 1, C), x.dtype, x.device)
-        initial_state = initial_state.contiguous()
-    x, weight = rows(x), weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    cu = cu_seqlens
+    try:
+        key = ("conv", activation, sig(x), sig(weight), sig(bias), sig(initial_state), sig(cu))
+        lay = plan(key)
+    except (AttributeError, TypeError):      # not tensors: the checks say which
+        key = lay = None
+    if lay is None:
+        silu = _silu(activation)
+        check_activations("x", x, (3,))
+        W = _check_filter(x, weight, bias)
+        B, T, C = x.shape
+        cu, nseq = offsets(cu_seqlens, B, T, x.device)
+        if initial_state is not None:
+            check_tensor("initial_state", initial_state, (nseq, W - 1, C), x.dtype, x.device)
+        given = (x, weight, bias, initial_state, cu_seqlens)
+        x, weight = rows(x), weight.contiguous()
+        bias, initial_state = _opt(bias, torch.Tensor.contiguous), _opt(initial_state, torch.Tensor.contiguous)
+        lay = _conv_layout(x, weight, nseq, silu)
+        if key is not None and all(a is b for a, b in zip(given, (x, weight, bias, initial_state, cu))):
+            _ops.keep_plan(key, lay)
     if wants_grad(x, weight, bias, initial_state):
-        return _CausalConv.apply(x, weight, bias, initial_state, cu, nseq, silu, return_state)
-    out, state = _conv_forward(x, weight, bias, initial_state, cu, nseq, silu, return_state)
+        return _CausalConv.apply(x, weight, bias, initial_state, cu, lay, return_state)
+    out, state = _conv_forward(lay, x, weight, bias, initial_state, cu, return_state)
     return (out, state) if return_state else out
 
 
@@ -142,27 +158,42 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     state [S, W - 1, C] (contiguous, x's type) is shifted in place: row slots[b] of it
     belongs to request b (row b without slots, S = B). Rows with a negative slot give 0
     and touch no state; two requests must not share a slot."""
-    silu = _silu(activation)
-    check_activations("x", x, (2,))
-    W = _check_filter(x, weight, bias)
-    B, C = x.shape
-    dev = x.device
-    _check_state("state", state, x.dtype, dev, (W - 1, C), B, slots)
-    s32, s64 = _ops.slot_pointers(slots, B, dev)
-    x, weight = rows(x), weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    out = torch.empty((B, C), dtype=x.dtype, device=dev)
+    try:
+        key = ("conv step", activation, sig(x), sig(state), sig(weight), sig(bias), sig(slots))
+        ints = plan(key)
+    except (AttributeError, TypeError):      # not tensors: the checks say which
+        key = ints = None
+    if ints is None:
+        silu = _silu(activation)
+        check_activations("x", x, (2,))
+        W = _check_filter(x, weight, bias)
+        B, C = x.shape
+        _check_state("state", state, x.dtype, x.device, (W - 1, C), B, slots)
+        _ops.check_slots(slots, B, x.device)
+        if any(t is not None and not t.is_contiguous() for t in (weight, bias)) or rows(x) is not x:
+            key = None
+            x, weight = rows(x), weight.contiguous()
+            bias = None if bias is None else bias.contiguous()
+        ints = (DTYPES[x.dtype], silu, W, B, C, state.shape[0], stride(x, 0), x.device.index)
+        if key is not None:
+            _ops.keep_plan(key, ints)
+    _no_grad_state(state)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s32, s64 = _ops.slot_pointers(slots)
     call("pe_causal_conv_step", _CONV_STEP.pack(
-        DTYPES[x.dtype], silu, W, B, C, state.shape[0], s32, s64, x.data_ptr(), weight.data_ptr(), ptr(bias),
-        stride(x, 0), state.data_ptr(), out.data_ptr()), dev)
+        *ints[:6], s32, s64, x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), ints[6],
+        state.data_ptr(), out.data_ptr()), ints[7])
     return out
+
+
+def _no_grad_state(state):
+    if state.requires_grad and torch.is_grad_enabled():
+        raise ValueError("state is updated in place and cannot require a gradient")
 
 
 def _check_state(name, state, dtype, dev, tail, batch, slots):
     if not isinstance(state, torch.Tensor) or state.dim() != 3:
         raise ValueError(f"{name} must have three dimensions, one row of {tail} a slot")
-    if state.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} is updated in place and cannot require a gradient")
     n = state.shape[0] if slots is not None else batch
     check_tensor(name, state, (n, *tail), dtype, dev)
     if not state.is_contiguous():
@@ -205,52 +236,50 @@ def _opt(t, f):
     return None if t is None else f(t)
 
 
-def _scan_fields(u, delta, A, B, C, D, z, bias, h0, cu, nseq, softplus, out, state, ckpt):
-    Bn, T, Dc = u.shape
-    return (DTYPES[u.dtype], softplus, Bn, T, Dc, A.shape[1], B.shape[2], nseq, ptr(cu), u.data_ptr(),
-            delta.data_ptr(), ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), ptr(D), ptr(bias), ptr(h0),
-            stride(u, 0), stride(u, 1), stride(delta, 0), stride(delta, 1), *((stride(z, 0), stride(z, 1)) if z is not None else (0, 0)),
-            stride(B, 0), stride(B, 1), stride(B, 2), stride(C, 0), stride(C, 1), stride(C, 2),
-            ptr(out), ptr(state), ptr(ckpt))
+def _scan_layout(u, delta, A, B, C, z, nseq, softplus):
+    zs = (0, 0) if z is None else (stride(z, 0), stride(z, 1))
+    return ((DTYPES[u.dtype], softplus, *u.shape, A.shape[1], B.shape[-2], nseq),
+            (stride(u, 0), stride(u, 1), stride(delta, 0), stride(delta, 1), *zs, stride(B, 0), stride(B, 1),
+             stride(B, -2), stride(C, 0), stride(C, 1), stride(C, -2)), u.device.index)
 
 
-def _scan_forward(u, delta, A, B, C, D, z, bias, h0, cu, nseq, softplus, want_state, want_ckpt):
-    Bn, T, Dc = u.shape
-    dev, N = u.device, A.shape[1]
-    out = torch.empty((Bn, T, Dc), dtype=u.dtype, device=dev)
-    state = torch.empty((nseq, Dc, N), dtype=torch.float32, device=dev) if want_state else None
-    ckpt = None
-    if want_ckpt:
-        ckpt = torch.empty(_core_ckpt(T, nseq, cu is not None, Dc, N), dtype=torch.float32, device=dev)
-    fields = _scan_fields(u, delta, A, B, C, D, z, bias, h0, cu, nseq, softplus, out, state, ckpt)
-    nbytes = _ops.sized("pe_scan_ws_bytes", _SCAN.pack(*fields, 0, 0), dev)
+def _scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, out, state, ckpt):
+    return (*lay[0], ptr(cu), u.data_ptr(), delta.data_ptr(), ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(),
+            ptr(D), ptr(bias), ptr(h0), *lay[1], ptr(out), ptr(state), ptr(ckpt))
+
+
+def _scan_forward(lay, u, delta, A, B, C, D, z, bias, h0, cu, want_state, want_ckpt):
+    dev, f32 = u.device, torch.float32
+    _, _, _, T, Dc, N, _, nseq = lay[0]
+    out = torch.empty(u.shape, dtype=u.dtype, device=dev)
+    state = torch.empty((nseq, Dc, N), dtype=f32, device=dev) if want_state else None
+    ckpt = torch.empty(_core_ckpt(T, nseq, cu is not None, Dc, N), dtype=f32, device=dev) if want_ckpt else None
+    fields = _scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, out, state, ckpt)
+    nbytes = _ops.sized("pe_scan_ws_bytes", _SCAN.pack(*fields, 0, 0), lay[2])
     ws = _ops.workspace(nbytes, dev)
-    call("pe_selective_scan", _SCAN.pack(*fields, ptr(ws), nbytes), dev)
+    call("pe_selective_scan", _SCAN.pack(*fields, ptr(ws), nbytes), lay[2])
     return out, state, ckpt
 
 
 def _core_ckpt(tokens, nseq, packed, channels, states) -> int:
-    import ctypes
-    fn = _ops.core_lib().pe_scan_ckpt_floats
-    fn.argtypes, fn.restype = [ctypes.c_int64] * 5, ctypes.c_int64
+    fn = _ops.function("pe_scan_ckpt_floats", restype=ctypes.c_int64, argtypes=[ctypes.c_int64] * 5)
     return fn(tokens, nseq, int(packed), channels, states)
 
 
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, cu, nseq, softplus, want_state):
+    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, cu, lay, want_state):
         ctx.set_materialize_grads(False)
-        out, state, ckpt = _scan_forward(u, delta, A, B, C, D, z, bias, h0, cu, nseq, softplus, want_state, True)
+        out, state, ckpt = _scan_forward(lay, u, delta, A, B, C, D, z, bias, h0, cu, want_state, True)
         ctx.save_for_backward(u, delta, A, B, C, D, z, bias, h0, cu, ckpt)
-        ctx.plan = nseq, softplus
+        ctx.lay = lay
         return (out, state) if want_state else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dstate=None):
         u, delta, A, B, C, D, z, bias, h0, cu, ckpt = ctx.saved_tensors
-        nseq, softplus = ctx.plan
-        dev, dt, f32 = u.device, u.dtype, torch.float32
+        lay, dev, dt, f32 = ctx.lay, u.device, u.dtype, torch.float32
         dout = torch.zeros(u.shape, dtype=dt, device=dev) if dout is None else rows(dout)
         dstate = _opt(dstate, torch.Tensor.contiguous)
 
@@ -259,13 +288,13 @@ class _SelectiveScan(torch.autograd.Function):
 
         du, ddelta, dz, dB, dC = (like(t, dt) for t in (u, delta, z, B, C))
         dA, dD, dbias, dh0 = (like(t, f32) for t in (A, D, bias, h0))
-        fields = (*_scan_fields(u, delta, A, B, C, D, z, bias, h0, cu, nseq, softplus, None, None, ckpt), 0, 0,
+        fields = (*_scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, None, None, ckpt), 0, 0,
                   dout.data_ptr(), stride(dout, 0), stride(dout, 1), ptr(dstate), ptr(du), ptr(ddelta), ptr(dz),
                   ptr(dB), ptr(dC), ptr(dA), ptr(dD), ptr(dbias), ptr(dh0))
-        nbytes = _ops.sized("pe_scan_grad_ws_bytes", _SCAN_GRAD.pack(*fields, 0, 0), dev)
+        nbytes = _ops.sized("pe_scan_grad_ws_bytes", _SCAN_GRAD.pack(*fields, 0, 0), lay[2])
         ws = _ops.workspace(nbytes, dev)
-        call("pe_selective_scan_grad", _SCAN_GRAD.pack(*fields, ptr(ws), nbytes), dev)
-        return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None
+        call("pe_selective_scan_grad", _SCAN_GRAD.pack(*fields, ptr(ws), nbytes), lay[2])
+        return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None
 
 
 def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softplus: bool = False,
@@ -277,21 +306,31 @@ def selective_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_
     channels in G equal groups. initial_state [S, Dc, N] float32 (zeros without it).
     Returns out [Bt, T, Dc], and with return_state the last states [S, Dc, N]
     float32. The last axes are contiguous, other strides are free."""
-    check_activations("u", u, (3,))
-    B, C = _check_scan(u, delta, A, B, C, D, z, delta_bias, u.shape[:2])
-    cu, nseq = offsets(cu_seqlens, u.shape[0], u.shape[1], u.device)
-    if initial_state is not None:
-        check_tensor("initial_state", initial_state, (nseq, *A.shape), torch.float32, u.device)
-        initial_state = initial_state.contiguous()
-    u, delta, B, C = rows(u), rows(delta), rows(B), rows(C)
-    z, A = _opt(z, rows), A.contiguous()
-    D, delta_bias = _opt(D, torch.Tensor.contiguous), _opt(delta_bias, torch.Tensor.contiguous)
-    softplus = int(bool(delta_softplus))
+    cu = cu_seqlens
+    try:
+        key = ("scan", delta_softplus, sig(u), sig(delta), sig(A), sig(B), sig(C), sig(D), sig(z), sig(delta_bias),
+               sig(initial_state), sig(cu))
+        lay = plan(key)
+    except (AttributeError, TypeError):      # not tensors: the checks say which
+        key = lay = None
+    if lay is None:
+        check_activations("u", u, (3,))
+        given = (u, delta, A, B, C, D, z, delta_bias, initial_state, cu_seqlens)
+        B, C = _check_scan(u, delta, A, B, C, D, z, delta_bias, u.shape[:2])
+        cu, nseq = offsets(cu_seqlens, u.shape[0], u.shape[1], u.device)
+        if initial_state is not None:
+            check_tensor("initial_state", initial_state, (nseq, *A.shape), torch.float32, u.device)
+            initial_state = initial_state.contiguous()
+        u, delta, B, C = rows(u), rows(delta), rows(B), rows(C)
+        z, A = _opt(z, rows), A.contiguous()
+        D, delta_bias = _opt(D, torch.Tensor.contiguous), _opt(delta_bias, torch.Tensor.contiguous)
+        lay = _scan_layout(u, delta, A, B, C, z, nseq, int(bool(delta_softplus)))
+        if key is not None and all(a is b for a, b in zip(given, (u, delta, A, B, C, D, z, delta_bias, initial_state,
+                                                                  cu))):
+            _ops.keep_plan(key, lay)
     if wants_grad(u, delta, A, B, C, D, z, delta_bias, initial_state):
-        return _SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, cu, nseq, softplus,
-                                    return_state)
-    out, state, _ = _scan_forward(u, delta, A, B, C, D, z, delta_bias, initial_state, cu, nseq, softplus,
-                                  return_state, False)
+        return _SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, cu, lay, return_state)
+    out, state, _ = _scan_forward(lay, u, delta, A, B, C, D, z, delta_bias, initial_state, cu, return_state, False)
     return (out, state) if return_state else out
 
 
@@ -303,21 +342,37 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     state [S, Dc, N] float32 (contiguous) is updated in place, in row slots[b] for
     request b (row b without slots, S = Bt). Rows with a negative slot give 0 and touch
     no state; two requests must not share a slot."""
-    check_activations("u", u, (2,))
-    Bt, Dc = u.shape
-    dev = u.device
-    B, C = _check_scan(u, delta, A, B, C, D, z, delta_bias, (Bt,))
-    _check_state("state", state, torch.float32, dev, tuple(A.shape), Bt, slots)
-    s32, s64 = _ops.slot_pointers(slots, Bt, dev)
-    u, delta, B, C = rows(u), rows(delta), rows(B), rows(C)
-    z, A = _opt(z, rows), A.contiguous()
-    D, delta_bias = _opt(D, torch.Tensor.contiguous), _opt(delta_bias, torch.Tensor.contiguous)
-    out = torch.empty((Bt, Dc), dtype=u.dtype, device=dev)
+    try:
+        key = ("scan step", delta_softplus, sig(state), sig(u), sig(delta), sig(A), sig(B), sig(C), sig(D), sig(z),
+               sig(delta_bias), sig(slots))
+        ints = plan(key)
+    except (AttributeError, TypeError):
+        key = ints = None
+    if ints is None:
+        check_activations("u", u, (2,))
+        Bt, Dc = u.shape
+        dev = u.device
+        B, C = _check_scan(u, delta, A, B, C, D, z, delta_bias, (Bt,))
+        _check_state("state", state, torch.float32, dev, tuple(A.shape), Bt, slots)
+        _ops.check_slots(slots, Bt, dev)
+        given = (u, delta, B, C, z, A, D, delta_bias)
+        u, delta, B, C = rows(u), rows(delta), rows(B), rows(C)
+        z, A = _opt(z, rows), A.contiguous()
+        D, delta_bias = _opt(D, torch.Tensor.contiguous), _opt(delta_bias, torch.Tensor.contiguous)
+        if any(a is not b for a, b in zip(given, (u, delta, B, C, z, A, D, delta_bias))):
+            key = None
+        ints = ((DTYPES[u.dtype], int(bool(delta_softplus)), Bt, Dc, A.shape[1], B.shape[1], state.shape[0]),
+                (stride(u, 0), stride(delta, 0), 0 if z is None else stride(z, 0), stride(B, 0), stride(B, 1),
+                 stride(C, 0), stride(C, 1)), dev.index)
+        if key is not None:
+            _ops.keep_plan(key, ints)
+    _no_grad_state(state)
+    out = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    s32, s64 = _ops.slot_pointers(slots)
     call("pe_selective_scan_step", _SCAN_STEP.pack(
-        DTYPES[u.dtype], int(bool(delta_softplus)), Bt, Dc, A.shape[1], B.shape[1], state.shape[0], s32, s64,
-        u.data_ptr(), delta.data_ptr(), ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), ptr(D), ptr(delta_bias),
-        stride(u, 0), stride(delta, 0), 0 if z is None else stride(z, 0), stride(B, 0), stride(B, 1), stride(C, 0),
-        stride(C, 1), state.data_ptr(), out.data_ptr()), dev)
+        *ints[0], s32, s64, u.data_ptr(), delta.data_ptr(), 0 if z is None else z.data_ptr(), B.data_ptr(),
+        C.data_ptr(), A.data_ptr(), 0 if D is None else D.data_ptr(),
+        0 if delta_bias is None else delta_bias.data_ptr(), *ints[1], state.data_ptr(), out.data_ptr()), ints[2])
     return out
 
 
