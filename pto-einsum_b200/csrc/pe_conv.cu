@@ -5,16 +5,18 @@
 //   g = dout act'(p),  dx[i] = sum_j w[W - 1 - j] g[i + j],  dw[k] = sum_t g[t] x[t - (W - 1) + k]
 //
 // All of it is bound by memory: two FMAs a tap against 2 (forward) or 3 (backward)
-// elements moved. A thread owns 16 bytes of channels and walks a tile of tokens with
-// the last W - 1 inputs in registers, four tokens' loads in flight, so that each
-// input is read once apart from the W - 1 tokens before (after) a tile.
+// elements moved (and, with silu, two special-function operations an element, which is
+// three quarters of the memory's time). A thread owns 16 bytes of channels and walks a
+// tile of tokens with the last W - 1 inputs in registers and the next seven on their
+// way to its own slots of shared memory, so that each input is read once apart from
+// the W - 1 tokens before (after) a tile.
 #include "pe_mixer.cuh"
 
 namespace pe {
 
 namespace {
 
-constexpr int U = 4;          // tokens loaded ahead
+constexpr int DEPTH = 8;      // slots of a thread's queue: seven tokens on their way
 constexpr int kBlock = 256;
 constexpr int kSiteOffsets = 34, kSiteSlot = 35;
 
@@ -29,42 +31,87 @@ struct ConvP {
     T *out, *state;
 };
 
+// V channels as pairs; a single channel is a pair whose other half stays zero.
+template <int V>
+constexpr int kPairs = (V + 1) / 2;
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Vec<T, V>& r, f32x2 (&f)[kPairs<V>]) {
+    if constexpr (V == 1)
+        f[0] = pack2(to_float(r.v[0]), 0.0f);
+    else
+        unpack_pairs(r, f);
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(const f32x2 (&f)[kPairs<V>]) {
+    if constexpr (V == 1) {
+        float lo, hi;
+        unpack2(f[0], lo, hi);
+        Vec<T, 1> r;
+        r.v[0] = from_float<T>(lo);
+        return r;
+    } else {
+        return pack_pairs<T, V>(f);
+    }
+}
+
 template <typename T, int W, int V>
 struct Filter {
-    float w[W][V], b[V];
+    static constexpr int Q = kPairs<V>;
+    f32x2 w[W][Q], b[Q];
     // weight [C][W]: the V channels' taps are V W consecutive elements, W loads
     __device__ __forceinline__ void load(const T* weight, const T* bias, int64_t c) {
-        Vec<T, V> r[W];
+        Vec<T, V> r[W], rb;
 #pragma unroll
         for (int k = 0; k < W; ++k) r[k] = load_vec<T, V>(weight + c * W + k * V);
+        if (bias) rb = load_vec<T, V>(bias + c);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            b[v] = 0.0f;
+        for (int k = 0; k < W; ++k) {
+            Vec<T, V> tap;
 #pragma unroll
-            for (int k = 0; k < W; ++k) w[k][v] = to_float(r[(v * W + k) / V].v[(v * W + k) % V]);
+            for (int v = 0; v < V; ++v) tap.v[v] = r[(v * W + k) / V].v[(v * W + k) % V];
+            widen<T, V>(tap, w[k]);
         }
-        if (bias) unpack(load_vec<T, V>(bias + c), b);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) b[q] = 0;
+        if (bias) widen<T, V>(rb, b);
+    }
+    __device__ __forceinline__ void apply(const f32x2 (&win)[W][Q], f32x2 (&p)[Q]) const {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            p[q] = b[q];
+#pragma unroll
+            for (int k = 0; k < W; ++k) p[q] = fma2(w[k][q], win[k][q], p[q]);
+        }
     }
 };
+template <int W, int Q>
+__device__ __forceinline__ void shift(f32x2 (&win)[W][Q]) {
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) win[k][q] = win[k + 1][q];
+}
 
 // Inputs before token `pos` (counted from the sequence's start): win[j] = x[pos - (W - 1) + j].
 template <typename T, int W, int V>
 __device__ __forceinline__ void load_before(const ConvP<T>& p, const T* xs, int64_t pos, int s, int64_t c,
-                                            float (&win)[W][V]) {
+                                            f32x2 (&win)[W][kPairs<V>]) {
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
         const int64_t i = pos - (W - 1) + j;
 #pragma unroll
-        for (int v = 0; v < V; ++v) win[j][v] = 0.0f;
+        for (int q = 0; q < kPairs<V>; ++q) win[j][q] = 0;
         if (i >= 0)
-            unpack(load_vec<T, V>(xs + i * p.x_st + c), win[j]);
+            widen<T, V>(load_vec<T, V>(xs + i * p.x_st + c), win[j]);
         else if (p.init)
-            unpack(load_vec<T, V>(p.init + ((int64_t)s * (W - 1) + (W - 1) + i) * p.C + c), win[j]);
+            widen<T, V>(load_vec<T, V>(p.init + ((int64_t)s * (W - 1) + (W - 1) + i) * p.C + c), win[j]);
     }
 }
 
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kBlock, 2) conv_fwd(const __grid_constant__ ConvP<T> p) {
+    constexpr int Q = kPairs<V>;
+    __shared__ __align__(16) Vec<T, V> queue[DEPTH * kBlock];
     if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.seqs, threadIdx.x, kSiteOffsets);
     int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
     const int64_t tile = id / p.CV, c = (id - tile * p.CV) * V;
@@ -74,51 +121,59 @@ __global__ void __launch_bounds__(kBlock, 2) conv_fwd(const __grid_constant__ Co
         if (!p.state || s >= p.seqs.nseq) return;
         const Span sp = seq_span(p.seqs, (int)s);
         const T* xs = p.x + sp.row * p.x_sb + sp.start * p.x_st;
-        float win[W][V];
+        f32x2 win[W][Q];
         load_before<T, W, V>(p, xs, sp.len, (int)s, c, win);
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) store_vec(p.state + (s * (W - 1) + j) * p.C + c, pack<T, V>(win[j]));
+        for (int j = 0; j < W - 1; ++j) store_vec(p.state + (s * (W - 1) + j) * p.C + c, narrow<T, V>(win[j]));
         return;
     }
-    Filter<T, W, V> f;
-    f.load(p.w, p.bias, c);
     const int64_t per = ceil_div(p.seqs.tokens, p.tile);   // tiles a row
     int64_t t = tile % per * p.tile;
     const int64_t end = min(p.seqs.tokens, t + p.tile);
+    const T* xr = p.x + (p.seqs.cu ? 0 : tile / per) * p.x_sb + c;
+    // the tile's inputs, DEPTH - 1 tokens ahead: a slot is filled again one token after it was read
+    Ring<T, V, DEPTH> ring(queue, kBlock);
+    const T* ahead = xr + t * p.x_st;
+    int left = (int)(end - t);   // tokens not yet on their way
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i, ahead += p.x_st, --left) {
+        ring.fetch(i, ahead, left > 0);
+        cp_commit();
+    }
+    Filter<T, W, V> f;
+    f.load(p.w, p.bias, c);
+    int slot = 0;
     int s = p.seqs.cu ? seq_of_token(p.seqs, t) : (int)(tile / per);
     for (; t < end && s < p.seqs.nseq; ++s) {
         const Span sp = seq_span(p.seqs, s);
         const int64_t stop = min(end, sp.start + sp.len);   // of the tile's tokens in this sequence
         if (stop <= t || sp.start > t) continue;
-        const T* xr = p.x + sp.row * p.x_sb + c;
-        T* o = p.out + sp.row * p.seqs.tokens * p.C + c;
-        float win[W][V];
+        T* o = p.out + (sp.row * p.seqs.tokens + t) * p.C + c;
+        f32x2 win[W][Q];
         load_before<T, W, V>(p, xr - c + sp.start * p.x_st, t - sp.start, s, c, win);
-        auto token = [&](const Vec<T, V>& raw, T* to) {
-            unpack(raw, win[W - 1]);
-            float y[V];
+#pragma unroll 4
+        for (; t < stop; ++t, ++slot, o += p.C) {
+            cp_wait_but<DEPTH - 2>();
+            widen<T, V>(ring.get(slot), win[W - 1]);
+            ring.fetch(slot + DEPTH - 1, ahead, left > 0);
+            cp_commit();
+            ahead += p.x_st;
+            --left;
+            f32x2 y[Q];
+            f.apply(win, y);
+            if (p.silu) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float a = f.b[v];
-#pragma unroll
-                for (int k = 0; k < W; ++k) a = fmaf(f.w[k][v], win[k][v], a);
-                y[v] = p.silu ? a * sigmoidf(a) : a;
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) win[k][v] = win[k + 1][v];
+                for (int q = 0; q < Q; ++q) {
+                    float lo, hi;
+                    unpack2(y[q], lo, hi);
+                    y[q] = mul2(y[q], pack2(sigmoidf(lo), sigmoidf(hi)));
+                }
             }
-            store_vec(to, pack<T, V>(y));
-        };
-        const T* xt = xr + t * p.x_st;
-        T* ot = o + t * p.C;
-        for (; t + U <= stop; t += U, xt += U * p.x_st, ot += U * p.C) {
-            Vec<T, V> raw[U];
-#pragma unroll
-            for (int i = 0; i < U; ++i) raw[i] = load_vec<T, V>(xt + i * p.x_st);
-#pragma unroll
-            for (int i = 0; i < U; ++i) token(raw[i], ot + i * p.C);
+            shift(win);
+            store_vec(o, narrow<T, V>(y));
         }
-        for (; t < stop; ++t, xt += p.x_st, ot += p.C) token(load_vec<T, V>(xt), ot);
     }
+    cp_wait();
 }
 
 // ---- backward -------------------------------------------------------------------
@@ -134,139 +189,123 @@ struct ConvGradP {
 
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kBlock, 2) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
-    __shared__ float red[(W + 1) * V * kBlock];
+    constexpr int Q = kPairs<V>;
+    // the queues, and once they are empty the block's sums
+    extern __shared__ __align__(16) unsigned char shared[];
     const ConvP<T>& f = p.f;
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) check_offsets(f.seqs, threadIdx.x, kSiteOffsets);
     const int by = kBlock / p.bx, x = threadIdx.x % p.bx, y = threadIdx.x / p.bx;
     const int64_t cv = (int64_t)blockIdx.y * p.bx + x, c = cv * V;
     const int64_t tile = (int64_t)blockIdx.x * by + y;
-    float dw[W][V], db[V];
+    f32x2 dw[W][Q], db[Q];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        db[v] = 0.0f;
+    for (int q = 0; q < Q; ++q) {
+        db[q] = 0;
 #pragma unroll
-        for (int k = 0; k < W; ++k) dw[k][v] = 0.0f;
+        for (int k = 0; k < W; ++k) dw[k][q] = 0;
     }
     if (cv < f.CV && tile < f.tiles) {
-        Filter<T, W, V> flt;
-        flt.load(f.w, f.bias, c);
         const int64_t per = ceil_div(f.seqs.tokens, f.tile);
         int64_t t = tile % per * f.tile;
-        const int64_t end = min(f.seqs.tokens, t + f.tile);
-        int s = f.seqs.cu ? seq_of_token(f.seqs, t) : (int)(tile / per);
+        const int64_t end = min(f.seqs.tokens, t + f.tile), row = f.seqs.cu ? 0 : tile / per;
+        const T* xr = f.x + row * f.x_sb + c;
+        const T* dor = p.dout + row * p.o_sb + c;
+        Vec<T, V>* queues = reinterpret_cast<Vec<T, V>*>(shared);
+        Ring<T, V, DEPTH> rx(queues, kBlock), ro(queues + DEPTH * kBlock, kBlock);
+        Filter<T, W, V> flt;
+        flt.load(f.w, f.bias, c);
+        int s = f.seqs.cu ? seq_of_token(f.seqs, t) : (int)row;
         for (; t < end && s < f.seqs.nseq; ++s) {
             const Span sp = seq_span(f.seqs, s);
             const int64_t fin = sp.start + sp.len, stop = min(end, fin);
             if (stop <= t || sp.start > t) continue;
-            const T* xr = f.x + sp.row * f.x_sb + c;
-            const T* dor = p.dout + sp.row * p.o_sb + c;
             T* dx = p.dx + sp.row * f.seqs.tokens * f.C + c;
-            float win[W][V], g[W][V];   // inputs and g of the tokens up to the current one
+            // g of the tokens t .. stop + W - 2 gives dx of t .. stop - 1 (and of the
+            // inputs before the sequence where t starts it)
+            const int64_t last = stop + W - 1, have = min(last, fin);
+            int64_t ahead = t;
+#pragma unroll
+            for (int i = 0; i < DEPTH - 1; ++i, ++ahead) {
+                rx.fetch(i, xr + ahead * f.x_st, ahead < have);
+                ro.fetch(i, dor + ahead * p.o_st, ahead < have);
+                cp_commit();
+            }
+            f32x2 win[W][Q], g[W][Q];   // inputs and g of the tokens up to the current one
             load_before<T, W, V>(f, xr - c + sp.start * f.x_st, t - sp.start, s, c, win);
 #pragma unroll
             for (int k = 0; k < W; ++k)
 #pragma unroll
-                for (int v = 0; v < V; ++v) g[k][v] = 0.0f;
-            // g of the tokens t .. stop + W - 2 gives dx of t .. stop - 1 (and of the
-            // inputs before the sequence where t starts it)
-            const int64_t last = stop + W - 1;
-            // a token's g, into the sums if it is the tile's own
-            auto slope = [&](const Vec<T, V>& rx, const Vec<T, V>& ro, bool own) {
-                unpack(rx, win[W - 1]);
-                unpack(ro, g[W - 1]);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
+                for (int q = 0; q < Q; ++q) g[k][q] = 0;
+            int slot = 0;
+#pragma unroll 4
+            for (int64_t k = t; k < last; ++k, ++slot, ++ahead) {
+                cp_wait_but<DEPTH - 2>();
+                widen<T, V>(rx.get(slot), win[W - 1]);
+                widen<T, V>(ro.get(slot), g[W - 1]);
+                rx.fetch(slot + DEPTH - 1, xr + ahead * f.x_st, ahead < have);
+                ro.fetch(slot + DEPTH - 1, dor + ahead * p.o_st, ahead < have);
+                cp_commit();
+                if (k < fin) {
                     if (f.silu) {
-                        float a = flt.b[v];
+                        f32x2 a[Q];
+                        flt.apply(win, a);
 #pragma unroll
-                        for (int q = 0; q < W; ++q) a = fmaf(flt.w[q][v], win[q][v], a);
-                        g[W - 1][v] *= silu_slope(a, sigmoidf(a));
+                        for (int q = 0; q < Q; ++q) {
+                            float lo, hi;
+                            unpack2(a[q], lo, hi);
+                            g[W - 1][q] = mul2(g[W - 1][q], pack2(silu_slope(lo, sigmoidf(lo)), silu_slope(hi, sigmoidf(hi))));
+                        }
                     }
-                    if (own) {
-                        db[v] += g[W - 1][v];
+                    if (k < stop) {   // the tile's own: into the sums
 #pragma unroll
-                        for (int q = 0; q < W; ++q) dw[q][v] = fmaf(g[W - 1][v], win[q][v], dw[q][v]);
+                        for (int q = 0; q < Q; ++q) {
+                            db[q] = add2(db[q], g[W - 1][q]);
+#pragma unroll
+                            for (int j = 0; j < W; ++j) dw[j][q] = fma2(g[W - 1][q], win[j][q], dw[j][q]);
+                        }
                     }
+                } else {
 #pragma unroll
-                    for (int q = 0; q < W - 1; ++q) win[q][v] = win[q + 1][v];
+                    for (int q = 0; q < Q; ++q) g[W - 1][q] = 0;
                 }
-            };
-            auto sum_taps = [&](float (&d)[V]) {
+                shift(win);
+                // dx of the input W - 1 tokens back, whose sum this completes
+                f32x2 d[Q];
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    d[v] = 0.0f;
+                for (int q = 0; q < Q; ++q) {
+                    d[q] = mul2(flt.w[W - 1][q], g[0][q]);
 #pragma unroll
-                    for (int j = 0; j < W; ++j) d[v] = fmaf(flt.w[W - 1 - j][v], g[j][v], d[v]);
-#pragma unroll
-                    for (int q = 0; q < W - 1; ++q) g[q][v] = g[q + 1][v];
+                    for (int j = 1; j < W; ++j) d[q] = fma2(flt.w[W - 1 - j][q], g[j][q], d[q]);
                 }
-            };
-            // U tokens from k0 on: their g, and dx of the inputs W - 1 earlier, whose sums they
-            // complete. Some may lie past the last one, and some inputs before the tile.
-            auto any = [&](int64_t k0) {
-                Vec<T, V> rx[U], ro[U];
-                const int64_t have = min(last, fin);
+                shift(g);
+                const int64_t i0 = k - (W - 1), pos = i0 - sp.start;
+                const bool first = pos < 0 && t == sp.start && p.dinit;   // an input before the sequence
+                if (i0 < t && !first) continue;
+                const int64_t j = pos + W - 1 - sp.len;                    // its place in the last state
+                if (p.dstate && j >= 0) {
+                    f32x2 e[Q];
+                    widen<T, V>(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
 #pragma unroll
-                for (int i = 0; i < U; ++i)
-                    if (k0 + i < have) {
-                        rx[i] = load_vec<T, V>(xr + (k0 + i) * f.x_st);
-                        ro[i] = load_vec<T, V>(dor + (k0 + i) * p.o_st);
-                    }
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const int64_t k = k0 + i;
-                    if (k >= last) break;
-                    if (k < fin) {
-                        slope(rx[i], ro[i], k < stop);
-                    } else {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) g[W - 1][v] = 0.0f;
-                    }
-                    float d[V];
-                    sum_taps(d);
-                    const int64_t i0 = k - (W - 1), pos = i0 - sp.start;
-                    const bool first = pos < 0 && t == sp.start && p.dinit;   // an input before the sequence
-                    if (i0 < t && !first) continue;
-                    const int64_t j = pos + W - 1 - sp.len;                    // its place in the last state
-                    if (p.dstate && j >= 0) {
-                        float e[V];
-                        unpack(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
-#pragma unroll
-                        for (int v = 0; v < V; ++v) d[v] += e[v];
-                    }
-                    T* to = first ? p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c : dx + i0 * f.C;
-                    store_vec(to, pack<T, V>(d));
+                    for (int q = 0; q < Q; ++q) d[q] = add2(d[q], e[q]);
                 }
-            };
-#pragma unroll 1
-            for (int64_t k = t; k < last; k += U) {
-                if (k == t || k + U > stop) {
-                    any(k);
-                    continue;
-                }
-                Vec<T, V> rx[U], ro[U];
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    rx[i] = load_vec<T, V>(xr + (k + i) * f.x_st);
-                    ro[i] = load_vec<T, V>(dor + (k + i) * p.o_st);
-                }
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    slope(rx[i], ro[i], true);
-                    float d[V];
-                    sum_taps(d);
-                    store_vec(dx + (k + i - (W - 1)) * f.C, pack<T, V>(d));
-                }
+                T* to = first ? p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c : dx + i0 * f.C;
+                store_vec(to, narrow<T, V>(d));
             }
+            cp_wait();
             t = stop;
         }
     }
     // the block's tiles, in order
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(shared);   // [(W + 1) V][kBlock]
 #pragma unroll
     for (int v = 0; v < V; ++v) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) red[(k * V + v) * kBlock + threadIdx.x] = dw[k][v];
-        red[(W * V + v) * kBlock + threadIdx.x] = db[v];
+        for (int k = 0; k <= W; ++k) {
+            float h[2];
+            unpack2(k < W ? dw[k < W ? k : 0][v / 2] : db[v / 2], h[0], h[1]);
+            red[(k * V + v) * kBlock + threadIdx.x] = h[v % 2];
+        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < (W + 1) * V * p.bx; i += kBlock) {
@@ -303,37 +342,43 @@ struct ConvStepP {
 
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(128) conv_step(const __grid_constant__ ConvStepP<T> p) {
+    constexpr int Q = kPairs<V>;
     const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x;
     const int64_t b = id / p.CV, c = (id - b * p.CV) * V;
     if (b >= p.batch) return;
     int64_t slot = b;
     if (p.s32) slot = __ldg(p.s32 + b);
     if (p.s64) slot = __ldg(p.s64 + b);
-    float y[V];
+    f32x2 y[Q];
     if (slot < 0 || slot >= p.slots) {
         if (slot >= 0 && c == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
 #pragma unroll
-        for (int v = 0; v < V; ++v) y[v] = 0.0f;
-        store_vec(p.out + b * p.C + c, pack<T, V>(y));
+        for (int q = 0; q < Q; ++q) y[q] = 0;
+        store_vec(p.out + b * p.C + c, narrow<T, V>(y));
         return;
     }
     T* st = p.state + slot * (W - 1) * p.C + c;
-    Vec<T, V> win[W];
+    Vec<T, V> raw[W];
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) win[k] = *reinterpret_cast<const Vec<T, V>*>(st + k * p.C);
-    win[W - 1] = load_vec<T, V>(p.x + b * p.x_sb + c);
+    for (int k = 0; k < W - 1; ++k) raw[k] = *reinterpret_cast<const Vec<T, V>*>(st + k * p.C);
+    raw[W - 1] = load_vec<T, V>(p.x + b * p.x_sb + c);
     Filter<T, W, V> f;
     f.load(p.w, p.bias, c);
+    f32x2 win[W][Q];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float a = f.b[v];
+    for (int k = 0; k < W; ++k) widen<T, V>(raw[k], win[k]);
+    f.apply(win, y);
+    if (p.silu) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) a = fmaf(f.w[k][v], to_float(win[k].v[v]), a);
-        y[v] = p.silu ? a * sigmoidf(a) : a;
+        for (int q = 0; q < Q; ++q) {
+            float lo, hi;
+            unpack2(y[q], lo, hi);
+            y[q] = mul2(y[q], pack2(sigmoidf(lo), sigmoidf(hi)));
+        }
     }
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) store_vec(st + k * p.C, win[k + 1]);
-    store_vec(p.out + b * p.C + c, pack<T, V>(y));
+    for (int k = 0; k < W - 1; ++k) store_vec(st + k * p.C, raw[k + 1]);
+    store_vec(p.out + b * p.C + c, narrow<T, V>(y));
 }
 
 // ---- host -------------------------------------------------------------------------
@@ -424,7 +469,12 @@ int conv_grad_run(const pe_conv_grad_args* g, cudaStream_t s) {
     const int64_t cblocks = ceil_div(p.f.CV, sh.bx);
     if (sh.rows > 0x7fffffffll || cblocks > 65535) return PE_ERR_UNSUPPORTED;
     if (sh.rows) {
-        conv_bwd<T, W, V><<<dim3((unsigned)sh.rows, (unsigned)cblocks), kBlock, 0, s>>>(p);
+        const int queues = 2 * DEPTH * kBlock * V * (int)sizeof(T), sums = (W + 1) * V * kBlock * 4;
+        const int smem = queues > sums ? queues : sums;
+        if (smem > 48 * 1024 && cudaFuncSetAttribute(conv_bwd<T, W, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     smem) != cudaSuccess)
+            return PE_ERR_CUDA;
+        conv_bwd<T, W, V><<<dim3((unsigned)sh.rows, (unsigned)cblocks), kBlock, smem, s>>>(p);
         count_launch();
         if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
@@ -502,7 +552,9 @@ int causal_conv(const pe_conv_args* a, cudaStream_t s) {
 int64_t conv_grad_ws_bytes(const pe_conv_grad_args* g) {
     if (!g || check_conv(&g->fwd) != PE_OK) return 0;
     const pe_conv_args* a = &g->fwd;
-    return grad_shape(a, grad_wide(g) ? 4 : 1).rows * a->channels * (a->width + 1) * 4;
+    // enough for either width of the loads: the size does not depend on addresses
+    const int64_t rows = grad_shape(a, 1).rows, wide_rows = a->channels % 4 ? rows : grad_shape(a, 4).rows;
+    return (rows > wide_rows ? rows : wide_rows) * a->channels * (a->width + 1) * 4;
 }
 
 int causal_conv_grad(const pe_conv_grad_args* g, cudaStream_t s) {

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "pe_common.cuh"
 
 namespace pe {
@@ -95,6 +97,98 @@ __device__ __forceinline__ float softplusf(float x) {
     // NaN stays NaN: fmaxf alone would drop it, the product with s does not
     return fmaxf(x, 0.0f) + 2.0f * s * r;
 }
+
+// ---- packed pairs --------------------------------------------------------------
+// Two fp32 lanes in one 64-bit register, one instruction for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
+    float lo, hi;
+    unpack2(x, lo, hi);
+    return pack2(exp2_fast(lo), exp2_fast(hi));
+}
+
+// V elements as V / 2 pairs (V even).
+template <typename T, int V>
+__device__ __forceinline__ void unpack_pairs(const Vec<T, V>& r, f32x2 (&f)[V / 2]) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) f[i] = pack2(to_float(r.v[2 * i]), to_float(r.v[2 * i + 1]));
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> pack_pairs(const f32x2 (&f)[V / 2]) {
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        float lo, hi;
+        unpack2(f[i], lo, hi);
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (std::is_same<T, __half>::value)
+                *reinterpret_cast<__half2*>(&r.v[2 * i]) = __floats2half2_rn(lo, hi);
+            else
+                *reinterpret_cast<__nv_bfloat162*>(&r.v[2 * i]) = __floats2bfloat162_rn(lo, hi);
+        } else {
+            r.v[2 * i] = from_float<T>(lo);
+            r.v[2 * i + 1] = from_float<T>(hi);
+        }
+    }
+    return r;
+}
+
+// ---- asynchronous copies ------------------------------------------------------------
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* dst, const void* src, int valid) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_wait() { cp_wait_but<0>(); }
+
+// A thread's own queue of vectors in shared memory: what it copies only it reads, so the
+// copies need no barrier, and DEPTH of them are under way without holding registers.
+// Slots of a block's threads lie side by side.
+template <typename T, int V, int DEPTH>
+struct Ring {
+    static_assert((DEPTH & (DEPTH - 1)) == 0, "a power of two");
+    using Elem = Vec<T, V>;
+    Elem* at;
+    int stride;
+    __device__ __forceinline__ Ring(Elem* block, int threads) : at(block + threadIdx.x), stride(threads) {}
+    __device__ __forceinline__ void fetch(int slot, const T* src, bool on) {
+        Elem* dst = at + (slot & (DEPTH - 1)) * stride;
+        if constexpr (sizeof(Elem) >= 4) {
+            if (on) cp_async<sizeof(Elem)>(dst, src, sizeof(Elem));
+        } else {
+            if (on) *dst = load_vec<T, V>(src);
+        }
+    }
+    __device__ __forceinline__ Elem get(int slot) const { return at[(slot & (DEPTH - 1)) * stride]; }
+};
 
 // ---- sequences ----------------------------------------------------------------
 // Uniform batches (cu == nullptr): nseq rows of `tokens` tokens. Packed: one row of

@@ -41,9 +41,11 @@ struct NormP {
 template <int NV>
 __device__ __forceinline__ void group_sum(float (&v)[NV], int L, float* red) {
     if (L <= 32) {
-        for (int m = L / 2; m >= 1; m /= 2)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
+        for (int m = 16; m >= 1; m /= 2)
+            if (m < L)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], m);
         return;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -123,20 +125,25 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
         for (int k = 0; k < K; ++k) {
             unpack(x[k], f[k]);
             if (p.mode == kGate) unpack(z[k], ga[k]);
+            float s = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) sum[0] += it.in[k] ? f[k][v] : 0.0f;
+            for (int v = 0; v < V; ++v) s += f[k][v];
+            sum[0] += it.in[k] ? s : 0.0f;
         }
         load(n + R);
         group_sum(sum, L, red);
         const float mean = sum[0] * inv;
         sum[0] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            float s = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 f[k][v] -= mean;
-                sum[0] += it.in[k] ? f[k][v] * f[k][v] : 0.0f;
+                s = fmaf(f[k][v], f[k][v], s);
             }
+            sum[0] += it.in[k] ? s : 0.0f;
+        }
         group_sum(sum, L, red);
         const float rstd = rsqrtf(sum[0] * inv + p.eps);
         if (!live || !on) continue;
@@ -547,6 +554,11 @@ int vec_of(const pe_norm_args* a, std::initializer_list<const void*> more, std::
     return v;
 }
 
+int widest(const pe_norm_args* a) {
+    const int v = a->dtype == PE_F32 ? 4 : 8;
+    return a->channels % v ? 1 : v;
+}
+
 struct Plan {
     int v;            // elements a load
     int lanes, k;     // groups in registers: lanes a group, loads a lane; lanes 0: too large for that
@@ -609,7 +621,7 @@ int launched() {
 }
 
 int64_t stats_floats(const pe_norm_args* a, const Plan& pl) {
-    return pl.lanes ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + (a->mean ? 0 : 2 * a->groups));
+    return pl.lanes ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->groups);
 }
 
 template <typename T, int V>
@@ -703,7 +715,10 @@ Plan grad_plan(const pe_norm_grad_args* g) {
 }  // namespace
 
 int64_t norm_ws_bytes(const pe_norm_args* a) {
-    return check_norm(a) == PE_OK ? stats_floats(a, plan_of(a, vec_of(a, {}, {}), false)) * 4 : 0;
+    if (check_norm(a) != PE_OK) return 0;
+    // enough for either width of the loads: the size does not depend on addresses
+    const int64_t x = stats_floats(a, plan_of(a, 1, false)), y = stats_floats(a, plan_of(a, widest(a), false));
+    return (x > y ? x : y) * 4;
 }
 
 int group_norm(const pe_norm_args* a, cudaStream_t s) {
@@ -717,7 +732,10 @@ int group_norm(const pe_norm_args* a, cudaStream_t s) {
 }
 
 int64_t norm_grad_ws_bytes(const pe_norm_grad_args* g) {
-    return g && check_norm(&g->fwd) == PE_OK ? grad_floats(&g->fwd, grad_plan(g)) * 4 : 0;
+    if (!g || check_norm(&g->fwd) != PE_OK) return 0;
+    const pe_norm_args* a = &g->fwd;
+    const int64_t x = grad_floats(a, plan_of(a, 1, true)), y = grad_floats(a, plan_of(a, widest(a), true));
+    return (x > y ? x : y) * 4;
 }
 
 int group_norm_grad(const pe_norm_grad_args* g, cudaStream_t s) {
@@ -731,7 +749,7 @@ int group_norm_grad(const pe_norm_grad_args* g, cudaStream_t s) {
     }
     if (!a->mean || !a->rstd || !g->dout || !g->dx || (a->gate && !g->dgate)) return PE_ERR_INVALID;
     const Plan pl = grad_plan(g);
-    const int64_t need = grad_floats(a, pl) * 4;
+    const int64_t need = grad_floats(a, pl) * 4;   // pe_group_norm_grad_ws_bytes is that or more
     if (!g->ws || g->ws_bytes < need) return PE_ERR_WORKSPACE;
     return norm_grad_any(g, pl, s);
 }

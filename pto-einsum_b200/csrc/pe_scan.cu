@@ -342,99 +342,131 @@ struct StepP {
     T* out;
 };
 
-// A lane has four states of one channel, LPC lanes a channel, for RB requests: A is read
+// Eight consecutive fp32, one 32-byte access each way (32-byte aligned).
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+    asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"f"(f[0]), "f"(f[1]), "f"(f[2]),
+                 "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]), "l"(p)
+                 : "memory");
+}
+// Eight consecutive elements of B or C as fp32.
+template <typename T>
+__device__ __forceinline__ void load_cols8(const T* p, float (&f)[8]) {
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < 8 / E; ++k) {
+        float g[E];
+        unpack(load_vec<T, E>(p + k * E), g);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[k * E + i] = g[i];
+    }
+}
+
+// A lane has eight states of one channel, LPC lanes a channel, for RB requests: A is read
 // once for them, and all their states are on the way before the first is used. Bound by
-// memory: the states, 8 bytes a (request, channel, state).
+// memory: the states, 8 bytes a (request, channel, state). Fewer states a lane repeat
+// what the channel needs (softplus, gate, loads) on more lanes; 256-bit accesses let
+// eight be one sector each.
 template <typename T, int LPC, int RB, bool VEC>
 __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ StepP<T> p) {
-    constexpr int CH = kThreads / LPC;
-    const int tid = threadIdx.x, q = tid % LPC, n0 = 4 * q;
+    constexpr int CH = kThreads / LPC, NS = 8;
+    const int tid = threadIdx.x, q = tid % LPC, n0 = NS * q;
     const int c = blockIdx.x * CH + tid / LPC;
-    const bool live = c < p.D;
+    const bool live = c < p.D, some = live && n0 < p.N;
     const int64_t b0 = (int64_t)blockIdx.y * RB, cn = (int64_t)c * p.N + n0;
-    bool in[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) in[i] = live && n0 + i < p.N;
-    float h[RB][4], B[RB][4], C[RB][4], A[4], u[RB], dt[RB], z[RB];
-    int64_t slot[RB];
+    const int nn = some ? min(NS, p.N - n0) : 0;   // this lane's states
+    float h[RB][NS], B[RB][NS], C[RB][NS], A[NS], u[RB], dt[RB], z[RB];
+    float* hp[RB];
     const int g = live ? c / p.Dg : 0;
+    const int rows = (int)min((int64_t)RB, p.batch - b0);
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-        const int64_t b = b0 + r;
-        slot[r] = b < p.batch ? (p.s32 ? (int64_t)__ldg(p.s32 + b) : p.s64 ? __ldg(p.s64 + b) : b) : -1;
-        if (slot[r] >= p.slots) {
-            if (blockIdx.x == 0 && tid == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
-            slot[r] = -1;
+        int64_t slot = -1;
+        if (r < rows) {
+            const int64_t b = b0 + r;
+            slot = p.s32 ? (int64_t)__ldg(p.s32 + b) : p.s64 ? __ldg(p.s64 + b) : b;
+            if (slot >= p.slots) {
+                if (blockIdx.x == 0 && tid == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
+                slot = -1;
+            }
         }
+        hp[r] = slot >= 0 ? p.state + slot * p.D * p.N + cn : nullptr;
     }
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-        const bool on = slot[r] >= 0;
-        const float* hp = p.state + slot[r] * p.D * p.N + cn;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) h[r][i] = 0.0f;
         if (VEC) {
-            const float4 v = on && in[0] ? __ldcs(reinterpret_cast<const float4*>(hp)) : make_float4(0, 0, 0, 0);
-            h[r][0] = v.x, h[r][1] = v.y, h[r][2] = v.z, h[r][3] = v.w;
+            if (hp[r] && some) load8(hp[r], h[r]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[r][i] = on && in[i] ? hp[i] : 0.0f;
+            for (int i = 0; i < NS; ++i)
+                if (hp[r] && i < nn) h[r][i] = hp[r][i];
         }
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) A[i] = 0.0f;
     if (VEC) {
-        const float4 v = in[0] ? __ldg(reinterpret_cast<const float4*>(p.A + cn)) : make_float4(0, 0, 0, 0);
-        A[0] = v.x * kLog2e, A[1] = v.y * kLog2e, A[2] = v.z * kLog2e, A[3] = v.w * kLog2e;
+        if (some) load_cols8(p.A + cn, A);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) A[i] = in[i] ? __ldg(p.A + cn + i) * kLog2e : 0.0f;
+        for (int i = 0; i < NS; ++i)
+            if (i < nn) A[i] = __ldg(p.A + cn + i);
     }
     const float bias = live && p.bias ? __ldg(p.bias + c) : 0.0f, Dw = live && p.Dw ? __ldg(p.Dw + c) : 0.0f;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
         const int64_t b = b0 + r;
-        const bool on = slot[r] >= 0;
-        u[r] = on && live ? to_float(__ldg(p.u + b * p.u_sb + c)) : 0.0f;
-        dt[r] = on && live ? to_float(__ldg(p.delta + b * p.d_sb + c)) + bias : 0.0f;
-        z[r] = on && live && p.z ? to_float(__ldg(p.z + b * p.z_sb + c)) : 0.0f;
+        const bool on = hp[r] && live;
+        u[r] = on ? to_float(__ldg(p.u + b * p.u_sb + c)) : 0.0f;
+        dt[r] = on ? to_float(__ldg(p.delta + b * p.d_sb + c)) + bias : 0.0f;
+        z[r] = on && p.z ? to_float(__ldg(p.z + b * p.z_sb + c)) : 0.0f;
+        const T* Bp = p.B + b * p.B_sb + g * p.B_sg + n0;
+        const T* Cp = p.C + b * p.C_sb + g * p.C_sg + n0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) B[r][i] = C[r][i] = 0.0f;
         if (VEC) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) B[r][i] = C[r][i] = 0.0f;
-            if (on && in[0]) {
-                unpack(load_vec<T, 4>(p.B + b * p.B_sb + g * p.B_sg + n0), B[r]);
-                unpack(load_vec<T, 4>(p.C + b * p.C_sb + g * p.C_sg + n0), C[r]);
+            if (on && some) {
+                load_cols8(Bp, B[r]);
+                load_cols8(Cp, C[r]);
             }
-            continue;
-        }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            B[r][i] = on && in[i] ? to_float(__ldg(p.B + b * p.B_sb + g * p.B_sg + n0 + i)) : 0.0f;
-            C[r][i] = on && in[i] ? to_float(__ldg(p.C + b * p.C_sb + g * p.C_sg + n0 + i)) : 0.0f;
+            for (int i = 0; i < NS; ++i)
+                if (on && i < nn) {
+                    B[r][i] = to_float(__ldg(Bp + i));
+                    C[r][i] = to_float(__ldg(Cp + i));
+                }
         }
     }
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-        if (b0 + r >= p.batch) break;
-        const float d = p.softplus ? softplusf(dt[r]) : dt[r], x = d * u[r];
+        if (r >= rows) break;
+        const float d = p.softplus ? softplusf(dt[r]) : dt[r], x = d * u[r], dl = d * kLog2e;
         float y = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h[r][i] = fmaf(exp2_fast(d * A[i]), h[r][i], x * B[r][i]);
+        for (int i = 0; i < NS; ++i) {
+            h[r][i] = fmaf(exp2_fast(dl * A[i]), h[r][i], x * B[r][i]);
             y = fmaf(C[r][i], h[r][i], y);
         }
-        if (slot[r] >= 0) {
-            float* hp = p.state + slot[r] * p.D * p.N + cn;
-            if (VEC) {
-                if (in[0]) __stcs(reinterpret_cast<float4*>(hp), make_float4(h[r][0], h[r][1], h[r][2], h[r][3]));
-            } else {
+        if (VEC) {
+            if (hp[r] && some) store8(hp[r], h[r]);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (in[i]) hp[i] = h[r][i];
-            }
+            for (int i = 0; i < NS; ++i)
+                if (hp[r] && i < nn) hp[r][i] = h[r][i];
         }
 #pragma unroll
         for (int m = LPC / 2; m >= 1; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
         if (live && q == 0) {
             y = fmaf(Dw, u[r], y);
             if (p.z) y *= z[r] * sigmoidf(z[r]);
-            p.out[(b0 + r) * p.D + c] = from_float<T>(slot[r] >= 0 ? y : 0.0f);
+            p.out[(b0 + r) * p.D + c] = from_float<T>(hp[r] ? y : 0.0f);
         }
     }
 }
@@ -521,10 +553,11 @@ int step_run(const pe_scan_step_args* a, cudaStream_t s) {
     p.B_sb = a->B_sb; p.B_sg = a->B_sg; p.C_sb = a->C_sb; p.C_sg = a->C_sg;
     p.state = a->state; p.out = (T*)a->out;
     const int64_t tiles = ceil_div(p.D, kThreads / LPC);
-    // four states at once: fp32 of the state and of A, and of B and C in their type
-    const int cb = 4 * sizeof(T);
-    const bool vec = p.N % 4 == 0 && ((uintptr_t)p.state | (uintptr_t)p.A) % 16 == 0 &&
-                     ((uintptr_t)p.B | (uintptr_t)p.C) % cb == 0 && (p.B_sb | p.B_sg | p.C_sb | p.C_sg) % 4 == 0;
+    // eight states at once: 32 bytes of the state, 16-byte loads of A, B and C
+    const int e = 16 / (int)sizeof(T);
+    const bool vec = p.N % 8 == 0 && (uintptr_t)p.state % 32 == 0 &&
+                     ((uintptr_t)p.A | (uintptr_t)p.B | (uintptr_t)p.C) % 16 == 0 &&
+                     (p.B_sb % e | p.B_sg % e | p.C_sb % e | p.C_sg % e) == 0;
     // two requests a thread once that still gives every SM its 16 blocks
     const bool two = tiles * a->batch >= 32ll * num_sms();
     const dim3 grid((unsigned)tiles, (unsigned)(two ? ceil_div(a->batch, 2) : a->batch));
@@ -541,7 +574,11 @@ int step_run(const pe_scan_step_args* a, cudaStream_t s) {
 }
 template <typename T>
 int step_type(const pe_scan_step_args* a, cudaStream_t s) {
-    PE_LANES(step_run, lanes_for(a->states), a, s)
+    if (a->states <= 8) return step_run<T, 1>(a, s);
+    if (a->states <= 16) return step_run<T, 2>(a, s);
+    if (a->states <= 32) return step_run<T, 4>(a, s);
+    if (a->states <= 64) return step_run<T, 8>(a, s);
+    return step_run<T, 16>(a, s);
 }
 
 int scan_any(const pe_scan_args* a, cudaStream_t s) { PE_TYPES(scan_type, a->dtype, a, s) }

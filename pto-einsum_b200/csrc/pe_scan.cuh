@@ -61,44 +61,7 @@ __device__ __forceinline__ Place place_of(const P& p) {
     return w;
 }
 
-// ---- packed pairs --------------------------------------------------------------
-// Two fp32 lanes in one 64-bit register, one instruction for both.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
-    float lo, hi;
-    unpack2(x, lo, hi);
-    return pack2(exp2_fast(lo), exp2_fast(hi));
-}
-
 // ---- copies to shared memory ------------------------------------------------------
-template <int BYTES>
-__device__ __forceinline__ void cp_async(void* dst, const void* src, int valid) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-
 // cnt (at most ROWS) rows of `width` (at most W) elements into rows of W, in chunks of
 // `cb` bytes that arrive asynchronously where the rows are aligned for them. Nothing
 // past the width or the count is read; there the tile stays as it was.

@@ -79,6 +79,25 @@ def sized(name: str, args: bytes, idx: int) -> int:
         return fn(args)
 
 
+_sizes: dict = {}
+
+
+def nbytes_of(name: str, lay, args) -> int:
+    """Workspace bytes of a call with this layout: they depend on its numbers alone."""
+    key = (name, lay[0], lay[2])
+    n = _sizes.get(key)
+    if n is None:
+        if len(_sizes) >= _MOST_PLANS:
+            _sizes.clear()
+        n = _sizes[key] = sized(name, args(), lay[2])
+    return n
+
+
+def empty(t):
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def workspace(nbytes: int, dev: torch.device):
     """Scratch from torch's caching allocator, so it belongs to the current stream."""
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None

@@ -34,12 +34,12 @@ def _fields(lay, x, weight, bias, gate, out, mean, rstd):
 
 def _forward(lay, x, weight, bias, gate, stats):
     dev = x.device
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    out = _ops.empty(x)
     mean = rstd = None
     if stats:
         mean, rstd = torch.empty((2, lay[0][2], lay[0][5]), dtype=torch.float32, device=dev).unbind(0)
     fields = _fields(lay, x, weight, bias, gate, out, mean, rstd)
-    nbytes = _ops.sized("pe_group_norm_ws_bytes", _NORM.pack(*fields, 0, 0), lay[2])
+    nbytes = _ops.nbytes_of("pe_group_norm_ws_bytes", lay, lambda: _NORM.pack(*fields, 0, 0))
     ws = _ops.workspace(nbytes, dev)
     call("pe_group_norm", _NORM.pack(*fields, ptr(ws), nbytes), lay[2])
     return out, mean, rstd
@@ -60,13 +60,10 @@ class _GroupNorm(torch.autograd.Function):
         lay, dev = ctx.lay, x.device
         dout = _fold(dout)
 
-        def like(t):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
-
-        dx, dw, db, dgate = like(x), like(weight), like(bias), like(gate)
+        dx, dw, db, dgate = [None if t is None else _ops.empty(t) for t in (x, weight, bias, gate)]
         fields = (*_fields(lay, x, weight, bias, gate, None, mean, rstd), 0, 0, dout.data_ptr(), *_strides(dout),
                   dx.data_ptr(), ptr(dgate), ptr(dw), ptr(db))
-        nbytes = _ops.sized("pe_group_norm_grad_ws_bytes", _NORM_GRAD.pack(*fields, 0, 0), lay[2])
+        nbytes = _ops.nbytes_of("pe_group_norm_grad_ws_bytes", lay, lambda: _NORM_GRAD.pack(*fields, 0, 0))
         ws = _ops.workspace(nbytes, dev)
         call("pe_group_norm_grad", _NORM_GRAD.pack(*fields, ptr(ws), nbytes), lay[2])
         return dx, dw, db, dgate, None

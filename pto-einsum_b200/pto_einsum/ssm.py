@@ -80,7 +80,7 @@ def _conv_fields(lay, x, weight, bias, init, cu, out, state):
 
 
 def _conv_forward(lay, x, weight, bias, init, cu, want_state):
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = _ops.empty(x)
     state = None
     if want_state:
         _, _, W, _, _, C, nseq = lay[0]
@@ -105,13 +105,10 @@ class _CausalConv(torch.autograd.Function):
         lay, dev, dt = ctx.lay, x.device, x.dtype
         dout = torch.zeros(x.shape, dtype=dt, device=dev) if dout is None else rows(dout)
         dstate = None if dstate is None else dstate.contiguous()
-        dx = torch.empty(x.shape, dtype=dt, device=dev)
-        dw = torch.empty(weight.shape, dtype=dt, device=dev)
-        db = torch.empty(bias.shape, dtype=dt, device=dev) if bias is not None else None
-        dinit = torch.empty(init.shape, dtype=dt, device=dev) if init is not None else None
+        dx, dw, db, dinit = _ops.empty(x), _ops.empty(weight), _opt(bias, _ops.empty), _opt(init, _ops.empty)
         fields = (*_conv_fields(lay, x, weight, bias, init, cu, None, None), dout.data_ptr(), ptr(dstate),
                   stride(dout, 0), stride(dout, 1), dx.data_ptr(), ptr(dinit), dw.data_ptr(), ptr(db))
-        nbytes = _ops.sized("pe_causal_conv_grad_ws_bytes", _CONV_GRAD.pack(*fields, 0, 0), lay[2])
+        nbytes = _ops.nbytes_of("pe_causal_conv_grad_ws_bytes", lay, lambda: _CONV_GRAD.pack(*fields, 0, 0))
         ws = _ops.workspace(nbytes, dev)
         call("pe_causal_conv_grad", _CONV_GRAD.pack(*fields, ptr(ws), nbytes), lay[2])
         return dx, dw, db, dinit, None, None, None
@@ -178,7 +175,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
         if key is not None:
             _ops.keep_plan(key, ints)
     _no_grad_state(state)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = _ops.empty(x)
     s32, s64 = _ops.slot_pointers(slots)
     call("pe_causal_conv_step", _CONV_STEP.pack(
         *ints[:6], s32, s64, x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), ints[6],
@@ -251,11 +248,12 @@ def _scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, out, state, ckpt):
 def _scan_forward(lay, u, delta, A, B, C, D, z, bias, h0, cu, want_state, want_ckpt):
     dev, f32 = u.device, torch.float32
     _, _, _, T, Dc, N, _, nseq = lay[0]
-    out = torch.empty(u.shape, dtype=u.dtype, device=dev)
+    out = _ops.empty(u)
     state = torch.empty((nseq, Dc, N), dtype=f32, device=dev) if want_state else None
     ckpt = torch.empty(_core_ckpt(T, nseq, cu is not None, Dc, N), dtype=f32, device=dev) if want_ckpt else None
     fields = _scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, out, state, ckpt)
-    nbytes = _ops.sized("pe_scan_ws_bytes", _SCAN.pack(*fields, 0, 0), lay[2])
+    nbytes = _ops.nbytes_of("pe_scan_ws_bytes", (lay[0] + (cu is None,), 0, lay[2]),
+                            lambda: _SCAN.pack(*fields, 0, 0))
     ws = _ops.workspace(nbytes, dev)
     call("pe_selective_scan", _SCAN.pack(*fields, ptr(ws), nbytes), lay[2])
     return out, state, ckpt
@@ -279,19 +277,16 @@ class _SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, dstate=None):
         u, delta, A, B, C, D, z, bias, h0, cu, ckpt = ctx.saved_tensors
-        lay, dev, dt, f32 = ctx.lay, u.device, u.dtype, torch.float32
+        lay, dev, dt = ctx.lay, u.device, u.dtype
         dout = torch.zeros(u.shape, dtype=dt, device=dev) if dout is None else rows(dout)
         dstate = _opt(dstate, torch.Tensor.contiguous)
 
-        def like(t, dtype):
-            return None if t is None else torch.empty(t.shape, dtype=dtype, device=dev)
-
-        du, ddelta, dz, dB, dC = (like(t, dt) for t in (u, delta, z, B, C))
-        dA, dD, dbias, dh0 = (like(t, f32) for t in (A, D, bias, h0))
+        du, ddelta, dz, dB, dC, dA, dD, dbias, dh0 = [_opt(t, _ops.empty) for t in (u, delta, z, B, C, A, D, bias, h0)]
         fields = (*_scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, None, None, ckpt), 0, 0,
                   dout.data_ptr(), stride(dout, 0), stride(dout, 1), ptr(dstate), ptr(du), ptr(ddelta), ptr(dz),
                   ptr(dB), ptr(dC), ptr(dA), ptr(dD), ptr(dbias), ptr(dh0))
-        nbytes = _ops.sized("pe_scan_grad_ws_bytes", _SCAN_GRAD.pack(*fields, 0, 0), lay[2])
+        nbytes = _ops.nbytes_of("pe_scan_grad_ws_bytes", (lay[0] + (cu is None,), 0, lay[2]),
+                                lambda: _SCAN_GRAD.pack(*fields, 0, 0))
         ws = _ops.workspace(nbytes, dev)
         call("pe_selective_scan_grad", _SCAN_GRAD.pack(*fields, ptr(ws), nbytes), lay[2])
         return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None
@@ -367,7 +362,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
         if key is not None:
             _ops.keep_plan(key, ints)
     _no_grad_state(state)
-    out = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    out = _ops.empty(u)
     s32, s64 = _ops.slot_pointers(slots)
     call("pe_selective_scan_step", _SCAN_STEP.pack(
         *ints[0], s32, s64, u.data_ptr(), delta.data_ptr(), 0 if z is None else z.data_ptr(), B.data_ptr(),
