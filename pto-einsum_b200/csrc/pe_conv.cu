@@ -31,29 +31,6 @@ struct ConvP {
     T *out, *state;
 };
 
-// V channels as pairs; a single channel is a pair whose other half stays zero.
-template <int V>
-constexpr int kPairs = (V + 1) / 2;
-template <typename T, int V>
-__device__ __forceinline__ void widen(const Vec<T, V>& r, f32x2 (&f)[kPairs<V>]) {
-    if constexpr (V == 1)
-        f[0] = pack2(to_float(r.v[0]), 0.0f);
-    else
-        unpack_pairs(r, f);
-}
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> narrow(const f32x2 (&f)[kPairs<V>]) {
-    if constexpr (V == 1) {
-        float lo, hi;
-        unpack2(f[0], lo, hi);
-        Vec<T, 1> r;
-        r.v[0] = from_float<T>(lo);
-        return r;
-    } else {
-        return pack_pairs<T, V>(f);
-    }
-}
-
 template <typename T, int W, int V>
 struct Filter {
     static constexpr int Q = kPairs<V>;
@@ -163,11 +140,7 @@ __global__ void __launch_bounds__(kBlock, 2) conv_fwd(const __grid_constant__ Co
             f.apply(win, y);
             if (p.silu) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    float lo, hi;
-                    unpack2(y[q], lo, hi);
-                    y[q] = mul2(y[q], pack2(sigmoidf(lo), sigmoidf(hi)));
-                }
+                for (int q = 0; q < Q; ++q) y[q] = mul2(y[q], sigmoid2(y[q]));
             }
             shift(win);
             store_vec(o, narrow<T, V>(y));
@@ -370,11 +343,7 @@ __global__ void __launch_bounds__(128) conv_step(const __grid_constant__ ConvSte
     f.apply(win, y);
     if (p.silu) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            float lo, hi;
-            unpack2(y[q], lo, hi);
-            y[q] = mul2(y[q], pack2(sigmoidf(lo), sigmoidf(hi)));
-        }
+        for (int q = 0; q < Q; ++q) y[q] = mul2(y[q], sigmoid2(y[q]));
     }
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) store_vec(st + k * p.C, raw[k + 1]);
@@ -419,21 +388,20 @@ ConvP<T> conv_params(const pe_conv_args* a, int v, int64_t tile) {
     return p;
 }
 
-// Tokens a thread walks in the forward pass: as many as leave two warps' worth of loads
-// to every scheduler (the W - 1 tokens read again and the filter weigh less on a longer
-// walk), 4 to 32.
-int64_t fwd_tile(const pe_conv_args* a, int v) {
-    const int64_t cells = a->tokens * a->batch * (a->channels / v), want = (int64_t)num_sms() * 1536;
-    int64_t tile = 4;
-    while (tile < 32 && cells / (2 * tile) >= want) tile *= 2;
-    return tile;
+// Tokens a thread walks: whole waves of the two blocks an SM holds, at most 64 tokens
+// each (the W - 1 tokens read again, the filter and the filling of the queue weigh less
+// on a longer walk; a last wave that is not full costs as much as one that is), at
+// least 4.
+int64_t tile_of(const pe_conv_args* a, int v) {
+    const int64_t cells = a->tokens * a->batch * (a->channels / v), wave = 2ll * num_sms() * kBlock;
+    const int64_t waves = ceil_div(cells, 64 * wave);
+    const int64_t tile = waves ? ceil_div(cells, waves * wave) : 4;
+    return tile < 4 ? 4 : tile;
 }
-// Backward, tokens a thread; the block's threads along the tokens add up their sums.
-constexpr int64_t kBwdTile = 32;
 
 template <typename T, int W, int V>
 int conv_run(const pe_conv_args* a, cudaStream_t s) {
-    const ConvP<T> p = conv_params<T>(a, V, fwd_tile(a, V));
+    const ConvP<T> p = conv_params<T>(a, V, tile_of(a, V));
     const int64_t ids = (p.tiles + (p.state ? a->nseq : 0)) * p.CV, blocks = ceil_div(ids, kBlock);
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     if (!blocks) return PE_OK;
@@ -450,7 +418,7 @@ ConvGradShape grad_shape(const pe_conv_args* a, int v) {
     const int64_t cv = a->channels / v;
     ConvGradShape g{1, 0};
     while (g.bx < 32 && g.bx < cv) g.bx *= 2;
-    g.rows = ceil_div(ceil_div(a->tokens, kBwdTile) * a->batch, kBlock / g.bx);
+    g.rows = ceil_div(ceil_div(a->tokens, tile_of(a, v)) * a->batch, kBlock / g.bx);
     return g;
 }
 
@@ -459,7 +427,7 @@ int conv_grad_run(const pe_conv_grad_args* g, cudaStream_t s) {
     const pe_conv_args* a = &g->fwd;
     const ConvGradShape sh = grad_shape(a, V);
     ConvGradP<T> p;
-    p.f = conv_params<T>(a, V, kBwdTile);
+    p.f = conv_params<T>(a, V, tile_of(a, V));
     p.dout = (const T*)g->dout; p.dstate = (const T*)g->dstate;
     p.o_sb = g->dout_sb; p.o_st = g->dout_st;
     p.dx = (T*)g->dx; p.dinit = (T*)g->dinit;

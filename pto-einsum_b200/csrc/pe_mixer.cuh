@@ -156,6 +156,43 @@ __device__ __forceinline__ Vec<T, V> pack_pairs(const f32x2 (&f)[V / 2]) {
     return r;
 }
 
+// V channels as pairs; a single channel is a pair whose other half stays zero.
+template <int V>
+constexpr int kPairs = (V + 1) / 2;
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Vec<T, V>& r, f32x2 (&f)[kPairs<V>]) {
+    if constexpr (V == 1)
+        f[0] = pack2(to_float(r.v[0]), 0.0f);
+    else
+        unpack_pairs(r, f);
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(const f32x2 (&f)[kPairs<V>]) {
+    if constexpr (V == 1) {
+        float lo, hi;
+        unpack2(f[0], lo, hi);
+        Vec<T, 1> r;
+        r.v[0] = from_float<T>(lo);
+        return r;
+    } else {
+        return pack_pairs<T, V>(f);
+    }
+}
+__device__ __forceinline__ f32x2 both(float x) { return pack2(x, x); }
+// A value a channel: 0 in the idle half of a single channel's pair.
+template <int V>
+__device__ __forceinline__ f32x2 each(float x) { return pack2(x, V == 1 ? 0.0f : x); }
+__device__ __forceinline__ float halves(f32x2 v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    return lo + hi;
+}
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
+    float lo, hi;
+    unpack2(x, lo, hi);
+    return pack2(sigmoidf(lo), sigmoidf(hi));
+}
+
 // ---- asynchronous copies ------------------------------------------------------------
 template <int BYTES>
 __device__ __forceinline__ void cp_async(void* dst, const void* src, int valid) {

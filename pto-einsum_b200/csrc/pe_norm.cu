@@ -7,7 +7,8 @@
 //
 // Bound by memory. A group of up to 1024 loads (512 backward; 16 bytes each where
 // the layout allows) stays in the registers of the lanes that share it: one read of x, two-pass
-// statistics. A larger one goes over the tensor twice: per-channel sums of row chunks,
+// statistics. A larger one stays in the shared memory of a cluster of up to eight blocks.
+// What that does not hold goes over the tensor twice: per-channel sums of row chunks,
 // their combination, then the result; the second read comes from L2 while the tensor
 // fits there. Variances are never formed as a difference of large squares: two passes
 // in registers, and sums shifted by a first value that are joined by Chan's formula
@@ -99,14 +100,18 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
     const int per = p.cg / V;
     const Items<V, K> it(l, L, per, live ? per * (int)p.S : 0, g * p.cg);
     const float inv = 1.0f / (float)(p.cg * (int)p.S);
+    constexpr int Q = kPairs<V>;
     int64_t xo[K], go[K];
-    Vec<T, V> w[K], b[K], x[K], z[K];
+    Vec<T, V> x[K], z[K];
+    f32x2 w[K][Q], b[K][Q];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         xo[k] = it.place[k] * p.x_sp + it.c[k];
         go[k] = it.place[k] * p.g_sp + it.c[k];
-        if (it.in[k] && p.w) w[k] = load_vec<T, V>(p.w + it.c[k]);
-        if (it.in[k] && p.b) b[k] = load_vec<T, V>(p.b + it.c[k]);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) w[k][q] = both(1.0f), b[k][q] = 0;
+        if (it.in[k] && p.w) widen<T, V>(load_vec<T, V>(p.w + it.c[k]), w[k]);
+        if (it.in[k] && p.b) widen<T, V>(load_vec<T, V>(p.b + it.c[k]), b[k]);
     }
     auto load = [&](int64_t n) {
 #pragma unroll
@@ -120,29 +125,31 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
     for (int64_t n0 = 0; n0 < p.N; n0 += R) {
         const int64_t n = n0 + r;
         const bool on = n < p.N;
-        float f[K][V], ga[K][V], sum[1] = {0.0f};
+        f32x2 f[K][Q], ga[K][Q];
+        float sum[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            unpack(x[k], f[k]);
-            if (p.mode == kGate) unpack(z[k], ga[k]);
-            float s = 0.0f;
+            widen<T, V>(x[k], f[k]);
+            if (p.mode == kGate) widen<T, V>(z[k], ga[k]);
+            f32x2 s = f[k][0];
 #pragma unroll
-            for (int v = 0; v < V; ++v) s += f[k][v];
-            sum[0] += it.in[k] ? s : 0.0f;
+            for (int q = 1; q < Q; ++q) s = add2(s, f[k][q]);
+            sum[0] += it.in[k] ? halves(s) : 0.0f;
         }
         load(n + R);
         group_sum(sum, L, red);
         const float mean = sum[0] * inv;
+        const f32x2 minus = each<V>(-mean);
         sum[0] = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float s = 0.0f;
+            f32x2 s = 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                f[k][v] -= mean;
-                s = fmaf(f[k][v], f[k][v], s);
+            for (int q = 0; q < Q; ++q) {
+                f[k][q] = add2(f[k][q], minus);
+                s = fma2(f[k][q], f[k][q], s);
             }
-            sum[0] += it.in[k] ? s : 0.0f;
+            sum[0] += it.in[k] ? halves(s) : 0.0f;
         }
         group_sum(sum, L, red);
         const float rstd = rsqrtf(sum[0] * inv + p.eps);
@@ -151,19 +158,18 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
             p.mean[n * p.G + g] = mean;
             p.rstd[n * p.G + g] = rstd;
         }
+        const f32x2 scale = both(rstd);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!it.in[k]) continue;
-            float y[V];
+            f32x2 y[Q];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                y[v] = f[k][v] * rstd;
-                if (p.w) y[v] *= to_float(w[k].v[v]);
-                if (p.b) y[v] += to_float(b[k].v[v]);
-                if (p.mode == kSilu) y[v] *= sigmoidf(y[v]);
-                if (p.mode == kGate) y[v] *= ga[k][v] * sigmoidf(ga[k][v]);
+            for (int q = 0; q < Q; ++q) {
+                y[q] = fma2(mul2(f[k][q], scale), w[k][q], b[k][q]);
+                if (p.mode == kSilu) y[q] = mul2(y[q], sigmoid2(y[q]));
+                if (p.mode == kGate) y[q] = mul2(y[q], mul2(ga[k][q], sigmoid2(ga[k][q])));
             }
-            store_vec(p.out + (n * p.S + it.place[k]) * p.C + it.c[k], pack<T, V>(y));
+            store_vec(p.out + (n * p.S + it.place[k]) * p.C + it.c[k], narrow<T, V>(y));
         }
     }
 }
@@ -186,11 +192,33 @@ __device__ __forceinline__ void through_act(int mode, const float (&xn)[V], cons
     }
 }
 
+// The same in pairs.
+__device__ __forceinline__ f32x2 silu_slope2(f32x2 x, f32x2 s) {
+    return mul2(s, fma2(x, add2(both(1.0f), mul2(s, both(-1.0f))), both(1.0f)));
+}
+template <int Q>
+__device__ __forceinline__ void through_act2(int mode, const f32x2 (&xn)[Q], const f32x2 (&w)[Q], const f32x2 (&b)[Q],
+                                             f32x2 (&go)[Q], f32x2 (&ga)[Q]) {
+    if (mode == kPlain) return;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const f32x2 val = fma2(xn[q], w[q], b[q]);
+        if (mode == kSilu) {
+            go[q] = mul2(go[q], silu_slope2(val, sigmoid2(val)));
+        } else {
+            const f32x2 s = sigmoid2(ga[q]), o = go[q];
+            go[q] = mul2(o, mul2(ga[q], s));
+            ga[q] = mul2(mul2(o, val), silu_slope2(ga[q], s));
+        }
+    }
+}
+
 // L lanes take rows r, r + R, ... of one group of channels (one place a row) and keep the
 // sums of g xn and g of their own channels: pw, pb [R][C].
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(const __grid_constant__ NormP<T> p, int L, int R, float* pw,
-                                                       float* pb) {
+__global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(const __grid_constant__ NormP<T> p, int L,
+                                                                            int R, float* pw, float* pb) {
+    constexpr int Q = kPairs<V>;
     __shared__ float red[16];
     const int unit = (int)(((int64_t)blockIdx.x * kBlock + threadIdx.x) / L), l = threadIdx.x % L;
     const bool live = unit / p.G < R;
@@ -198,19 +226,15 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
     const int per = p.cg / V;
     const Items<V, K> it(l, L, per, live ? per : 0, g * p.cg);
     const float inv = 1.0f / (float)p.cg;
-    float aw[K][V], ab[K][V];
-    Vec<T, V> w[K], b[K], x[K], z[K], o[K];
+    f32x2 aw[K][Q], ab[K][Q], w[K][Q], b[K][Q];
+    Vec<T, V> x[K], z[K], o[K];
     float mean = 0.0f, rstd = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            aw[k][v] = ab[k][v] = 0.0f;
-            w[k].v[v] = from_float<T>(1.0f);
-            b[k].v[v] = from_float<T>(0.0f);
-        }
-        if (it.in[k] && p.w) w[k] = load_vec<T, V>(p.w + it.c[k]);
-        if (it.in[k] && p.b) b[k] = load_vec<T, V>(p.b + it.c[k]);
+        for (int q = 0; q < Q; ++q) aw[k][q] = ab[k][q] = b[k][q] = 0, w[k][q] = each<V>(1.0f);
+        if (it.in[k] && p.w) widen<T, V>(load_vec<T, V>(p.w + it.c[k]), w[k]);
+        if (it.in[k] && p.b) widen<T, V>(load_vec<T, V>(p.b + it.c[k]), b[k]);
     }
     auto load = [&](int64_t n) {
         if (n < p.N) {
@@ -229,40 +253,41 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
     for (int64_t n0 = 0; n0 < p.N; n0 += R) {
         const int64_t n = n0 + r;
         const bool on = n < p.N;
-        const float scale = rstd;
-        float xn[K][V], go[K][V], sum[2] = {0.0f, 0.0f};
+        const f32x2 minus = each<V>(-mean), scale = both(rstd);
+        f32x2 xn[K][Q], go[K][Q];
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!it.in[k] || !on) continue;
-            float ga[V], wf[V], bf[V];
-            unpack(x[k], xn[k]);
-            unpack(o[k], go[k]);
-            unpack(w[k], wf);
-            unpack(b[k], bf);
-            if (p.mode == kGate) unpack(z[k], ga);
+            f32x2 ga[Q], s0 = 0, s1 = 0;
+            widen<T, V>(x[k], xn[k]);
+            widen<T, V>(o[k], go[k]);
+            if (p.mode == kGate) widen<T, V>(z[k], ga);
 #pragma unroll
-            for (int v = 0; v < V; ++v) xn[k][v] = (xn[k][v] - mean) * rstd;
-            through_act<V>(p.mode, xn[k], wf, bf, go[k], ga);
-            if (p.mode == kGate) store_vec(p.dgate + n * p.C + it.c[k], pack<T, V>(ga));
+            for (int q = 0; q < Q; ++q) xn[k][q] = mul2(add2(xn[k][q], minus), scale);
+            through_act2<Q>(p.mode, xn[k], w[k], b[k], go[k], ga);
+            if (p.mode == kGate) store_vec(p.dgate + n * p.C + it.c[k], narrow<T, V>(ga));
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                aw[k][v] = fmaf(go[k][v], xn[k][v], aw[k][v]);
-                ab[k][v] += go[k][v];
-                go[k][v] *= wf[v];
-                sum[0] += go[k][v];
-                sum[1] = fmaf(go[k][v], xn[k][v], sum[1]);
+            for (int q = 0; q < Q; ++q) {
+                aw[k][q] = fma2(go[k][q], xn[k][q], aw[k][q]);
+                ab[k][q] = add2(ab[k][q], go[k][q]);
+                go[k][q] = mul2(go[k][q], w[k][q]);
+                s0 = add2(s0, go[k][q]);
+                s1 = fma2(go[k][q], xn[k][q], s1);
             }
+            sum[0] += halves(s0);
+            sum[1] += halves(s1);
         }
         load(n + R);
         group_sum(sum, L, red);
-        const float m0 = sum[0] * inv, m1 = sum[1] * inv;
+        const f32x2 m0 = both(-sum[0] * inv), m1 = both(-sum[1] * inv);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!it.in[k] || !on) continue;
-            float d[V];
+            f32x2 d[Q];
 #pragma unroll
-            for (int v = 0; v < V; ++v) d[v] = scale * (go[k][v] - m0 - xn[k][v] * m1);
-            store_vec(p.dx + n * p.C + it.c[k], pack<T, V>(d));
+            for (int q = 0; q < Q; ++q) d[q] = mul2(scale, fma2(xn[k][q], m1, add2(go[k][q], m0)));
+            store_vec(p.dx + n * p.C + it.c[k], narrow<T, V>(d));
         }
     }
     if (!pw) return;
@@ -271,10 +296,297 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
         if (!it.in[k]) continue;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            pw[(int64_t)r * p.C + it.c[k] + v] = aw[k][v];
-            pb[(int64_t)r * p.C + it.c[k] + v] = ab[k][v];
+            float a[2], c[2];
+            unpack2(aw[k][v / 2], a[0], a[1]);
+            unpack2(ab[k][v / 2], c[0], c[1]);
+            pw[(int64_t)r * p.C + it.c[k] + v] = a[v % 2];
+            pb[(int64_t)r * p.C + it.c[k] + v] = c[v % 2];
         }
     }
+}
+
+// ---- groups in a cluster's shared memory ------------------------------------------------
+// A cluster of R blocks takes a slab of whole groups (CS channels) of one row, each block
+// its P places, which stay in shared memory: one read of the tensor and one launch. The
+// blocks exchange their sums of each group through distributed shared memory and add
+// them in rank order.
+struct Slab {
+    int CS, slabs, R, P;
+};
+
+__device__ __forceinline__ float remote(const float* own, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(own), rank)) : "memory");
+    return v;
+}
+
+// A block's part of the layout: channel vector x of row lane y (of by).
+template <typename T, int V>
+struct SlabPlace {
+    int64_t n, c0, s0;
+    int cs, pc, cvn, by, x, y;   // channels and places here, vectors a place
+    bool on;
+    __device__ __forceinline__ SlabPlace(const NormP<T>& p, const Slab& q) {
+        const int rank = (int)cluster_rank();
+        const int64_t unit = blockIdx.x / q.R;
+        n = unit / q.slabs;
+        c0 = (unit - n * q.slabs) * q.CS;
+        cs = (int)min((int64_t)q.CS, p.C - c0);
+        s0 = (int64_t)rank * q.P;
+        pc = (int)max((int64_t)0, min((int64_t)q.P, p.S - s0));
+        cvn = cs / V;
+        by = kBlock / cvn;
+        x = threadIdx.x % cvn;
+        y = threadIdx.x / cvn;
+        on = y < by;
+    }
+    // this block's places of a tensor into shared memory [P][cs]
+    __device__ __forceinline__ void copy(T* dst, const T* src, int64_t sb, int64_t sp) const {
+        if (!on) return;
+        const T* from = src + n * sb + s0 * sp + c0 + x * V;
+        for (int i = y; i < pc; i += by) {
+            if constexpr (V * sizeof(T) >= 8)
+                cp_async<V * sizeof(T)>(dst + i * cs + x * V, from + i * sp, V * sizeof(T));
+            else
+                dst[i * cs + x * V] = __ldg(from + i * sp);
+        }
+    }
+    __device__ __forceinline__ void get(const T* tile, int i, f32x2 (&f)[kPairs<V>]) const {
+        widen<T, V>(*reinterpret_cast<const Vec<T, V>*>(tile + i * cs + x * V), f);
+    }
+    // Sums of a value a channel over the block's row lanes: sums[ch], via red [cs][by].
+    __device__ __forceinline__ void channel_sums(const f32x2 (&v)[kPairs<V>], float* red, float* sums) const {
+        if (on)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float h[2];
+                unpack2(v[k / 2], h[0], h[1]);
+                red[(x * V + k) * by + y] = h[k % 2];
+            }
+        __syncthreads();
+        const int lane = threadIdx.x & 31;
+        if (by <= 8) {
+            for (int c = threadIdx.x; c < cs; c += kBlock) {
+                float a = 0.0f;
+                for (int i = 0; i < by; ++i) a += red[c * by + i];
+                sums[c] = a;
+            }
+        } else {
+            for (int c = threadIdx.x / 32; c < cs; c += kBlock / 32) {
+                float a = 0.0f;
+                for (int i = lane; i < by; i += 32) a += red[c * by + i];
+#pragma unroll
+                for (int m = 16; m >= 1; m /= 2) a += __shfl_xor_sync(0xffffffffu, a, m);
+                if (lane == 0) sums[c] = a;
+            }
+        }
+        __syncthreads();
+    }
+};
+
+// Sums over each group's channels of a(c), into g; the block's own share.
+template <typename F>
+__device__ __forceinline__ void slab_groups(int groups, int cg, float* g, F a) {
+    const int lane = threadIdx.x & 31;
+    for (int j = threadIdx.x / 32; j < groups; j += kBlock / 32) {
+        float s = 0.0f;
+        for (int i = lane; i < cg; i += 32) s += a(j * cg + i);
+#pragma unroll
+        for (int m = 16; m >= 1; m /= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
+        if (lane == 0) g[j] = s;
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kBlock, 2) norm_slab(const __grid_constant__ NormP<T> p, const Slab q) {
+    constexpr int Q = kPairs<V>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* red = reinterpret_cast<float*>(smem);        // [kBlock V]
+    float *sums = red + kBlock * V, *share = sums + q.CS, *own = share + 2 * q.CS;   // a channel; 2 a group; a group
+    T* tile = reinterpret_cast<T*>(own + q.CS);
+    const SlabPlace<T, V> at(p, q);
+    const int groups = at.cs / p.cg;
+    at.copy(tile, p.x, p.x_sb, p.x_sp);
+    cp_commit();
+    f32x2 w[Q], b[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) w[k] = each<V>(1.0f), b[k] = 0;
+    if (at.on && p.w) widen<T, V>(load_vec<T, V>(p.w + at.c0 + at.x * V), w);
+    if (at.on && p.b) widen<T, V>(load_vec<T, V>(p.b + at.c0 + at.x * V), b);
+    const float inv = 1.0f / ((float)p.cg * (float)p.S);
+    cp_wait();
+    // own places only: a thread reads what it copied
+    f32x2 mean[Q], rstd[Q], s[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) s[k] = 0;
+    if (at.on)
+#pragma unroll 4
+        for (int i = at.y; i < at.pc; i += at.by) {
+            f32x2 f[Q];
+            at.get(tile, i, f);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) s[k] = add2(s[k], f[k]);
+        }
+    // (sum over all places of each group) inv, a channel's pair
+    auto over_group = [&](float* to, f32x2 (&out)[Q]) {
+        at.channel_sums(s, red, sums);
+        slab_groups(groups, p.cg, to, [&](int c) { return sums[c]; });
+        __syncthreads();
+        cluster_sync();
+        for (int j = threadIdx.x; j < groups; j += kBlock) {
+            float a = 0.0f;
+            for (int r = 0; r < q.R; ++r) a += remote(to + j, r);
+            own[j] = a * inv;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            const int c = at.on ? at.x * V + 2 * k : 0;
+            out[k] = pack2(own[c / p.cg], V == 1 ? 0.0f : own[(c + 1) / p.cg]);
+        }
+    };
+    over_group(share, mean);
+    float keep = 0.0f;
+    if (threadIdx.x < groups) keep = own[threadIdx.x];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < Q; ++k) s[k] = 0, mean[k] = mul2(mean[k], both(-1.0f));
+    if (at.on)
+#pragma unroll 4
+        for (int i = at.y; i < at.pc; i += at.by) {
+            f32x2 f[Q];
+            at.get(tile, i, f);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+                f[k] = add2(f[k], mean[k]);
+                s[k] = fma2(f[k], f[k], s[k]);
+            }
+        }
+    over_group(share + q.CS, rstd);
+    if (cluster_rank() == 0 && p.mean && threadIdx.x < groups) {
+        const int64_t g = at.n * p.G + at.c0 / p.cg + threadIdx.x;
+        p.mean[g] = keep;
+        p.rstd[g] = rsqrtf(own[threadIdx.x] + p.eps);
+    }
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        float lo, hi;
+        unpack2(rstd[k], lo, hi);
+        rstd[k] = pack2(rsqrtf(lo + p.eps), rsqrtf(hi + p.eps));
+    }
+    if (at.on) {
+        const int64_t c = at.c0 + at.x * V;
+        const T* gate = p.mode == kGate ? p.gate + at.n * p.g_sb + at.s0 * p.g_sp + c : nullptr;
+        T* out = p.out + (at.n * p.S + at.s0) * p.C + c;
+#pragma unroll 4
+        for (int i = at.y; i < at.pc; i += at.by) {
+            f32x2 f[Q], ga[Q];
+            if (gate) widen<T, V>(load_vec<T, V>(gate + i * p.g_sp), ga);
+            at.get(tile, i, f);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+                f[k] = fma2(mul2(add2(f[k], mean[k]), rstd[k]), w[k], b[k]);
+                if (p.mode == kSilu) f[k] = mul2(f[k], sigmoid2(f[k]));
+                if (gate) f[k] = mul2(f[k], mul2(ga[k], sigmoid2(ga[k])));
+            }
+            store_vec(out + (int64_t)i * p.C, narrow<T, V>(f));
+        }
+    }
+    cluster_sync();   // the others may still read this block's sums
+}
+
+// Backward: x and dout stay in shared memory, the gate is read twice. pw, pb [N R][C]: a
+// block's share of the sums of g xn and g.
+template <typename T, int V>
+__global__ void __launch_bounds__(kBlock, 2) norm_slab_bwd(const __grid_constant__ NormP<T> p, const Slab q, float* pw,
+                                                           float* pb) {
+    constexpr int Q = kPairs<V>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* red = reinterpret_cast<float*>(smem);        // [kBlock V]
+    float *sw = red + kBlock * V, *sb = sw + q.CS, *share = sb + q.CS, *own = share + 2 * q.CS;
+    T* tx = reinterpret_cast<T*>(own + 2 * q.CS);
+    T* to = tx + (int64_t)q.P * q.CS;
+    const SlabPlace<T, V> at(p, q);
+    const int groups = at.cs / p.cg;
+    at.copy(tx, p.x, p.x_sb, p.x_sp);
+    at.copy(to, p.dout, p.o_sb, p.o_sp);
+    cp_commit();
+    const int64_t c = at.c0 + at.x * V;
+    f32x2 w[Q], b[Q], mean[Q], rstd[Q], a0[Q], a1[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) w[k] = each<V>(1.0f), b[k] = a0[k] = a1[k] = mean[k] = rstd[k] = 0;
+    if (at.on) {
+        if (p.w) widen<T, V>(load_vec<T, V>(p.w + c), w);
+        if (p.b) widen<T, V>(load_vec<T, V>(p.b + c), b);
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            const int64_t g0 = at.n * p.G + (int)(c + 2 * k) / p.cg, g1 = at.n * p.G + (int)(c + 2 * k + (V > 1)) / p.cg;
+            mean[k] = pack2(-__ldg(p.mean + g0), V == 1 ? 0.0f : -__ldg(p.mean + g1));
+            rstd[k] = pack2(__ldg(p.rstd + g0), V == 1 ? 0.0f : __ldg(p.rstd + g1));
+        }
+    }
+    const T* gate = p.mode == kGate ? p.gate + at.n * p.g_sb + at.s0 * p.g_sp + c : nullptr;
+    auto load = [&](int i, f32x2 (&xn)[Q], f32x2 (&go)[Q], f32x2 (&ga)[Q]) {
+        if (gate) widen<T, V>(load_vec<T, V>(gate + i * p.g_sp), ga);
+        at.get(tx, i, xn);
+        at.get(to, i, go);
+#pragma unroll
+        for (int k = 0; k < Q; ++k) xn[k] = mul2(add2(xn[k], mean[k]), rstd[k]);
+        through_act2<Q>(p.mode, xn, w, b, go, ga);
+    };
+    cp_wait();
+    if (at.on)
+#pragma unroll 2
+        for (int i = at.y; i < at.pc; i += at.by) {
+            f32x2 xn[Q], go[Q], ga[Q];
+            load(i, xn, go, ga);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+                a0[k] = add2(a0[k], go[k]);
+                a1[k] = fma2(go[k], xn[k], a1[k]);
+            }
+        }
+    at.channel_sums(a1, red, sw);
+    at.channel_sums(a0, red, sb);
+    if (pw)
+        for (int i = threadIdx.x; i < at.cs; i += kBlock) {
+            const int64_t row = at.n * q.R + cluster_rank();
+            pw[row * p.C + at.c0 + i] = sw[i];
+            pb[row * p.C + at.c0 + i] = sb[i];
+        }
+    auto weight = [&](int i) { return p.w ? to_float(__ldg(p.w + at.c0 + i)) : 1.0f; };
+    slab_groups(groups, p.cg, share, [&](int i) { return weight(i) * sb[i]; });
+    slab_groups(groups, p.cg, share + q.CS, [&](int i) { return weight(i) * sw[i]; });
+    __syncthreads();
+    cluster_sync();
+    const float inv = 1.0f / ((float)p.cg * (float)p.S);
+    for (int j = threadIdx.x; j < groups; j += kBlock) {
+        float m0 = 0.0f, m1 = 0.0f;
+        for (int r = 0; r < q.R; ++r) m0 += remote(share + j, r), m1 += remote(share + q.CS + j, r);
+        own[j] = -m0 * inv;
+        own[q.CS + j] = -m1 * inv;
+    }
+    __syncthreads();
+    if (at.on) {
+        f32x2 m0[Q], m1[Q];
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            const int i = at.x * V + 2 * k, g0 = i / p.cg, g1 = V == 1 ? g0 : (i + 1) / p.cg;
+            m0[k] = pack2(own[g0], own[g1]);
+            m1[k] = pack2(own[q.CS + g0], own[q.CS + g1]);
+        }
+#pragma unroll 2
+        for (int i = at.y; i < at.pc; i += at.by) {
+            f32x2 xn[Q], go[Q], ga[Q];
+            load(i, xn, go, ga);
+            const int64_t o = (at.n * p.S + at.s0 + i) * p.C + c;
+            if (gate) store_vec(p.dgate + o, narrow<T, V>(ga));
+#pragma unroll
+            for (int k = 0; k < Q; ++k) go[k] = mul2(rstd[k], fma2(xn[k], m1[k], fma2(go[k], w[k], m0[k])));
+            store_vec(p.dx + o, narrow<T, V>(go));
+        }
+    }
+    cluster_sync();   // the others may still read this block's sums
 }
 
 // ---- larger groups ------------------------------------------------------------------
@@ -563,8 +875,36 @@ struct Plan {
     int v;            // elements a load
     int lanes, k;     // groups in registers: lanes a group, loads a lane; lanes 0: too large for that
     int64_t R;        // in registers: rows at work, a lane takes every R-th
+    Slab slab;        // in a cluster's shared memory: R > 0
     Chunks q;
 };
+
+int64_t slab_smem(int64_t cs, int64_t P, int v, int64_t es, bool grad) {
+    return (kBlock * v + (grad ? 6 : 4) * cs) * 4 + (grad ? 2 : 1) * ceil_div(P * cs * es, 16) * 16;
+}
+
+// The slab of a group that is too large for registers: whole groups and whole loads, 64
+// bytes a place or more where there are so many channels; blocks enough to hold it at
+// two an SM (one where it must be), and to give every SM one. R 0: too large.
+Slab slab_of(const pe_norm_args* a, int v, bool grad) {
+    Slab s{0, 0, 0, 0};
+    const int64_t cg = a->channels / a->groups, es = a->dtype == PE_F32 ? 4 : 2;
+    int64_t base = cg;
+    while (base % v) base += cg;
+    int64_t cs = base;
+    while (cs * es < 64 && cs + base <= a->channels) cs += base;
+    if (cs / v > kBlock || a->places > (1 << 24)) return s;
+    const int64_t slabs = ceil_div(a->channels, cs);
+    for (int64_t room : {100 * 1024, 200 * 1024})
+        for (int r = 1; r <= 8; r *= 2) {
+            const int64_t P = ceil_div(a->places, r);
+            if (slab_smem(cs, P, v, es, grad) > room) continue;
+            if (room == 100 * 1024 && r < 8 && a->batch * slabs * r < num_sms() && P * (cs / v) > 2 * kBlock) continue;
+            s.CS = (int)cs; s.slabs = (int)slabs; s.R = r; s.P = (int)P;
+            return s;
+        }
+    return s;
+}
 
 Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
     Plan p{};
@@ -591,6 +931,8 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
         return p;
     }
     p.v = vec;
+    p.slab = slab_of(a, vec, grad);
+    if (p.slab.R) return p;
     const int64_t cv = a->channels / vec;
     p.q.bx = 32;
     while (p.q.bx > 1 && ceil_div(cv, p.q.bx) * p.q.bx * 8 > cv * 9) p.q.bx /= 2;
@@ -621,7 +963,30 @@ int launched() {
 }
 
 int64_t stats_floats(const pe_norm_args* a, const Plan& pl) {
-    return pl.lanes ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->groups);
+    return pl.lanes || pl.slab.R ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->groups);
+}
+
+template <typename K, typename... A>
+int launch_slab(K kernel, int64_t rows, const Slab& q, int64_t smem, cudaStream_t s, A... args) {
+    const int64_t blocks = rows * q.slabs * q.R;
+    if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return PE_ERR_CUDA;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = q.R;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kBlock);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) return PE_ERR_CUDA;
+    count_launch();
+    return PE_OK;
 }
 
 template <typename T, int V>
@@ -636,6 +1001,9 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
         else norm_reg<T, V, 4><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
         return launched();
     }
+    if (pl.slab.R)
+        return launch_slab(norm_slab<T, V>, p.N, pl.slab, slab_smem(pl.slab.CS, pl.slab.P, V, sizeof(T), false), s, p,
+                           pl.slab);
     float* part = (float*)a->ws;
     if (!p.mean) {
         p.mean = part + p.N * pl.q.chunks * 2 * p.C;
@@ -654,6 +1022,7 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
 
 int64_t grad_floats(const pe_norm_args* a, const Plan& pl) {
     if (pl.lanes) return 2 * pl.R * a->channels;
+    if (pl.slab.R) return 2 * a->batch * pl.slab.R * a->channels;
     return a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->channels + 2 * a->groups);
 }
 
@@ -677,6 +1046,14 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
         if (pl.k == 1) norm_reg_bwd<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R, pw, sb);
         else norm_reg_bwd<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R, pw, sb);
         if (int rc = launched()) return rc;
+    } else if (pl.slab.R) {
+        rows = p.N * pl.slab.R;
+        sw = ws;
+        sb = ws + rows * p.C;
+        float* pw = ga->dweight || ga->dbias ? sw : nullptr;
+        if (int rc = launch_slab(norm_slab_bwd<T, V>, p.N, pl.slab,
+                                 slab_smem(pl.slab.CS, pl.slab.P, V, sizeof(T), true), s, p, pl.slab, pw, sb))
+            return rc;
     } else {
         float* part = ws;
         sw = part + p.N * pl.q.chunks * 2 * p.C;
