@@ -161,7 +161,7 @@ struct ConvGradP {
 };
 
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(kBlock, 2) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
+__global__ void __launch_bounds__(kBlock, 1) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
     constexpr int Q = kPairs<V>;
     // the queues, and once they are empty the block's sums
     extern __shared__ __align__(16) unsigned char shared[];
@@ -224,9 +224,7 @@ __global__ void __launch_bounds__(kBlock, 2) conv_bwd(const __grid_constant__ Co
                         flt.apply(win, a);
 #pragma unroll
                         for (int q = 0; q < Q; ++q) {
-                            float lo, hi;
-                            unpack2(a[q], lo, hi);
-                            g[W - 1][q] = mul2(g[W - 1][q], pack2(silu_slope(lo, sigmoidf(lo)), silu_slope(hi, sigmoidf(hi))));
+                            g[W - 1][q] = mul2(g[W - 1][q], silu_slope2(a[q], sigmoid2(a[q])));
                         }
                     }
                     if (k < stop) {   // the tile's own: into the sums
@@ -388,20 +386,26 @@ ConvP<T> conv_params(const pe_conv_args* a, int v, int64_t tile) {
     return p;
 }
 
-// Tokens a thread walks: whole waves of the two blocks an SM holds, at most 64 tokens
-// each (the W - 1 tokens read again, the filter and the filling of the queue weigh less
-// on a longer walk; a last wave that is not full costs as much as one that is), at
-// least 4.
-int64_t tile_of(const pe_conv_args* a, int v) {
-    const int64_t cells = a->tokens * a->batch * (a->channels / v), wave = 2ll * num_sms() * kBlock;
-    const int64_t waves = ceil_div(cells, 64 * wave);
-    const int64_t tile = waves ? ceil_div(cells, waves * wave) : 4;
+// Tokens a thread walks: whole waves of the blocks an SM holds (two forward, one
+// backward), at most 64 tokens each (the W - 1 tokens read again, the filter and the
+// filling of the queue weigh less on a longer walk; a last wave that is not full costs as
+// much as one that is), at least 4. by: a block's threads along the tokens, where the
+// block is laid out by channels.
+int64_t tile_of(const pe_conv_args* a, int64_t columns, int resident, int by) {
+    const int64_t rows = a->batch, slots = (int64_t)num_sms() * resident, threads = slots * kBlock;
+    const int64_t cells = a->tokens * rows * columns, waves = ceil_div(cells, 64 * threads);
+    if (!waves) return 4;
+    int64_t tile = ceil_div(cells, waves * threads);
+    if (by > 1) {   // blocks are whole: lengthen the walk until they fit
+        const int64_t per = ceil_div(columns, kBlock / by);
+        while (tile < 64 && ceil_div(ceil_div(a->tokens, tile) * rows, by) * per > waves * slots) ++tile;
+    }
     return tile < 4 ? 4 : tile;
 }
 
 template <typename T, int W, int V>
 int conv_run(const pe_conv_args* a, cudaStream_t s) {
-    const ConvP<T> p = conv_params<T>(a, V, tile_of(a, V));
+    const ConvP<T> p = conv_params<T>(a, V, tile_of(a, a->channels / V, 2, 1));
     const int64_t ids = (p.tiles + (p.state ? a->nseq : 0)) * p.CV, blocks = ceil_div(ids, kBlock);
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     if (!blocks) return PE_OK;
@@ -412,13 +416,14 @@ int conv_run(const pe_conv_args* a, cudaStream_t s) {
 
 struct ConvGradShape {
     int bx;
-    int64_t rows;       // blocks along the tokens
+    int64_t tile, rows;   // tokens a thread, blocks along the tokens
 };
 ConvGradShape grad_shape(const pe_conv_args* a, int v) {
     const int64_t cv = a->channels / v;
-    ConvGradShape g{1, 0};
+    ConvGradShape g{1, 4, 0};
     while (g.bx < 32 && g.bx < cv) g.bx *= 2;
-    g.rows = ceil_div(ceil_div(a->tokens, tile_of(a, v)) * a->batch, kBlock / g.bx);
+    g.tile = tile_of(a, cv, 1, kBlock / g.bx);
+    g.rows = ceil_div(ceil_div(a->tokens, g.tile) * a->batch, kBlock / g.bx);
     return g;
 }
 
@@ -427,7 +432,7 @@ int conv_grad_run(const pe_conv_grad_args* g, cudaStream_t s) {
     const pe_conv_args* a = &g->fwd;
     const ConvGradShape sh = grad_shape(a, V);
     ConvGradP<T> p;
-    p.f = conv_params<T>(a, V, tile_of(a, V));
+    p.f = conv_params<T>(a, V, sh.tile);
     p.dout = (const T*)g->dout; p.dstate = (const T*)g->dstate;
     p.o_sb = g->dout_sb; p.o_st = g->dout_st;
     p.dx = (T*)g->dx; p.dinit = (T*)g->dinit;
@@ -492,14 +497,8 @@ int conv_step_w(const pe_conv_step_args* a, cudaStream_t s) { PE_CONV_W(conv_ste
         default: return vec ? F<__nv_bfloat16, 8>(__VA_ARGS__) : F<__nv_bfloat16, 1>(__VA_ARGS__);  \
     }
 int conv_any(const pe_conv_args* a, bool vec, cudaStream_t s) { PE_CONV_T(conv_w, a->dtype, vec, a, s) }
-// The backward pass keeps 2 (W + 1) sums and taps a channel besides two windows: four
-// channels a thread in every type.
 int conv_grad_any(const pe_conv_grad_args* a, bool vec, cudaStream_t s) {
-    switch (a->fwd.dtype) {
-        case PE_F32: return vec ? conv_grad_w<float, 4>(a, s) : conv_grad_w<float, 1>(a, s);
-        case PE_F16: return vec ? conv_grad_w<__half, 4>(a, s) : conv_grad_w<__half, 1>(a, s);
-        default: return vec ? conv_grad_w<__nv_bfloat16, 4>(a, s) : conv_grad_w<__nv_bfloat16, 1>(a, s);
-    }
+    PE_CONV_T(conv_grad_w, a->fwd.dtype, vec, a, s)
 }
 int conv_step_any(const pe_conv_step_args* a, bool vec, cudaStream_t s) { PE_CONV_T(conv_step_w, a->dtype, vec, a, s) }
 
@@ -521,7 +520,8 @@ int64_t conv_grad_ws_bytes(const pe_conv_grad_args* g) {
     if (!g || check_conv(&g->fwd) != PE_OK) return 0;
     const pe_conv_args* a = &g->fwd;
     // enough for either width of the loads: the size does not depend on addresses
-    const int64_t rows = grad_shape(a, 1).rows, wide_rows = a->channels % 4 ? rows : grad_shape(a, 4).rows;
+    const int v = 16 / elem_bytes(a->dtype);
+    const int64_t rows = grad_shape(a, 1).rows, wide_rows = a->channels % v ? rows : grad_shape(a, v).rows;
     return (rows > wide_rows ? rows : wide_rows) * a->channels * (a->width + 1) * 4;
 }
 

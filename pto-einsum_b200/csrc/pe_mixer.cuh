@@ -193,6 +193,11 @@ __device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
     return pack2(sigmoidf(lo), sigmoidf(hi));
 }
 
+// d silu(x) / dx with s = sigmoid(x), in pairs.
+__device__ __forceinline__ f32x2 silu_slope2(f32x2 x, f32x2 s) {
+    return mul2(s, fma2(x, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
+}
+
 // ---- asynchronous copies ------------------------------------------------------------
 template <int BYTES>
 __device__ __forceinline__ void cp_async(void* dst, const void* src, int valid) {

@@ -88,7 +88,7 @@ struct Items {
     }
 };
 
-// L lanes share a group and take its rows r, r + R, ...; the next row's loads are on the
+// L lanes share a group and take its rows r, r + R, ...; the next three rows are on their
 // way while the current one is reduced. All lanes make the same number of rounds, for
 // the shuffles take all of them.
 template <typename T, int V, int K>
@@ -101,8 +101,11 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
     const Items<V, K> it(l, L, per, live ? per * (int)p.S : 0, g * p.cg);
     const float inv = 1.0f / (float)(p.cg * (int)p.S);
     constexpr int Q = kPairs<V>;
+    constexpr int DEPTH = 4;   // three rows on their way
+    extern __shared__ __align__(16) unsigned char queues[];
+    Vec<T, V>* slots = reinterpret_cast<Vec<T, V>*>(queues);
+    Ring<T, V, DEPTH * K> rx(slots, kBlock), rz(slots + DEPTH * K * kBlock, kBlock);
     int64_t xo[K], go[K];
-    Vec<T, V> x[K], z[K];
     f32x2 w[K][Q], b[K][Q];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -113,30 +116,34 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
         if (it.in[k] && p.w) widen<T, V>(load_vec<T, V>(p.w + it.c[k]), w[k]);
         if (it.in[k] && p.b) widen<T, V>(load_vec<T, V>(p.b + it.c[k]), b[k]);
     }
-    auto load = [&](int64_t n) {
+    auto fetch = [&](int64_t n, int step) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (it.in[k] && n < p.N) {
-                x[k] = load_vec<T, V>(p.x + n * p.x_sb + xo[k]);
-                if (p.mode == kGate) z[k] = load_vec<T, V>(p.gate + n * p.g_sb + go[k]);
-            }
+        for (int k = 0; k < K; ++k) {
+            const bool on = it.in[k] && n < p.N;
+            rx.fetch(step * K + k, p.x + n * p.x_sb + xo[k], on);
+            if (p.mode == kGate) rz.fetch(step * K + k, p.gate + n * p.g_sb + go[k], on);
+        }
+        cp_commit();
     };
-    load(r);
-    for (int64_t n0 = 0; n0 < p.N; n0 += R) {
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i) fetch(r + (int64_t)i * R, i);
+    int step = 0;
+    for (int64_t n0 = 0; n0 < p.N; n0 += R, ++step) {
         const int64_t n = n0 + r;
         const bool on = n < p.N;
         f32x2 f[K][Q], ga[K][Q];
         float sum[1] = {0.0f};
+        cp_wait_but<DEPTH - 2>();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            widen<T, V>(x[k], f[k]);
-            if (p.mode == kGate) widen<T, V>(z[k], ga[k]);
+            widen<T, V>(rx.get(step * K + k), f[k]);
+            if (p.mode == kGate) widen<T, V>(rz.get(step * K + k), ga[k]);
             f32x2 s = f[k][0];
 #pragma unroll
             for (int q = 1; q < Q; ++q) s = add2(s, f[k][q]);
             sum[0] += it.in[k] ? halves(s) : 0.0f;
         }
-        load(n + R);
+        fetch(n + (DEPTH - 1) * (int64_t)R, step + DEPTH - 1);   // into the slots of the row before this one
         group_sum(sum, L, red);
         const float mean = sum[0] * inv;
         const f32x2 minus = each<V>(-mean);
@@ -172,6 +179,7 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
             store_vec(p.out + (n * p.S + it.place[k]) * p.C + it.c[k], narrow<T, V>(y));
         }
     }
+    cp_wait();
 }
 
 // g = dL / dv, and the gate's gradient in place of `ga`.
@@ -193,9 +201,6 @@ __device__ __forceinline__ void through_act(int mode, const float (&xn)[V], cons
 }
 
 // The same in pairs.
-__device__ __forceinline__ f32x2 silu_slope2(f32x2 x, f32x2 s) {
-    return mul2(s, fma2(x, add2(both(1.0f), mul2(s, both(-1.0f))), both(1.0f)));
-}
 template <int Q>
 __device__ __forceinline__ void through_act2(int mode, const f32x2 (&xn)[Q], const f32x2 (&w)[Q], const f32x2 (&b)[Q],
                                              f32x2 (&go)[Q], f32x2 (&ga)[Q]) {
@@ -226,9 +231,13 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
     const int per = p.cg / V;
     const Items<V, K> it(l, L, per, live ? per : 0, g * p.cg);
     const float inv = 1.0f / (float)p.cg;
+    constexpr int DEPTH = 4;
+    extern __shared__ __align__(16) unsigned char queues[];
+    Vec<T, V>* slots = reinterpret_cast<Vec<T, V>*>(queues);
+    constexpr int each_queue = DEPTH * K * kBlock;
+    Ring<T, V, DEPTH * K> rx(slots, kBlock), ro(slots + each_queue, kBlock), rz(slots + 2 * each_queue, kBlock);
     f32x2 aw[K][Q], ab[K][Q], w[K][Q], b[K][Q];
-    Vec<T, V> x[K], z[K], o[K];
-    float mean = 0.0f, rstd = 0.0f;
+    float mean = 0.0f, rstd = 0.0f, mean2 = 0.0f, rstd2 = 0.0f;   // of this row and the next
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -236,23 +245,33 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
         if (it.in[k] && p.w) widen<T, V>(load_vec<T, V>(p.w + it.c[k]), w[k]);
         if (it.in[k] && p.b) widen<T, V>(load_vec<T, V>(p.b + it.c[k]), b[k]);
     }
-    auto load = [&](int64_t n) {
-        if (n < p.N) {
-            mean = __ldg(p.mean + n * p.G + g);
-            rstd = __ldg(p.rstd + n * p.G + g);
-        }
+    auto fetch = [&](int64_t n, int step) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (it.in[k] && n < p.N) {
-                x[k] = load_vec<T, V>(p.x + n * p.x_sb + it.c[k]);
-                o[k] = load_vec<T, V>(p.dout + n * p.o_sb + it.c[k]);
-                if (p.mode == kGate) z[k] = load_vec<T, V>(p.gate + n * p.g_sb + it.c[k]);
-            }
+        for (int k = 0; k < K; ++k) {
+            const bool on = it.in[k] && n < p.N;
+            rx.fetch(step * K + k, p.x + n * p.x_sb + it.c[k], on);
+            ro.fetch(step * K + k, p.dout + n * p.o_sb + it.c[k], on);
+            if (p.mode == kGate) rz.fetch(step * K + k, p.gate + n * p.g_sb + it.c[k], on);
+        }
+        cp_commit();
     };
-    load(r);
-    for (int64_t n0 = 0; n0 < p.N; n0 += R) {
+    auto stats = [&](int64_t n) {
+        if (n < p.N) {
+            mean2 = __ldg(p.mean + n * p.G + g);
+            rstd2 = __ldg(p.rstd + n * p.G + g);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i) fetch(r + (int64_t)i * R, i);
+    stats(r);
+    int step = 0;
+    for (int64_t n0 = 0; n0 < p.N; n0 += R, ++step) {
         const int64_t n = n0 + r;
         const bool on = n < p.N;
+        mean = mean2;
+        rstd = rstd2;
+        stats(n + R);
+        cp_wait_but<DEPTH - 2>();
         const f32x2 minus = each<V>(-mean), scale = both(rstd);
         f32x2 xn[K][Q], go[K][Q];
         float sum[2] = {0.0f, 0.0f};
@@ -260,9 +279,9 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
         for (int k = 0; k < K; ++k) {
             if (!it.in[k] || !on) continue;
             f32x2 ga[Q], s0 = 0, s1 = 0;
-            widen<T, V>(x[k], xn[k]);
-            widen<T, V>(o[k], go[k]);
-            if (p.mode == kGate) widen<T, V>(z[k], ga);
+            widen<T, V>(rx.get(step * K + k), xn[k]);
+            widen<T, V>(ro.get(step * K + k), go[k]);
+            if (p.mode == kGate) widen<T, V>(rz.get(step * K + k), ga);
 #pragma unroll
             for (int q = 0; q < Q; ++q) xn[k][q] = mul2(add2(xn[k][q], minus), scale);
             through_act2<Q>(p.mode, xn[k], w[k], b[k], go[k], ga);
@@ -278,7 +297,7 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
             sum[0] += halves(s0);
             sum[1] += halves(s1);
         }
-        load(n + R);
+        fetch(n + (DEPTH - 1) * (int64_t)R, step + DEPTH - 1);   // into the slots of the row before this one
         group_sum(sum, L, red);
         const f32x2 m0 = both(-sum[0] * inv), m1 = both(-sum[1] * inv);
 #pragma unroll
@@ -290,6 +309,7 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
             store_vec(p.dx + n * p.C + it.c[k], narrow<T, V>(d));
         }
     }
+    cp_wait();
     if (!pw) return;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -313,6 +333,9 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
 struct Slab {
     int CS, slabs, R, P;
 };
+__host__ __device__ __forceinline__ int slab_floats(int n) { return (n + 3) / 4 * 16; }   // their bytes, whole 16s
+// Floats of the segments' sums: at most kBlock segments, or one a channel.
+__host__ __device__ __forceinline__ int slab_sums(int cs) { return (cs > kBlock ? cs : kBlock) + 3 & ~3; }
 
 __device__ __forceinline__ float remote(const float* own, int rank) {
     float v;
@@ -328,9 +351,9 @@ struct SlabPlace {
     bool on;
     __device__ __forceinline__ SlabPlace(const NormP<T>& p, const Slab& q) {
         const int rank = (int)cluster_rank();
-        const int64_t unit = blockIdx.x / q.R;
-        n = unit / q.slabs;
-        c0 = (unit - n * q.slabs) * q.CS;
+        const unsigned unit = blockIdx.x / (unsigned)q.R;
+        n = unit / (unsigned)q.slabs;
+        c0 = (int64_t)(unit % (unsigned)q.slabs) * q.CS;
         cs = (int)min((int64_t)q.CS, p.C - c0);
         s0 = (int64_t)rank * q.P;
         pc = (int)max((int64_t)0, min((int64_t)q.P, p.S - s0));
@@ -339,6 +362,7 @@ struct SlabPlace {
         x = threadIdx.x % cvn;
         y = threadIdx.x / cvn;
         on = y < by;
+        segs = max(1, min(by, kBlock / cs));
     }
     // this block's places of a tensor into shared memory [P][cs]
     __device__ __forceinline__ void copy(T* dst, const T* src, int64_t sb, int64_t sp) const {
@@ -354,7 +378,9 @@ struct SlabPlace {
     __device__ __forceinline__ void get(const T* tile, int i, f32x2 (&f)[kPairs<V>]) const {
         widen<T, V>(*reinterpret_cast<const Vec<T, V>*>(tile + i * cs + x * V), f);
     }
-    // Sums of a value a channel over the block's row lanes: sums[ch], via red [cs][by].
+    // Sums of a value a channel over the block's row lanes, in `segs` segments a channel:
+    // sums[ch * segs + i], via red [cs][by].
+    int segs;
     __device__ __forceinline__ void channel_sums(const f32x2 (&v)[kPairs<V>], float* red, float* sums) const {
         if (on)
 #pragma unroll
@@ -364,36 +390,38 @@ struct SlabPlace {
                 red[(x * V + k) * by + y] = h[k % 2];
             }
         __syncthreads();
-        const int lane = threadIdx.x & 31;
-        if (by <= 8) {
-            for (int c = threadIdx.x; c < cs; c += kBlock) {
-                float a = 0.0f;
-                for (int i = 0; i < by; ++i) a += red[c * by + i];
-                sums[c] = a;
-            }
-        } else {
-            for (int c = threadIdx.x / 32; c < cs; c += kBlock / 32) {
-                float a = 0.0f;
-                for (int i = lane; i < by; i += 32) a += red[c * by + i];
-#pragma unroll
-                for (int m = 16; m >= 1; m /= 2) a += __shfl_xor_sync(0xffffffffu, a, m);
-                if (lane == 0) sums[c] = a;
-            }
+        const int len = (by + segs - 1) / segs;
+        for (int i = threadIdx.x; i < cs * segs; i += kBlock) {
+            const int c = i / segs, from = (i - c * segs) * len, to = min(by, from + len);
+            float a = 0.0f;
+            for (int k = from; k < to; ++k) a += red[c * by + k];
+            sums[i] = a;
         }
         __syncthreads();
     }
 };
 
-// Sums over each group's channels of a(c), into g; the block's own share.
+// Sums over each group's `items` of a(j, i), into g: the block's own share. A warp a group.
 template <typename F>
-__device__ __forceinline__ void slab_groups(int groups, int cg, float* g, F a) {
+__device__ __forceinline__ void slab_groups(int groups, int items, float* g, F a) {
     const int lane = threadIdx.x & 31;
     for (int j = threadIdx.x / 32; j < groups; j += kBlock / 32) {
         float s = 0.0f;
-        for (int i = lane; i < cg; i += 32) s += a(j * cg + i);
+        for (int i = lane; i < items; i += 32) s += a(j * items + i);
 #pragma unroll
         for (int m = 16; m >= 1; m /= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
         if (lane == 0) g[j] = s;
+    }
+}
+// The blocks' shares of each group added in a fixed order: total[j] = scale * sum. Lane r of
+// a warp reads block r's.
+__device__ __forceinline__ void cluster_groups(int groups, int R, const float* share, float* total, float scale) {
+    const int lane = threadIdx.x & 31;
+    for (int j = threadIdx.x / 32; j < groups; j += kBlock / 32) {
+        float s = lane < R ? remote(share + j, lane) : 0.0f;
+#pragma unroll
+        for (int m = 4; m >= 1; m /= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
+        if (lane == 0) total[j] = s * scale;
     }
 }
 
@@ -402,8 +430,8 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab(const __grid_constant__ N
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) unsigned char smem[];
     float* red = reinterpret_cast<float*>(smem);        // [kBlock V]
-    float *sums = red + kBlock * V, *share = sums + q.CS, *own = share + 2 * q.CS;   // a channel; 2 a group; a group
-    T* tile = reinterpret_cast<T*>(own + q.CS);
+    float *sums = red + kBlock * V, *share = sums + slab_sums(q.CS), *own = share + 2 * q.CS;   // 2 a group; a group
+    T* tile = reinterpret_cast<T*>(smem + slab_floats(kBlock * V + slab_sums(q.CS) + 3 * q.CS));
     const SlabPlace<T, V> at(p, q);
     const int groups = at.cs / p.cg;
     at.copy(tile, p.x, p.x_sb, p.x_sp);
@@ -417,8 +445,14 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab(const __grid_constant__ N
     cp_wait();
     // own places only: a thread reads what it copied
     f32x2 mean[Q], rstd[Q], s[Q];
+    int g0[Q], g1[Q];   // the channels' groups in the slab
 #pragma unroll
-    for (int k = 0; k < Q; ++k) s[k] = 0;
+    for (int k = 0; k < Q; ++k) {
+        const int c = at.on ? at.x * V + 2 * k : 0;
+        s[k] = 0;
+        g0[k] = c / p.cg;
+        g1[k] = (c + (V > 1)) / p.cg;
+    }
     if (at.on)
 #pragma unroll 4
         for (int i = at.y; i < at.pc; i += at.by) {
@@ -430,20 +464,13 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab(const __grid_constant__ N
     // (sum over all places of each group) inv, a channel's pair
     auto over_group = [&](float* to, f32x2 (&out)[Q]) {
         at.channel_sums(s, red, sums);
-        slab_groups(groups, p.cg, to, [&](int c) { return sums[c]; });
+        slab_groups(groups, p.cg * at.segs, to, [&](int i) { return sums[i]; });
         __syncthreads();
         cluster_sync();
-        for (int j = threadIdx.x; j < groups; j += kBlock) {
-            float a = 0.0f;
-            for (int r = 0; r < q.R; ++r) a += remote(to + j, r);
-            own[j] = a * inv;
-        }
+        cluster_groups(groups, q.R, to, own, inv);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-            const int c = at.on ? at.x * V + 2 * k : 0;
-            out[k] = pack2(own[c / p.cg], V == 1 ? 0.0f : own[(c + 1) / p.cg]);
-        }
+        for (int k = 0; k < Q; ++k) out[k] = pack2(own[g0[k]], V == 1 ? 0.0f : own[g1[k]]);
     };
     over_group(share, mean);
     float keep = 0.0f;
@@ -503,8 +530,8 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab_bwd(const __grid_constant
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) unsigned char smem[];
     float* red = reinterpret_cast<float*>(smem);        // [kBlock V]
-    float *sw = red + kBlock * V, *sb = sw + q.CS, *share = sb + q.CS, *own = share + 2 * q.CS;
-    T* tx = reinterpret_cast<T*>(own + 2 * q.CS);
+    float *sw = red + kBlock * V, *sb = sw + slab_sums(q.CS), *share = sb + slab_sums(q.CS), *own = share + 2 * q.CS;
+    T* tx = reinterpret_cast<T*>(smem + slab_floats(kBlock * V + 2 * slab_sums(q.CS) + 4 * q.CS));
     T* to = tx + (int64_t)q.P * q.CS;
     const SlabPlace<T, V> at(p, q);
     const int groups = at.cs / p.cg;
@@ -551,21 +578,19 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab_bwd(const __grid_constant
     if (pw)
         for (int i = threadIdx.x; i < at.cs; i += kBlock) {
             const int64_t row = at.n * q.R + cluster_rank();
-            pw[row * p.C + at.c0 + i] = sw[i];
-            pb[row * p.C + at.c0 + i] = sb[i];
+            float a = 0.0f, b = 0.0f;
+            for (int k = 0; k < at.segs; ++k) a += sw[i * at.segs + k], b += sb[i * at.segs + k];
+            pw[row * p.C + at.c0 + i] = a;
+            pb[row * p.C + at.c0 + i] = b;
         }
-    auto weight = [&](int i) { return p.w ? to_float(__ldg(p.w + at.c0 + i)) : 1.0f; };
-    slab_groups(groups, p.cg, share, [&](int i) { return weight(i) * sb[i]; });
-    slab_groups(groups, p.cg, share + q.CS, [&](int i) { return weight(i) * sw[i]; });
+    auto weight = [&](int i) { return p.w ? to_float(__ldg(p.w + at.c0 + i / at.segs)) : 1.0f; };
+    slab_groups(groups, p.cg * at.segs, share, [&](int i) { return weight(i) * sb[i]; });
+    slab_groups(groups, p.cg * at.segs, share + q.CS, [&](int i) { return weight(i) * sw[i]; });
     __syncthreads();
     cluster_sync();
     const float inv = 1.0f / ((float)p.cg * (float)p.S);
-    for (int j = threadIdx.x; j < groups; j += kBlock) {
-        float m0 = 0.0f, m1 = 0.0f;
-        for (int r = 0; r < q.R; ++r) m0 += remote(share + j, r), m1 += remote(share + q.CS + j, r);
-        own[j] = -m0 * inv;
-        own[q.CS + j] = -m1 * inv;
-    }
+    cluster_groups(groups, q.R, share, own, -inv);
+    cluster_groups(groups, q.R, share + q.CS, own + q.CS, -inv);
     __syncthreads();
     if (at.on) {
         f32x2 m0[Q], m1[Q];
@@ -880,7 +905,7 @@ struct Plan {
 };
 
 int64_t slab_smem(int64_t cs, int64_t P, int v, int64_t es, bool grad) {
-    return (kBlock * v + (grad ? 6 : 4) * cs) * 4 + (grad ? 2 : 1) * ceil_div(P * cs * es, 16) * 16;
+    return slab_floats(kBlock * v + (grad ? 2 : 1) * slab_sums((int)cs) + (grad ? 4 : 3) * (int)cs) + (grad ? 2 : 1) * ceil_div(P * cs * es, 16) * 16;
 }
 
 // The slab of a group that is too large for registers: whole groups and whole loads, 64
@@ -899,7 +924,7 @@ Slab slab_of(const pe_norm_args* a, int v, bool grad) {
         for (int r = 1; r <= 8; r *= 2) {
             const int64_t P = ceil_div(a->places, r);
             if (slab_smem(cs, P, v, es, grad) > room) continue;
-            if (room == 100 * 1024 && r < 8 && a->batch * slabs * r < num_sms() && P * (cs / v) > 2 * kBlock) continue;
+            if (room == 100 * 1024 && r < 8 && a->batch * slabs * r * 4 < num_sms() * 3 && P * (cs / v) > 2 * kBlock) continue;
             s.CS = (int)cs; s.slabs = (int)slabs; s.R = r; s.P = (int)P;
             return s;
         }
@@ -966,6 +991,20 @@ int64_t stats_floats(const pe_norm_args* a, const Plan& pl) {
     return pl.lanes || pl.slab.R ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->groups);
 }
 
+// Shared memory of the register kernels' queues: four rows of k loads a lane and stream.
+template <typename T, int V>
+int queue_bytes(int k, int streams) {
+    return 4 * k * streams * kBlock * V * (int)sizeof(T);
+}
+template <typename K, typename... A>
+int launch_reg(K kernel, int64_t blocks, int smem, cudaStream_t s, A... args) {
+    if (smem > 40 * 1024 &&   // the kernels have some static shared memory too
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return PE_ERR_CUDA;
+    kernel<<<(unsigned)blocks, kBlock, smem, s>>>(args...);
+    return launched();
+}
+
 template <typename K, typename... A>
 int launch_slab(K kernel, int64_t rows, const Slab& q, int64_t smem, cudaStream_t s, A... args) {
     const int64_t blocks = rows * q.slabs * q.R;
@@ -996,10 +1035,10 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
     if (pl.lanes) {
         const int64_t blocks = ceil_div(pl.R * p.G * pl.lanes, kBlock);
         if (blocks > 0x7fffffll) return PE_ERR_UNSUPPORTED;
-        if (pl.k == 1) norm_reg<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
-        else if (pl.k == 2) norm_reg<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
-        else norm_reg<T, V, 4><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R);
-        return launched();
+        const int streams = p.mode == kGate ? 2 : 1;
+        if (pl.k == 1) return launch_reg(norm_reg<T, V, 1>, blocks, queue_bytes<T, V>(1, streams), s, p, pl.lanes, (int)pl.R);
+        if (pl.k == 2) return launch_reg(norm_reg<T, V, 2>, blocks, queue_bytes<T, V>(2, streams), s, p, pl.lanes, (int)pl.R);
+        return launch_reg(norm_reg<T, V, 4>, blocks, queue_bytes<T, V>(4, streams), s, p, pl.lanes, (int)pl.R);
     }
     if (pl.slab.R)
         return launch_slab(norm_slab<T, V>, p.N, pl.slab, slab_smem(pl.slab.CS, pl.slab.P, V, sizeof(T), false), s, p,
@@ -1043,9 +1082,12 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
         sw = ws;
         sb = ws + rows * p.C;
         float* pw = sums ? sw : nullptr;
-        if (pl.k == 1) norm_reg_bwd<T, V, 1><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R, pw, sb);
-        else norm_reg_bwd<T, V, 2><<<(unsigned)blocks, kBlock, 0, s>>>(p, pl.lanes, (int)pl.R, pw, sb);
-        if (int rc = launched()) return rc;
+        const int streams = p.mode == kGate ? 3 : 2;
+        const int rc = pl.k == 1 ? launch_reg(norm_reg_bwd<T, V, 1>, blocks, queue_bytes<T, V>(1, streams), s, p, pl.lanes,
+                                              (int)pl.R, pw, sb)
+                                 : launch_reg(norm_reg_bwd<T, V, 2>, blocks, queue_bytes<T, V>(2, streams), s, p, pl.lanes,
+                                              (int)pl.R, pw, sb);
+        if (rc) return rc;
     } else if (pl.slab.R) {
         rows = p.N * pl.slab.R;
         sw = ws;
