@@ -10,6 +10,7 @@
 // B and C in fp32; the sums over states are reduced for LPC tokens together
 // (reduce_scatter: LPC - 1 shuffles for LPC tokens).
 #include <cmath>
+#include <cstddef>
 
 #include "pe_scan.cuh"
 
@@ -61,6 +62,64 @@ struct FwdSmem {
     float y[2][STATE_ONLY ? 4 : TS * L::Y];
 };
 
+// The copies of a tile where every row allows 16-byte chunks: the chunks of all tensors
+// in one list, a thread's entries of it worked out once.
+template <typename T, int LPC, bool STATE_ONLY>
+struct Feeder {
+    using L = Lanes<LPC>;
+    using F = FwdSmem<T, LPC, STATE_ONLY>;
+    static constexpr int E = 16 / (int)sizeof(T);
+    static constexpr int PC = L::CH / E, PN = L::NP / E;   // chunks a row
+    static constexpr bool POSSIBLE = L::CH % E == 0 && L::NP % E == 0;
+    static constexpr int TOTAL = TS * ((STATE_ONLY ? 2 : 3) * PC + (STATE_ONLY ? 1 : 2) * PN);
+    static constexpr int J = (TOTAL + kThreads - 1) / kThreads;
+    const T* src[J];
+    int64_t step[J];      // elements a tile
+    int to[J], valid[J];  // offset in the raw buffer; bytes
+    int t[J];             // row of the tile (TS: none)
+
+    __device__ __forceinline__ void init(const ScanP<T>& p, const Place& w, const T* u, const T* d, const T* z,
+                                         const T* b, const T* c) {
+        using Raw = typename F::Raw;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            int i = threadIdx.x + j * kThreads;
+            t[j] = TS;
+            src[j] = u;
+            to[j] = valid[j] = 0;
+            step[j] = 0;
+            auto entry = [&](const T* from, int64_t st, int per, int width, int base, int row) {
+                if (i >= 0 && i < TS * per && from) {
+                    const int r = i / per, k = i % per * E;
+                    if (k < width) {
+                        t[j] = r;
+                        src[j] = from + r * st + k;
+                        step[j] = TS * st;
+                        to[j] = base + (r * row + k) * (int)sizeof(T);
+                        valid[j] = min(16, (width - k) * (int)sizeof(T));
+                    }
+                }
+                i -= TS * per;
+            };
+            entry(u, p.u_st, PC, w.nch, (int)offsetof(Raw, u), L::CH);
+            entry(d, p.d_st, PC, w.nch, (int)offsetof(Raw, d), L::CH);
+            entry(b, p.B_st, PN, p.N, (int)offsetof(Raw, b), L::NP);
+            if constexpr (!STATE_ONLY) {
+                entry(c, p.C_st, PN, p.N, (int)offsetof(Raw, c), L::NP);
+                entry(z, p.z_st, PC, w.nch, (int)offsetof(Raw, z), L::CH);
+            }
+        }
+    }
+    // the next tile, of cnt tokens
+    __device__ __forceinline__ void copy(void* raw, int cnt) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (t[j] < cnt) cp_async<16>((char*)raw + to[j], src[j], valid[j]);
+            src[j] += step[j];
+        }
+    }
+};
+
 // STATE_ONLY: a piece's last state from a zero start and its sum of dt (first half of
 // a split scan); else the whole, starting from what the sequence's earlier pieces left.
 //
@@ -91,9 +150,18 @@ __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
     const T* B = p.B + w.sp.row * p.B_sb + row0 * p.B_st + w.g * p.B_sg;
     const T* C = p.C + w.sp.row * p.C_sb + row0 * p.C_st + w.g * p.C_sg;
     const int64_t count = w.t1 - w.t0;                        // tokens
-    auto copy = [&](int64_t t, int b) {
+    using Feed = Feeder<T, LPC, STATE_ONLY>;
+    Feed feed;
+    const bool fast = Feed::POSSIBLE && p.fast;
+    if (fast) feed.init(p, w, u, delta, z, B, C);
+    auto copy = [&](int64_t t, int b) {   // tiles in order
         if (t < count) {
             const int cnt = (int)min((int64_t)TS, count - t);
+            if (fast) {
+                feed.copy(&m.raw[b], cnt);
+                cp_commit();
+                return;
+            }
             stage<TS, CH>(m.raw[b].u, u + t * p.u_st, p.u_st, cnt, w.nch, p.u_cb);
             stage<TS, CH>(m.raw[b].d, delta + t * p.d_st, p.d_st, cnt, w.nch, p.d_cb);
             stage<TS, NP>(m.raw[b].b, B + t * p.B_st, p.B_st, cnt, p.N, p.B_cb);
@@ -508,6 +576,7 @@ int scan_run(const pe_scan_args* a, cudaStream_t s) {
     const int64_t piece = piece_tokens(a);
     if (piece) {
         p.piece = piece;
+        p.longest_first = false;
         const int64_t n = piece_count(p.seqs, piece);
         p.hloc = (float*)a->ws;
         p.dtsum = p.hloc + n * p.D * p.N;

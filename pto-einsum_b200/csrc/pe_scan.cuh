@@ -27,7 +27,9 @@ struct ScanP {
     float *state, *ckpt;
     // copies to shared memory: rows of these tensors in chunks (see chunk_of), 0 = element by element
     int u_cb, d_cb, z_cb, B_cb, C_cb;
+    bool fast;            // all of them in chunks of 16
     bool pairs;           // out's rows take aligned pairs of elements
+    bool longest_first;   // packed sequences are taken in the order of their lengths
     int64_t piece;        // tokens a piece (a multiple of KCK, or more than any sequence has)
     float *hloc, *dtsum;  // ws of a split scan: each piece's own last state and sum of dt
 };
@@ -43,6 +45,25 @@ struct Place {
     bool any;              // false: a number that stands for no piece
 };
 
+// The sequence with `rank` longer ones (equal lengths in order), for up to kThreads of
+// them: blocks that take whole sequences of very different lengths start with the longest,
+// or the last one to start would end long after the others.
+__device__ __forceinline__ int seq_of_rank(const Seqs& q, int rank) {
+    __shared__ int found;
+    const int i = threadIdx.x;
+    if (i < q.nseq) {
+        const int64_t len = seq_span(q, i).len;
+        int longer = 0;
+        for (int j = 0; j < q.nseq; ++j) {
+            const int64_t l = seq_span(q, j).len;
+            longer += l > len || (l == len && j < i);
+        }
+        if (longer == rank) found = i;
+    }
+    __syncthreads();
+    return found;
+}
+
 template <int CH, typename P>
 __device__ __forceinline__ Place place_of(const P& p) {
     Place w;
@@ -51,6 +72,7 @@ __device__ __forceinline__ Place place_of(const P& p) {
     b /= p.ntile;
     w.g = (int)(b % p.G);
     w.number = b / p.G;
+    if (p.longest_first && w.number < p.seqs.nseq) w.number = seq_of_rank(p.seqs, (int)w.number);
     piece_find(p.seqs, w.number, p.piece, w.s, w.j);
     w.sp = seq_span(p.seqs, w.s);
     w.t0 = w.j * p.piece;
@@ -134,6 +156,7 @@ ScanP<T> scan_params(const pe_scan_args* a, int ch, int nc) {
     p.C_sb = a->C_sb; p.C_st = a->C_st; p.C_sg = a->C_sg;
     p.out = (T*)a->out; p.state = a->state; p.ckpt = a->ckpt;
     p.piece = (a->tokens / KCK + 1) * KCK;   // longer than any sequence: one piece each, numbered like it
+    p.longest_first = a->cu && a->nseq > 1 && a->nseq <= kThreads;   // whole sequences; a split clears it
     p.hloc = p.dtsum = nullptr;
     const int es = sizeof(T);
     const int64_t step = p.G > 1 ? p.Dg : ch, row = (int64_t)ch * es;   // of a block's first channel
@@ -143,6 +166,7 @@ ScanP<T> scan_params(const pe_scan_args* a, int ch, int nc) {
     p.z_cb = p.z ? chunk_of(p.z, es, row, {p.z_sb, p.z_st, (int64_t)ch}, step) : 0;
     p.B_cb = chunk_of(p.B, es, cols, {p.B_sb, p.B_st, p.B_sg}, nc);
     p.C_cb = chunk_of(p.C, es, cols, {p.C_sb, p.C_st, p.C_sg}, nc);
+    p.fast = p.u_cb == 16 && p.d_cb == 16 && (!p.z || p.z_cb == 16) && p.B_cb == 16 && p.C_cb == 16;
     p.pairs = p.Dg % 2 == 0;
     return p;
 }
