@@ -45,20 +45,37 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const __grid_constant__ 
     }
 }
 
+// The same for a few rows: a thread a column.
+__global__ void __launch_bounds__(256) sum_few_rows(const __grid_constant__ Jobs jobs) {
+    const SumJob& j = jobs.j[blockIdx.y];
+    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < j.cols; c += (int64_t)gridDim.x * 256) {
+        float a = 0.0f;
+#pragma unroll 8
+        for (int64_t r = 0; r < j.rows; ++r) a += __ldg(j.part + r * j.cols + c);
+        store_sum(j, c, a);
+    }
+}
+
 }  // namespace
 
 int sum_rows(const SumJob* jobs, int count, cudaStream_t s) {
     Jobs all{};
     int n = 0;
-    int64_t most = 0;
+    int64_t most = 0, rows = 0;
     for (int i = 0; i < count; ++i)
         if (jobs[i].out && jobs[i].cols > 0) {
             all.j[n++] = jobs[i];
             most = jobs[i].cols > most ? jobs[i].cols : most;
+            rows = jobs[i].rows > rows ? jobs[i].rows : rows;
         }
     if (!n) return PE_OK;
-    const int64_t blocks = ceil_div(most, 32);
-    sum_rows_kernel<<<dim3((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), n), 1024, 0, s>>>(all);
+    const bool few = rows <= 16;   // no more loads a thread than the other kernel's columns take
+    const int64_t blocks = ceil_div(most, few ? 256 : 32);
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), n);
+    if (few)
+        sum_few_rows<<<grid, 256, 0, s>>>(all);
+    else
+        sum_rows_kernel<<<grid, 1024, 0, s>>>(all);
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }

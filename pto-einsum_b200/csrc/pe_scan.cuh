@@ -84,30 +84,30 @@ __device__ __forceinline__ Place place_of(const P& p) {
 }
 
 // ---- copies to shared memory ------------------------------------------------------
-// cnt (at most ROWS) rows of `width` (at most W) elements into rows of W, in chunks of
+// By the NT threads of the block: cnt (at most ROWS) rows of `width` (at most W) elements into rows of W, in chunks of
 // `cb` bytes that arrive asynchronously where the rows are aligned for them. Nothing
 // past the width or the count is read; there the tile stays as it was.
-template <int ROWS, int W, int BYTES, typename T>
+template <int ROWS, int W, int BYTES, int NT, typename T>
 __device__ __forceinline__ void stage_chunks(T* dst, const T* src, int64_t st, int cnt, int width) {
     constexpr int E = BYTES / (int)sizeof(T), PER = W / E;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < ROWS * PER; i += kThreads) {
+    for (int i = threadIdx.x; i < ROWS * PER; i += NT) {
         const int t = i / PER, k = i % PER * E;
         if (t < cnt && k < width)
             cp_async<BYTES>(dst + t * W + k, src + t * st + k, min(BYTES, (width - k) * (int)sizeof(T)));
     }
 }
-template <int ROWS, int W, typename T>
+template <int ROWS, int W, int NT = kThreads, typename T>
 __device__ __forceinline__ void stage(T* dst, const T* src, int64_t st, int cnt, int width, int cb) {
     constexpr int ROW = W * (int)sizeof(T);
     static_assert(ROW % 8 == 0, "rows of whole chunks");
     if (ROW % 16 == 0 && cb == 16) {
-        stage_chunks<ROWS, W, 16>(dst, src, st, cnt, width);
+        stage_chunks<ROWS, W, 16, NT>(dst, src, st, cnt, width);
     } else if (cb >= 8) {
-        stage_chunks<ROWS, W, 8>(dst, src, st, cnt, width);
+        stage_chunks<ROWS, W, 8, NT>(dst, src, st, cnt, width);
     } else {
 #pragma unroll 4
-        for (int i = threadIdx.x; i < ROWS * W; i += kThreads) {
+        for (int i = threadIdx.x; i < ROWS * W; i += NT) {
             const int t = i / W, k = i % W;
             if (t < cnt && k < width) dst[i] = __ldg(src + t * st + k);
         }
@@ -178,11 +178,11 @@ inline int grid_of(int64_t blocks, unsigned* grid) {
 }
 
 template <typename K, typename P>
-int launch(K kernel, const P& p, unsigned grid, int smem, cudaStream_t s) {
+int launch(K kernel, const P& p, unsigned grid, int smem, cudaStream_t s, int threads = kThreads) {
     if (smem > 48 * 1024 &&
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return PE_ERR_CUDA;
-    kernel<<<grid, kThreads, smem, s>>>(p);
+    kernel<<<grid, threads, smem, s>>>(p);
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }

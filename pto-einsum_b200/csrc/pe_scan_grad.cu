@@ -20,11 +20,11 @@ __device__ __forceinline__ int at_token(int t) { return t / K * SEG + t % K; }
 
 // B or C of a tile's tokens, rows of NC states as in memory, into fp32 [state][token];
 // zero past the last token (a token there must leave the state alone) and state.
-template <int LT, int NC, typename T>
+template <int LT, int NC, int NT, typename T>
 __device__ __forceinline__ void widen_cols(float* dst, const T* src, int cnt, int nn) {
     constexpr int TT = Tile<LT>::TT, RS = Tile<LT>::RS;
 #pragma unroll
-    for (int i = threadIdx.x; i < TT * NC / 4; i += kThreads) {
+    for (int i = threadIdx.x; i < TT * NC / 4; i += NT) {
         const int t = i / (NC / 4), n = i % (NC / 4) * 4;
         const Vec<T, 4> v = *reinterpret_cast<const Vec<T, 4>*>(src + t * NC + n);
 #pragma unroll
@@ -61,36 +61,16 @@ __device__ __forceinline__ float product(const Pairs& a) {
     unpack2(mul2(mul2(a.p[0], a.p[1]), mul2(a.p[2], a.p[3])), lo, hi);
     return lo * hi;
 }
-__device__ __forceinline__ f32x2 shfl2_up(f32x2 v, int d, int width) {
-    float lo, hi;
-    unpack2(v, lo, hi);
-    return pack2(__shfl_up_sync(0xffffffffu, lo, d, width), __shfl_up_sync(0xffffffffu, hi, d, width));
-}
 __device__ __forceinline__ f32x2 shfl2_down(f32x2 v, int d, int width) {
     float lo, hi;
     unpack2(v, lo, hi);
     return pack2(__shfl_down_sync(0xffffffffu, lo, d, width), __shfl_down_sync(0xffffffffu, hi, d, width));
 }
 
-// What the lanes of a channel pair do to the state, composed along the tokens. Lane tl
-// maps the state before it, h, to P h + H (both channels at once). Returns the state
-// before the lane, and in `last` the state after it, given the state `h0` before lane 0.
-template <int LT>
-__device__ __forceinline__ f32x2 scan_lanes_up(f32x2 P, f32x2 H, f32x2 h0, int tl, f32x2& last) {
-    if (tl == 0) H = fma2(P, h0, H);
-#pragma unroll
-    for (int d = 1; d < LT; d *= 2) {
-        const f32x2 Hu = shfl2_up(H, d, LT), Pu = shfl2_up(P, d, LT);
-        if (tl >= d) {
-            H = fma2(P, Hu, H);
-            P = mul2(P, Pu);
-        }
-    }
-    last = H;
-    const f32x2 before = shfl2_up(H, 1, LT);
-    return tl == 0 ? h0 : before;
-}
-// The same from the last token to the first.
+// What the lanes of a channel pair do to the adjoint state, composed from the last token
+// to the first. Lane tl maps the state after it, g, to P g + H (both channels at once).
+// Returns the state after the lane, and in `last` the state before lane 0, given the
+// state `h0` after the last lane.
 template <int LT>
 __device__ __forceinline__ f32x2 scan_lanes_down(f32x2 P, f32x2 H, f32x2 h0, int tl, f32x2& last) {
     if (tl == LT - 1) H = fma2(P, h0, H);
@@ -104,6 +84,37 @@ __device__ __forceinline__ f32x2 scan_lanes_down(f32x2 P, f32x2 H, f32x2 h0, int
     }
     last = H;
     const f32x2 after = shfl2_down(H, 1, LT);
+    return tl == LT - 1 ? h0 : after;
+}
+
+// One channel, and from the first token to the last.
+template <int LT>
+__device__ __forceinline__ float scan_lanes_up(float P, float H, float h0, int tl) {
+    if (tl == 0) H = fmaf(P, h0, H);
+#pragma unroll
+    for (int d = 1; d < LT; d *= 2) {
+        const float Hu = __shfl_up_sync(0xffffffffu, H, d, LT), Pu = __shfl_up_sync(0xffffffffu, P, d, LT);
+        if (tl >= d) {
+            H = fmaf(P, Hu, H);
+            P *= Pu;
+        }
+    }
+    const float before = __shfl_up_sync(0xffffffffu, H, 1, LT);
+    return tl == 0 ? h0 : before;
+}
+template <int LT>
+__device__ __forceinline__ float scan_lanes_down(float P, float H, float h0, int tl, float& last) {
+    if (tl == LT - 1) H = fmaf(P, h0, H);
+#pragma unroll
+    for (int d = 1; d < LT; d *= 2) {
+        const float Hu = __shfl_down_sync(0xffffffffu, H, d, LT), Pu = __shfl_down_sync(0xffffffffu, P, d, LT);
+        if (tl < LT - d) {
+            H = fmaf(P, Hu, H);
+            P *= Pu;
+        }
+    }
+    last = H;
+    const float after = __shfl_down_sync(0xffffffffu, H, 1, LT);
     return tl == LT - 1 ? h0 : after;
 }
 
@@ -128,31 +139,35 @@ struct GradP {
     float *gloc, *dtsum;   // split: each piece's own adjoint state at its start, later the one after it; sum of dt
 };
 
+constexpr int kGradThreads = 256, kGradWarps = kGradThreads / 32;
+static_assert(CB == 32 / LT * kGradWarps, "a channel for every eight lanes");
+
 template <typename T>
 struct GradSmem {
-    static constexpr int NC = sizeof(T) == 2 ? 16 : 8;   // states at a time: two blocks fit an SM
+    static constexpr int NC = 8;                         // states at a time: two blocks fit an SM
     alignas(16) T u[TT * CB];                            // as in memory
     T d[TT * CB], z[TT * CB], o[TT * CB], b[TT * NC], c[TT * NC];
     // fp32, [channel or state][token]; the first three end as du, q u + r and y + D u
     alignas(16) float dt[CB * RS];
     float x[CB * RS], dy[CB * RS];
     float B[NC * RS], C[NC * RS];
-    float red[kWarps][NC][2][TT];                        // a warp's share of dB and dC
+    float red[kGradWarps][NC][2][TT];                    // a warp's share of dB and dC
     float rows[];   // [N][CB] adjoint states, A log2(e), dA; [CB][N] checkpoint
 };
 
 // One block takes 32 channels through a sequence (or a piece of it), tile by tile from
-// its end. Per
-// state n a lane composes the maps of its K tokens forwards (from the checkpoint) and
-// backwards (from the tile after), scans them with the other lanes of its channels, and
-// runs both recurrences again in registers:
+// its end. Per state n a lane composes the maps of its K tokens of its channel forwards
+// (from the checkpoint) and backwards (from the tile after), scans them with the other
+// seven lanes of the channel, and runs both recurrences again in registers:
 //   h = a h' + b,  a = exp(dt A),  b = dt u B;   g = C dy + a' g'
 //   q = sum_n g B,  r = sum_n g a h' A:   du = q dt + D dy,  ddt = q u + r
 //   dB = sum_c g dt u,  dC = sum_c dy h,  dA = sum_t g a h' dt
+// Bound by the instructions issued (about 150 a lane for four states of a token) and by
+// their latencies: sixteen warps an SM at 128 registers.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ GradP<T> p) {
+__global__ void __launch_bounds__(kGradThreads, 2) scan_bwd(const __grid_constant__ GradP<T> p) {
     using M = GradSmem<T>;
-    constexpr int NC = M::NC;
+    constexpr int NC = M::NC, NT = kGradThreads;
     extern __shared__ __align__(16) unsigned char smem[];
     M& m = *reinterpret_cast<M*>(smem);
     const ScanP<T>& f = p.f;
@@ -160,12 +175,12 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
     if (blockIdx.x == 0 && tid < 32) check_offsets(f.seqs, lane, kSiteOffsets);
     const Place w = place_of<CB>(f);
-    const int tl = lane % LT, cl = lane / LT, c = 2 * (warp * (32 / LT) + cl);
+    const int tl = lane % LT, c = warp * (32 / LT) + lane / LT;
     const int64_t DN = (int64_t)f.D * f.N;
     const int tile = (w.c0 - w.g * f.Dg) / CB;
 
     if (!w.any) {   // a number that stands for no piece: nothing in the sums
-        for (int i = tid; i < w.nch * f.N; i += kThreads) p.pA[w.number * DN + (int64_t)w.c0 * f.N + i] = 0.0f;
+        for (int i = tid; i < w.nch * f.N; i += NT) p.pA[w.number * DN + (int64_t)w.c0 * f.N + i] = 0.0f;
         if (tid < w.nch) p.pD[w.number * f.D + w.c0 + tid] = p.pb[w.number * f.D + w.c0 + tid] = 0.0f;
         return;
     }
@@ -181,24 +196,24 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
     const float* ckpt = f.ckpt + piece_base(f.seqs, w.s, KCK) * DN + (int64_t)w.c0 * f.N;
     auto copy_states = [&](int64_t t, int n0) {
         const int cnt = (int)min((int64_t)TT, len - t), nn = min(NC, f.N - n0);
-        stage<TT, NC>(m.b, B + t * f.B_st + n0, f.B_st, cnt, nn, f.B_cb);
-        stage<TT, NC>(m.c, C + t * f.C_st + n0, f.C_st, cnt, nn, f.C_cb);
+        stage<TT, NC, NT>(m.b, B + t * f.B_st + n0, f.B_st, cnt, nn, f.B_cb);
+        stage<TT, NC, NT>(m.c, C + t * f.C_st + n0, f.C_st, cnt, nn, f.C_cb);
     };
     auto copy = [&](int64_t t) {
         const int cnt = (int)min((int64_t)TT, len - t);
-        stage<TT, CB>(m.u, u + t * f.u_st, f.u_st, cnt, w.nch, f.u_cb);
-        stage<TT, CB>(m.d, delta + t * f.d_st, f.d_st, cnt, w.nch, f.d_cb);
-        stage<TT, CB>(m.o, dout + t * p.o_st, p.o_st, cnt, w.nch, p.o_cb);
-        if (z) stage<TT, CB>(m.z, z + t * f.z_st, f.z_st, cnt, w.nch, f.z_cb);
+        stage<TT, CB, NT>(m.u, u + t * f.u_st, f.u_st, cnt, w.nch, f.u_cb);
+        stage<TT, CB, NT>(m.d, delta + t * f.d_st, f.d_st, cnt, w.nch, f.d_cb);
+        stage<TT, CB, NT>(m.o, dout + t * p.o_st, p.o_st, cnt, w.nch, p.o_cb);
+        if (z) stage<TT, CB, NT>(m.z, z + t * f.z_st, f.z_st, cnt, w.nch, f.z_cb);
         copy_states(t, 0);
         const float* k = ckpt + t / KCK * DN;
-        for (int i = tid; i < w.nch * f.N; i += kThreads) cp_async<4>(sK + i, k + i, 4);
+        for (int i = tid; i < w.nch * f.N; i += NT) cp_async<4>(sK + i, k + i, 4);
     };
     const int64_t top = len > w.t0 ? (len - 1) / TT * TT : -1;
     if (top >= 0) copy(top);
     cp_commit();
     const float* from = p.gloc ? p.gloc + w.number * DN : p.dstate ? p.dstate + w.s * DN : nullptr;
-    for (int i = tid; i < CB * f.N; i += kThreads) {
+    for (int i = tid; i < CB * f.N; i += NT) {
         const int ci = i / f.N, n = i - ci * f.N;
         const int64_t k = (int64_t)(w.c0 + ci) * f.N + n;
         const bool in = ci < w.nch;
@@ -207,166 +222,135 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
         sD[n * CB + ci] = 0.0f;
         if (!in) sK[i] = 0.0f;
     }
-    float Dw[2], dD[2] = {0.0f, 0.0f}, db[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) Dw[e] = f.Dw && c + e < w.nch ? __ldg(f.Dw + w.c0 + c + e) : 0.0f;
-    // of the element-wise work: channels cp, cp + 1
-    const int cp = tid % (CB / 2) * 2;
+    const float Dw = f.Dw && c < w.nch ? __ldg(f.Dw + w.c0 + c) : 0.0f;
+    float dD = 0.0f, db[2] = {0.0f, 0.0f};
+    // of the element-wise work: channels cp, cp + 1 of four tokens t4 (a thread's only item)
+    const int cp = tid % (CB / 2) * 2, t4 = tid / (CB / 2) * 4;
+    static_assert(TT / 4 * (CB / 2) == NT, "one item a thread");
     float bias[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) bias[e] = f.bias && cp + e < w.nch ? __ldg(f.bias + w.c0 + cp + e) : 0.0f;
     float* dtr = m.dt + c * RS + tl * SEG;
     float* xr = m.x + c * RS + tl * SEG;
     float* dyr = m.dy + c * RS + tl * SEG;
+    using T2 = Vec<T, 2>;
+    auto raw = [&](const T* a, int k) { return *reinterpret_cast<const T2*>(a + (t4 + k) * CB + cp); };
 
     for (int64_t t = top; t >= w.t0; t -= TT) {
         const int cnt = (int)min((int64_t)TT, len - t);
-        Pairs dt[2], x[2], dy[2], y[2], q[2], r[2];
+        Pairs dt, x, dy, y, q, r;
         for (int n0 = 0; n0 < f.N; n0 += NC) {
             const int nn = min(NC, f.N - n0);
             cp_wait();
             __syncthreads();
             if (n0 == 0) {
                 // dt, u and dy = dout silu(z), transposed; zero past the last token and channel
-#pragma unroll 2
-                for (int i = tid; i < TT / 4 * (CB / 2); i += kThreads) {
-                    const int t4 = i / (CB / 2) * 4;
+                float fd[2][4], fu[2][4], fy[2][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const T2 vd = raw(m.d, k), vu = raw(m.u, k), vo = raw(m.o, k);
+                    T2 vz = vo;
+                    if (z) vz = raw(m.z, k);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float fd[4], fu[4], fy[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int at = (t4 + k) * CB + cp + e;
-                            const bool ok = cp + e < w.nch && t4 + k < cnt;
-                            float v = to_float(m.d[at]) + bias[e];
-                            if (f.softplus) v = softplusf(v);
-                            fd[k] = ok ? v : 0.0f;
-                            fu[k] = ok ? to_float(m.u[at]) : 0.0f;
-                            v = to_float(m.o[at]);
-                            if (z) {
-                                const float zv = to_float(m.z[at]);
-                                v *= zv * sigmoidf(zv);
-                            }
-                            fy[k] = ok ? v : 0.0f;
+                        const bool ok = cp + e < w.nch && t4 + k < cnt;
+                        float v = to_float(vd.v[e]) + bias[e];
+                        if (f.softplus) v = softplusf(v);
+                        fd[e][k] = ok ? v : 0.0f;
+                        fu[e][k] = ok ? to_float(vu.v[e]) : 0.0f;
+                        v = to_float(vo.v[e]);
+                        if (z) {
+                            const float zv = to_float(vz.v[e]);
+                            v *= zv * sigmoidf(zv);
                         }
-                        const int to = (cp + e) * RS + at_token(t4);
-                        *reinterpret_cast<float4*>(m.dt + to) = make_float4(fd[0], fd[1], fd[2], fd[3]);
-                        *reinterpret_cast<float4*>(m.x + to) = make_float4(fu[0], fu[1], fu[2], fu[3]);
-                        *reinterpret_cast<float4*>(m.dy + to) = make_float4(fy[0], fy[1], fy[2], fy[3]);
+                        fy[e][k] = ok ? v : 0.0f;
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int to = (cp + e) * RS + at_token(t4);
+                    *reinterpret_cast<float4*>(m.dt + to) = make_float4(fd[e][0], fd[e][1], fd[e][2], fd[e][3]);
+                    *reinterpret_cast<float4*>(m.x + to) = make_float4(fu[e][0], fu[e][1], fu[e][2], fu[e][3]);
+                    *reinterpret_cast<float4*>(m.dy + to) = make_float4(fy[e][0], fy[e][1], fy[e][2], fy[e][3]);
+                }
             }
-            widen_cols<LT, NC>(m.B, m.b, cnt, nn);
-            widen_cols<LT, NC>(m.C, m.c, cnt, nn);
+            widen_cols<LT, NC, NT>(m.B, m.b, cnt, nn);
+            widen_cols<LT, NC, NT>(m.C, m.c, cnt, nn);
             __syncthreads();
             if (n0 + NC < f.N) {
                 copy_states(t, n0 + NC);
                 cp_commit();
             }
             if (n0 == 0) {
+                dt = load_pairs(dtr);
+                x = load_pairs(xr);
+                dy = load_pairs(dyr);
+                f32x2 s = 0;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    dt[e] = load_pairs(dtr + e * RS);
-                    x[e] = load_pairs(xr + e * RS);
-                    dy[e] = load_pairs(dyr + e * RS);
-                    f32x2 s = 0;
-#pragma unroll
-                    for (int i = 0; i < K / 2; ++i) {
-                        s = fma2(x[e].p[i], dy[e].p[i], s);
-                        x[e].p[i] = mul2(dt[e].p[i], x[e].p[i]);
-                        y[e].p[i] = q[e].p[i] = r[e].p[i] = 0;
-                    }
-                    float lo, hi;
-                    unpack2(s, lo, hi);
-                    dD[e] += lo + hi;
+                for (int i = 0; i < K / 2; ++i) {
+                    s = fma2(x.p[i], dy.p[i], s);
+                    x.p[i] = mul2(dt.p[i], x.p[i]);
+                    y.p[i] = q.p[i] = r.p[i] = 0;
                 }
+                dD += halves(s);
             }
 #pragma unroll 1
             for (int n = 0; n < nn; ++n) {
                 const Pairs Bn = load_pairs(m.B + n * RS + tl * SEG), Cn = load_pairs(m.C + n * RS + tl * SEG);
                 const int at = (n0 + n) * CB + c;
-                const float2 A = *reinterpret_cast<const float2*>(sA + at);
-                f32x2* gp = reinterpret_cast<f32x2*>(sG + at);
-                const f32x2 g0 = *gp, h0 = pack2(sK[c * f.N + n0 + n], sK[(c + 1) * f.N + n0 + n]);
-                float a[2][K], b[2][K], v[2][K], P[2], H[2], G[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float Ae = e ? A.y : A.x;
-                    const f32x2 A2 = pack2(Ae, Ae);
+                const float g0 = sG[at], h0 = sK[c * f.N + n0 + n];
+                const f32x2 A2 = both(sA[at]);
+                float a[K], b[K], v[K], P;
+                {
                     Pairs ap, bp, vp;
 #pragma unroll
                     for (int i = 0; i < K / 2; ++i) {
-                        ap.p[i] = exp2_2(mul2(dt[e].p[i], A2));
-                        bp.p[i] = mul2(x[e].p[i], Bn.p[i]);
-                        vp.p[i] = mul2(dy[e].p[i], Cn.p[i]);
+                        ap.p[i] = exp2_2(mul2(dt.p[i], A2));
+                        bp.p[i] = mul2(x.p[i], Bn.p[i]);
+                        vp.p[i] = mul2(dy.p[i], Cn.p[i]);
                     }
-                    P[e] = product(ap);
-                    to_scalars(ap, a[e]);
-                    to_scalars(bp, b[e]);
-                    to_scalars(vp, v[e]);
-                    H[e] = b[e][0];
-                    G[e] = v[e][K - 1];
-#pragma unroll
-                    for (int k = 1; k < K; ++k) {
-                        H[e] = fmaf(a[e][k], H[e], b[e][k]);
-                        G[e] = fmaf(a[e][K - k], G[e], v[e][K - 1 - k]);
-                    }
-                    G[e] *= a[e][0];
+                    P = product(ap);
+                    to_scalars(ap, a);
+                    to_scalars(bp, b);
+                    to_scalars(vp, v);
                 }
-                f32x2 last;
-                const f32x2 P2 = pack2(P[0], P[1]);
-                const f32x2 before = scan_lanes_up<LT>(P2, pack2(H[0], H[1]), h0, tl, last);
-                const f32x2 after = scan_lanes_down<LT>(P2, pack2(G[0], G[1]), g0, tl, last);
-                if (tl == 0) *gp = last;   // the last lane read it before the shuffles
-                float hb[2], ga[2], da[2];
-                unpack2(before, hb[0], hb[1]);
-                unpack2(after, ga[0], ga[1]);
-                Pairs dB, dC;
+                float H = b[0], G = v[K - 1], last;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float Ae = e ? A.y : A.x;
-                    const f32x2 A2 = pack2(Ae, Ae);
-                    float h = hb[e], g = ga[e], s[K], gs[K], hs[K];   // s = a h'
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        s[k] = a[e][k] * h;
-                        h = hs[k] = s[k] + b[e][k];
-                    }
-#pragma unroll
-                    for (int k = K - 1; k >= 0; --k) {
-                        gs[k] = g + v[e][k];
-                        g = gs[k] * a[e][k];
-                    }
-                    f32x2 sum = 0;
-#pragma unroll
-                    for (int i = 0; i < K / 2; ++i) {
-                        const f32x2 g2 = pack2(gs[2 * i], gs[2 * i + 1]), h2 = pack2(hs[2 * i], hs[2 * i + 1]);
-                        y[e].p[i] = fma2(Cn.p[i], h2, y[e].p[i]);
-                        q[e].p[i] = fma2(Bn.p[i], g2, q[e].p[i]);
-                        const f32x2 e2 = mul2(g2, pack2(s[2 * i], s[2 * i + 1]));
-                        r[e].p[i] = fma2(e2, A2, r[e].p[i]);
-                        sum = fma2(e2, dt[e].p[i], sum);
-                        dB.p[i] = e ? fma2(g2, x[e].p[i], dB.p[i]) : mul2(g2, x[e].p[i]);
-                        dC.p[i] = e ? fma2(h2, dy[e].p[i], dC.p[i]) : mul2(h2, dy[e].p[i]);
-                    }
-                    float lo, hi;
-                    unpack2(sum, lo, hi);
-                    da[e] = lo + hi;
+                for (int k = 1; k < K; ++k) {
+                    H = fmaf(a[k], H, b[k]);
+                    G = fmaf(a[K - k], G, v[K - 1 - k]);
                 }
+                G *= a[0];
+                float h = scan_lanes_up<LT>(P, H, h0, tl);
+                float g = scan_lanes_down<LT>(P, G, g0, tl, last);
+                if (tl == 0) sG[at] = last;   // the last lane read it before the shuffles
+                float s[K], gs[K], hs[K];     // s = a h'
 #pragma unroll
-                for (int d = LT / 2; d >= 1; d /= 2) {
-                    da[0] += __shfl_xor_sync(0xffffffffu, da[0], d);
-                    da[1] += __shfl_xor_sync(0xffffffffu, da[1], d);
+                for (int k = 0; k < K; ++k) {
+                    s[k] = a[k] * h;
+                    gs[K - 1 - k] = g + v[K - 1 - k];
+                    h = hs[k] = s[k] + b[k];
+                    g = gs[K - 1 - k] * a[K - 1 - k];
                 }
-                if (tl == 0) {
-                    float2* o = reinterpret_cast<float2*>(sD + at);
-                    *o = make_float2(o->x + da[0], o->y + da[1]);
-                }
-                // over the warp's four channel pairs: lanes 16 .. 31 end with dC, odd pairs with
-                // the second half of the tokens
+                f32x2 sum = 0;
                 float vb[K], vc[K];
-                to_scalars(dB, vb);
-                to_scalars(dC, vc);
+#pragma unroll
+                for (int i = 0; i < K / 2; ++i) {
+                    const f32x2 g2 = pack2(gs[2 * i], gs[2 * i + 1]), h2 = pack2(hs[2 * i], hs[2 * i + 1]);
+                    y.p[i] = fma2(Cn.p[i], h2, y.p[i]);
+                    q.p[i] = fma2(Bn.p[i], g2, q.p[i]);
+                    const f32x2 e2 = mul2(g2, pack2(s[2 * i], s[2 * i + 1]));
+                    r.p[i] = fma2(e2, A2, r.p[i]);
+                    sum = fma2(e2, dt.p[i], sum);
+                    unpack2(mul2(g2, x.p[i]), vb[2 * i], vb[2 * i + 1]);
+                    unpack2(mul2(h2, dy.p[i]), vc[2 * i], vc[2 * i + 1]);
+                }
+                float da = halves(sum);
+#pragma unroll
+                for (int d = LT / 2; d >= 1; d /= 2) da += __shfl_xor_sync(0xffffffffu, da, d);
+                if (tl == 0) sD[at] += da;
+                // over the warp's four channels: lanes 16 .. 31 end with dC, the odd channels with
+                // the second half of the tokens
                 const bool hi = lane & 16, odd = lane & 8;
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
@@ -382,34 +366,31 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
                     make_float4(vb[0], vb[1], vb[2], vb[3]);
             }
             __syncthreads();
-            for (int i = tid; i < nn * 2 * TT; i += kThreads) {
+            for (int i = tid; i < nn * 2 * TT; i += NT) {
                 const int k = i % TT, which = i / TT % 2, n = i / (2 * TT);
                 if (k >= cnt) continue;
                 float s = 0.0f;
 #pragma unroll
-                for (int v = 0; v < kWarps; ++v) s += m.red[v][n][which][k];
+                for (int v = 0; v < kGradWarps; ++v) s += m.red[v][n][which][k];
                 p.pBC[((((int64_t)which * f.ntile + tile) * f.G + w.g) * f.N + n0 + n) * rows + row0 + t + k] = s;
             }
         }
         // a lane's own parts of the rows take what the element-wise work needs
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const Pairs uv = load_pairs(xr + e * RS);
-            const f32x2 D2 = pack2(Dw[e], Dw[e]), ln2 = pack2(kLn2, kLn2);
+        {
+            const Pairs uv = load_pairs(xr);
+            const f32x2 D2 = both(Dw), ln2 = both(kLn2);
 #pragma unroll
             for (int i = 0; i < K / 2; ++i) {
-                dt[e].p[i] = fma2(q[e].p[i], dt[e].p[i], mul2(D2, dy[e].p[i]));
-                r[e].p[i] = fma2(q[e].p[i], uv.p[i], mul2(ln2, r[e].p[i]));
-                y[e].p[i] = fma2(D2, uv.p[i], y[e].p[i]);
+                dt.p[i] = fma2(q.p[i], dt.p[i], mul2(D2, dy.p[i]));
+                r.p[i] = fma2(q.p[i], uv.p[i], mul2(ln2, r.p[i]));
+                y.p[i] = fma2(D2, uv.p[i], y.p[i]);
             }
-            store_pairs(dtr + e * RS, dt[e]);
-            store_pairs(xr + e * RS, r[e]);
-            store_pairs(dyr + e * RS, y[e]);
+            store_pairs(dtr, dt);
+            store_pairs(xr, r);
+            store_pairs(dyr, y);
         }
         __syncthreads();
-#pragma unroll 2
-        for (int i = tid; i < TT / 4 * (CB / 2); i += kThreads) {
-            const int t4 = i / (CB / 2) * 4;
+        {
             float du[2][4], dd[2][4], yv[2][4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -421,28 +402,30 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
                 dd[e][0] = v1.x, dd[e][1] = v1.y, dd[e][2] = v1.z, dd[e][3] = v1.w;
                 yv[e][0] = v2.x, yv[e][1] = v2.y, yv[e][2] = v2.z, yv[e][3] = v2.w;
             }
+            int64_t o = (row0 + t + t4) * f.D + w.c0 + cp;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 4; ++k, o += f.D) {
                 if (t4 + k >= cnt || cp >= w.nch) break;
-                Vec<T, 2> vu, vd, vz;
+                T2 vu, vd, vz;
+                const T2 rd = raw(m.d, k), ro = raw(m.o, k);
+                T2 rz = ro;
+                if (p.dz) rz = raw(m.z, k);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int at = (t4 + k) * CB + cp + e;
                     float g = dd[e][k];
-                    if (f.softplus) g *= sigmoidf(to_float(m.d[at]) + bias[e]);
+                    if (f.softplus) g *= sigmoidf(to_float(rd.v[e]) + bias[e]);
                     if (cp + e < w.nch) db[e] += g;
                     vu.v[e] = from_float<T>(du[e][k]);
                     vd.v[e] = from_float<T>(g);
                     if (p.dz) {
-                        const float zv = to_float(m.z[at]);
-                        vz.v[e] = from_float<T>(to_float(m.o[at]) * silu_slope(zv, sigmoidf(zv)) * yv[e][k]);
+                        const float zv = to_float(rz.v[e]);
+                        vz.v[e] = from_float<T>(to_float(ro.v[e]) * silu_slope(zv, sigmoidf(zv)) * yv[e][k]);
                     }
                 }
-                const int64_t o = (row0 + t + t4 + k) * f.D + w.c0 + cp;
                 if (f.pairs) {
-                    *reinterpret_cast<Vec<T, 2>*>(p.du + o) = vu;
-                    *reinterpret_cast<Vec<T, 2>*>(p.ddelta + o) = vd;
-                    if (p.dz) *reinterpret_cast<Vec<T, 2>*>(p.dz + o) = vz;
+                    *reinterpret_cast<T2*>(p.du + o) = vu;
+                    *reinterpret_cast<T2*>(p.ddelta + o) = vd;
+                    if (p.dz) *reinterpret_cast<T2*>(p.dz + o) = vz;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
@@ -461,23 +444,21 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
         }
     }
     __syncthreads();
-    for (int i = tid; i < w.nch * f.N; i += kThreads) {
+    for (int i = tid; i < w.nch * f.N; i += NT) {
         const int ci = i / f.N, n = i - ci * f.N;
         const int64_t k = (int64_t)(w.c0 + ci) * f.N + n;
         p.pA[w.number * DN + k] = sD[n * CB + ci];
         if (p.dh0 && w.j == 0) p.dh0[w.s * DN + k] = sG[n * CB + ci];
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int d = LT / 2; d >= 1; d /= 2) dD += __shfl_xor_sync(0xffffffffu, dD, d);
+    if (tl == 0 && c < w.nch) p.pD[w.number * f.D + w.c0 + c] = dD;
 #pragma unroll
-        for (int d = LT / 2; d >= 1; d /= 2) dD[e] += __shfl_xor_sync(0xffffffffu, dD[e], d);
-        if (tl == 0 && c + e < w.nch) p.pD[w.number * f.D + w.c0 + c + e] = dD[e];
-        m.dt[e * kThreads + tid] = db[e];
-    }
+    for (int e = 0; e < 2; ++e) m.dt[e * NT + tid] = db[e];
     __syncthreads();
     if (tid < w.nch) {
         float s = 0.0f;
-        for (int k = tid / 2; k < kThreads; k += CB / 2) s += m.dt[tid % 2 * kThreads + k];
+        for (int k = tid / 2; k < NT; k += CB / 2) s += m.dt[tid % 2 * NT + k];
         p.pb[w.number * f.D + w.c0 + tid] = s;
     }
 }
@@ -487,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd(const __grid_constant__ 
 // nothing but g's recurrence.
 template <typename T>
 struct AdjSmem {
-    static constexpr int NC = GradSmem<T>::NC;
+    static constexpr int NC = 16;
     alignas(16) T d[TT * CB];
     T z[TT * CB], o[TT * CB], c[TT * NC];
     alignas(16) float dt[CB * RS];
@@ -570,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_adjoint(const __grid_constan
                     }
                 }
             }
-            widen_cols<LT, NC>(m.C, m.c, cnt, nn);
+            widen_cols<LT, NC, kThreads>(m.C, m.c, cnt, nn);
             __syncthreads();
             if (n0 + NC < f.N) {
                 copy_states(t, n0 + NC);
@@ -755,7 +736,7 @@ int grad_type(const pe_scan_grad_args* a, cudaStream_t s) {
         if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
     }
     if (grid)
-        if (int rc = launch(scan_bwd<T>, p, grid, sizeof(GradSmem<T>) + 4 * p.f.N * CB * 4, s)) return rc;
+        if (int rc = launch(scan_bwd<T>, p, grid, sizeof(GradSmem<T>) + 4 * p.f.N * CB * 4, s, kGradThreads)) return rc;
     const int64_t rows = f->tokens * (f->cu ? 1 : f->nseq), cols = f->groups * f->states;
     if (rows) {
         if (ceil_div(rows, 32) > 0x7fffffffll || ceil_div(cols, 32) > 65535) return PE_ERR_UNSUPPORTED;
