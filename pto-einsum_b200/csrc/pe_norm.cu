@@ -7,7 +7,8 @@
 //
 // Bound by memory. A group of up to 1024 loads (512 backward; 16 bytes each where
 // the layout allows) stays in the registers of the lanes that share it: one read of x, two-pass
-// statistics. A larger one stays in the shared memory of a cluster of up to eight blocks.
+// statistics. A larger one of a single place is a block's, in L1; of several places it stays
+// in the shared memory of a cluster of up to eight blocks.
 // What that does not hold goes over the tensor twice: per-channel sums of row chunks,
 // their combination, then the result; the second read comes from L2 while the tensor
 // fits there. Variances are never formed as a difference of large squares: two passes
@@ -323,6 +324,134 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
             pb[(int64_t)r * p.C + it.c[k] + v] = c[v % 2];
         }
     }
+}
+
+// ---- one place a row, too many channels for registers ------------------------------------
+// A block takes a group of one row; the passes after the first find it in L1.
+template <typename T, int V>
+__global__ void __launch_bounds__(kBlock) norm_wide(const __grid_constant__ NormP<T> p) {
+    constexpr int Q = kPairs<V>;
+    __shared__ float red[8];
+    const int64_t n = blockIdx.x / (unsigned)p.G;
+    const int g = blockIdx.x % (unsigned)p.G, c0 = g * p.cg;
+    const T* x = p.x + n * p.x_sb + c0;
+    const float inv = 1.0f / (float)p.cg;
+    f32x2 s = 0;
+    float sum[1];
+#pragma unroll 4
+    for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
+        f32x2 f[Q];
+        widen<T, V>(load_vec<T, V>(x + c), f);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) s = add2(s, f[q]);
+    }
+    sum[0] = halves(s);
+    group_sum(sum, kBlock, red);
+    const float mean = sum[0] * inv;
+    const f32x2 minus = each<V>(-mean);
+    s = 0;
+#pragma unroll 4
+    for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
+        f32x2 f[Q];
+        widen<T, V>(load_vec<T, V>(x + c), f);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            f[q] = add2(f[q], minus);
+            s = fma2(f[q], f[q], s);
+        }
+    }
+    sum[0] = halves(s);
+    group_sum(sum, kBlock, red);
+    const float rstd = rsqrtf(sum[0] * inv + p.eps);
+    if (threadIdx.x == 0 && p.mean) {
+        p.mean[blockIdx.x] = mean;
+        p.rstd[blockIdx.x] = rstd;
+    }
+    const f32x2 scale = both(rstd);
+#pragma unroll 2
+    for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
+        f32x2 f[Q], w[Q], b[Q], ga[Q];
+        widen<T, V>(load_vec<T, V>(x + c), f);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) w[q] = both(1.0f), b[q] = 0;
+        if (p.w) widen<T, V>(load_vec<T, V>(p.w + c0 + c), w);
+        if (p.b) widen<T, V>(load_vec<T, V>(p.b + c0 + c), b);
+        if (p.mode == kGate) widen<T, V>(load_vec<T, V>(p.gate + n * p.g_sb + c0 + c), ga);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            f[q] = fma2(mul2(add2(f[q], minus), scale), w[q], b[q]);
+            if (p.mode == kSilu) f[q] = mul2(f[q], sigmoid2(f[q]));
+            if (p.mode == kGate) f[q] = mul2(f[q], mul2(ga[q], sigmoid2(ga[q])));
+        }
+        store_vec(p.out + n * p.C + c0 + c, narrow<T, V>(f));
+    }
+}
+
+// Backward: rows r, r + R, ... of one group a block, the sums of g xn and g of its
+// channels in shared memory, each with the thread that has the channel.
+template <typename T, int V>
+__global__ void __launch_bounds__(kBlock) norm_wide_bwd(const __grid_constant__ NormP<T> p, int R, float* pw, float* pb) {
+    constexpr int Q = kPairs<V>;
+    extern __shared__ __align__(16) f32x2 acc[];   // [cg / V][2][Q], g xn and g
+    __shared__ float red[16];
+    const int r = blockIdx.x / (unsigned)p.G, g = blockIdx.x % (unsigned)p.G, c0 = g * p.cg;
+    const float inv = 1.0f / (float)p.cg;
+    for (int c = threadIdx.x; c < p.cg / V; c += kBlock)
+#pragma unroll
+        for (int q = 0; q < 2 * Q; ++q) acc[c * 2 * Q + q] = 0;
+    for (int64_t n = r; n < p.N; n += R) {
+        const f32x2 minus = each<V>(-__ldg(p.mean + n * p.G + g)), scale = both(__ldg(p.rstd + n * p.G + g));
+        auto load = [&](int c, f32x2 (&xn)[Q], f32x2 (&go)[Q], f32x2 (&ga)[Q], f32x2 (&w)[Q]) {
+            f32x2 b[Q];
+            widen<T, V>(load_vec<T, V>(p.x + n * p.x_sb + c0 + c), xn);
+            widen<T, V>(load_vec<T, V>(p.dout + n * p.o_sb + c0 + c), go);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) w[q] = each<V>(1.0f), b[q] = 0;
+            if (p.w) widen<T, V>(load_vec<T, V>(p.w + c0 + c), w);
+            if (p.b) widen<T, V>(load_vec<T, V>(p.b + c0 + c), b);
+            if (p.mode == kGate) widen<T, V>(load_vec<T, V>(p.gate + n * p.g_sb + c0 + c), ga);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) xn[q] = mul2(add2(xn[q], minus), scale);
+            through_act2<Q>(p.mode, xn, w, b, go, ga);
+        };
+        f32x2 s0 = 0, s1 = 0;
+#pragma unroll 2
+        for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
+            f32x2 xn[Q], go[Q], ga[Q], w[Q];
+            load(c, xn, go, ga, w);
+            f32x2* a = acc + c / V * 2 * Q;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                a[q] = fma2(go[q], xn[q], a[q]);
+                a[Q + q] = add2(a[Q + q], go[q]);
+                go[q] = mul2(go[q], w[q]);
+                s0 = add2(s0, go[q]);
+                s1 = fma2(go[q], xn[q], s1);
+            }
+        }
+        float sum[2] = {halves(s0), halves(s1)};
+        group_sum(sum, kBlock, red);
+        const f32x2 m0 = both(-sum[0] * inv), m1 = both(-sum[1] * inv);
+#pragma unroll 2
+        for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
+            f32x2 xn[Q], go[Q], ga[Q], w[Q];
+            load(c, xn, go, ga, w);
+            if (p.mode == kGate) store_vec(p.dgate + n * p.C + c0 + c, narrow<T, V>(ga));
+#pragma unroll
+            for (int q = 0; q < Q; ++q) go[q] = mul2(scale, fma2(xn[q], m1, fma2(go[q], w[q], m0)));
+            store_vec(p.dx + n * p.C + c0 + c, narrow<T, V>(go));
+        }
+    }
+    if (!pw) return;
+    for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float a[2], b[2];
+            unpack2(acc[c / V * 2 * Q + v / 2], a[0], a[1]);
+            unpack2(acc[c / V * 2 * Q + Q + v / 2], b[0], b[1]);
+            pw[(int64_t)r * p.C + c0 + c + v] = a[v % 2];
+            pb[(int64_t)r * p.C + c0 + c + v] = b[v % 2];
+        }
 }
 
 // ---- groups in a cluster's shared memory ------------------------------------------------
@@ -900,6 +1029,7 @@ struct Plan {
     int v;            // elements a load
     int lanes, k;     // groups in registers: lanes a group, loads a lane; lanes 0: too large for that
     int64_t R;        // in registers: rows at work, a lane takes every R-th
+    bool wide;        // a block a group of one place
     Slab slab;        // in a cluster's shared memory: R > 0
     Chunks q;
 };
@@ -955,6 +1085,16 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
         p.R = a->batch < want ? a->batch : want < 1 ? 1 : want;
         return p;
     }
+    // one place a row: a block a group while its sums fit shared memory
+    const int64_t smem = cg / vr * 2 * ((vr + 1) / 2) * 8;
+    if (a->places == 1 && smem <= 200 * 1024) {
+        p.v = vr;
+        p.wide = true;
+        const int64_t resident = smem > 100 * 1024 ? 1 : smem > 50 * 1024 ? 2 : 4;
+        const int64_t want = ceil_div((int64_t)num_sms() * resident, a->groups);
+        p.R = a->batch < want ? a->batch : want;
+        return p;
+    }
     p.v = vec;
     p.slab = slab_of(a, vec, grad);
     if (p.slab.R) return p;
@@ -988,7 +1128,7 @@ int launched() {
 }
 
 int64_t stats_floats(const pe_norm_args* a, const Plan& pl) {
-    return pl.lanes || pl.slab.R ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->groups);
+    return pl.lanes || pl.wide || pl.slab.R ? 0 : a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->groups);
 }
 
 // Shared memory of the register kernels' queues: four rows of k loads a lane and stream.
@@ -1040,6 +1180,11 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
         if (pl.k == 2) return launch_reg(norm_reg<T, V, 2>, blocks, queue_bytes<T, V>(2, streams), s, p, pl.lanes, (int)pl.R);
         return launch_reg(norm_reg<T, V, 4>, blocks, queue_bytes<T, V>(4, streams), s, p, pl.lanes, (int)pl.R);
     }
+    if (pl.wide) {
+        if (units > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+        norm_wide<T, V><<<(unsigned)units, kBlock, 0, s>>>(p);
+        return launched();
+    }
     if (pl.slab.R)
         return launch_slab(norm_slab<T, V>, p.N, pl.slab, slab_smem(pl.slab.CS, pl.slab.P, V, sizeof(T), false), s, p,
                            pl.slab);
@@ -1060,7 +1205,7 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
 }
 
 int64_t grad_floats(const pe_norm_args* a, const Plan& pl) {
-    if (pl.lanes) return 2 * pl.R * a->channels;
+    if (pl.lanes || pl.wide) return 2 * pl.R * a->channels;
     if (pl.slab.R) return 2 * a->batch * pl.slab.R * a->channels;
     return a->batch * (pl.q.chunks * 2 * a->channels + 2 * a->channels + 2 * a->groups);
 }
@@ -1088,6 +1233,15 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
                                  : launch_reg(norm_reg_bwd<T, V, 2>, blocks, queue_bytes<T, V>(2, streams), s, p, pl.lanes,
                                               (int)pl.R, pw, sb);
         if (rc) return rc;
+    } else if (pl.wide) {
+        rows = pl.R;
+        sw = ws;
+        sb = ws + rows * p.C;
+        const int smem = p.cg / V * 2 * kPairs<V> * 8;
+        if (pl.R * p.G > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+        if (int rc = launch_reg(norm_wide_bwd<T, V>, pl.R * p.G, smem, s, p, (int)pl.R,
+                                ga->dweight || ga->dbias ? sw : nullptr, sb))
+            return rc;
     } else if (pl.slab.R) {
         rows = p.N * pl.slab.R;
         sw = ws;

@@ -34,7 +34,8 @@ def rand(*shape, seed, dtype=F32, device="cuda"):
 CASES = [  # shape, groups
     ((1, 8), 1), ((5, 64), 4), ((300, 256), 8), ((7, 33), 3), ((64, 4096), 32), ((3, 8192), 1), ((2, 20000), 2),
     ((9, 16, 32), 4), ((2, 5, 7, 24), 3), ((2, 1024, 320), 32), ((1, 33, 31, 96), 1), ((3, 700, 50), 5),
-    ((2, 9000, 8), 8), ((1, 5000, 7), 7), ((0, 16), 4), ((2, 0, 16), 4), ((1, 3, 260, 128), 2), ((4, 130), 130)]
+    ((2, 9000, 8), 8), ((1, 5000, 7), 7), ((0, 16), 4), ((2, 0, 16), 4), ((1, 3, 260, 128), 2), ((4, 130), 130),
+    ((70, 2722), 2), ((5, 24000), 2), ((3, 70000), 1), ((3, 40, 2600), 2), ((2, 31, 5000), 1)]
 
 
 def inputs(shape, dt, seed=0):
