@@ -88,7 +88,7 @@ __device__ __forceinline__ void load_before(const ConvP<T>& p, const T* xs, int6
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kBlock, 2) conv_fwd(const __grid_constant__ ConvP<T> p) {
     constexpr int Q = kPairs<V>;
-    __shared__ __align__(16) Vec<T, V> queue[DEPTH * kBlock];
+    __shared__ __align__(16) unsigned char queue[DEPTH * kBlock * kSlotBytes<T, V>];
     if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.seqs, threadIdx.x, kSiteOffsets);
     int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
     const int64_t tile = id / p.CV, c = (id - tile * p.CV) * V;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kBlock, 2) conv_fwd(const __grid_constant__ Co
 #pragma unroll 4
         for (; t < stop; ++t, ++slot, o += p.C) {
             cp_wait_but<DEPTH - 2>();
-            widen<T, V>(ring.get(slot), win[W - 1]);
+            widen<T, V>(ring.get(slot, xr + t * p.x_st), win[W - 1]);
             ring.fetch(slot + DEPTH - 1, ahead, left > 0);
             cp_commit();
             ahead += p.x_st;
@@ -160,8 +160,11 @@ struct ConvGradP {
     int bx;             // channel vectors a block (power of two <= 32)
 };
 
+// Blocks an SM holds: by the registers of V channels' taps, sums and windows.
+__host__ __device__ constexpr int bwd_blocks(int v) { return v <= 4 ? 2 : 1; }
+
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(kBlock, 1) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
+__global__ void __launch_bounds__(kBlock, bwd_blocks(V)) conv_bwd(const __grid_constant__ ConvGradP<T> p) {
     constexpr int Q = kPairs<V>;
     // the queues, and once they are empty the block's sums
     extern __shared__ __align__(16) unsigned char shared[];
@@ -183,8 +186,7 @@ __global__ void __launch_bounds__(kBlock, 1) conv_bwd(const __grid_constant__ Co
         const int64_t end = min(f.seqs.tokens, t + f.tile), row = f.seqs.cu ? 0 : tile / per;
         const T* xr = f.x + row * f.x_sb + c;
         const T* dor = p.dout + row * p.o_sb + c;
-        Vec<T, V>* queues = reinterpret_cast<Vec<T, V>*>(shared);
-        Ring<T, V, DEPTH> rx(queues, kBlock), ro(queues + DEPTH * kBlock, kBlock);
+        Ring<T, V, DEPTH> rx(shared, kBlock), ro(shared + DEPTH * kBlock * kSlotBytes<T, V>, kBlock);
         Filter<T, W, V> flt;
         flt.load(f.w, f.bias, c);
         int s = f.seqs.cu ? seq_of_token(f.seqs, t) : (int)row;
@@ -213,8 +215,8 @@ __global__ void __launch_bounds__(kBlock, 1) conv_bwd(const __grid_constant__ Co
 #pragma unroll 4
             for (int64_t k = t; k < last; ++k, ++slot, ++ahead) {
                 cp_wait_but<DEPTH - 2>();
-                widen<T, V>(rx.get(slot), win[W - 1]);
-                widen<T, V>(ro.get(slot), g[W - 1]);
+                widen<T, V>(rx.get(slot, xr + k * f.x_st), win[W - 1]);
+                widen<T, V>(ro.get(slot, dor + k * p.o_st), g[W - 1]);
                 rx.fetch(slot + DEPTH - 1, xr + ahead * f.x_st, ahead < have);
                 ro.fetch(slot + DEPTH - 1, dor + ahead * p.o_st, ahead < have);
                 cp_commit();
@@ -386,8 +388,7 @@ ConvP<T> conv_params(const pe_conv_args* a, int v, int64_t tile) {
     return p;
 }
 
-// Tokens a thread walks: whole waves of the blocks an SM holds (two forward, one
-// backward), at most 64 tokens each (the W - 1 tokens read again, the filter and the
+// Tokens a thread walks: whole waves of the blocks an SM holds, at most 64 tokens each (the W - 1 tokens read again, the filter and the
 // filling of the queue weigh less on a longer walk; a last wave that is not full costs as
 // much as one that is), at least 4. by: a block's threads along the tokens, where the
 // block is laid out by channels.
@@ -422,7 +423,7 @@ ConvGradShape grad_shape(const pe_conv_args* a, int v) {
     const int64_t cv = a->channels / v;
     ConvGradShape g{1, 4, 0};
     while (g.bx < 32 && g.bx < cv) g.bx *= 2;
-    g.tile = tile_of(a, cv, 1, kBlock / g.bx);
+    g.tile = tile_of(a, cv, bwd_blocks(v), kBlock / g.bx);
     g.rows = ceil_div(ceil_div(a->tokens, g.tile) * a->batch, kBlock / g.bx);
     return g;
 }
@@ -442,7 +443,7 @@ int conv_grad_run(const pe_conv_grad_args* g, cudaStream_t s) {
     const int64_t cblocks = ceil_div(p.f.CV, sh.bx);
     if (sh.rows > 0x7fffffffll || cblocks > 65535) return PE_ERR_UNSUPPORTED;
     if (sh.rows) {
-        const int queues = 2 * DEPTH * kBlock * V * (int)sizeof(T), sums = (W + 1) * V * kBlock * 4;
+        const int queues = 2 * DEPTH * kBlock * kSlotBytes<T, V>, sums = (W + 1) * V * kBlock * 4;
         const int smem = queues > sums ? queues : sums;
         if (smem > 48 * 1024 && cudaFuncSetAttribute(conv_bwd<T, W, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                      smem) != cudaSuccess)

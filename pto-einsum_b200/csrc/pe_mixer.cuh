@@ -23,6 +23,17 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// One element. Not __ldg of the 16-bit types: CUDA's headers write that as assembly
+// without "volatile", which the compiler may move out of the condition that guards it,
+// to addresses that are not there.
+__device__ __forceinline__ float load_one(const float* p) { return __ldg(p); }
+__device__ __forceinline__ __half load_one(const __half* p) {
+    return __ushort_as_half(__ldg(reinterpret_cast<const unsigned short*>(p)));
+}
+__device__ __forceinline__ __nv_bfloat16 load_one(const __nv_bfloat16* p) {
+    return __ushort_as_bfloat16(__ldg(reinterpret_cast<const unsigned short*>(p)));
+}
+
 // V elements that one load moves (V * sizeof(T) is 16 or 8 bytes, or V is 1).
 template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {
@@ -39,7 +50,7 @@ __device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
     } else {
         static_assert(V == 1, "16 or 8 bytes, or one element");
         Vec<T, V> r;
-        r.v[0] = __ldg(p);
+        r.v[0] = load_one(p);
         return r;
     }
 }
@@ -213,24 +224,40 @@ __device__ __forceinline__ void cp_wait() { cp_wait_but<0>(); }
 
 // A thread's own queue of vectors in shared memory: what it copies only it reads, so the
 // copies need no barrier, and DEPTH of them are under way without holding registers.
-// Slots of a block's threads lie side by side.
+// Slots of a block's threads lie side by side. A 2-byte element comes as the aligned
+// 4-byte word that holds it (its own half alone where that is the first).
 template <typename T, int V, int DEPTH>
 struct Ring {
     static_assert((DEPTH & (DEPTH - 1)) == 0, "a power of two");
     using Elem = Vec<T, V>;
-    Elem* at;
+    static constexpr bool kHalf = sizeof(Elem) == 2;
+    using Slot = typename std::conditional<kHalf, uint32_t, Elem>::type;
+    Slot* at;
     int stride;
-    __device__ __forceinline__ Ring(Elem* block, int threads) : at(block + threadIdx.x), stride(threads) {}
+    __device__ __forceinline__ Ring(void* block, int threads)
+        : at(reinterpret_cast<Slot*>(block) + threadIdx.x), stride(threads) {}
     __device__ __forceinline__ void fetch(int slot, const T* src, bool on) {
-        Elem* dst = at + (slot & (DEPTH - 1)) * stride;
-        if constexpr (sizeof(Elem) >= 4) {
-            if (on) cp_async<sizeof(Elem)>(dst, src, sizeof(Elem));
+        Slot* dst = at + (slot & (DEPTH - 1)) * stride;
+        if constexpr (kHalf) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(src);
+            if (on) cp_async<4>(dst, reinterpret_cast<const void*>(a & ~(uintptr_t)3), a & 2 ? 4 : 2);
         } else {
-            if (on) *dst = load_vec<T, V>(src);
+            if (on) cp_async<sizeof(Elem)>(dst, src, sizeof(Elem));
         }
     }
-    __device__ __forceinline__ Elem get(int slot) const { return at[(slot & (DEPTH - 1)) * stride]; }
+    // src: the address that the slot was filled from
+    __device__ __forceinline__ Elem get(int slot, const T* src) const {
+        const Slot s = at[(slot & (DEPTH - 1)) * stride];
+        if constexpr (kHalf) {
+            const unsigned short h = (unsigned short)(reinterpret_cast<uintptr_t>(src) & 2 ? s >> 16 : s);
+            return *reinterpret_cast<const Elem*>(&h);
+        } else {
+            return s;
+        }
+    }
 };
+template <typename T, int V>
+constexpr int kSlotBytes = V * sizeof(T) < 4 ? 4 : V * (int)sizeof(T);
 
 // ---- sequences ----------------------------------------------------------------
 // Uniform batches (cu == nullptr): nseq rows of `tokens` tokens. Packed: one row of

@@ -6,7 +6,7 @@
 //   dx = rstd (g w - mean(g w) - xn mean(g w xn))          (means over the group)
 //
 // Bound by memory. A group of up to 1024 loads (512 backward; 16 bytes each where
-// the layout allows) stays in the registers of the lanes that share it: one read of x, two-pass
+// the layout allows, else 256 of an element) stays in the registers of the lanes that share it: one read of x, two-pass
 // statistics. A larger one of a single place is a block's, in L1; of several places it stays
 // in the shared memory of a cluster of up to eight blocks.
 // What that does not hold goes over the tensor twice: per-channel sums of row chunks,
@@ -68,8 +68,9 @@ __device__ __forceinline__ void group_sum(float (&v)[NV], int L, float* red) {
     }
 }
 
-// Blocks an SM holds of the kernels below, by loads a lane.
-__host__ __device__ constexpr int reg_blocks(int k, bool grad) {
+// Blocks an SM holds of the kernels below, by loads a lane and elements a load.
+__host__ __device__ constexpr int reg_blocks(int k, int v, bool grad) {
+    if (v == 1) return k <= 2 ? 4 : 2;
     return grad ? (k == 1 ? 2 : 1) : k == 1 ? 3 : k == 2 ? 2 : 1;
 }
 
@@ -93,7 +94,7 @@ struct Items {
 // way while the current one is reduced. All lanes make the same number of rounds, for
 // the shuffles take all of them.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const __grid_constant__ NormP<T> p, int L, int R) {
+__global__ void __launch_bounds__(kBlock, reg_blocks(K, V, false)) norm_reg(const __grid_constant__ NormP<T> p, int L, int R) {
     __shared__ float red[8];
     const int unit = (int)(((int64_t)blockIdx.x * kBlock + threadIdx.x) / L), l = threadIdx.x % L;
     const bool live = unit / p.G < R;
@@ -104,14 +105,13 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
     constexpr int Q = kPairs<V>;
     constexpr int DEPTH = 4;   // three rows on their way
     extern __shared__ __align__(16) unsigned char queues[];
-    Vec<T, V>* slots = reinterpret_cast<Vec<T, V>*>(queues);
-    Ring<T, V, DEPTH * K> rx(slots, kBlock), rz(slots + DEPTH * K * kBlock, kBlock);
-    int64_t xo[K], go[K];
+    constexpr int each_queue = DEPTH * K * kBlock * kSlotBytes<T, V>;
+    Ring<T, V, DEPTH * K> rx(queues, kBlock), rz(queues + each_queue, kBlock);
+    auto at_x = [&](int64_t n, int k) { return p.x + n * p.x_sb + it.place[k] * p.x_sp + it.c[k]; };
+    auto at_gate = [&](int64_t n, int k) { return p.gate + n * p.g_sb + it.place[k] * p.g_sp + it.c[k]; };
     f32x2 w[K][Q], b[K][Q];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        xo[k] = it.place[k] * p.x_sp + it.c[k];
-        go[k] = it.place[k] * p.g_sp + it.c[k];
 #pragma unroll
         for (int q = 0; q < Q; ++q) w[k][q] = both(1.0f), b[k][q] = 0;
         if (it.in[k] && p.w) widen<T, V>(load_vec<T, V>(p.w + it.c[k]), w[k]);
@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const bool on = it.in[k] && n < p.N;
-            rx.fetch(step * K + k, p.x + n * p.x_sb + xo[k], on);
-            if (p.mode == kGate) rz.fetch(step * K + k, p.gate + n * p.g_sb + go[k], on);
+            rx.fetch(step * K + k, at_x(n, k), on);
+            if (p.mode == kGate) rz.fetch(step * K + k, at_gate(n, k), on);
         }
         cp_commit();
     };
@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
         cp_wait_but<DEPTH - 2>();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            widen<T, V>(rx.get(step * K + k), f[k]);
-            if (p.mode == kGate) widen<T, V>(rz.get(step * K + k), ga[k]);
+            widen<T, V>(rx.get(step * K + k, at_x(n, k)), f[k]);
+            if (p.mode == kGate) widen<T, V>(rz.get(step * K + k, at_gate(n, k)), ga[k]);
             f32x2 s = f[k][0];
 #pragma unroll
             for (int q = 1; q < Q; ++q) s = add2(s, f[k][q]);
@@ -184,24 +184,6 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, false)) norm_reg(const _
 }
 
 // g = dL / dv, and the gate's gradient in place of `ga`.
-template <int V>
-__device__ __forceinline__ void through_act(int mode, const float (&xn)[V], const float (&w)[V], const float (&b)[V],
-                                            float (&go)[V], float (&ga)[V]) {
-    if (mode == kPlain) return;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const float val = fmaf(xn[v], w[v], b[v]);
-        if (mode == kSilu) {
-            go[v] *= silu_slope(val, sigmoidf(val));
-        } else {
-            const float s = sigmoidf(ga[v]), o = go[v];
-            go[v] = o * ga[v] * s;
-            ga[v] = o * val * silu_slope(ga[v], s);
-        }
-    }
-}
-
-// The same in pairs.
 template <int Q>
 __device__ __forceinline__ void through_act2(int mode, const f32x2 (&xn)[Q], const f32x2 (&w)[Q], const f32x2 (&b)[Q],
                                              f32x2 (&go)[Q], f32x2 (&ga)[Q]) {
@@ -222,7 +204,7 @@ __device__ __forceinline__ void through_act2(int mode, const f32x2 (&xn)[Q], con
 // L lanes take rows r, r + R, ... of one group of channels (one place a row) and keep the
 // sums of g xn and g of their own channels: pw, pb [R][C].
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(const __grid_constant__ NormP<T> p, int L,
+__global__ void __launch_bounds__(kBlock, reg_blocks(K, V, true)) norm_reg_bwd(const __grid_constant__ NormP<T> p, int L,
                                                                             int R, float* pw, float* pb) {
     constexpr int Q = kPairs<V>;
     __shared__ float red[16];
@@ -234,9 +216,8 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
     const float inv = 1.0f / (float)p.cg;
     constexpr int DEPTH = 4;
     extern __shared__ __align__(16) unsigned char queues[];
-    Vec<T, V>* slots = reinterpret_cast<Vec<T, V>*>(queues);
-    constexpr int each_queue = DEPTH * K * kBlock;
-    Ring<T, V, DEPTH * K> rx(slots, kBlock), ro(slots + each_queue, kBlock), rz(slots + 2 * each_queue, kBlock);
+    constexpr int each_queue = DEPTH * K * kBlock * kSlotBytes<T, V>;
+    Ring<T, V, DEPTH * K> rx(queues, kBlock), ro(queues + each_queue, kBlock), rz(queues + 2 * each_queue, kBlock);
     f32x2 aw[K][Q], ab[K][Q], w[K][Q], b[K][Q];
     float mean = 0.0f, rstd = 0.0f, mean2 = 0.0f, rstd2 = 0.0f;   // of this row and the next
 #pragma unroll
@@ -280,9 +261,9 @@ __global__ void __launch_bounds__(kBlock, reg_blocks(K, true)) norm_reg_bwd(cons
         for (int k = 0; k < K; ++k) {
             if (!it.in[k] || !on) continue;
             f32x2 ga[Q], s0 = 0, s1 = 0;
-            widen<T, V>(rx.get(step * K + k), xn[k]);
-            widen<T, V>(ro.get(step * K + k), go[k]);
-            if (p.mode == kGate) widen<T, V>(rz.get(step * K + k), ga);
+            widen<T, V>(rx.get(step * K + k, p.x + n * p.x_sb + it.c[k]), xn[k]);
+            widen<T, V>(ro.get(step * K + k, p.dout + n * p.o_sb + it.c[k]), go[k]);
+            if (p.mode == kGate) widen<T, V>(rz.get(step * K + k, p.gate + n * p.g_sb + it.c[k]), ga);
 #pragma unroll
             for (int q = 0; q < Q; ++q) xn[k][q] = mul2(add2(xn[k][q], minus), scale);
             through_act2<Q>(p.mode, xn[k], w[k], b[k], go[k], ga);
@@ -390,7 +371,7 @@ __global__ void __launch_bounds__(kBlock) norm_wide(const __grid_constant__ Norm
 // Backward: rows r, r + R, ... of one group a block, the sums of g xn and g of its
 // channels in shared memory, each with the thread that has the channel.
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock) norm_wide_bwd(const __grid_constant__ NormP<T> p, int R, float* pw, float* pb) {
+__global__ void __launch_bounds__(kBlock, 2) norm_wide_bwd(const __grid_constant__ NormP<T> p, int R, float* pw, float* pb) {
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) f32x2 acc[];   // [cg / V][2][Q], g xn and g
     __shared__ float red[16];
@@ -415,7 +396,7 @@ __global__ void __launch_bounds__(kBlock) norm_wide_bwd(const __grid_constant__ 
             through_act2<Q>(p.mode, xn, w, b, go, ga);
         };
         f32x2 s0 = 0, s1 = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
             f32x2 xn[Q], go[Q], ga[Q], w[Q];
             load(c, xn, go, ga, w);
@@ -459,12 +440,13 @@ __global__ void __launch_bounds__(kBlock) norm_wide_bwd(const __grid_constant__ 
 // its P places, which stay in shared memory: one read of the tensor and one launch. The
 // blocks exchange their sums of each group through distributed shared memory and add
 // them in rank order.
+constexpr int kSlab = 512;   // threads: one block an SM
 struct Slab {
     int CS, slabs, R, P;
 };
 __host__ __device__ __forceinline__ int slab_floats(int n) { return (n + 3) / 4 * 16; }   // their bytes, whole 16s
-// Floats of the segments' sums: at most kBlock segments, or one a channel.
-__host__ __device__ __forceinline__ int slab_sums(int cs) { return (cs > kBlock ? cs : kBlock) + 3 & ~3; }
+// Floats of the segments' sums: at most kSlab segments, or one a channel.
+__host__ __device__ __forceinline__ int slab_sums(int cs) { return (cs > kSlab ? cs : kSlab) + 3 & ~3; }
 
 __device__ __forceinline__ float remote(const float* own, int rank) {
     float v;
@@ -487,11 +469,11 @@ struct SlabPlace {
         s0 = (int64_t)rank * q.P;
         pc = (int)max((int64_t)0, min((int64_t)q.P, p.S - s0));
         cvn = cs / V;
-        by = kBlock / cvn;
+        by = kSlab / cvn;
         x = threadIdx.x % cvn;
         y = threadIdx.x / cvn;
         on = y < by;
-        segs = max(1, min(by, kBlock / cs));
+        segs = max(1, min(by, kSlab / cs));
     }
     // this block's places of a tensor into shared memory [P][cs]
     __device__ __forceinline__ void copy(T* dst, const T* src, int64_t sb, int64_t sp) const {
@@ -501,7 +483,7 @@ struct SlabPlace {
             if constexpr (V * sizeof(T) >= 8)
                 cp_async<V * sizeof(T)>(dst + i * cs + x * V, from + i * sp, V * sizeof(T));
             else
-                dst[i * cs + x * V] = __ldg(from + i * sp);
+                dst[i * cs + x * V] = load_one(from + i * sp);
         }
     }
     __device__ __forceinline__ void get(const T* tile, int i, f32x2 (&f)[kPairs<V>]) const {
@@ -520,7 +502,7 @@ struct SlabPlace {
             }
         __syncthreads();
         const int len = (by + segs - 1) / segs;
-        for (int i = threadIdx.x; i < cs * segs; i += kBlock) {
+        for (int i = threadIdx.x; i < cs * segs; i += kSlab) {
             const int c = i / segs, from = (i - c * segs) * len, to = min(by, from + len);
             float a = 0.0f;
             for (int k = from; k < to; ++k) a += red[c * by + k];
@@ -534,7 +516,7 @@ struct SlabPlace {
 template <typename F>
 __device__ __forceinline__ void slab_groups(int groups, int items, float* g, F a) {
     const int lane = threadIdx.x & 31;
-    for (int j = threadIdx.x / 32; j < groups; j += kBlock / 32) {
+    for (int j = threadIdx.x / 32; j < groups; j += kSlab / 32) {
         float s = 0.0f;
         for (int i = lane; i < items; i += 32) s += a(j * items + i);
 #pragma unroll
@@ -546,7 +528,7 @@ __device__ __forceinline__ void slab_groups(int groups, int items, float* g, F a
 // a warp reads block r's.
 __device__ __forceinline__ void cluster_groups(int groups, int R, const float* share, float* total, float scale) {
     const int lane = threadIdx.x & 31;
-    for (int j = threadIdx.x / 32; j < groups; j += kBlock / 32) {
+    for (int j = threadIdx.x / 32; j < groups; j += kSlab / 32) {
         float s = lane < R ? remote(share + j, lane) : 0.0f;
 #pragma unroll
         for (int m = 4; m >= 1; m /= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
@@ -555,12 +537,12 @@ __device__ __forceinline__ void cluster_groups(int groups, int R, const float* s
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock, 2) norm_slab(const __grid_constant__ NormP<T> p, const Slab q) {
+__global__ void __launch_bounds__(kSlab, 1) norm_slab(const __grid_constant__ NormP<T> p, const Slab q) {
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) unsigned char smem[];
-    float* red = reinterpret_cast<float*>(smem);        // [kBlock V]
-    float *sums = red + kBlock * V, *share = sums + slab_sums(q.CS), *own = share + 2 * q.CS;   // 2 a group; a group
-    T* tile = reinterpret_cast<T*>(smem + slab_floats(kBlock * V + slab_sums(q.CS) + 3 * q.CS));
+    float* red = reinterpret_cast<float*>(smem);        // [kSlab V]
+    float *sums = red + kSlab * V, *share = sums + slab_sums(q.CS), *own = share + 2 * q.CS;   // 2 a group; a group
+    T* tile = reinterpret_cast<T*>(smem + slab_floats(kSlab * V + slab_sums(q.CS) + 3 * q.CS));
     const SlabPlace<T, V> at(p, q);
     const int groups = at.cs / p.cg;
     at.copy(tile, p.x, p.x_sb, p.x_sp);
@@ -654,13 +636,13 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab(const __grid_constant__ N
 // Backward: x and dout stay in shared memory, the gate is read twice. pw, pb [N R][C]: a
 // block's share of the sums of g xn and g.
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock, 2) norm_slab_bwd(const __grid_constant__ NormP<T> p, const Slab q, float* pw,
+__global__ void __launch_bounds__(kSlab, 1) norm_slab_bwd(const __grid_constant__ NormP<T> p, const Slab q, float* pw,
                                                            float* pb) {
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) unsigned char smem[];
-    float* red = reinterpret_cast<float*>(smem);        // [kBlock V]
-    float *sw = red + kBlock * V, *sb = sw + slab_sums(q.CS), *share = sb + slab_sums(q.CS), *own = share + 2 * q.CS;
-    T* tx = reinterpret_cast<T*>(smem + slab_floats(kBlock * V + 2 * slab_sums(q.CS) + 4 * q.CS));
+    float* red = reinterpret_cast<float*>(smem);        // [kSlab V]
+    float *sw = red + kSlab * V, *sb = sw + slab_sums(q.CS), *share = sb + slab_sums(q.CS), *own = share + 2 * q.CS;
+    T* tx = reinterpret_cast<T*>(smem + slab_floats(kSlab * V + 2 * slab_sums(q.CS) + 4 * q.CS));
     T* to = tx + (int64_t)q.P * q.CS;
     const SlabPlace<T, V> at(p, q);
     const int groups = at.cs / p.cg;
@@ -705,14 +687,14 @@ __global__ void __launch_bounds__(kBlock, 2) norm_slab_bwd(const __grid_constant
     at.channel_sums(a1, red, sw);
     at.channel_sums(a0, red, sb);
     if (pw)
-        for (int i = threadIdx.x; i < at.cs; i += kBlock) {
+        for (int i = threadIdx.x; i < at.cs; i += kSlab) {
             const int64_t row = at.n * q.R + cluster_rank();
             float a = 0.0f, b = 0.0f;
             for (int k = 0; k < at.segs; ++k) a += sw[i * at.segs + k], b += sb[i * at.segs + k];
             pw[row * p.C + at.c0 + i] = a;
             pb[row * p.C + at.c0 + i] = b;
         }
-    auto weight = [&](int i) { return p.w ? to_float(__ldg(p.w + at.c0 + i / at.segs)) : 1.0f; };
+    auto weight = [&](int i) { return p.w ? to_float(load_one(p.w + at.c0 + i / at.segs)) : 1.0f; };
     slab_groups(groups, p.cg * at.segs, share, [&](int i) { return weight(i) * sb[i]; });
     slab_groups(groups, p.cg * at.segs, share + q.CS, [&](int i) { return weight(i) * sw[i]; });
     __syncthreads();
@@ -820,11 +802,21 @@ __global__ void __launch_bounds__(kBlock) norm_join(const float* part, int64_t S
     const int g = (int)(blockIdx.x - n * G);
     Moments m{0.0f, 0.0f, 0.0f};
     const int64_t items = q.chunks * cg;
-    for (int64_t i = threadIdx.x; i < items; i += kBlock) {
-        const int64_t chunk = i / cg, c = (int64_t)g * cg + (i - chunk * cg);
-        const float cnt = (float)(min(S, (chunk + 1) * q.rows) - chunk * q.rows);
-        const float* b = part + (n * q.chunks + chunk) * 2 * C + c;
-        m.join(cnt, b[0], b[C]);
+    for (int i0 = threadIdx.x; i0 < (int)items; i0 += 8 * kBlock) {   // eight loads on their way
+        float cnt[8], mean8[8], m28[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * kBlock, chunk = i / cg, c = g * cg + (i - chunk * cg);
+            cnt[k] = 0.0f;
+            if (i >= (int)items) continue;
+            const float* b = part + (n * q.chunks + chunk) * 2 * C + c;
+            cnt[k] = (float)(min(S, (chunk + 1) * q.rows) - chunk * q.rows);
+            mean8[k] = __ldg(b);
+            m28[k] = __ldg(b + C);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (cnt[k] > 0.0f) m.join(cnt[k], mean8[k], m28[k]);
     }
     for (int h = kBlock / 2; h >= 1; h /= 2) {
         red[0][threadIdx.x] = m.n;
@@ -842,23 +834,26 @@ __global__ void __launch_bounds__(kBlock) norm_join(const float* part, int64_t S
 
 template <typename T, int V>
 struct Channel {
-    float w[V], b[V], mean[V], rstd[V];
+    static constexpr int Q = kPairs<V>;
+    f32x2 w[Q], b[Q], minus[Q], rstd[Q];   // minus the mean
     __device__ __forceinline__ Channel(const NormP<T>& p, int64_t n, int64_t c) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) w[v] = 1.0f, b[v] = 0.0f;
-        if (p.w) unpack(load_vec<T, V>(p.w + c), w);
-        if (p.b) unpack(load_vec<T, V>(p.b + c), b);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int64_t g = n * p.G + (int)(c + v) / p.cg;
-            mean[v] = __ldg(p.mean + g);
-            rstd[v] = __ldg(p.rstd + g);
+        for (int q = 0; q < Q; ++q) {
+            const int64_t g0 = n * p.G + (int)(c + 2 * q) / p.cg, g1 = n * p.G + (int)(c + 2 * q + (V > 1)) / p.cg;
+            w[q] = each<V>(1.0f);
+            b[q] = 0;
+            minus[q] = pack2(-__ldg(p.mean + g0), V == 1 ? 0.0f : -__ldg(p.mean + g1));
+            rstd[q] = pack2(__ldg(p.rstd + g0), __ldg(p.rstd + g1));
         }
+        if (p.w) widen<T, V>(load_vec<T, V>(p.w + c), w);
+        if (p.b) widen<T, V>(load_vec<T, V>(p.b + c), b);
     }
+    __device__ __forceinline__ f32x2 xn(int q, f32x2 x) const { return mul2(add2(x, minus[q]), rstd[q]); }
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock) norm_apply(const __grid_constant__ NormP<T> p, Chunks q) {
+__global__ void __launch_bounds__(kBlock, 2) norm_apply(const __grid_constant__ NormP<T> p, Chunks q) {
+    constexpr int Q = kPairs<V>;
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
     const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
@@ -867,52 +862,56 @@ __global__ void __launch_bounds__(kBlock) norm_apply(const __grid_constant__ Nor
     const Channel<T, V> ch(p, n, c);
 #pragma unroll 4
     for (int64_t i = s0 + y; i < s1; i += by) {
-        float f[V], ga[V];
-        unpack(load_vec<T, V>(p.x + n * p.x_sb + i * p.x_sp + c), f);
-        if (p.mode == kGate) unpack(load_vec<T, V>(p.gate + n * p.g_sb + i * p.g_sp + c), ga);
+        f32x2 f[Q], ga[Q];
+        widen<T, V>(load_vec<T, V>(p.x + n * p.x_sb + i * p.x_sp + c), f);
+        if (p.mode == kGate) widen<T, V>(load_vec<T, V>(p.gate + n * p.g_sb + i * p.g_sp + c), ga);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            f[v] = fmaf((f[v] - ch.mean[v]) * ch.rstd[v], ch.w[v], ch.b[v]);
-            if (p.mode == kSilu) f[v] *= sigmoidf(f[v]);
-            if (p.mode == kGate) f[v] *= ga[v] * sigmoidf(ga[v]);
+        for (int k = 0; k < Q; ++k) {
+            f[k] = fma2(ch.xn(k, f[k]), ch.w[k], ch.b[k]);
+            if (p.mode == kSilu) f[k] = mul2(f[k], sigmoid2(f[k]));
+            if (p.mode == kGate) f[k] = mul2(f[k], mul2(ga[k], sigmoid2(ga[k])));
         }
-        store_vec(p.out + (n * p.S + i) * p.C + c, pack<T, V>(f));
+        store_vec(p.out + (n * p.S + i) * p.C + c, narrow<T, V>(f));
     }
 }
 
 // Per-channel sums of g xn and g over a chunk's places: part [n][chunk][2][C].
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock) norm_sums(const __grid_constant__ NormP<T> p, Chunks q, float* part) {
+__global__ void __launch_bounds__(kBlock, 2) norm_sums(const __grid_constant__ NormP<T> p, Chunks q, float* part) {
+    constexpr int Q = kPairs<V>;
     __shared__ float red[2][V][kBlock];
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
     const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
     const int64_t s0 = chunk * q.rows, s1 = min(p.S, s0 + q.rows);
-    float aw[V], ab[V];
+    f32x2 aw[Q], ab[Q];
 #pragma unroll
-    for (int v = 0; v < V; ++v) aw[v] = ab[v] = 0.0f;
+    for (int k = 0; k < Q; ++k) aw[k] = ab[k] = 0;
     if (c < p.C) {
         const Channel<T, V> ch(p, n, c);
-#pragma unroll 2
+#pragma unroll 4
         for (int64_t i = s0 + y; i < s1; i += by) {
-            float xn[V], go[V], ga[V];
-            unpack(load_vec<T, V>(p.x + n * p.x_sb + i * p.x_sp + c), xn);
-            unpack(load_vec<T, V>(p.dout + n * p.o_sb + i * p.o_sp + c), go);
-            if (p.mode == kGate) unpack(load_vec<T, V>(p.gate + n * p.g_sb + i * p.g_sp + c), ga);
+            f32x2 xn[Q], go[Q], ga[Q];
+            widen<T, V>(load_vec<T, V>(p.x + n * p.x_sb + i * p.x_sp + c), xn);
+            widen<T, V>(load_vec<T, V>(p.dout + n * p.o_sb + i * p.o_sp + c), go);
+            if (p.mode == kGate) widen<T, V>(load_vec<T, V>(p.gate + n * p.g_sb + i * p.g_sp + c), ga);
 #pragma unroll
-            for (int v = 0; v < V; ++v) xn[v] = (xn[v] - ch.mean[v]) * ch.rstd[v];
-            through_act<V>(p.mode, xn, ch.w, ch.b, go, ga);
+            for (int k = 0; k < Q; ++k) xn[k] = ch.xn(k, xn[k]);
+            through_act2<Q>(p.mode, xn, ch.w, ch.b, go, ga);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                aw[v] = fmaf(go[v], xn[v], aw[v]);
-                ab[v] += go[v];
+            for (int k = 0; k < Q; ++k) {
+                aw[k] = fma2(go[k], xn[k], aw[k]);
+                ab[k] = add2(ab[k], go[k]);
             }
         }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        red[0][v][threadIdx.x] = aw[v];
-        red[1][v][threadIdx.x] = ab[v];
+        float a[2], b[2];
+        unpack2(aw[v / 2], a[0], a[1]);
+        unpack2(ab[v / 2], b[0], b[1]);
+        red[0][v][threadIdx.x] = a[v % 2];
+        red[1][v][threadIdx.x] = b[v % 2];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < q.bx * V * 2; i += kBlock) {
@@ -938,13 +937,14 @@ __global__ void __launch_bounds__(kBlock) norm_sums_join(const __grid_constant__
         const int64_t c = (int64_t)g * p.cg + i;
         const float* b = part + n * q.chunks * 2 * p.C + c;
         float aw = 0.0f, ab = 0.0f;
+#pragma unroll 8
         for (int64_t k = 0; k < q.chunks; ++k) {
             aw += __ldg(b + 2 * k * p.C);
             ab += __ldg(b + (2 * k + 1) * p.C);
         }
         sw[n * p.C + c] = aw;
         sb[n * p.C + c] = ab;
-        const float w = p.w ? to_float(__ldg(p.w + c)) : 1.0f;
+        const float w = p.w ? to_float(load_one(p.w + c)) : 1.0f;
         s0 = fmaf(w, ab, s0);
         s1 = fmaf(w, aw, s1);
     }
@@ -963,35 +963,37 @@ __global__ void __launch_bounds__(kBlock) norm_sums_join(const __grid_constant__
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock) norm_apply_bwd(const __grid_constant__ NormP<T> p, Chunks q,
-                                                         const float* gm) {
+__global__ void __launch_bounds__(kBlock, 2) norm_apply_bwd(const __grid_constant__ NormP<T> p, Chunks q,
+                                                            const float* gm) {
+    constexpr int Q = kPairs<V>;
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
     const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
     const int64_t c = ((int64_t)blockIdx.y * q.bx + x) * V;
     if (c >= p.C) return;
     const int64_t s0 = chunk * q.rows, s1 = min(p.S, s0 + q.rows);
     const Channel<T, V> ch(p, n, c);
-    float m0[V], m1[V];
+    f32x2 m0[Q], m1[Q];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int64_t g = n * p.G + (int)(c + v) / p.cg;
-        m0[v] = __ldg(gm + 2 * g);
-        m1[v] = __ldg(gm + 2 * g + 1);
+    for (int k = 0; k < Q; ++k) {
+        const float* a = gm + 2 * (n * p.G + (int)(c + 2 * k) / p.cg);
+        const float* b = gm + 2 * (n * p.G + (int)(c + 2 * k + (V > 1)) / p.cg);
+        m0[k] = pack2(-__ldg(a), -__ldg(b));
+        m1[k] = pack2(-__ldg(a + 1), -__ldg(b + 1));
     }
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t i = s0 + y; i < s1; i += by) {
-        float xn[V], go[V], ga[V];
+        f32x2 xn[Q], go[Q], ga[Q];
         const int64_t o = (n * p.S + i) * p.C + c;
-        unpack(load_vec<T, V>(p.x + n * p.x_sb + i * p.x_sp + c), xn);
-        unpack(load_vec<T, V>(p.dout + n * p.o_sb + i * p.o_sp + c), go);
-        if (p.mode == kGate) unpack(load_vec<T, V>(p.gate + n * p.g_sb + i * p.g_sp + c), ga);
+        widen<T, V>(load_vec<T, V>(p.x + n * p.x_sb + i * p.x_sp + c), xn);
+        widen<T, V>(load_vec<T, V>(p.dout + n * p.o_sb + i * p.o_sp + c), go);
+        if (p.mode == kGate) widen<T, V>(load_vec<T, V>(p.gate + n * p.g_sb + i * p.g_sp + c), ga);
 #pragma unroll
-        for (int v = 0; v < V; ++v) xn[v] = (xn[v] - ch.mean[v]) * ch.rstd[v];
-        through_act<V>(p.mode, xn, ch.w, ch.b, go, ga);
-        if (p.mode == kGate) store_vec(p.dgate + o, pack<T, V>(ga));
+        for (int k = 0; k < Q; ++k) xn[k] = ch.xn(k, xn[k]);
+        through_act2<Q>(p.mode, xn, ch.w, ch.b, go, ga);
+        if (p.mode == kGate) store_vec(p.dgate + o, narrow<T, V>(ga));
 #pragma unroll
-        for (int v = 0; v < V; ++v) go[v] = ch.rstd[v] * (go[v] * ch.w[v] - m0[v] - xn[v] * m1[v]);
-        store_vec(p.dx + o, pack<T, V>(go));
+        for (int k = 0; k < Q; ++k) go[k] = mul2(ch.rstd[k], fma2(xn[k], m1[k], fma2(go[k], ch.w[k], m0[k])));
+        store_vec(p.dx + o, narrow<T, V>(go));
     }
 }
 
@@ -1035,12 +1037,12 @@ struct Plan {
 };
 
 int64_t slab_smem(int64_t cs, int64_t P, int v, int64_t es, bool grad) {
-    return slab_floats(kBlock * v + (grad ? 2 : 1) * slab_sums((int)cs) + (grad ? 4 : 3) * (int)cs) + (grad ? 2 : 1) * ceil_div(P * cs * es, 16) * 16;
+    return slab_floats(kSlab * v + (grad ? 2 : 1) * slab_sums((int)cs) + (grad ? 4 : 3) * (int)cs) + (grad ? 2 : 1) * ceil_div(P * cs * es, 16) * 16;
 }
 
 // The slab of a group that is too large for registers: whole groups and whole loads, 64
-// bytes a place or more where there are so many channels; blocks enough to hold it at
-// two an SM (one where it must be), and to give every SM one. R 0: too large.
+// bytes a place or more where there are so many channels; blocks enough to hold it, and to
+// give three SMs in four one. R 0: too large.
 Slab slab_of(const pe_norm_args* a, int v, bool grad) {
     Slab s{0, 0, 0, 0};
     const int64_t cg = a->channels / a->groups, es = a->dtype == PE_F32 ? 4 : 2;
@@ -1048,16 +1050,15 @@ Slab slab_of(const pe_norm_args* a, int v, bool grad) {
     while (base % v) base += cg;
     int64_t cs = base;
     while (cs * es < 64 && cs + base <= a->channels) cs += base;
-    if (cs / v > kBlock || a->places > (1 << 24)) return s;
+    if (cs / v > kSlab || a->places > (1 << 24)) return s;
     const int64_t slabs = ceil_div(a->channels, cs);
-    for (int64_t room : {100 * 1024, 200 * 1024})
-        for (int r = 1; r <= 8; r *= 2) {
-            const int64_t P = ceil_div(a->places, r);
-            if (slab_smem(cs, P, v, es, grad) > room) continue;
-            if (room == 100 * 1024 && r < 8 && a->batch * slabs * r * 4 < num_sms() * 3 && P * (cs / v) > 2 * kBlock) continue;
-            s.CS = (int)cs; s.slabs = (int)slabs; s.R = r; s.P = (int)P;
-            return s;
-        }
+    for (int r = 1; r <= 8; r *= 2) {
+        const int64_t P = ceil_div(a->places, r);
+        if (slab_smem(cs, P, v, es, grad) > 200 * 1024) continue;
+        if (r < 8 && a->batch * slabs * r * 4 < num_sms() * 3 && P * (cs / v) > 2 * kSlab) continue;
+        s.CS = (int)cs; s.slabs = (int)slabs; s.R = r; s.P = (int)P;
+        return s;
+    }
     return s;
 }
 
@@ -1067,9 +1068,10 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
     const int vr = cg % vec == 0 ? vec : 1;      // in registers a load stays within its group
     const int64_t items = a->places <= 1024 ? cg / vr * a->places : 1 << 20;
     // the backward pass keeps sums a channel in registers, where an item is a channel vector
-    // (two loads a lane at most: four need more registers than there are)
-    const int most = grad ? 2 : 4;
-    if (items <= most * kBlock && (!grad || a->places == 1)) {
+    // (loads a lane at most: by the registers they need; groups that take a whole block are
+    // slower element by element than the block a group further down)
+    const int most = vr == 1 ? 8 : grad ? 2 : 4;
+    if (items <= (vr == 1 ? 32 * most : most * kBlock) && (!grad || a->places == 1)) {
         p.v = vr;
         if (items <= 32 * most) {
             p.lanes = 1;
@@ -1078,10 +1080,10 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
             p.lanes = kBlock;
         }
         const int64_t k = ceil_div(items, p.lanes);
-        p.k = k <= 1 ? 1 : k <= 2 ? 2 : 4;
+        p.k = k <= 1 ? 1 : k <= 2 ? 2 : k <= 4 ? 4 : 8;
         // rows of groups at work: one wave of blocks; each then takes further rows, so that
         // its filter and its sums weigh less
-        const int64_t want = (int64_t)num_sms() * reg_blocks(p.k, grad) * kBlock / p.lanes / a->groups;
+        const int64_t want = (int64_t)num_sms() * reg_blocks(p.k, p.v, grad) * kBlock / p.lanes / a->groups;
         p.R = a->batch < want ? a->batch : want < 1 ? 1 : want;
         return p;
     }
@@ -1134,7 +1136,7 @@ int64_t stats_floats(const pe_norm_args* a, const Plan& pl) {
 // Shared memory of the register kernels' queues: four rows of k loads a lane and stream.
 template <typename T, int V>
 int queue_bytes(int k, int streams) {
-    return 4 * k * streams * kBlock * V * (int)sizeof(T);
+    return 4 * k * streams * kBlock * kSlotBytes<T, V>;
 }
 template <typename K, typename... A>
 int launch_reg(K kernel, int64_t blocks, int smem, cudaStream_t s, A... args) {
@@ -1158,7 +1160,7 @@ int launch_slab(K kernel, int64_t rows, const Slab& q, int64_t smem, cudaStream_
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kBlock);
+    cfg.blockDim = dim3(kSlab);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cfg.attrs = at;
@@ -1178,6 +1180,9 @@ int norm_run(const pe_norm_args* a, const Plan& pl, cudaStream_t s) {
         const int streams = p.mode == kGate ? 2 : 1;
         if (pl.k == 1) return launch_reg(norm_reg<T, V, 1>, blocks, queue_bytes<T, V>(1, streams), s, p, pl.lanes, (int)pl.R);
         if (pl.k == 2) return launch_reg(norm_reg<T, V, 2>, blocks, queue_bytes<T, V>(2, streams), s, p, pl.lanes, (int)pl.R);
+        if constexpr (V == 1)
+            if (pl.k == 8)
+                return launch_reg(norm_reg<T, V, 8>, blocks, queue_bytes<T, V>(8, streams), s, p, pl.lanes, (int)pl.R);
         return launch_reg(norm_reg<T, V, 4>, blocks, queue_bytes<T, V>(4, streams), s, p, pl.lanes, (int)pl.R);
     }
     if (pl.wide) {
@@ -1228,10 +1233,16 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
         sb = ws + rows * p.C;
         float* pw = sums ? sw : nullptr;
         const int streams = p.mode == kGate ? 3 : 2;
-        const int rc = pl.k == 1 ? launch_reg(norm_reg_bwd<T, V, 1>, blocks, queue_bytes<T, V>(1, streams), s, p, pl.lanes,
-                                              (int)pl.R, pw, sb)
-                                 : launch_reg(norm_reg_bwd<T, V, 2>, blocks, queue_bytes<T, V>(2, streams), s, p, pl.lanes,
-                                              (int)pl.R, pw, sb);
+        auto go = [&](auto kernel, int k) {
+            return launch_reg(kernel, blocks, queue_bytes<T, V>(k, streams), s, p, pl.lanes, (int)pl.R, pw, sb);
+        };
+        int rc = PE_ERR_INVALID;
+        if (pl.k == 1) rc = go(norm_reg_bwd<T, V, 1>, 1);
+        if (pl.k == 2) rc = go(norm_reg_bwd<T, V, 2>, 2);
+        if constexpr (V == 1) {
+            if (pl.k == 4) rc = go(norm_reg_bwd<T, V, 4>, 4);
+            if (pl.k == 8) rc = go(norm_reg_bwd<T, V, 8>, 8);
+        }
         if (rc) return rc;
     } else if (pl.wide) {
         rows = pl.R;

@@ -127,7 +127,7 @@ struct Feeder {
 // the element-wise work before tile i + 1 and after tile i - 1, and the recurrence of
 // tile i; what one barrier interval writes, the next one reads. Tokens past the end have
 // dt = 0 and B = 0: they leave the state as it is.
-template <typename T, int LPC, bool STATE_ONLY>
+template <typename T, int LPC, bool STATE_ONLY, bool FAST>
 __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
     scan_fwd(const __grid_constant__ ScanP<T> p) {
     using L = Lanes<LPC>;
@@ -152,25 +152,46 @@ __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
     const int64_t count = w.t1 - w.t0;                        // tokens
     using Feed = Feeder<T, LPC, STATE_ONLY>;
     Feed feed;
-    const bool fast = Feed::POSSIBLE && p.fast;
-    if (fast) feed.init(p, w, u, delta, z, B, C);
+    Elements<TS, CH, kThreads, T> eu, ed, ez;
+    Elements<TS, NP, kThreads, T> eb, ec;
+    if constexpr (FAST) feed.init(p, w, u, delta, z, B, C);
     auto copy = [&](int64_t t, int b) {   // tiles in order
         if (t < count) {
             const int cnt = (int)min((int64_t)TS, count - t);
-            if (fast) {
+            if constexpr (FAST) {
                 feed.copy(&m.raw[b], cnt);
-                cp_commit();
-                return;
-            }
-            stage<TS, CH>(m.raw[b].u, u + t * p.u_st, p.u_st, cnt, w.nch, p.u_cb);
-            stage<TS, CH>(m.raw[b].d, delta + t * p.d_st, p.d_st, cnt, w.nch, p.d_cb);
-            stage<TS, NP>(m.raw[b].b, B + t * p.B_st, p.B_st, cnt, p.N, p.B_cb);
-            if constexpr (!STATE_ONLY) {
-                stage<TS, NP>(m.raw[b].c, C + t * p.C_st, p.C_st, cnt, p.N, p.C_cb);
-                if (z) stage<TS, CH>(m.raw[b].z, z + t * p.z_st, p.z_st, cnt, w.nch, p.z_cb);
+            } else if (p.chunks) {
+                stage<TS, CH>(m.raw[b].u, u + t * p.u_st, p.u_st, cnt, w.nch, p.u_cb);
+                stage<TS, CH>(m.raw[b].d, delta + t * p.d_st, p.d_st, cnt, w.nch, p.d_cb);
+                stage<TS, NP>(m.raw[b].b, B + t * p.B_st, p.B_st, cnt, p.N, p.B_cb);
+                if constexpr (!STATE_ONLY) {
+                    stage<TS, NP>(m.raw[b].c, C + t * p.C_st, p.C_st, cnt, p.N, p.C_cb);
+                    if (z) stage<TS, CH>(m.raw[b].z, z + t * p.z_st, p.z_st, cnt, w.nch, p.z_cb);
+                }
+            } else {
+                eu.load(u + t * p.u_st, p.u_st, cnt, w.nch);
+                ed.load(delta + t * p.d_st, p.d_st, cnt, w.nch);
+                eb.load(B + t * p.B_st, p.B_st, cnt, p.N);
+                if constexpr (!STATE_ONLY) {
+                    ec.load(C + t * p.C_st, p.C_st, cnt, p.N);
+                    if (z) ez.load(z + t * p.z_st, p.z_st, cnt, w.nch);
+                }
             }
         }
         cp_commit();
+    };
+    // the second half of a copy of elements
+    auto land = [&](int b) {
+        if constexpr (!FAST) {
+            if (p.chunks) return;
+            eu.store(m.raw[b].u);
+            ed.store(m.raw[b].d);
+            eb.store(m.raw[b].b);
+            if constexpr (!STATE_ONLY) {
+                ec.store(m.raw[b].c);
+                if (z) ez.store(m.raw[b].z);
+            }
+        }
     };
     copy(0, 0);
 
@@ -282,10 +303,12 @@ __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
         }
     };
 
+    land(0);
     cp_wait();
     __syncthreads();
     copy(TS, 1);
     before(0, 0);
+    land(1);
     int b = 0;
     for (int64_t t = 0; t < count; t += TS, b ^= 1) {
         cp_wait();
@@ -343,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
                 }
             }
         }
+        land(b);
     }
     if (!STATE_ONLY && count > 0) {
         __syncthreads();
@@ -491,9 +515,9 @@ __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ St
     for (int r = 0; r < RB; ++r) {
         const int64_t b = b0 + r;
         const bool on = hp[r] && live;
-        u[r] = on ? to_float(__ldg(p.u + b * p.u_sb + c)) : 0.0f;
-        dt[r] = on ? to_float(__ldg(p.delta + b * p.d_sb + c)) + bias : 0.0f;
-        z[r] = on && p.z ? to_float(__ldg(p.z + b * p.z_sb + c)) : 0.0f;
+        u[r] = on ? to_float(load_one(p.u + b * p.u_sb + c)) : 0.0f;
+        dt[r] = on ? to_float(load_one(p.delta + b * p.d_sb + c)) + bias : 0.0f;
+        z[r] = on && p.z ? to_float(load_one(p.z + b * p.z_sb + c)) : 0.0f;
         const T* Bp = p.B + b * p.B_sb + g * p.B_sg + n0;
         const T* Cp = p.C + b * p.C_sb + g * p.C_sg + n0;
 #pragma unroll
@@ -507,8 +531,8 @@ __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ St
 #pragma unroll
             for (int i = 0; i < NS; ++i)
                 if (on && i < nn) {
-                    B[r][i] = to_float(__ldg(Bp + i));
-                    C[r][i] = to_float(__ldg(Cp + i));
+                    B[r][i] = to_float(load_one(Bp + i));
+                    C[r][i] = to_float(load_one(Cp + i));
                 }
         }
     }
@@ -570,6 +594,18 @@ int64_t piece_tokens(const pe_scan_args* a) {
     return max((int64_t)KCK, ceil_div(ceil_div(a->tokens, pieces), KCK) * KCK);
 }
 
+template <typename T, int LPC, bool FAST>
+int scan_launch(const ScanP<T>& p, unsigned grid, bool split, cudaStream_t s) {
+    if (split) {
+        if (int rc = launch(scan_fwd<T, LPC, true, FAST>, p, grid, sizeof(FwdSmem<T, LPC, true>), s)) return rc;
+        const dim3 blocks((unsigned)ceil_div((int64_t)p.D * p.N, kThreads), (unsigned)p.seqs.nseq);
+        scan_carry<T><<<blocks, kThreads, 0, s>>>(p);
+        count_launch();
+        if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
+    }
+    return launch(scan_fwd<T, LPC, false, FAST>, p, grid, sizeof(FwdSmem<T, LPC, false>), s);
+}
+
 template <typename T, int LPC>
 int scan_run(const pe_scan_args* a, cudaStream_t s) {
     ScanP<T> p = scan_params<T>(a, kThreads / LPC, 4 * LPC);
@@ -583,14 +619,9 @@ int scan_run(const pe_scan_args* a, cudaStream_t s) {
     }
     unsigned grid;
     if (int rc = grid_of(piece_count(p.seqs, p.piece) * p.G * p.ntile, &grid)) return rc;
-    if (piece) {
-        if (int rc = launch(scan_fwd<T, LPC, true>, p, grid, sizeof(FwdSmem<T, LPC, true>), s)) return rc;
-        const dim3 blocks((unsigned)ceil_div((int64_t)p.D * p.N, kThreads), (unsigned)p.seqs.nseq);
-        scan_carry<T><<<blocks, kThreads, 0, s>>>(p);
-        count_launch();
-        if (cudaGetLastError() != cudaSuccess) return PE_ERR_CUDA;
-    }
-    return launch(scan_fwd<T, LPC, false>, p, grid, sizeof(FwdSmem<T, LPC, false>), s);
+    if constexpr (Feeder<T, LPC, false>::POSSIBLE)
+        if (p.fast) return scan_launch<T, LPC, true>(p, grid, piece, s);
+    return scan_launch<T, LPC, false>(p, grid, piece, s);
 }
 
 #define PE_LANES(F, l, ...)                    \

@@ -27,7 +27,7 @@ struct ScanP {
     float *state, *ckpt;
     // copies to shared memory: rows of these tensors in chunks (see chunk_of), 0 = element by element
     int u_cb, d_cb, z_cb, B_cb, C_cb;
-    bool fast;            // all of them in chunks of 16
+    bool fast, chunks;    // all of them in chunks of 16; of 8 or 16
     bool pairs;           // out's rows take aligned pairs of elements
     bool longest_first;   // packed sequences are taken in the order of their lengths
     int64_t piece;        // tokens a piece (a multiple of KCK, or more than any sequence has)
@@ -109,10 +109,32 @@ __device__ __forceinline__ void stage(T* dst, const T* src, int64_t st, int cnt,
 #pragma unroll 4
         for (int i = threadIdx.x; i < ROWS * W; i += NT) {
             const int t = i / W, k = i % W;
-            if (t < cnt && k < width) dst[i] = __ldg(src + t * st + k);
+            if (t < cnt && k < width) dst[i] = load_one(src + t * st + k);
         }
     }
 }
+
+// Rows that no chunk fits, element by element in two halves, so that the loads of all
+// tensors are on their way together: load() before other work, store() after it.
+template <int ROWS, int W, int NT, typename T>
+struct Elements {
+    static constexpr int J = (ROWS * W + NT - 1) / NT;
+    T r[J];
+    __device__ __forceinline__ void load(const T* src, int64_t st, int cnt, int width) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = threadIdx.x + j * NT, t = i / W, k = i % W;
+            if (t < cnt && k < width) r[j] = load_one(src + t * st + k);
+        }
+    }
+    __device__ __forceinline__ void store(T* dst) const {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = threadIdx.x + j * NT;
+            if (i < ROWS * W) dst[i] = r[j];
+        }
+    }
+};
 
 // ---- host -------------------------------------------------------------------------
 inline int check_scan(const pe_scan_args* a) {
@@ -167,6 +189,7 @@ ScanP<T> scan_params(const pe_scan_args* a, int ch, int nc) {
     p.B_cb = chunk_of(p.B, es, cols, {p.B_sb, p.B_st, p.B_sg}, nc);
     p.C_cb = chunk_of(p.C, es, cols, {p.C_sb, p.C_st, p.C_sg}, nc);
     p.fast = p.u_cb == 16 && p.d_cb == 16 && (!p.z || p.z_cb == 16) && p.B_cb == 16 && p.C_cb == 16;
+    p.chunks = p.u_cb && p.d_cb && (!p.z || p.z_cb) && p.B_cb && p.C_cb;
     p.pairs = p.Dg % 2 == 0;
     return p;
 }

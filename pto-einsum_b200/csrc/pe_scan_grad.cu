@@ -201,13 +201,31 @@ __global__ void __launch_bounds__(kGradThreads, 2) scan_bwd(const __grid_constan
     };
     auto copy = [&](int64_t t) {
         const int cnt = (int)min((int64_t)TT, len - t);
+        const float* k = ckpt + t / KCK * DN;
+        for (int i = tid; i < w.nch * f.N; i += NT) cp_async<4>(sK + i, k + i, 4);
+        if (!f.chunks || !p.o_cb) {
+            Elements<TT, CB, NT, T> eu, ed, eo, ez;
+            Elements<TT, NC, NT, T> eb, ec;
+            const int nn = min(NC, f.N);
+            eu.load(u + t * f.u_st, f.u_st, cnt, w.nch);
+            ed.load(delta + t * f.d_st, f.d_st, cnt, w.nch);
+            eo.load(dout + t * p.o_st, p.o_st, cnt, w.nch);
+            if (z) ez.load(z + t * f.z_st, f.z_st, cnt, w.nch);
+            eb.load(B + t * f.B_st, f.B_st, cnt, nn);
+            ec.load(C + t * f.C_st, f.C_st, cnt, nn);
+            eu.store(m.u);
+            ed.store(m.d);
+            eo.store(m.o);
+            if (z) ez.store(m.z);
+            eb.store(m.b);
+            ec.store(m.c);
+            return;
+        }
         stage<TT, CB, NT>(m.u, u + t * f.u_st, f.u_st, cnt, w.nch, f.u_cb);
         stage<TT, CB, NT>(m.d, delta + t * f.d_st, f.d_st, cnt, w.nch, f.d_cb);
         stage<TT, CB, NT>(m.o, dout + t * p.o_st, p.o_st, cnt, w.nch, p.o_cb);
         if (z) stage<TT, CB, NT>(m.z, z + t * f.z_st, f.z_st, cnt, w.nch, f.z_cb);
         copy_states(t, 0);
-        const float* k = ckpt + t / KCK * DN;
-        for (int i = tid; i < w.nch * f.N; i += NT) cp_async<4>(sK + i, k + i, 4);
     };
     const int64_t top = len > w.t0 ? (len - 1) / TT * TT : -1;
     if (top >= 0) copy(top);
@@ -499,6 +517,16 @@ __global__ void __launch_bounds__(kThreads, 3) scan_adjoint(const __grid_constan
     };
     auto copy = [&](int64_t t) {
         const int cnt = (int)min((int64_t)TT, len - t);
+        if (!f.d_cb || !p.o_cb || (z && !f.z_cb)) {
+            Elements<TT, CB, kThreads, T> ed, eo, ez;
+            ed.load(delta + t * f.d_st, f.d_st, cnt, w.nch);
+            eo.load(dout + t * p.o_st, p.o_st, cnt, w.nch);
+            if (z) ez.load(z + t * f.z_st, f.z_st, cnt, w.nch);
+            ed.store(m.d);
+            eo.store(m.o);
+            if (z) ez.store(m.z);
+            return;
+        }
         stage<TT, CB>(m.d, delta + t * f.d_st, f.d_st, cnt, w.nch, f.d_cb);
         stage<TT, CB>(m.o, dout + t * p.o_st, p.o_st, cnt, w.nch, p.o_cb);
         if (z) stage<TT, CB>(m.z, z + t * f.z_st, f.z_st, cnt, w.nch, f.z_cb);
