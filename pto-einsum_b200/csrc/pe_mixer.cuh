@@ -96,7 +96,12 @@ __device__ __forceinline__ float silu_slope(float x, float s) { return s * (1.0f
 // leaves a relative error below (1/9)^7 / 15 = 1.4e-8. A logarithm of the
 // rounded 1 + e would lose the small step sizes (e = 1e-3 keeps 13 bits).
 __device__ __forceinline__ float softplusf(float x) {
-    const float e = exp2_fast(-kLog2e * fabsf(x));
+    // the product -|x| log2(e) in two parts: rounded to one, small step sizes (x = -7) would
+    // be off by 4e-7, more than all that follows
+    const float a = fmaxf(-fabsf(x), -150.0f), hi = a * kLog2e;   // finite: exp(-150) is 0 here
+    const float lo = fmaf(a, kLog2e, -hi) + a * 1.925963033500011e-8f;   // log2(e) - kLog2e
+    float e = exp2_fast(hi);
+    e = fmaf(e, lo * kLn2, e);
     const float s = e * rcp_fast(2.0f + e);
     const float q = s * s;
     float r = fmaf(q, 1.0f / 13, 1.0f / 11);
@@ -105,8 +110,7 @@ __device__ __forceinline__ float softplusf(float x) {
     r = fmaf(r, q, 1.0f / 5);
     r = fmaf(r, q, 1.0f / 3);
     r = fmaf(r, q, 1.0f);
-    // NaN stays NaN: fmaxf alone would drop it, the product with s does not
-    return fmaxf(x, 0.0f) + 2.0f * s * r;
+    return (x < 0.0f ? 0.0f : x) + 2.0f * s * r;   // NaN stays NaN
 }
 
 // ---- packed pairs --------------------------------------------------------------

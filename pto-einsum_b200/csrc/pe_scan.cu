@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
                 const float2 dx = m.fp[b].dx[k0 + k][ch];
                 const f32x2 dt2 = pack2(dx.x, dx.x), x2 = pack2(dx.y, dx.y);
                 const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&m.fp[b].B[(k0 + k) * NP + n0]);
-                a[k][0] = exp2_2(mul2(dt2, A01));
-                a[k][1] = exp2_2(mul2(dt2, A23));
+                a[k][0] = decay2(dt2, A01);
+                a[k][1] = decay2(dt2, A23);
                 x[k][0] = mul2(x2, bv.x);
                 x[k][1] = mul2(x2, bv.y);
                 if constexpr (STATE_ONLY) dtsum += dx.x;
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ St
         float y = 0.0f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            h[r][i] = fmaf(exp2_fast(dl * A[i]), h[r][i], x * B[r][i]);
+            h[r][i] = fmaf(decay(dl, A[i]), h[r][i], x * B[r][i]);
             y = fmaf(C[r][i], h[r][i], y);
         }
         if (VEC) {

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) scan_bwd(const __grid_constan
                     Pairs ap, bp, vp;
 #pragma unroll
                     for (int i = 0; i < K / 2; ++i) {
-                        ap.p[i] = exp2_2(mul2(dt.p[i], A2));
+                        ap.p[i] = decay2(dt.p[i], A2);
                         bp.p[i] = mul2(x.p[i], Bn.p[i]);
                         vp.p[i] = mul2(dy.p[i], Cn.p[i]);
                     }
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_adjoint(const __grid_constan
                     float a[K], v[K];
 #pragma unroll
                     for (int i = 0; i < K / 2; ++i) {
-                        ap.p[i] = exp2_2(mul2(dt[e].p[i], A2));
+                        ap.p[i] = decay2(dt[e].p[i], A2);
                         vp.p[i] = mul2(dy[e].p[i], Cn.p[i]);
                     }
                     P[e] = product(ap);
