@@ -27,41 +27,42 @@ _NORM = packer("6q" "d" "4Q" "4q" "Q" "2Q" "Qq")
 _NORM_GRAD = packer("6q" "d" "4Q" "4q" "Q" "2Q" "Qq" "Q" "2q" "4Q" "Qq")
 
 
-def _fields(lay, x, weight, bias, gate, out, mean, rstd):
+def _fields(lay, x, weight, bias, gate, out, stats):
+    """stats [2, N, G]: means, then reciprocal deviations."""
     ints, strides, _ = lay
-    return (*ints, x.data_ptr(), ptr(weight), ptr(bias), ptr(gate), *strides, ptr(out), ptr(mean), ptr(rstd))
+    mean = ptr(stats)
+    return (*ints, x.data_ptr(), ptr(weight), ptr(bias), ptr(gate), *strides, ptr(out), mean,
+            mean + 4 * ints[2] * ints[5] if mean else 0)
 
 
 def _forward(lay, x, weight, bias, gate, stats):
     dev = x.device
     out = _ops.empty(x)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, lay[0][2], lay[0][5]), dtype=torch.float32, device=dev).unbind(0)
-    fields = _fields(lay, x, weight, bias, gate, out, mean, rstd)
+    stats = torch.empty((2, lay[0][2], lay[0][5]), dtype=torch.float32, device=dev) if stats else None
+    fields = _fields(lay, x, weight, bias, gate, out, stats)
     nbytes = _ops.nbytes_of("pe_group_norm_ws_bytes", lay, lambda: _NORM.pack(*fields, 0, 0))
     ws = _ops.workspace(nbytes, dev)
     call("pe_group_norm", _NORM.pack(*fields, ptr(ws), nbytes), lay[2])
-    return out, mean, rstd
+    return out, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gate, lay):
-        out, mean, rstd = _forward(lay, x, weight, bias, gate, True)
-        ctx.save_for_backward(x, weight, bias, gate, mean, rstd)
+        out, stats = _forward(lay, x, weight, bias, gate, True)
+        ctx.save_for_backward(x, weight, bias, gate, stats)
         ctx.lay = lay
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        x, weight, bias, gate, mean, rstd = ctx.saved_tensors
+        x, weight, bias, gate, stats = ctx.saved_tensors
         lay, dev = ctx.lay, x.device
         dout = _fold(dout)
 
         dx, dw, db, dgate = [None if t is None else _ops.empty(t) for t in (x, weight, bias, gate)]
-        fields = (*_fields(lay, x, weight, bias, gate, None, mean, rstd), 0, 0, dout.data_ptr(), *_strides(dout),
+        fields = (*_fields(lay, x, weight, bias, gate, None, stats), 0, 0, dout.data_ptr(), *_strides(dout),
                   dx.data_ptr(), ptr(dgate), ptr(dw), ptr(db))
         nbytes = _ops.nbytes_of("pe_group_norm_grad_ws_bytes", lay, lambda: _NORM_GRAD.pack(*fields, 0, 0))
         ws = _ops.workspace(nbytes, dev)
