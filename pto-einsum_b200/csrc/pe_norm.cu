@@ -368,18 +368,55 @@ __global__ void __launch_bounds__(kBlock) norm_wide(const __grid_constant__ Norm
     }
 }
 
-// Backward: rows r, r + R, ... of one group a block, the sums of g xn and g of its
-// channels in shared memory, each with the thread that has the channel.
-template <typename T, int V>
+// The sums of V channels, from and to memory.
+template <int V>
+__device__ __forceinline__ void load_sums(const float* from, f32x2 (&s)[kPairs<V>]) {
+    if constexpr (V == 1) {
+        s[0] = pack2(*from, 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(from)[i];
+            s[2 * i] = pack2(v.x, v.y);
+            s[2 * i + 1] = pack2(v.z, v.w);
+        }
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_sums(float* to, const f32x2 (&s)[kPairs<V>]) {
+    float h[2 * kPairs<V>];
+#pragma unroll
+    for (int q = 0; q < kPairs<V>; ++q) unpack2(s[q], h[2 * q], h[2 * q + 1]);
+    if constexpr (V == 1) {
+        *to = h[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            reinterpret_cast<float4*>(to)[i] = make_float4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+    }
+}
+
+// Backward: rows r, r + R, ... of one group a block. The sums of g xn and g of a channel
+// belong to the thread that has the channel: in shared memory (LOCAL; a plane for each
+// element of a load, for no two lanes share a bank then), or, where that is too small,
+// in their places of pw and pb.
+template <typename T, int V, bool LOCAL>
 __global__ void __launch_bounds__(kBlock, 2) norm_wide_bwd(const __grid_constant__ NormP<T> p, int R, float* pw, float* pb) {
     constexpr int Q = kPairs<V>;
-    extern __shared__ __align__(16) f32x2 acc[];   // [cg / V][2][Q], g xn and g
+    extern __shared__ __align__(16) f32x2 acc[];   // [2][Q][cg / V], g xn and g
     __shared__ float red[16];
     const int r = blockIdx.x / (unsigned)p.G, g = blockIdx.x % (unsigned)p.G, c0 = g * p.cg;
     const float inv = 1.0f / (float)p.cg;
-    for (int c = threadIdx.x; c < p.cg / V; c += kBlock)
+    const int cv = p.cg / V;
+    if (LOCAL)
+        for (int c = threadIdx.x; c < cv; c += kBlock)
 #pragma unroll
-        for (int q = 0; q < 2 * Q; ++q) acc[c * 2 * Q + q] = 0;
+            for (int q = 0; q < 2 * Q; ++q) acc[q * cv + c] = 0;
+    float *ow = nullptr, *ob = nullptr;
+    if (pw) {
+        ow = pw + (int64_t)r * p.C + c0;
+        ob = pb + (int64_t)r * p.C + c0;
+    }
     for (int64_t n = r; n < p.N; n += R) {
         const f32x2 minus = each<V>(-__ldg(p.mean + n * p.G + g)), scale = both(__ldg(p.rstd + n * p.G + g));
         auto load = [&](int c, f32x2 (&xn)[Q], f32x2 (&go)[Q], f32x2 (&ga)[Q], f32x2 (&w)[Q]) {
@@ -400,11 +437,31 @@ __global__ void __launch_bounds__(kBlock, 2) norm_wide_bwd(const __grid_constant
         for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
             f32x2 xn[Q], go[Q], ga[Q], w[Q];
             load(c, xn, go, ga, w);
-            f32x2* a = acc + c / V * 2 * Q;
+            if (LOCAL) {
+                f32x2* a = acc + c / V;
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    a[q * cv] = fma2(go[q], xn[q], a[q * cv]);
+                    a[(Q + q) * cv] = add2(a[(Q + q) * cv], go[q]);
+                }
+            } else if (ow) {
+                f32x2 aw[Q], ab[Q];
+#pragma unroll
+                for (int q = 0; q < Q; ++q) aw[q] = ab[q] = 0;
+                if (n != r) {
+                    load_sums<V>(ow + c, aw);
+                    load_sums<V>(ob + c, ab);
+                }
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    aw[q] = fma2(go[q], xn[q], aw[q]);
+                    ab[q] = add2(ab[q], go[q]);
+                }
+                store_sums<V>(ow + c, aw);
+                store_sums<V>(ob + c, ab);
+            }
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                a[q] = fma2(go[q], xn[q], a[q]);
-                a[Q + q] = add2(a[Q + q], go[q]);
                 go[q] = mul2(go[q], w[q]);
                 s0 = add2(s0, go[q]);
                 s1 = fma2(go[q], xn[q], s1);
@@ -423,16 +480,17 @@ __global__ void __launch_bounds__(kBlock, 2) norm_wide_bwd(const __grid_constant
             store_vec(p.dx + n * p.C + c0 + c, narrow<T, V>(go));
         }
     }
-    if (!pw) return;
-    for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V)
+    if (!LOCAL || !pw) return;
+    for (int c = threadIdx.x * V; c < p.cg; c += kBlock * V) {
+        f32x2 a[Q], b[Q];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float a[2], b[2];
-            unpack2(acc[c / V * 2 * Q + v / 2], a[0], a[1]);
-            unpack2(acc[c / V * 2 * Q + Q + v / 2], b[0], b[1]);
-            pw[(int64_t)r * p.C + c0 + c + v] = a[v % 2];
-            pb[(int64_t)r * p.C + c0 + c + v] = b[v % 2];
+        for (int q = 0; q < Q; ++q) {
+            a[q] = acc[q * cv + c / V];
+            b[q] = acc[(Q + q) * cv + c / V];
         }
+        store_sums<V>(ow + c, a);
+        store_sums<V>(ob + c, b);
+    }
 }
 
 // ---- groups in a cluster's shared memory ------------------------------------------------
@@ -440,7 +498,7 @@ __global__ void __launch_bounds__(kBlock, 2) norm_wide_bwd(const __grid_constant
 // its P places, which stay in shared memory: one read of the tensor and one launch. The
 // blocks exchange their sums of each group through distributed shared memory and add
 // them in rank order.
-constexpr int kSlab = 512;   // threads: one block an SM
+constexpr int kSlab = 256;   // threads
 struct Slab {
     int CS, slabs, R, P;
 };
@@ -537,7 +595,7 @@ __device__ __forceinline__ void cluster_groups(int groups, int R, const float* s
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kSlab, 1) norm_slab(const __grid_constant__ NormP<T> p, const Slab q) {
+__global__ void __launch_bounds__(kSlab, 3) norm_slab(const __grid_constant__ NormP<T> p, const Slab q) {
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) unsigned char smem[];
     float* red = reinterpret_cast<float*>(smem);        // [kSlab V]
@@ -636,7 +694,7 @@ __global__ void __launch_bounds__(kSlab, 1) norm_slab(const __grid_constant__ No
 // Backward: x and dout stay in shared memory, the gate is read twice. pw, pb [N R][C]: a
 // block's share of the sums of g xn and g.
 template <typename T, int V>
-__global__ void __launch_bounds__(kSlab, 1) norm_slab_bwd(const __grid_constant__ NormP<T> p, const Slab q, float* pw,
+__global__ void __launch_bounds__(kSlab, 2) norm_slab_bwd(const __grid_constant__ NormP<T> p, const Slab q, float* pw,
                                                            float* pb) {
     constexpr int Q = kPairs<V>;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -1031,7 +1089,7 @@ struct Plan {
     int v;            // elements a load
     int lanes, k;     // groups in registers: lanes a group, loads a lane; lanes 0: too large for that
     int64_t R;        // in registers: rows at work, a lane takes every R-th
-    bool wide;        // a block a group of one place
+    bool wide, local; // a block a group of one place; its sums in shared memory
     Slab slab;        // in a cluster's shared memory: R > 0
     Chunks q;
 };
@@ -1055,7 +1113,8 @@ Slab slab_of(const pe_norm_args* a, int v, bool grad) {
     for (int r = 1; r <= 8; r *= 2) {
         const int64_t P = ceil_div(a->places, r);
         if (slab_smem(cs, P, v, es, grad) > 200 * 1024) continue;
-        if (r < 8 && a->batch * slabs * r * 4 < num_sms() * 3 && P * (cs / v) > 2 * kSlab) continue;
+        if (r < 8 && slab_smem(cs, P, v, es, grad) > (grad ? 100 : 64) * 1024 && P * (cs / v) > 2 * kSlab) continue;
+        if (a->batch * slabs * r > num_sms() * (grad ? 2 : 3)) return s;
         s.CS = (int)cs; s.slabs = (int)slabs; s.R = r; s.P = (int)P;
         return s;
     }
@@ -1070,7 +1129,7 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
     // the backward pass keeps sums a channel in registers, where an item is a channel vector
     // (loads a lane at most: by the registers they need; groups that take a whole block are
     // slower element by element than the block a group further down)
-    const int most = vr == 1 ? 8 : grad ? 2 : 4;
+    const int most = vr == 1 ? 8 : grad || a->places == 1 ? 2 : 4;
     if (items <= (vr == 1 ? 32 * most : most * kBlock) && (!grad || a->places == 1)) {
         p.v = vr;
         if (items <= 32 * most) {
@@ -1089,10 +1148,11 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
     }
     // one place a row: a block a group while its sums fit shared memory
     const int64_t smem = cg / vr * 2 * ((vr + 1) / 2) * 8;
-    if (a->places == 1 && smem <= 200 * 1024) {
+    if (a->places == 1) {
         p.v = vr;
         p.wide = true;
-        const int64_t resident = smem > 100 * 1024 ? 1 : smem > 50 * 1024 ? 2 : 4;
+        p.local = smem <= 200 * 1024;
+        const int64_t resident = !p.local ? 2 : smem > 100 * 1024 ? 1 : smem > 50 * 1024 ? 2 : 4;
         const int64_t want = ceil_div((int64_t)num_sms() * resident, a->groups);
         p.R = a->batch < want ? a->batch : want;
         return p;
@@ -1250,9 +1310,10 @@ int norm_grad_run(const pe_norm_grad_args* ga, const Plan& pl, cudaStream_t s) {
         sb = ws + rows * p.C;
         const int smem = p.cg / V * 2 * kPairs<V> * 8;
         if (pl.R * p.G > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
-        if (int rc = launch_reg(norm_wide_bwd<T, V>, pl.R * p.G, smem, s, p, (int)pl.R,
-                                ga->dweight || ga->dbias ? sw : nullptr, sb))
-            return rc;
+        float* pw = ga->dweight || ga->dbias ? sw : nullptr;
+        const int rc = pl.local ? launch_reg(norm_wide_bwd<T, V, true>, pl.R * p.G, smem, s, p, (int)pl.R, pw, sb)
+                                : launch_reg(norm_wide_bwd<T, V, false>, pl.R * p.G, 0, s, p, (int)pl.R, pw, sb);
+        if (rc) return rc;
     } else if (pl.slab.R) {
         rows = p.N * pl.slab.R;
         sw = ws;
