@@ -69,7 +69,7 @@ int sum_rows(const SumJob* jobs, int count, cudaStream_t s) {
             rows = jobs[i].rows > rows ? jobs[i].rows : rows;
         }
     if (!n) return PE_OK;
-    const bool few = rows <= 16;   // no more loads a thread than the other kernel's columns take
+    const bool few = rows <= 16 && ceil_div(most, 32) > 2 * num_sms();
     const int64_t blocks = ceil_div(most, few ? 256 : 32);
     const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), n);
     if (few)
