@@ -50,14 +50,15 @@ struct Place {
 // or the last one to start would end long after the others.
 __device__ __forceinline__ int seq_of_rank(const Seqs& q, int rank) {
     __shared__ int found;
+    __shared__ int64_t lens[kThreads];
     const int i = threadIdx.x;
+    const int64_t len = i < q.nseq ? seq_span(q, i).len : -1;
+    if (i < kThreads) lens[i] = len;
+    __syncthreads();
     if (i < q.nseq) {
-        const int64_t len = seq_span(q, i).len;
         int longer = 0;
-        for (int j = 0; j < q.nseq; ++j) {
-            const int64_t l = seq_span(q, j).len;
-            longer += l > len || (l == len && j < i);
-        }
+#pragma unroll 8
+        for (int j = 0; j < q.nseq; ++j) longer += lens[j] > len || (lens[j] == len && j < i);
         if (longer == rank) found = i;
     }
     __syncthreads();
@@ -98,6 +99,7 @@ __device__ __forceinline__ float decay(float dt, float A) { return exp2_fast(fma
 template <int ROWS, int W, int BYTES, int NT, typename T>
 __device__ __forceinline__ void stage_chunks(T* dst, const T* src, int64_t st, int cnt, int width) {
     constexpr int E = BYTES / (int)sizeof(T), PER = W / E;
+    static_assert(W % E == 0, "rows of whole chunks");
 #pragma unroll 4
     for (int i = threadIdx.x; i < ROWS * PER; i += NT) {
         const int t = i / PER, k = i % PER * E;
@@ -109,9 +111,13 @@ template <int ROWS, int W, int NT = kThreads, typename T>
 __device__ __forceinline__ void stage(T* dst, const T* src, int64_t st, int cnt, int width, int cb) {
     constexpr int ROW = W * (int)sizeof(T);
     static_assert(ROW % 8 == 0, "rows of whole chunks");
-    if (ROW % 16 == 0 && cb == 16) {
-        stage_chunks<ROWS, W, 16, NT>(dst, src, st, cnt, width);
-    } else if (cb >= 8) {
+    if constexpr (ROW % 16 == 0) {
+        if (cb == 16) {
+            stage_chunks<ROWS, W, 16, NT>(dst, src, st, cnt, width);
+            return;
+        }
+    }
+    if (cb >= 8) {
         stage_chunks<ROWS, W, 8, NT>(dst, src, st, cnt, width);
     } else {
 #pragma unroll 4

@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(256) sum_tiles(const float* __restrict__ part,
 int64_t grad_piece(const pe_scan_args* a) {
     const int64_t tiles = a->groups * ceil_div(a->channels / a->groups, CB), rows = a->cu ? 1 : a->nseq;
     const int64_t blocks = a->nseq * tiles;
-    if (blocks < 1 || a->nseq > 65535 || blocks * 10 >= num_sms() * 6 || a->tokens / (a->nseq / rows) < 4 * KCK)
+    if (blocks < 1 || a->nseq > 65535 || blocks >= num_sms() || a->tokens / (a->nseq / rows) < 4 * KCK)
         return 0;
     int64_t pieces = 2 * num_sms() / (rows * tiles) - (a->cu ? a->nseq : 0);
     if (pieces < 2) return 0;
