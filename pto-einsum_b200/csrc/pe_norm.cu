@@ -910,7 +910,7 @@ struct Channel {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kBlock, 2) norm_apply(const __grid_constant__ NormP<T> p, Chunks q) {
+__global__ void __launch_bounds__(kBlock, 4) norm_apply(const __grid_constant__ NormP<T> p, Chunks q) {
     constexpr int Q = kPairs<V>;
     const int by = kBlock / q.bx, x = threadIdx.x % q.bx, y = threadIdx.x / q.bx;
     const int64_t n = blockIdx.x / (unsigned)q.chunks, chunk = blockIdx.x % (unsigned)q.chunks;
@@ -1114,7 +1114,8 @@ Slab slab_of(const pe_norm_args* a, int v, bool grad) {
         const int64_t P = ceil_div(a->places, r);
         if (slab_smem(cs, P, v, es, grad) > 200 * 1024) continue;
         if (r < 8 && slab_smem(cs, P, v, es, grad) > (grad ? 100 : 64) * 1024 && P * (cs / v) > 2 * kSlab) continue;
-        if (a->batch * slabs * r > num_sms() * (grad ? 2 : 3)) return s;
+        const int64_t resident = min((int64_t)(grad ? 2 : 3), 220 * 1024 / slab_smem(cs, P, v, es, grad));
+        if (a->batch * slabs * r > num_sms() * resident) return s;
         s.CS = (int)cs; s.slabs = (int)slabs; s.R = r; s.P = (int)P;
         return s;
     }
@@ -1163,10 +1164,19 @@ Plan plan_of(const pe_norm_args* a, int vec, bool grad) {
     const int64_t cv = a->channels / vec;
     p.q.bx = 32;
     while (p.q.bx > 1 && ceil_div(cv, p.q.bx) * p.q.bx * 8 > cv * 9) p.q.bx /= 2;
-    const int64_t blocks = ceil_div(cv, p.q.bx) * a->batch, by = kBlock / p.q.bx;
-    const int64_t want = ceil_div((int64_t)num_sms() * 8, blocks > 0 ? blocks : 1);
-    p.q.rows = ceil_div(ceil_div(a->places, want), by) * by;
-    if (p.q.rows < 4 * by) p.q.rows = 4 * by;
+    // chunks a row: whole waves of the blocks that the SMs hold, where a block costs its
+    // places and about six more (its filter, its statistics, the sums over its lanes)
+    const int64_t blocks = max((int64_t)1, ceil_div(cv, p.q.bx) * a->batch), by = kBlock / p.q.bx;
+    const int64_t slots = (int64_t)num_sms() * (grad ? 2 : 4);
+    int64_t best = 0;
+    for (int64_t w = 1; w <= 8; ++w) {
+        const int64_t rows = ceil_div(ceil_div(a->places, max((int64_t)1, w * slots / blocks)), by) * by;
+        const int64_t cost = ceil_div(blocks * ceil_div(a->places, rows), slots) * (rows / by + 6);
+        if (w == 1 || cost < best) {
+            best = cost;
+            p.q.rows = rows;
+        }
+    }
     p.q.chunks = ceil_div(a->places, p.q.rows);
     return p;
 }
