@@ -63,13 +63,6 @@ __device__ __forceinline__ void unpack(const Vec<T, V>& r, float (&f)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = to_float(r.v[i]);
 }
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
-    Vec<T, V> r;
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(f[i]);
-    return r;
-}
 
 // 2^x and 1/x of one instruction each (relative errors of 2^-22 and 2^-23; denormal
 // arguments and results count as zero).

@@ -8,8 +8,8 @@ namespace {
 // out[c] = sum_r part[r][c] of each job (blockIdx.y). A block has 32 columns and 32 row
 // lanes: lane y adds the rows y, y + 32, ..., eight loads in flight, then the 32 sums are
 // added in order, so that the same input gives the same bits. Reads of a warp are 128
-// contiguous bytes. Bound by latency at the usual sizes (a few hundred rows), so all of
-// an operator's sums go in one launch.
+// contiguous bytes. Bound by latency at the usual sizes (a few hundred rows: 4 us on a
+// B200), so all of an operator's sums go in one launch.
 struct Jobs {
     SumJob j[3];
 };
@@ -45,7 +45,10 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const __grid_constant__ 
     }
 }
 
-// The same for a few rows: a thread a column.
+// The same for a few rows: a thread a column, where the columns alone fill the GPU. The
+// scan's training step of 2 x 256 tokens, 4096 channels and 16 states: 128 us, 140 with
+// the kernel above; the norm's of 16 rows and 4096 channels, which that rule leaves to the
+// kernel above: 20.7 and 16.6.
 __global__ void __launch_bounds__(256) sum_few_rows(const __grid_constant__ Jobs jobs) {
     const SumJob& j = jobs.j[blockIdx.y];
     for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < j.cols; c += (int64_t)gridDim.x * 256) {

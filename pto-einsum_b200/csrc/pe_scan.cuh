@@ -47,7 +47,8 @@ struct Place {
 
 // The sequence with `rank` longer ones (equal lengths in order), for up to kThreads of
 // them: blocks that take whole sequences of very different lengths start with the longest,
-// or the last one to start would end long after the others.
+// or the last one to start would end long after the others (17 sequences in 8192 tokens,
+// 4096 channels: 253 us, 368 in the order of the table; 60 sequences 306 and 312).
 __device__ __forceinline__ int seq_of_rank(const Seqs& q, int rank) {
     __shared__ int found;
     __shared__ int64_t lens[kThreads];
@@ -93,9 +94,10 @@ __device__ __forceinline__ f32x2 decay2(f32x2 dt, f32x2 A) { return exp2_2(fma2(
 __device__ __forceinline__ float decay(float dt, float A) { return exp2_fast(fmaf(dt, A, kLow)); }
 
 // ---- copies to shared memory ------------------------------------------------------
-// By the NT threads of the block: cnt (at most ROWS) rows of `width` (at most W) elements into rows of W, in chunks of
-// `cb` bytes that arrive asynchronously where the rows are aligned for them. Nothing
-// past the width or the count is read; there the tile stays as it was.
+// By the NT threads of the block: cnt (at most ROWS) rows of `width` (at most W) elements
+// into rows of W, in chunks of `cb` bytes that arrive asynchronously where the rows are
+// aligned for them. Nothing past the width or the count is read; there the tile stays as
+// it was.
 template <int ROWS, int W, int BYTES, int NT, typename T>
 __device__ __forceinline__ void stage_chunks(T* dst, const T* src, int64_t st, int cnt, int width) {
     constexpr int E = BYTES / (int)sizeof(T), PER = W / E;

@@ -162,8 +162,12 @@ struct GradSmem {
 //   h = a h' + b,  a = exp(dt A),  b = dt u B;   g = C dy + a' g'
 //   q = sum_n g B,  r = sum_n g a h' A:   du = q dt + D dy,  ddt = q u + r
 //   dB = sum_c g dt u,  dC = sum_c dy h,  dA = sum_t g a h' dt
-// Bound by the instructions issued (about 150 a lane for four states of a token) and by
-// their latencies: sixteen warps an SM at 128 registers.
+// Bound by the instructions issued (about 160 a warp for what the forward pass does in 42)
+// and by their latencies: sixteen warps an SM at 128 registers issue in half of the clocks.
+// 4 x 2048 tokens of 2048 channels and 16 states take 600 us, 0.45 T states a second. Run
+// backwards in time instead, a channel's states stored every tile and recomputed, it took
+// 170 instructions, at a quarter of the parallelism. Two channels a lane and eight warps
+// were as fast at twice the registers.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads, 2) scan_bwd(const __grid_constant__ GradP<T> p) {
     using M = GradSmem<T>;
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) scan_bwd(const __grid_constan
 
 // The first half of a backward pass split along the tokens: the adjoint state at a
 // piece's start that the piece's own tokens give, and its sum of dt. As scan_bwd, with
-// nothing but g's recurrence.
+// nothing but g's recurrence; half of scan_bwd's time for the same tokens.
 template <typename T>
 struct AdjSmem {
     static constexpr int NC = 16;
@@ -677,7 +681,7 @@ __global__ void __launch_bounds__(kThreads) adjoint_carry(const __grid_constant_
 }
 
 // dB and dC [row][G N] from the channel tiles' shares [tile][G N][row]: 32 rows by 32
-// columns a block, transposed in shared memory; blockIdx.z 0 is dB, 1 dC.
+// columns a block, transposed in shared memory; blockIdx.z 0 is dB, 1 dC. Bound by memory.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_tiles(const float* __restrict__ part, int ntile, int64_t rows, int cols,
                                                  T* dB, T* dC) {
@@ -706,8 +710,11 @@ __global__ void __launch_bounds__(256) sum_tiles(const float* __restrict__ part,
 // ---- host -------------------------------------------------------------------------
 // Tokens a piece of the backward pass; 0 = whole sequences. A block that has an SM to
 // itself leaves most of it idle, and the pass that finds the adjoint states between
-// pieces costs half as much as the pass itself: split where the sequences' blocks fill
-// less than 0.6 of the SMs, into as many pieces as two blocks an SM take.
+// pieces costs half as much as the pass itself: split where there are fewer blocks than
+// SMs, into as many pieces as two blocks an SM take. Forward and backward of a bf16
+// sequence with 16 states, split against whole: 1024 x 256 62 and 237 us, 4096 x 2048
+// 585 and 1028, 4096 x 4096 (128 blocks) 1107 and 1153; two blocks an SM and more give a
+// rule of this form one piece.
 int64_t grad_piece(const pe_scan_args* a) {
     const int64_t tiles = a->groups * ceil_div(a->channels / a->groups, CB), rows = a->cu ? 1 : a->nseq;
     const int64_t blocks = a->nseq * tiles;
