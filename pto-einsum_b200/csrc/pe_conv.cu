@@ -168,10 +168,12 @@ struct ConvGradP {
 // One thread does for its channels and tokens what each of the three results needs: the
 // slope of silu from the recomputed sum, dx from the window of g, the sums of dw and
 // dbias in registers to the end of the walk, then over the block's threads in order, and
-// over blocks by sum_rows. Bound by instructions at few warps: 4 x 2048 x 2048 f16 34 us,
-// 3.0 TB/s. Eight channels a thread and one block an SM beat four channels and two (51 us):
-// what a token costs beside its channels is paid half as often. Elements (V = 1), forward
-// and backward of 8000 x 2049 bf16: 174 us, 54 for x 2048 in 16-byte accesses.
+// over blocks by sum_rows. Bound by instructions at few warps: 4 x 2048 x 2048 f16 31 us,
+// 3.2 TB/s; 16384 x 4352 bf16 102 us, 4.2 TB/s. Eight channels a thread and one block an SM
+// beat four channels and two (51 us against 34 at the time): what a token costs beside its
+// channels is paid half as often. The tokens inside a tile have a loop without the ends'
+// conditions: 194 us with them for 16384 x 4352 and its forward pass, 179 without. Elements
+// (V = 1), forward and backward of 8000 x 2049 bf16: 124 us, 50 for x 2048 in 16-byte accesses.
 // Blocks an SM holds: by the registers of V channels' taps, sums and windows.
 __host__ __device__ constexpr int bwd_blocks(int v) { return v <= 4 ? 2 : 1; }
 
@@ -224,24 +226,27 @@ __global__ void __launch_bounds__(kBlock, bwd_blocks(V)) conv_bwd(const __grid_c
 #pragma unroll
                 for (int q = 0; q < Q; ++q) g[k][q] = 0;
             int slot = 0;
-#pragma unroll 4
-            for (int64_t k = t; k < last; ++k, ++slot, ++ahead) {
+            // EDGE false: a token of the tile and of the sequence whose g completes the dx of an
+            // input of the tile, which is none of the last state's
+            auto token = [&](int64_t k, auto edge) {
+                constexpr bool EDGE = decltype(edge)::value;
                 cp_wait_but<DEPTH - 2>();
                 widen<T, V>(rx.get(slot, xr + k * f.x_st), win[W - 1]);
                 widen<T, V>(ro.get(slot, dor + k * p.o_st), g[W - 1]);
                 rx.fetch(slot + DEPTH - 1, xr + ahead * f.x_st, ahead < have);
                 ro.fetch(slot + DEPTH - 1, dor + ahead * p.o_st, ahead < have);
                 cp_commit();
-                if (k < fin) {
+                ++slot;
+                ++ahead;
+                if (!EDGE || k < fin) {
                     if (f.silu) {
                         f32x2 a[Q];
                         flt.apply(win, a);
 #pragma unroll
-                        for (int q = 0; q < Q; ++q) {
+                        for (int q = 0; q < Q; ++q)
                             g[W - 1][q] = mul2(g[W - 1][q], silu_slope2(a[q], sigmoid2(a[q])));
-                        }
                     }
-                    if (k < stop) {   // the tile's own: into the sums
+                    if (!EDGE || k < stop) {   // the tile's own: into the sums
 #pragma unroll
                         for (int q = 0; q < Q; ++q) {
                             db[q] = add2(db[q], g[W - 1][q]);
@@ -263,19 +268,30 @@ __global__ void __launch_bounds__(kBlock, bwd_blocks(V)) conv_bwd(const __grid_c
                     for (int j = 1; j < W; ++j) d[q] = fma2(flt.w[W - 1 - j][q], g[j][q], d[q]);
                 }
                 shift(g);
-                const int64_t i0 = k - (W - 1), pos = i0 - sp.start;
-                const bool first = pos < 0 && t == sp.start && p.dinit;   // an input before the sequence
-                if (i0 < t && !first) continue;
-                const int64_t j = pos + W - 1 - sp.len;                    // its place in the last state
-                if (p.dstate && j >= 0) {
-                    f32x2 e[Q];
-                    widen<T, V>(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
+                const int64_t i0 = k - (W - 1);
+                T* to = dx + i0 * f.C;
+                if constexpr (EDGE) {
+                    const int64_t pos = i0 - sp.start;
+                    const bool first = pos < 0 && t == sp.start && p.dinit;   // an input before the sequence
+                    if (i0 < t && !first) return;
+                    const int64_t j = pos + W - 1 - sp.len;                    // its place in the last state
+                    if (p.dstate && j >= 0) {
+                        f32x2 e[Q];
+                        widen<T, V>(load_vec<T, V>(p.dstate + ((int64_t)s * (W - 1) + j) * f.C + c), e);
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) d[q] = add2(d[q], e[q]);
+                        for (int q = 0; q < Q; ++q) d[q] = add2(d[q], e[q]);
+                    }
+                    if (first) to = p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c;
                 }
-                T* to = first ? p.dinit + ((int64_t)s * (W - 1) + W - 1 + pos) * f.C + c : dx + i0 * f.C;
                 store_vec(to, narrow<T, V>(d));
-            }
+            };
+            int64_t k = t;
+#pragma unroll 1
+            for (const int64_t head = min(stop, t + W - 1); k < head; ++k) token(k, std::true_type());
+#pragma unroll(V == 1 ? 4 : 2)
+            for (; k < stop; ++k) token(k, std::false_type());
+#pragma unroll 1
+            for (; k < last; ++k) token(k, std::true_type());
             cp_wait();
             t = stop;
         }
@@ -403,28 +419,28 @@ ConvP<T> conv_params(const pe_conv_args* a, int v, int64_t tile) {
     return p;
 }
 
-// Tokens a thread walks: whole waves of the blocks an SM holds, at most 64 tokens each (the
-// W - 1 tokens read again, the filter and the filling of the queue weigh less on a longer
-// walk; a last wave that is not full costs as much as one that is), at least 4. by: a
-// block's threads along the tokens, where the block is laid out by channels. Forward
-// (with backward), bf16, by this rule, by 8, 64 and 256 tokens: 300 x 1024 6, 6, 17, 43
-// (19, 19, 49, 133) us; 8192 x 2048 17, 23, 21, 55 (54, 99, 63, 176); 16384 x 4352 56, 93,
-// 58, 62 (195, 391, 201, 185).
-int64_t tile_of(const pe_conv_args* a, int64_t columns, int resident, int by) {
+// Tokens a thread walks: whole waves of the blocks an SM holds, at most `most` tokens each
+// (the W - 1 tokens read again, the filter and the filling of the queue weigh less on a
+// longer walk, the backward pass's sums too; a last wave that is not full costs as much as
+// one that is), at least 4. by: a block's threads along the tokens, where the block is laid
+// out by channels. Forward, bf16, by this rule (at most 64), by 8, 64 and 256 tokens:
+// 300 x 1024 6, 6, 17, 43 us; 8192 x 2048 17, 23, 21, 55; 16384 x 4352 56, 93, 58, 62. With the
+// backward pass (at most 256): 17, 19, 46, 109; 50, 99, 55, 155; 158, 388, 183, 165.
+int64_t tile_of(const pe_conv_args* a, int64_t columns, int resident, int by, int64_t most) {
     const int64_t rows = a->batch, slots = (int64_t)num_sms() * resident, threads = slots * kBlock;
-    const int64_t cells = a->tokens * rows * columns, waves = ceil_div(cells, 64 * threads);
+    const int64_t cells = a->tokens * rows * columns, waves = ceil_div(cells, most * threads);
     if (!waves) return 4;
     int64_t tile = ceil_div(cells, waves * threads);
     if (by > 1) {   // blocks are whole: lengthen the walk until they fit
         const int64_t per = ceil_div(columns, kBlock / by);
-        while (tile < 64 && ceil_div(ceil_div(a->tokens, tile) * rows, by) * per > waves * slots) ++tile;
+        while (tile < most && ceil_div(ceil_div(a->tokens, tile) * rows, by) * per > waves * slots) ++tile;
     }
     return tile < 4 ? 4 : tile;
 }
 
 template <typename T, int W, int V>
 int conv_run(const pe_conv_args* a, cudaStream_t s) {
-    const ConvP<T> p = conv_params<T>(a, V, tile_of(a, a->channels / V, 2, 1));
+    const ConvP<T> p = conv_params<T>(a, V, tile_of(a, a->channels / V, 2, 1, 64));
     const int64_t ids = (p.tiles + (p.state ? a->nseq : 0)) * p.CV, blocks = ceil_div(ids, kBlock);
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     if (!blocks) return PE_OK;
@@ -441,7 +457,7 @@ ConvGradShape grad_shape(const pe_conv_args* a, int v) {
     const int64_t cv = a->channels / v;
     ConvGradShape g{1, 4, 0};
     while (g.bx < 32 && g.bx < cv) g.bx *= 2;
-    g.tile = tile_of(a, cv, bwd_blocks(v), kBlock / g.bx);
+    g.tile = tile_of(a, cv, bwd_blocks(v), kBlock / g.bx, 256);
     g.rows = ceil_div(ceil_div(a->tokens, g.tile) * a->batch, kBlock / g.bx);
     return g;
 }
