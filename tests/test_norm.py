@@ -115,6 +115,16 @@ def test_forward_and_gradients(shape, groups, layout, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", [
+    ((640, 26000), 1), ((310, 26001), 1),                         # rows that share their sums' places in memory
+    ((310, 8192), 1), ((700, 4104), 8),                           # and in shared memory
+    ((40, 256, 1280), 32), ((8, 2100, 320), 32), ((2, 20000, 64), 4)])   # chunks in several waves
+def test_many_rows_and_chunks(shape, groups, dt):
+    test_forward_and_gradients(shape, groups, "plain", dt)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape,groups", [((40, 64), 4), ((2, 3000, 64), 4)])
 def test_gradients_against_differences(shape, groups):
     x, w, b, z = inputs(shape, F32)
