@@ -471,83 +471,109 @@ __device__ __forceinline__ void load_cols8(const T* p, float (&f)[8]) {
     }
 }
 
-// A lane has eight states of one channel, LPC lanes a channel, of one request. Bound by
+// A lane has eight states of one channel, LPC lanes a channel, for RB requests: A is read
+// once for them, and all their states are on the way before the first is used. Bound by
 // memory: the states, 8 bytes a (request, channel, state). Fewer states a lane repeat
 // what the channel needs (softplus, gate, loads) on more lanes (four states a lane: 43 us a
-// call, eight 29, of which the kernel has 25, 5.4 TB/s of states, for 256 requests of 4096
-// channels and 16 states);
-// 256-bit accesses let eight be one sector each. VEC against elements: 200 requests of
-// 2048 x 32 and of 2049 x 31 states 21 and 54 us. Two requests a thread, sharing A, were
-// no faster.
-template <typename T, int LPC, bool VEC>
+// call, eight 29, of which the kernel has 23, 5.9 TB/s of states, for 256 requests of 4096
+// channels and 16 states); 256-bit accesses let eight be one sector each. VEC against
+// elements: 200 requests of 2048 x 32 and of 2049 x 31 states 21 and 54 us.
+template <typename T, int LPC, int RB, bool VEC>
 __global__ void __launch_bounds__(kThreads) scan_step(const __grid_constant__ StepP<T> p) {
     constexpr int CH = kThreads / LPC, NS = 8;
     const int tid = threadIdx.x, q = tid % LPC, n0 = NS * q;
     const int c = blockIdx.x * CH + tid / LPC;
     const bool live = c < p.D, some = live && n0 < p.N;
-    const int64_t b = blockIdx.y, cn = (int64_t)c * p.N + n0;
+    const int64_t b0 = (int64_t)blockIdx.y * RB, cn = (int64_t)c * p.N + n0;
     const int nn = some ? min(NS, p.N - n0) : 0;   // this lane's states
+    float h[RB][NS], B[RB][NS], C[RB][NS], A[NS], u[RB], dt[RB], z[RB];
+    float* hp[RB];
     const int g = live ? c / p.Dg : 0;
-    int64_t slot = p.s32 ? (int64_t)__ldg(p.s32 + b) : p.s64 ? __ldg(p.s64 + b) : b;
-    if (slot >= p.slots) {
-        if (blockIdx.x == 0 && tid == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
-        slot = -1;
-    }
-    float* hp = slot >= 0 ? p.state + slot * p.D * p.N + cn : nullptr;
-    const bool on = hp && live;
-    float h[NS], A[NS], B[NS], C[NS];
+    const int rows = (int)min((int64_t)RB, p.batch - b0);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) h[i] = A[i] = B[i] = C[i] = 0.0f;
-    const T* Bp = p.B + b * p.B_sb + g * p.B_sg + n0;
-    const T* Cp = p.C + b * p.C_sb + g * p.C_sg + n0;
+    for (int r = 0; r < RB; ++r) {
+        int64_t slot = -1;
+        if (r < rows) {
+            const int64_t b = b0 + r;
+            slot = p.s32 ? (int64_t)__ldg(p.s32 + b) : p.s64 ? __ldg(p.s64 + b) : b;
+            if (slot >= p.slots) {
+                if (blockIdx.x == 0 && tid == 0) record_error(PE_ERR_INVALID | (kSiteSlot << 8));
+                slot = -1;
+            }
+        }
+        hp[r] = slot >= 0 ? p.state + slot * p.D * p.N + cn : nullptr;
+    }
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) h[r][i] = 0.0f;
+        if (VEC) {
+            if (hp[r] && some) load8(hp[r], h[r]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (hp[r] && i < nn) h[r][i] = hp[r][i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) A[i] = 0.0f;
     if (VEC) {
-        if (hp && some) load8(hp, h);
         if (some) load_cols8(p.A + cn, A);
     } else {
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (hp && i < nn) h[i] = hp[i];
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             if (i < nn) A[i] = __ldg(p.A + cn + i);
     }
     const float bias = live && p.bias ? __ldg(p.bias + c) : 0.0f, Dw = live && p.Dw ? __ldg(p.Dw + c) : 0.0f;
-    const float u = on ? to_float(load_one(p.u + b * p.u_sb + c)) : 0.0f;
-    const float dt = on ? to_float(load_one(p.delta + b * p.d_sb + c)) + bias : 0.0f;
-    const float z = on && p.z ? to_float(load_one(p.z + b * p.z_sb + c)) : 0.0f;
-    if (VEC) {
-        if (on && some) {
-            load_cols8(Bp, B);
-            load_cols8(Cp, C);
-        }
-    } else {
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (on && i < nn) {
-                B[i] = to_float(load_one(Bp + i));
-                C[i] = to_float(load_one(Cp + i));
+    for (int r = 0; r < RB; ++r) {
+        const int64_t b = b0 + r;
+        const bool on = hp[r] && live;
+        u[r] = on ? to_float(load_one(p.u + b * p.u_sb + c)) : 0.0f;
+        dt[r] = on ? to_float(load_one(p.delta + b * p.d_sb + c)) + bias : 0.0f;
+        z[r] = on && p.z ? to_float(load_one(p.z + b * p.z_sb + c)) : 0.0f;
+        const T* Bp = p.B + b * p.B_sb + g * p.B_sg + n0;
+        const T* Cp = p.C + b * p.C_sb + g * p.C_sg + n0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) B[r][i] = C[r][i] = 0.0f;
+        if (VEC) {
+            if (on && some) {
+                load_cols8(Bp, B[r]);
+                load_cols8(Cp, C[r]);
             }
-    }
-    const float d = p.softplus ? softplusf(dt) : dt, x = d * u, dl = d * kLog2e;
-    float y = 0.0f;
+        } else {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        h[i] = fmaf(decay(dl, A[i]), h[i], x * B[i]);
-        y = fmaf(C[i], h[i], y);
-    }
-    if (VEC) {
-        if (hp && some) store8(hp, h);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (hp && i < nn) hp[i] = h[i];
+            for (int i = 0; i < NS; ++i)
+                if (on && i < nn) {
+                    B[r][i] = to_float(load_one(Bp + i));
+                    C[r][i] = to_float(load_one(Cp + i));
+                }
+        }
     }
 #pragma unroll
-    for (int m = LPC / 2; m >= 1; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
-    if (live && q == 0) {
-        y = fmaf(Dw, u, y);
-        if (p.z) y *= z * sigmoidf(z);
-        p.out[b * p.D + c] = from_float<T>(hp ? y : 0.0f);
+    for (int r = 0; r < RB; ++r) {
+        if (r >= rows) break;
+        const float d = p.softplus ? softplusf(dt[r]) : dt[r], x = d * u[r], dl = d * kLog2e;
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            h[r][i] = fmaf(decay(dl, A[i]), h[r][i], x * B[r][i]);
+            y = fmaf(C[r][i], h[r][i], y);
+        }
+        if (VEC) {
+            if (hp[r] && some) store8(hp[r], h[r]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (hp[r] && i < nn) hp[r][i] = h[r][i];
+        }
+#pragma unroll
+        for (int m = LPC / 2; m >= 1; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
+        if (live && q == 0) {
+            y = fmaf(Dw, u[r], y);
+            if (p.z) y *= z[r] * sigmoidf(z[r]);
+            p.out[(b0 + r) * p.D + c] = from_float<T>(hp[r] ? y : 0.0f);
+        }
     }
 }
 
@@ -650,11 +676,19 @@ int step_run(const pe_scan_step_args* a, cudaStream_t s) {
     const bool vec = p.N % 8 == 0 && (uintptr_t)p.state % 32 == 0 &&
                      ((uintptr_t)p.A | (uintptr_t)p.B | (uintptr_t)p.C) % 16 == 0 &&
                      (p.B_sb % e | p.B_sg % e | p.C_sb % e | p.C_sg % e) == 0;
-    const dim3 grid((unsigned)tiles, (unsigned)a->batch);
-    if (vec)
-        scan_step<T, LPC, true><<<grid, kThreads, 0, s>>>(p);
+    // two requests a thread once that still gives every SM its 16 blocks: fp16, 16 states, two
+    // against one, 256 x 4096 22.8 and 25.0 us, 512 x 4096 51.6 and 56.0; 64 x 2048, below the
+    // rule, 6.4 both
+    const bool two = tiles * a->batch >= 32ll * num_sms();
+    const dim3 grid((unsigned)tiles, (unsigned)(two ? ceil_div(a->batch, 2) : a->batch));
+    if (vec && two)
+        scan_step<T, LPC, 2, true><<<grid, kThreads, 0, s>>>(p);
+    else if (two)
+        scan_step<T, LPC, 2, false><<<grid, kThreads, 0, s>>>(p);
+    else if (vec)
+        scan_step<T, LPC, 1, true><<<grid, kThreads, 0, s>>>(p);
     else
-        scan_step<T, LPC, false><<<grid, kThreads, 0, s>>>(p);
+        scan_step<T, LPC, 1, false><<<grid, kThreads, 0, s>>>(p);
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PE_OK : PE_ERR_CUDA;
 }
