@@ -8,8 +8,8 @@ namespace {
 constexpr int K = 8;         // tokens a lane
 constexpr int SEG = K + 4;   // a lane's K tokens in a shared row: float4 reads of eight lanes fall on
                              // all banks once
-// A warp takes 32 / LT channel pairs and LT K consecutive tokens, a lane one pair's K
-// tokens; the block's warps have other channels and the same tokens.
+// A warp takes LT K consecutive tokens, a lane K of them, for 32 / LT channels (scan_bwd) or
+// channel pairs (scan_adjoint); the block's warps have other channels and the same tokens.
 template <int LT>
 struct Tile {
     static constexpr int TT = LT * K;                 // tokens
@@ -67,10 +67,10 @@ __device__ __forceinline__ f32x2 shfl2_down(f32x2 v, int d, int width) {
     return pack2(__shfl_down_sync(0xffffffffu, lo, d, width), __shfl_down_sync(0xffffffffu, hi, d, width));
 }
 
-// What the lanes of a channel pair do to the adjoint state, composed from the last token
-// to the first. Lane tl maps the state after it, g, to P g + H (both channels at once).
-// Returns the state after the lane, and in `last` the state before lane 0, given the
-// state `h0` after the last lane.
+// What the lanes of a channel (or of a pair, both at once) do to the adjoint state, composed
+// from the last token to the first. Lane tl maps the state after it, g, to P g + H. Returns
+// the state after the lane, and in `last` the state before lane 0, given the state `h0`
+// after the last lane.
 template <int LT>
 __device__ __forceinline__ f32x2 scan_lanes_down(f32x2 P, f32x2 H, f32x2 h0, int tl, f32x2& last) {
     if (tl == LT - 1) H = fma2(P, h0, H);
