@@ -1073,6 +1073,9 @@ int check_norm(const pe_norm_args* a) {
     return PE_OK;
 }
 
+// Nothing to normalise, and nothing that plan_of could divide into rows and chunks.
+bool empty(const pe_norm_args* a) { return a->batch == 0 || a->places == 0; }
+
 // Elements a load: 16 bytes where all rows start on that boundary, else one (8000 gated
 // rows of 8 groups, 4096 and 4008 bf16 channels, groups of 501: 43 and 197 us forward).
 int vec_of(const pe_norm_args* a, std::initializer_list<const void*> more, std::initializer_list<int64_t> strides) {
@@ -1385,7 +1388,7 @@ Plan grad_plan(const pe_norm_grad_args* g) {
 }  // namespace
 
 int64_t norm_ws_bytes(const pe_norm_args* a) {
-    if (check_norm(a) != PE_OK) return 0;
+    if (check_norm(a) != PE_OK || empty(a)) return 0;
     // enough for either width of the loads: the size does not depend on addresses
     const int64_t x = stats_floats(a, plan_of(a, 1, false)), y = stats_floats(a, plan_of(a, widest(a), false));
     return (x > y ? x : y) * 4;
@@ -1393,7 +1396,7 @@ int64_t norm_ws_bytes(const pe_norm_args* a) {
 
 int group_norm(const pe_norm_args* a, cudaStream_t s) {
     if (int rc = check_norm(a)) return rc;
-    if (a->batch == 0 || a->places == 0) return PE_OK;
+    if (empty(a)) return PE_OK;
     if (!a->out || !a->mean != !a->rstd) return PE_ERR_INVALID;
     const Plan pl = plan_of(a, vec_of(a, {}, {}), false);
     const int64_t need = stats_floats(a, pl) * 4;
@@ -1402,7 +1405,7 @@ int group_norm(const pe_norm_args* a, cudaStream_t s) {
 }
 
 int64_t norm_grad_ws_bytes(const pe_norm_grad_args* g) {
-    if (!g || check_norm(&g->fwd) != PE_OK) return 0;
+    if (!g || check_norm(&g->fwd) != PE_OK || empty(&g->fwd)) return 0;
     const pe_norm_args* a = &g->fwd;
     const int64_t x = grad_floats(a, plan_of(a, 1, true)), y = grad_floats(a, plan_of(a, widest(a), true));
     return (x > y ? x : y) * 4;
@@ -1412,7 +1415,7 @@ int group_norm_grad(const pe_norm_grad_args* g, cudaStream_t s) {
     if (!g) return PE_ERR_INVALID;
     const pe_norm_args* a = &g->fwd;
     if (int rc = check_norm(a)) return rc;
-    if (a->batch == 0 || a->places == 0) {
+    if (empty(a)) {
         const SumJob none[2] = {{nullptr, 0, a->channels, (int)a->dtype, g->dweight},
                                 {nullptr, 0, a->channels, (int)a->dtype, g->dbias}};
         return sum_rows(none, 2, s);

@@ -1,0 +1,49 @@
+"""The recurrent-mixer operators called in other ways than the plain one: empty tensors, states that
+change in place, derivatives of other kinds, arguments at the ends of their range, the C entries."""
+import ctypes
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from pto_einsum import _ops, norm
+from pto_einsum.norm import group_norm
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def rand(*shape, seed, dtype=F32, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(dtype).to(device)
+
+
+# ---------------------------------------------------------------------------- empty tensors
+def norm_grad_ws_bytes(N, places, C, groups, dtype):
+    args = norm._NORM_GRAD.pack(dtype, 0, N, places, C, groups, 1e-5, *[0] * (len(norm._NORM_GRAD.unpack(
+        bytes(norm._NORM_GRAD.size))) - 7))
+    return _ops.function("pe_group_norm_grad_ws_bytes", ctypes.c_int64, (ctypes.c_char_p,))(args)
+
+
+EMPTY = [(1000, 0, 64, 4), (2, 0, 4096, 1), (0, 7, 64, 4)]
+
+
+def test_workspaces_of_empty_norms():
+    """In a process of its own: a host that divides by the places of a row ends."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import sys; sys.path[:0] = [%r, %r]\nfrom test_operator_calls import *\n"
+            "assert [norm_grad_ws_bytes(*e, dt) for e in EMPTY for dt in (0, 1, 2)] == [0] * 9"
+            % (here, os.path.join(os.path.dirname(here), "pto-einsum_b200")))
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,places,C,groups", EMPTY)
+def test_gradients_of_empty_norms(N, places, C, groups):
+    x, w = rand(N, places, C, seed=1).requires_grad_(), rand(C, seed=2).requires_grad_()
+    b = rand(C, seed=3).requires_grad_()
+    y = group_norm(x, groups, w, b, activation="silu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+    assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
