@@ -720,6 +720,7 @@ int64_t scan_ws_bytes(const pe_scan_args* a) {
 int selective_scan(const pe_scan_args* a, cudaStream_t s) {
     if (int rc = check_scan(a)) return rc;
     if (a->nseq == 0) return PE_OK;
+    if (a->tokens && !a->out) return PE_ERR_INVALID;
     const int64_t need = scan_ws_bytes(a);
     if (need && (!a->ws || a->ws_bytes < need)) return PE_ERR_WORKSPACE;
     return scan_any(a, s);

@@ -8,7 +8,7 @@ import sys
 import pytest
 import torch
 
-from pto_einsum import _ops, norm
+from pto_einsum import _core, _ops, norm, ssm
 from pto_einsum.norm import group_norm
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -47,3 +47,15 @@ def test_gradients_of_empty_norms(N, places, C, groups):
     y = group_norm(x, groups, w, b, activation="silu")
     dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
     assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
+
+
+# ---------------------------------------------------------------------------- the C entries
+def test_a_scan_without_a_place_for_its_output_is_refused():
+    """The arguments are checked before anything is launched: no address here is ever used."""
+    some = 4096
+    args = dict(zip(("dtype", "softplus", "batch", "tokens", "channels", "states", "groups", "nseq"),
+                    (1, 1, 2, 10, 16, 16, 1, 2)))
+    fields = [*args.values(), 0, some, some, 0, some, some, some, 0, 0, 0, 160, 16, 160, 16, 0, 0, 160, 16, 16, 160, 16, 16]
+    call = _ops.function("pe_selective_scan")
+    assert call(ssm._SCAN.pack(*fields, 0, 0, 0, 0, 0), None) == 1
+    assert _core.core_lib().pe_last_error() == 1
