@@ -28,7 +28,7 @@ struct ScanP {
     // copies to shared memory: rows of these tensors in chunks (see chunk_of), 0 = element by element
     int u_cb, d_cb, z_cb, B_cb, C_cb;
     bool fast, chunks;    // all of them in chunks of 16; of 8 or 16
-    bool pairs;           // out's rows take aligned pairs of elements
+    bool pairs;           // the results' rows take aligned pairs of elements
     bool longest_first;   // packed sequences are taken in the order of their lengths
     int64_t piece;        // tokens a piece (a multiple of KCK, or more than any sequence has)
     float *hloc, *dtsum;  // ws of a split scan: each piece's own last state and sum of dt
@@ -206,7 +206,7 @@ ScanP<T> scan_params(const pe_scan_args* a, int ch, int nc) {
     p.C_cb = chunk_of(p.C, es, cols, {p.C_sb, p.C_st, p.C_sg}, nc);
     p.fast = p.u_cb == 16 && p.d_cb == 16 && (!p.z || p.z_cb == 16) && p.B_cb == 16 && p.C_cb == 16;
     p.chunks = p.u_cb && p.d_cb && (!p.z || p.z_cb) && p.B_cb && p.C_cb;
-    p.pairs = p.Dg % 2 == 0;
+    p.pairs = p.Dg % 2 == 0 && (uintptr_t)p.out % (2 * es) == 0;
     return p;
 }
 

@@ -755,6 +755,8 @@ int grad_type(const pe_scan_grad_args* a, cudaStream_t s) {
     p.dstate = a->dstate;
     p.du = (T*)a->du; p.ddelta = (T*)a->ddelta; p.dz = (T*)a->dz;
     p.dh0 = a->dh0;
+    p.f.pairs = p.f.Dg % 2 == 0 &&
+                ((uintptr_t)p.du | (uintptr_t)p.ddelta | (uintptr_t)p.dz) % (2 * sizeof(T)) == 0;
     p.pBC = ws + w.bc; p.pA = ws + w.a; p.pD = ws + w.d; p.pb = ws + w.b;
     p.gloc = p.dtsum = nullptr;
     unsigned grid;

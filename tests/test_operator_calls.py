@@ -10,6 +10,7 @@ import torch
 
 from pto_einsum import _core, _ops, norm, ssm
 from pto_einsum.norm import group_norm
+from pto_einsum.ssm import selective_scan
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -59,3 +60,39 @@ def test_a_scan_without_a_place_for_its_output_is_refused():
     call = _ops.function("pe_selective_scan")
     assert call(ssm._SCAN.pack(*fields, 0, 0, 0, 0, 0), None) == 1
     assert _core.core_lib().pe_last_error() == 1
+
+
+def scan_inputs(B, T, D, N, dt=F32):
+    return dict(u=rand(B, T, D, seed=1, dtype=dt), delta=rand(B, T, D, seed=2, dtype=dt), A=-torch.exp(rand(D, N, seed=3)),
+                B=rand(B, T, 1, N, seed=4, dtype=dt), C=rand(B, T, 1, N, seed=5, dtype=dt), D=rand(D, seed=6),
+                z=rand(B, T, D, seed=7, dtype=dt), delta_bias=rand(D, seed=8) - 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_scan_results_at_any_element(dt):
+    """Results one element past an aligned address, which a caller of the C entries may choose."""
+    B, T, D, N = 2, 70, 48, 16
+    k = scan_inputs(B, T, D, N, dt)
+    own = {m: t.clone().requires_grad_() for m, t in k.items()}
+    y = selective_scan(**own, delta_softplus=True)
+    dy = rand(B, T, D, seed=9, dtype=dt)
+    want = torch.autograd.grad(y, list(own.values()), dy)
+    off = {m: torch.empty(B * T * D + 1, dtype=dt, device="cuda")[1:].view(B, T, D) for m in ("out", "u", "delta", "z")}
+    rest = {m: torch.empty_like(k[m]) for m in ("A", "B", "C", "D", "delta_bias")}
+    lay = ssm._scan_layout(*(k[m] for m in ("u", "delta", "A", "B", "C", "z")), B, 1)
+    ckpt = torch.empty(ssm._core_ckpt(T, B, False, D, N), device="cuda")
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+
+    def fields(out):
+        return ssm._scan_fields(lay, *(k[m] for m in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")), None,
+                                None, out, None, ckpt)
+
+    _ops.call("pe_selective_scan", ssm._SCAN.pack(*fields(off["out"]), ws.data_ptr(), ws.numel()), 0)
+    assert torch.equal(off["out"], y)
+    _ops.call("pe_selective_scan_grad", ssm._SCAN_GRAD.pack(
+        *fields(None), 0, 0, dy.data_ptr(), *dy.stride()[:2], 0,
+        *(t.data_ptr() for t in (off["u"], off["delta"], off["z"], rest["B"], rest["C"], rest["A"], rest["D"],
+                                 rest["delta_bias"])), 0, ws.data_ptr(), ws.numel()), 0)
+    for m, g in zip(own, want):
+        assert torch.equal(off[m] if m in off else rest[m], g), m
