@@ -1381,8 +1381,9 @@ int norm_grad_any(const pe_norm_grad_args* a, const Plan& pl, cudaStream_t s) {
     PE_NORM_T(norm_grad_run, a->fwd.dtype, pl.v, a, pl, s)
 }
 
+// ws: norm_wide_bwd keeps sums in it that it reads and writes in vectors.
 Plan grad_plan(const pe_norm_grad_args* g) {
-    return plan_of(&g->fwd, vec_of(&g->fwd, {g->dout, g->dx, g->dgate}, {g->dout_sb, g->dout_sp}), true);
+    return plan_of(&g->fwd, vec_of(&g->fwd, {g->dout, g->dx, g->dgate, g->ws}, {g->dout_sb, g->dout_sp}), true);
 }
 
 }  // namespace

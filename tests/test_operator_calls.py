@@ -96,3 +96,35 @@ def test_scan_results_at_any_element(dt):
                                  rest["delta_bias"])), 0, ws.data_ptr(), ws.numel()), 0)
     for m, g in zip(own, want):
         assert torch.equal(off[m] if m in off else rest[m], g), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", [((700, 26000), 1), ((300, 4096), 8), ((4, 3000, 320), 32)])
+def test_norm_gradients_with_a_workspace_at_any_float(shape, groups, dt):
+    N, C = shape[0], shape[-1]
+    t = [rand(*shape, seed=1, dtype=dt), rand(C, seed=2, dtype=dt), rand(C, seed=3, dtype=dt)]
+    own = [v.clone().requires_grad_() for v in t]
+    y = group_norm(own[0], groups, own[1], own[2], activation="silu")
+    dy = rand(*shape, seed=4, dtype=dt)
+    want = torch.autograd.grad(y, own, dy)
+    places = shape[1] if len(shape) > 2 else 1
+    stats = torch.empty(2, N, groups, device="cuda")
+    lay = ((norm.DTYPES[dt], 1, N, places, C, groups, 1e-5), (*norm._strides(t[0]), 0, 0), 0)
+    got = [torch.empty_like(v) for v in t]
+    out = torch.empty_like(t[0])
+
+    def call(name, pack, tail, out):
+        fields = (*norm._fields(lay, *t, None, out, stats), *tail)
+        n = _ops.sized(name + "_ws_bytes", pack(*fields, 0, 0), 0)
+        ws = torch.empty(n // 4 + 1, device="cuda")[1:]
+        _ops.call(name, pack(*fields, ws.data_ptr(), n), 0)
+
+    call("pe_group_norm", norm._NORM.pack, (), out)
+    call("pe_group_norm_grad", norm._NORM_GRAD.pack, (0, 0, dy.data_ptr(), *norm._strides(dy), got[0].data_ptr(), 0,
+                                                      got[1].data_ptr(), got[2].data_ptr()), None)
+    # the same sums in another order: a few fp32 roundings, then one to the type
+    assert torch.equal(out, y)
+    for g, h in zip(got, want):
+        off = (g.double() - h.double()).norm() / h.double().norm()
+        assert off <= 2 * torch.finfo(dt).eps + 2.0 ** -18, off
