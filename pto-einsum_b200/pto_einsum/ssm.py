@@ -32,6 +32,7 @@ import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _ops
 from ._ops import (DTYPES, call, check_activations, check_tensor, offsets, packer, plan, ptr, rows, sig, stride,
@@ -180,6 +181,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     call("pe_causal_conv_step", _CONV_STEP.pack(
         *ints[:6], s32, s64, x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), ints[6],
         state.data_ptr(), out.data_ptr()), ints[7])
+    increment_version(state)   # autograd sees the kernel's writes as its own in-place operations
     return out
 
 
@@ -269,20 +271,22 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, u, delta, A, B, C, D, z, bias, h0, cu, lay, want_state):
         ctx.set_materialize_grads(False)
         out, state, ckpt = _scan_forward(lay, u, delta, A, B, C, D, z, bias, h0, cu, want_state, True)
-        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, h0, cu, ckpt)
-        ctx.lay = lay
+        # not h0: its values are in the checkpoints, and a decode step may go on in its place
+        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, cu, ckpt)
+        ctx.lay, ctx.has_h0 = lay, h0 is not None
         return (out, state) if want_state else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dstate=None):
-        u, delta, A, B, C, D, z, bias, h0, cu, ckpt = ctx.saved_tensors
+        u, delta, A, B, C, D, z, bias, cu, ckpt = ctx.saved_tensors
         lay, dev, dt = ctx.lay, u.device, u.dtype
         dout = torch.zeros(u.shape, dtype=dt, device=dev) if dout is None else rows(dout)
         dstate = _opt(dstate, torch.Tensor.contiguous)
 
-        du, ddelta, dz, dB, dC, dA, dD, dbias, dh0 = [_opt(t, _ops.empty) for t in (u, delta, z, B, C, A, D, bias, h0)]
-        fields = (*_scan_fields(lay, u, delta, A, B, C, D, z, bias, h0, cu, None, None, ckpt), 0, 0,
+        du, ddelta, dz, dB, dC, dA, dD, dbias = [_opt(t, _ops.empty) for t in (u, delta, z, B, C, A, D, bias)]
+        dh0 = torch.empty((lay[0][7], *A.shape), dtype=torch.float32, device=dev) if ctx.has_h0 else None
+        fields = (*_scan_fields(lay, u, delta, A, B, C, D, z, bias, None, cu, None, None, ckpt), 0, 0,
                   dout.data_ptr(), stride(dout, 0), stride(dout, 1), ptr(dstate), ptr(du), ptr(ddelta), ptr(dz),
                   ptr(dB), ptr(dC), ptr(dA), ptr(dD), ptr(dbias), ptr(dh0))
         nbytes = _ops.nbytes_of("pe_scan_grad_ws_bytes", (lay[0] + (cu is None,), 0, lay[2]),
@@ -368,6 +372,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
         *ints[0], s32, s64, u.data_ptr(), delta.data_ptr(), 0 if z is None else z.data_ptr(), B.data_ptr(),
         C.data_ptr(), A.data_ptr(), 0 if D is None else D.data_ptr(),
         0 if delta_bias is None else delta_bias.data_ptr(), *ints[1], state.data_ptr(), out.data_ptr()), ints[2])
+    increment_version(state)
     return out
 
 

@@ -10,7 +10,7 @@ import torch
 
 from pto_einsum import _core, _ops, norm, ssm
 from pto_einsum.norm import group_norm
-from pto_einsum.ssm import selective_scan
+from pto_einsum.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -128,3 +128,43 @@ def test_norm_gradients_with_a_workspace_at_any_float(shape, groups, dt):
     for g, h in zip(got, want):
         off = (g.double() - h.double()).norm() / h.double().norm()
         assert off <= 2 * torch.finfo(dt).eps + 2.0 ** -18, off
+
+
+# ---------------------------------------------------------------------------- states in place
+def token(k, t):
+    return {m: v[:, t] if m in ("u", "delta", "B", "C", "z") else v for m, v in k.items()}
+
+
+@pytest.mark.gpu
+def test_a_state_that_a_gradient_still_needs():
+    """The steps write through the state's address; autograd has to know."""
+    x, w, s = rand(2, 9, 16, seed=1), rand(16, 4, seed=2).requires_grad_(), rand(2, 3, 16, seed=3)
+    y = causal_conv(x, w, initial_state=s)
+    with torch.no_grad():
+        causal_conv_step(x[:, 0], s, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    k, s = scan_inputs(2, 3, 16, 16), rand(2, 16, 16, seed=9)
+    y = (rand(2, 16, 16, seed=10).requires_grad_() * s).sum()
+    with torch.no_grad():
+        selective_scan_step(s, **token(k, 0), delta_softplus=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        s = torch.zeros(2, 16, 16, device="cuda")
+        selective_scan_step(s, **token(k, 0), delta_softplus=True)
+
+
+@pytest.mark.gpu
+def test_scan_gradients_after_the_first_state_went_on():
+    """The scan's backward pass starts from its checkpoints: the state itself may be used again."""
+    k, got = scan_inputs(2, 9, 16, 16), []
+    for change in (False, True):
+        s = rand(2, 16, 16, seed=9)
+        own = {m: t.clone().requires_grad_() for m, t in k.items()}
+        y = selective_scan(**own, initial_state=s, delta_softplus=True)
+        if change:
+            with torch.no_grad():
+                selective_scan_step(s, **token(k, 0), delta_softplus=True)
+        got.append(torch.autograd.grad(y.sum(), list(own.values())))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
