@@ -6,6 +6,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from ._core import core_lib, error_string
 from .builder import _raw_stream_getter
@@ -184,8 +185,14 @@ def slot_pointers(slots):
 
 
 def wants_grad(*tensors) -> bool:
+    """Whether autograd has to see the call: gradients are recorded for an input, or one
+    carries a tangent (forward mode, which no_grad leaves on)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) >= 0:   # inside dual_level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
     return False

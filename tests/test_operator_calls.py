@@ -7,6 +7,7 @@ import sys
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from pto_einsum import _core, _ops, norm, ssm
 from pto_einsum.norm import group_norm
@@ -168,3 +169,27 @@ def test_scan_gradients_after_the_first_state_went_on():
                 selective_scan_step(s, **token(k, 0), delta_softplus=True)
         got.append(torch.autograd.grad(y.sum(), list(own.values())))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ---------------------------------------------------------------------------- other derivatives
+def test_tangents_are_seen():
+    x = torch.ones(3)
+    assert not _ops.wants_grad(x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        with torch.no_grad():
+            assert _ops.wants_grad(None, x, dual) and not _ops.wants_grad(x, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_derivatives_are_refused(grad):
+    """The operators have none: torch's error for that, not an output without a tangent."""
+    x, w, k = rand(2, 9, 16, seed=1), rand(16, 4, seed=2), scan_inputs(2, 9, 16, 16)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: causal_conv(dual, w), lambda: selective_scan(**{**k, "u": dual}, delta_softplus=True),
+                  lambda: group_norm(dual, 4), lambda: group_norm(x, 4, gate=dual)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                f()
+        causal_conv(x, w)
