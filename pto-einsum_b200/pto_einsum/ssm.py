@@ -155,7 +155,8 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
 
     state [S, W - 1, C] (contiguous, x's type) is shifted in place: row slots[b] of it
     belongs to request b (row b without slots, S = B). Rows with a negative slot give 0
-    and touch no state; two requests must not share a slot."""
+    and touch no state; two requests must not share a slot. There is no gradient: inputs
+    that require one are refused outside torch.no_grad()."""
     try:
         key = ("conv step", activation, sig(x), sig(state), sig(weight), sig(bias), sig(slots))
         ints = plan(key)
@@ -175,7 +176,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
         ints = (DTYPES[x.dtype], silu, W, B, C, state.shape[0], stride(x, 0), x.device.index)
         if key is not None:
             _ops.keep_plan(key, ints)
-    _no_grad_state(state)
+    _no_gradients("causal_conv_step", state, x, weight, bias)
     out = _ops.empty(x)
     s32, s64 = _ops.slot_pointers(slots)
     call("pe_causal_conv_step", _CONV_STEP.pack(
@@ -185,9 +186,11 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     return out
 
 
-def _no_grad_state(state):
+def _no_gradients(name, state, *inputs):
     if state.requires_grad and torch.is_grad_enabled():
         raise ValueError("state is updated in place and cannot require a gradient")
+    if wants_grad(state, *inputs):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or the prompt form on one token")
 
 
 def _check_state(name, state, dtype, dev, tail, batch, slots):
@@ -340,7 +343,8 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
 
     state [S, Dc, N] float32 (contiguous) is updated in place, in row slots[b] for
     request b (row b without slots, S = Bt). Rows with a negative slot give 0 and touch
-    no state; two requests must not share a slot."""
+    no state; two requests must not share a slot. There is no gradient: inputs that
+    require one are refused outside torch.no_grad()."""
     try:
         key = ("scan step", delta_softplus, sig(state), sig(u), sig(delta), sig(A), sig(B), sig(C), sig(D), sig(z),
                sig(delta_bias), sig(slots))
@@ -365,7 +369,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
                  stride(C, 0), stride(C, 1)), dev.index)
         if key is not None:
             _ops.keep_plan(key, ints)
-    _no_grad_state(state)
+    _no_gradients("selective_scan_step", state, u, delta, A, B, C, D, z, delta_bias)
     out = _ops.empty(u)
     s32, s64 = _ops.slot_pointers(slots)
     call("pe_selective_scan_step", _SCAN_STEP.pack(

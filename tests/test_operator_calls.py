@@ -193,3 +193,22 @@ def test_forward_derivatives_are_refused(grad):
             with pytest.raises(NotImplementedError, match="jvp"):
                 f()
         causal_conv(x, w)
+
+
+@pytest.mark.gpu
+def test_steps_refuse_gradients():
+    """Their outputs carry none: an input that asks for one, or has a tangent, is an error."""
+    x, w, k = rand(2, 16, seed=1), rand(16, 4, seed=2), token(scan_inputs(2, 1, 16, 16), 0)
+    cs, ss = rand(2, 3, 16, seed=3), rand(2, 16, 16, seed=4)
+    before = cs.clone(), ss.clone()
+    for a in ((x.clone().requires_grad_(), w), (x, w.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="no gradient"):
+            causal_conv_step(a[0], cs, a[1])
+    for m in k:
+        with pytest.raises(ValueError, match="no gradient"):
+            selective_scan_step(ss, **{**k, m: k[m].clone().requires_grad_()})
+    with torch.no_grad(), forward_ad.dual_level(), pytest.raises(ValueError, match="no gradient"):
+        causal_conv_step(forward_ad.make_dual(x, x.clone()), cs, w)
+    assert torch.equal(cs, before[0]) and torch.equal(ss, before[1])
+    with torch.no_grad():
+        causal_conv_step(x, cs, w.clone().requires_grad_())
