@@ -47,14 +47,16 @@ class _Contract(torch.autograd.Function):
         backend, eq = ctx.plan
         ins, z = eq.replace(" ", "").split("->")
         x, y = ins.split(",")
-        da = backend.contract(f"{z},{y}->{x}", dout, b).to(a.dtype) if ctx.needs_input_grad[2] else None
-        db = backend.contract(f"{x},{z}->{y}", a, dout).to(b.dtype) if ctx.needs_input_grad[3] else None
+        # by the differentiable form: gradients of gradients are contractions again
+        da = contract(backend, f"{z},{y}->{x}", dout, b).to(a.dtype) if ctx.needs_input_grad[2] else None
+        db = contract(backend, f"{x},{z}->{y}", a, dout).to(b.dtype) if ctx.needs_input_grad[3] else None
         return None, None, da, db
 
 
 def contract(backend: GDNChunked, eq: str, a, b):
-    """A contraction on the backend's runners, in the operands' type, differentiable. Every
-    label of an operand has to appear in the other operand or the output."""
+    """A contraction on the backend's runners, in the operands' type, differentiable any
+    number of times. Every label of an operand has to appear in the other operand or the
+    output."""
     return _Contract.apply(backend, eq, a, b)
 
 

@@ -10,6 +10,7 @@ import torch
 from torch.autograd import forward_ad
 
 from pto_einsum import _core, _ops, norm, ssm
+from pto_einsum.mixer import SelectiveMixer, contract
 from pto_einsum.norm import group_norm, group_norm_reference
 from pto_einsum.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
@@ -232,3 +233,36 @@ def test_norms_of_large_finite_maps(dt):
         assert ((y - r).norm() / r.norm()).item() <= 1000 * 2.0 ** -24 + 2.0 ** -20
     else:
         assert (y == 0).all()
+
+
+# ---------------------------------------------------------------------------- second derivatives
+class Detached:
+    """A backend whose results know no gradient, as the compiled runners' do not."""
+
+    def contract(self, eq, a, b):
+        return torch.einsum(eq, a.detach(), b.detach())
+
+
+def test_second_derivatives_of_contractions():
+    a = rand(2, 3, 4, seed=1, device="cpu").double().requires_grad_()
+    b = rand(4, 5, seed=2, device="cpu").double().requires_grad_()
+    g = rand(2, 3, 5, seed=3, device="cpu").double()
+
+    def second(f):
+        y = f("bte,ef->btf", a, b)
+        da, db = torch.autograd.grad((y * y * g).sum(), (a, b), create_graph=True)
+        return torch.autograd.grad((da ** 3).sum() + (db ** 2).sum(), (a, b))
+
+    for u, v in zip(second(lambda eq, a, b: contract(Detached(), eq, a, b)), second(torch.einsum)):
+        assert torch.allclose(u, v, rtol=1e-12)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_of_the_layer_are_refused():
+    """Its other operators have first derivatives only, and say so."""
+    mix = SelectiveMixer(32, 64, heads=2, dtype=F32, device="cuda", seed=3, requires_grad=True)
+    y = mix(rand(2, 24, 32, seed=1))
+    d, = torch.autograd.grad((y * y).sum(), mix.params["w_in"], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (d * d).sum().backward()
+    mix.cleanup()
