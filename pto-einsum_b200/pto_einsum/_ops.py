@@ -165,6 +165,8 @@ def offsets(cu_seqlens, batch: int, tokens: int, dev):
         raise ValueError(f"cu_seqlens must be one row of at least two offsets (got {tuple(cu_seqlens.shape)})")
     if cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"cu_seqlens must be int32 or int64 (got {cu_seqlens.dtype})")
+    if cu_seqlens.dtype == torch.int64:      # an offset past the row stays past it, and is reported
+        cu_seqlens = cu_seqlens.clamp(-1, min(tokens + 1, 2 ** 31 - 1))
     return cu_seqlens.to(torch.int32).contiguous(), cu_seqlens.shape[0] - 1   # itself if it is that
 
 

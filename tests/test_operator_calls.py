@@ -266,3 +266,16 @@ def test_second_derivatives_of_the_layer_are_refused():
     with pytest.raises(RuntimeError, match="once_differentiable"):
         (d * d).sum().backward()
     mix.cleanup()
+
+
+# ---------------------------------------------------------------------------- offsets
+@pytest.mark.gpu
+def test_offsets_past_32_bits_are_reported():
+    """64-bit offsets whose low halves would make a table."""
+    x, w = rand(1, 10, 16, seed=1), rand(16, 4, seed=2)
+    assert _core.device_error() == 0
+    for cu in ([0, 2 ** 32 + 5, 10], [2 ** 32, 5, 10], [0, 5, 10 - 2 ** 32], [0, 5, 2 ** 32 + 10]):
+        causal_conv(x, w, cu_seqlens=torch.tensor(cu, device="cuda"))
+        assert _core.device_error() & 0xFF == 1, cu
+    causal_conv(x, w, cu_seqlens=torch.tensor([0, 5, 10], device="cuda"))
+    assert _core.device_error() == 0
