@@ -155,7 +155,10 @@ def offsets(cu_seqlens, batch: int, tokens: int, dev):
     if tokens > 2 ** 31 - 1:
         raise ValueError("cu_seqlens takes rows of less than 2**31 tokens")
     if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.device.type == "cpu":
-        cu = [int(v) for v in (cu_seqlens.tolist() if hasattr(cu_seqlens, "tolist") else cu_seqlens)]
+        given = list(cu_seqlens.tolist() if hasattr(cu_seqlens, "tolist") else cu_seqlens)
+        cu = [int(v) for v in given]
+        if cu != given:
+            raise ValueError("cu_seqlens must be whole numbers")
         if len(cu) < 2 or cu[0] != 0 or cu[-1] != tokens or any(a > b for a, b in zip(cu, cu[1:])):
             raise ValueError(f"cu_seqlens must rise from 0 to the {tokens} tokens of the row")
         return torch.tensor(cu, dtype=torch.int32, device=dev), len(cu) - 1

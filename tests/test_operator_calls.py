@@ -279,3 +279,14 @@ def test_offsets_past_32_bits_are_reported():
         assert _core.device_error() & 0xFF == 1, cu
     causal_conv(x, w, cu_seqlens=torch.tensor([0, 5, 10], device="cuda"))
     assert _core.device_error() == 0
+
+
+def test_host_offsets_are_whole_numbers():
+    cpu = torch.device("cpu")
+    for cu in ([0, 2.5, 4], torch.tensor([0.0, 2.5, 4.0])):
+        with pytest.raises(ValueError, match="whole numbers"):
+            _ops.offsets(cu, 1, 4, cpu)
+    for cu in ([0, 2, 4], (0, 2, 4), torch.tensor([0, 2, 4]), torch.tensor([0, 2, 4]).numpy(), range(0, 6, 2),
+               [torch.tensor(0), torch.tensor(2), torch.tensor(4)]):
+        table, n = _ops.offsets(cu, 1, 4, cpu)
+        assert table.tolist() == [0, 2, 4] and n == 2
