@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, LPC >= 4 ? 4 : LPC == 2 ? 3 : 2)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const bool in = live && n0 + i < p.N;
-        A[i] = in ? __ldg(p.A + (int64_t)c * p.N + n0 + i) * kLog2e : 0.0f;
+        A[i] = in ? rate(__ldg(p.A + (int64_t)c * p.N + n0 + i)) : 0.0f;
         h[i] = 0.0f;
     }
     const int64_t DN = (int64_t)p.D * p.N, cn = (int64_t)c * p.N + n0;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) scan_carry(const __grid_constant__ S
     const int64_t len = seq_span(p.seqs, s).len, base = piece_base(p.seqs, s, p.piece);
     const int64_t n = len > p.piece ? ceil_div(len, p.piece) : 1;
     const int c = (int)(i / p.N);
-    const float A = __ldg(p.A + i) * kLog2e;
+    const float A = rate(__ldg(p.A + i));
     float h = p.h0 ? __ldg(p.h0 + s * DN + i) : 0.0f;
     float* hp = p.hloc + base * DN + i;
     const float* sp = p.dtsum + base * p.D + c;

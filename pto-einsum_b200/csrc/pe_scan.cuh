@@ -2,6 +2,7 @@
 // placement of blocks, tiles and staging, and the host's checks.
 #pragma once
 
+#include <cfloat>
 #include <initializer_list>
 
 #include "pe_mixer.cuh"
@@ -92,6 +93,12 @@ __device__ __forceinline__ Place place_of(const P& p) {
 constexpr float kLow = 1.7e-8f;
 __device__ __forceinline__ f32x2 decay2(f32x2 dt, f32x2 A) { return exp2_2(fma2(dt, A, both(kLow))); }
 __device__ __forceinline__ float decay(float dt, float A) { return exp2_fast(fmaf(dt, A, kLow)); }
+// A in those units, and finite: where A is -inf the state forgets everything, but a token past the
+// end, with dt = 0, has to leave it as it is, and 0 times infinity is neither.
+__device__ __forceinline__ float rate(float A) {
+    const float a = A * kLog2e;
+    return a < -FLT_MAX ? -FLT_MAX : a;
+}
 
 // ---- copies to shared memory ------------------------------------------------------
 // By the NT threads of the block: cnt (at most ROWS) rows of `width` (at most W) elements

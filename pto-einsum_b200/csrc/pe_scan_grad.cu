@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) scan_bwd(const __grid_constan
         const int64_t k = (int64_t)(w.c0 + ci) * f.N + n;
         const bool in = ci < w.nch;
         sG[n * CB + ci] = in && from ? from[k] : 0.0f;
-        sA[n * CB + ci] = in ? __ldg(f.A + k) * kLog2e : 0.0f;
+        sA[n * CB + ci] = in ? rate(__ldg(f.A + k)) : 0.0f;
         sD[n * CB + ci] = 0.0f;
         if (!in) sK[i] = 0.0f;
     }
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_adjoint(const __grid_constan
     for (int i = tid; i < CB * f.N; i += kThreads) {
         const int ci = i / f.N, n = i - ci * f.N;
         sG[n * CB + ci] = 0.0f;
-        sA[n * CB + ci] = ci < w.nch ? __ldg(f.A + (int64_t)(w.c0 + ci) * f.N + n) * kLog2e : 0.0f;
+        sA[n * CB + ci] = ci < w.nch ? rate(__ldg(f.A + (int64_t)(w.c0 + ci) * f.N + n)) : 0.0f;
     }
     const int cp = tid % (CB / 2) * 2;
     float bias[2], dtsum[2] = {0.0f, 0.0f};
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kThreads) adjoint_carry(const __grid_constant_
     const int s = blockIdx.y;
     const int64_t len = seq_span(f.seqs, s).len, base = piece_base(f.seqs, s, f.piece);
     const int64_t n = len > f.piece ? ceil_div(len, f.piece) : 1;
-    const float A = __ldg(f.A + i) * kLog2e;
+    const float A = rate(__ldg(f.A + i));
     float g = p.dstate ? __ldg(p.dstate + s * DN + i) : 0.0f;
     float* gp = p.gloc + base * DN + i;
     const float* sp = p.dtsum + base * f.D + i / f.N;

@@ -12,7 +12,8 @@ from torch.autograd import forward_ad
 from pto_einsum import _core, _ops, norm, ssm
 from pto_einsum.mixer import SelectiveMixer, contract
 from pto_einsum.norm import group_norm, group_norm_reference
-from pto_einsum.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+from pto_einsum.ssm import (causal_conv, causal_conv_step, selective_scan, selective_scan_reference,
+                            selective_scan_step)
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -290,3 +291,28 @@ def test_host_offsets_are_whole_numbers():
                [torch.tensor(0), torch.tensor(2), torch.tensor(4)]):
         table, n = _ops.offsets(cu, 1, 4, cpu)
         assert table.tolist() == [0, 2, 4] and n == 2
+
+
+# ---------------------------------------------------------------------------- infinite rates
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,D", [(2, 20, 16), (1, 5000, 48)])
+def test_states_that_forget_everything(B, T, D):
+    """A = -inf: each token starts from nothing, and the last state is its own. A tile's rows past the
+    last token, whose steps are zero, must not take part. Whole sequences and one split along time."""
+    k = scan_inputs(B, T, D, 16)
+    k["A"][:, 3] = -float("inf")
+    y, end = selective_scan(**k, delta_softplus=True, return_state=True)
+    r, rend = selective_scan_reference(**k, delta_softplus=True)
+    tol = 2.0 ** -20 + T ** 0.5 * 2.0 ** -18
+    for a, b in ((y, r), (end, rend)):
+        assert torch.isfinite(a).all() and ((a - b).norm() / b.norm()).item() <= tol
+    # the gradients are those of a rate so large that it forgets as well
+    got = []
+    for rate in (-float("inf"), -1e30):
+        own = {m: t.clone().requires_grad_() for m, t in k.items()}
+        with torch.no_grad():
+            own["A"][:, 3] = rate
+        y, end = selective_scan(**own, delta_softplus=True, return_state=True)
+        got.append(torch.autograd.grad([y, end], list(own.values()), [torch.ones_like(y), torch.ones_like(end)]))
+    for m, a, b in zip(k, *got):
+        assert torch.isfinite(a).all() and torch.equal(a, b), m
