@@ -629,8 +629,7 @@ int scan_run(const pe_scan_args* a, cudaStream_t s) {
     ScanP<T> p = scan_params<T>(a, kThreads / LPC, 4 * LPC);
     const int64_t piece = piece_tokens(a);
     if (piece) {
-        p.piece = piece;
-        p.longest_first = false;
+        p.split(piece);
         const int64_t n = piece_count(p.seqs, piece);
         p.hloc = (float*)a->ws;
         p.dtsum = p.hloc + n * p.D * p.N;

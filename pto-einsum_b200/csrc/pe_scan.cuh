@@ -33,6 +33,11 @@ struct ScanP {
     bool longest_first;   // packed sequences are taken in the order of their lengths
     int64_t piece;        // tokens a piece (a multiple of KCK, or more than any sequence has)
     float *hloc, *dtsum;  // ws of a split scan: each piece's own last state and sum of dt
+
+    void split(int64_t tokens) {   // pieces have about one length, and a place of their own in the order
+        piece = tokens;
+        longest_first = false;
+    }
 };
 
 // Where a block works: channel tile, group and piece.
@@ -201,7 +206,7 @@ ScanP<T> scan_params(const pe_scan_args* a, int ch, int nc) {
     p.C_sb = a->C_sb; p.C_st = a->C_st; p.C_sg = a->C_sg;
     p.out = (T*)a->out; p.state = a->state; p.ckpt = a->ckpt;
     p.piece = (a->tokens / KCK + 1) * KCK;   // longer than any sequence: one piece each, numbered like it
-    p.longest_first = a->cu && a->nseq > 1 && a->nseq <= kThreads;   // whole sequences; a split clears it
+    p.longest_first = a->cu && a->nseq > 1 && a->nseq <= kThreads;
     p.hloc = p.dtsum = nullptr;
     const int es = sizeof(T);
     const int64_t step = p.G > 1 ? p.Dg : ch, row = (int64_t)ch * es;   // of a block's first channel

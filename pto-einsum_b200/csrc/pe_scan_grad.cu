@@ -763,7 +763,7 @@ int grad_type(const pe_scan_grad_args* a, cudaStream_t s) {
     if (int rc = grid_of(w.pieces * p.f.G * p.f.ntile, &grid)) return rc;
     if (f->nseq == 0) grid = 0;
     if (grid && w.piece) {
-        p.f.piece = w.piece;
+        p.f.split(w.piece);
         p.gloc = ws + w.g;
         p.dtsum = ws + w.s;
         if (int rc = launch(scan_adjoint<T>, p, grid, sizeof(AdjSmem<T>) + 2 * p.f.N * CB * 4, s)) return rc;
