@@ -803,13 +803,9 @@ struct Moments {
     float n, mean, m2;
     __device__ __forceinline__ void join(float bn, float bmean, float bm2) {
         if (bn == 0.0f) return;
-        if (n == 0.0f) {   // the other whole: its mean is no distance, and its square may overflow
-            n = bn, mean = bmean, m2 = bm2;
-            return;
-        }
         const float t = n + bn, d = bmean - mean, f = bn / t;
         mean = fmaf(d, f, mean);
-        m2 += bm2 + d * (d * (n * f));   // in this order nothing overflows that the sum does not
+        m2 += bm2 + (d * n) * (d * f);   // 0 from n = 0, and no overflow that the sum does not have
         n = t;
     }
 };
