@@ -30,6 +30,14 @@ def sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
+def sigs(*tensors):
+    """That of several, and where gradients are recorded whether they ask for one."""
+    if not torch.is_grad_enabled():
+        return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device(), t.requires_grad)
+                  for t in tensors])
+
+
 def plan(key):
     return _plans.get(key)
 
@@ -59,10 +67,10 @@ def function(name: str, restype=ctypes.c_int, argtypes=(ctypes.c_char_p, ctypes.
 def call(name: str, args: bytes, idx: int):
     """Enqueue on the current stream of device `idx`; a nonzero status raises RuntimeError."""
     global _raw_stream
-    if _raw_stream is None:
-        _raw_stream = _raw_stream_getter()
     fn = _fns.get(name) or function(name)
     if idx == _get_device():
+        if _raw_stream is None:
+            _raw_stream = _raw_stream_getter()
         rc = fn(args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
@@ -196,7 +204,7 @@ def wants_grad(*tensors) -> bool:
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    if getattr(forward_ad, "_current_level", 0) >= 0:   # inside dual_level
+    if forward_ad._current_level >= 0:   # inside dual_level
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True

@@ -31,6 +31,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -158,7 +159,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     and touch no state; two requests must not share a slot. There is no gradient: inputs
     that require one are refused outside torch.no_grad()."""
     try:
-        key = ("conv step", activation, sig(x), sig(state), sig(weight), sig(bias), sig(slots))
+        key = ("conv step", activation, _ops.sigs(x, state, weight, bias, slots))
         ints = plan(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = ints = None
@@ -173,17 +174,23 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
             key = None
             x, weight = rows(x), weight.contiguous()
             bias = None if bias is None else bias.contiguous()
-        ints = (DTYPES[x.dtype], silu, W, B, C, state.shape[0], stride(x, 0), x.device.index)
+        ints = (DTYPES[x.dtype], silu, W, B, C, state.shape[0], stride(x, 0), x.device.index,
+                _ask_for_gradients(x, state, weight, bias), x.is_contiguous())
         if key is not None:
             _ops.keep_plan(key, ints)
-    _no_gradients("causal_conv_step", state, x, weight, bias)
-    out = _ops.empty(x)
-    s32, s64 = _ops.slot_pointers(slots)
+    if ints[8] or forward_ad._current_level >= 0:
+        _no_gradients("causal_conv_step", state, x, weight, bias)
+    out = torch.empty_like(x) if ints[9] else _ops.empty(x)
+    s32, s64 = (0, 0) if slots is None else _ops.slot_pointers(slots)
     call("pe_causal_conv_step", _CONV_STEP.pack(
         *ints[:6], s32, s64, x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), ints[6],
         state.data_ptr(), out.data_ptr()), ints[7])
     increment_version(state)   # autograd sees the kernel's writes as its own in-place operations
     return out
+
+
+def _ask_for_gradients(*tensors) -> bool:
+    return any(t is not None and t.requires_grad for t in tensors)
 
 
 def _no_gradients(name, state, *inputs):
@@ -346,8 +353,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
     no state; two requests must not share a slot. There is no gradient: inputs that
     require one are refused outside torch.no_grad()."""
     try:
-        key = ("scan step", delta_softplus, sig(state), sig(u), sig(delta), sig(A), sig(B), sig(C), sig(D), sig(z),
-               sig(delta_bias), sig(slots))
+        key = ("scan step", delta_softplus, _ops.sigs(state, u, delta, A, B, C, D, z, delta_bias, slots))
         ints = plan(key)
     except (AttributeError, TypeError):
         key = ints = None
@@ -366,12 +372,14 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, *, z=None, delta_bias=
             key = None
         ints = ((DTYPES[u.dtype], int(bool(delta_softplus)), Bt, Dc, A.shape[1], B.shape[1], state.shape[0]),
                 (stride(u, 0), stride(delta, 0), 0 if z is None else stride(z, 0), stride(B, 0), stride(B, 1),
-                 stride(C, 0), stride(C, 1)), dev.index)
+                 stride(C, 0), stride(C, 1)), dev.index, _ask_for_gradients(state, u, delta, A, B, C, D, z, delta_bias),
+                u.is_contiguous())
         if key is not None:
             _ops.keep_plan(key, ints)
-    _no_gradients("selective_scan_step", state, u, delta, A, B, C, D, z, delta_bias)
-    out = _ops.empty(u)
-    s32, s64 = _ops.slot_pointers(slots)
+    if ints[3] or forward_ad._current_level >= 0:
+        _no_gradients("selective_scan_step", state, u, delta, A, B, C, D, z, delta_bias)
+    out = torch.empty_like(u) if ints[4] else _ops.empty(u)
+    s32, s64 = (0, 0) if slots is None else _ops.slot_pointers(slots)
     call("pe_selective_scan_step", _SCAN_STEP.pack(
         *ints[0], s32, s64, u.data_ptr(), delta.data_ptr(), 0 if z is None else z.data_ptr(), B.data_ptr(),
         C.data_ptr(), A.data_ptr(), 0 if D is None else D.data_ptr(),
