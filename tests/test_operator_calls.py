@@ -316,3 +316,26 @@ def test_states_that_forget_everything(B, T, D):
         got.append(torch.autograd.grad([y, end], list(own.values()), [torch.ones_like(y), torch.ones_like(end)]))
     for m, a, b in zip(k, *got):
         assert torch.isfinite(a).all() and torch.equal(a, b), m
+
+
+# ---------------------------------------------------------------------------- shared memory
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("N", [1, 6, 7, 8, 9, 11, 12, 40])
+def test_split_scans_of_any_number_of_states(N, dt):
+    """The launches' shared memory grows with the states, past what a block has without asking for more."""
+    k = scan_inputs(1, 600, 40, N, dt)
+    k["delta_bias"] = k["delta_bias"] - 2
+    own = {m: t.clone().requires_grad_() for m, t in k.items()}
+    ref = {m: t.double().requires_grad_() for m, t in k.items()}
+    n0 = _core.launch_count()
+    y, r = selective_scan(**own, delta_softplus=True), selective_scan_reference(**ref, delta_softplus=True)[0]
+    assert _core.launch_count() == n0 + 3
+    dy = rand(*y.shape, seed=9, dtype=dt)
+    got = torch.autograd.grad(y, list(own.values()), dy)
+    assert _core.launch_count() == n0 + 8
+    want = torch.autograd.grad(r, list(ref.values()), dy.double())
+    for m, a, b in zip(k, got, want):
+        unit = torch.finfo(a.dtype).eps / 2
+        tol = 4 * (unit + 2.0 ** -20 + 600 ** 0.5 * 2.0 ** -18)
+        assert torch.isfinite(a).all() and ((a - b).norm() / b.norm()).item() <= tol, m
