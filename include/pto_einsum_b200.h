@@ -186,7 +186,8 @@ int pe_permute(const pe_permute_plan* plan, const void* in, void* out, void* str
  * rows of `tokens` tokens (nseq = batch); else batch is 1 and sequence s is tokens
  * cu[s] .. cu[s + 1] - 1 of the row, cu[0] = 0, cu[nseq] = tokens, never falling (a
  * table that is not so gives PE_ERR_INVALID in the device word and outputs of no
- * meaning). Sequences may be empty. Every field is 8 bytes wide.
+ * meaning). Sequences may be empty. Every field is 8 bytes wide. Addresses need their
+ * elements' alignment (ws: 4 bytes); 16 bytes is the fast path.
  */
 
 /*

@@ -165,15 +165,15 @@ struct ConvGradP {
     int bx;             // channel vectors a block (power of two <= 32)
 };
 
-// One thread does for its channels and tokens what each of the three results needs: the
-// slope of silu from the recomputed sum, dx from the window of g, the sums of dw and
-// dbias in registers to the end of the walk, then over the block's threads in order, and
-// over blocks by sum_rows. Bound by instructions at few warps: 4 x 2048 x 2048 f16 31 us,
-// 3.2 TB/s; 16384 x 4352 bf16 102 us, 4.2 TB/s. Eight channels a thread and one block an SM
-// beat four channels and two (51 us against 34 at the time): what a token costs beside its
-// channels is paid half as often. The tokens inside a tile have a loop without the ends'
-// conditions: 194 us with them for 16384 x 4352 and its forward pass, 179 without. Elements
-// (V = 1), forward and backward of 8000 x 2049 bf16: 124 us, 50 for x 2048 in 16-byte accesses.
+// One thread does for its channels and tokens what each of the three results needs: the slope of
+// silu from the recomputed sum, dx from the window of g, the sums of dw and dbias in registers to
+// the end of the walk, then over the block's threads in order, and over blocks by sum_rows. Bound
+// by instructions at few warps: 4 x 2048 x 2048 f16 31 us, 3.2 TB/s; 16384 x 4352 bf16 102 us, 4.2
+// TB/s. Eight channels a thread and one block an SM beat four channels and two (51 us against 34,
+// both before the loop below had its form without edges): what a token costs beside its channels is
+// paid half as often. The tokens inside a tile have a loop without the ends' conditions: 194 us
+// with them for 16384 x 4352 and its forward pass, 179 without. Elements (V = 1), forward and
+// backward of 8000 x 2049 bf16: 124 us, 50 for x 2048 in 16-byte accesses.
 // Blocks an SM holds: by the registers of V channels' taps, sums and windows.
 __host__ __device__ constexpr int bwd_blocks(int v) { return v <= 4 ? 2 : 1; }
 

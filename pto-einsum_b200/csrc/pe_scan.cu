@@ -130,11 +130,12 @@ struct Feeder {
 // tile i; what one barrier interval writes, the next one reads. Tokens past the end have
 // dt = 0 and B = 0: they leave the state as it is.
 //
-// Bound by instructions issued, 42 a warp and four states of a token: 17 packed fp16 prompts of 8192 tokens
-// in all, 4096 channels, 16 states take 253 us, 2.7 T exponentials a second (57% of 16 a
-// clock an SM). More tiles than 16 tokens' would take the shared memory of a block (four an
-// SM; five, at 96 registers, were 3% slower). A form parallel along the tokens, lanes
-// composing their tokens' maps, needed 64 instructions and 1.6 times the time.
+// Instructions, 42 a warp and four states of a token, and their latency at four warps a scheduler
+// count about alike: it issues in 62% of the clocks. 17 packed fp16 prompts of 8192 tokens in all,
+// 4096 channels, 16 states take 253 us, 2.7 T exponentials a second (57% of 16 a clock an SM). More
+// tiles than 16 tokens' would take the shared memory of a block (four an SM; five, at 96 registers,
+// were 3% slower). A form parallel along the tokens, lanes composing their tokens' maps, needed 64
+// instructions and 1.6 times the time.
 //
 // FAST: 16-byte asynchronous copies, where all rows allow them, against elements through
 // registers: 2 x 8000 tokens of 2048 and of 2049 channels 447 and 605 us.

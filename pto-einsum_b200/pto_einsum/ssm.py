@@ -17,14 +17,15 @@ Spaces", 2023, algorithm 2), per channel d of group g and state n:
 
 Packed prompts: with ``cu_seqlens`` (S + 1 rising offsets, as in `pto_einsum.gdn`, but
 any lengths, empty ones too) the batch is one row that holds S sequences. A list or a
-host tensor is checked by the host; an int32 tensor on the device costs no
-synchronisation, and a wrong one shows in `_core.device_error`.
+host tensor is checked by the host and copied, which waits for the stream; an int32
+tensor on the device costs no synchronisation, and a wrong one shows in
+`_core.device_error`.
 
 Both prompt operators are differentiable in every floating argument. Their gradients
 are written by kernels that add in a fixed order: the same inputs give the same bits.
 The `_step` forms take one token of each request and update the states in place, in
 rows picked by ``slots`` where the states live in a pool (a negative slot skips the
-request).
+request). A scan step takes up to 65535 requests.
 """
 from __future__ import annotations
 
